@@ -471,6 +471,113 @@ typedef struct {
 
 int sfl_prefill_layers(const sfl_prefill_args* args, void* stream);
 
+/* ---- drafted tokens over a bounded KV cache -----------------------------------
+ * No counterpart in the reference: the calls of a serving step that verifies
+ * several drafted tokens of each sequence at once and keeps the cache within a
+ * budget. A cache is k, v [batch, kv_heads, capacity, head_dim] of one dtype
+ * (F32, BF16 or F16); sequence b has lengths[b] committed rows in slots
+ * [0, lengths[b]) and its drafts' rows from slot lengths[b] on. head_dim 16, 32,
+ * 64 or 128. `strides`: one array of strides in elements, per tensor {batch,
+ * head, row}; the last dimension is contiguous. Lengths, counts, positions and
+ * paths are read on the device: values outside their range are clamped or their
+ * rows left out, never followed out of a buffer.
+ */
+
+/*
+ * Norm, rotation and cache append of new tokens, in one pass:
+ *   x = x / sqrt(mean(x^2) + eps) * gain        (q and k; where a gain is given)
+ *   (x1, x2) = (x1 cos - x2 sin, x2 cos + x1 sin) over the first rotary_dim dims,
+ *   pairs (i, i + rotary_dim/2) with half_layout, else (2i, 2i + 1)
+ * in fp32, rounded once. cos, sin [table, rotary_dim/2] fp32 by position; a position
+ * outside [0, table) gives NaN.
+ *   q [batch, q_heads, tokens], k, v [batch, kv_heads, tokens] rows of head_dim
+ *   positions [batch, tokens] int32
+ *   q_gain, k_gain [head_dim] of gain_dtype (dtype or F32) or NULL
+ *   start   [batch] int32 or NULL: k and v rows of token t go to slot start[b] + t of
+ *           k_out, v_out (rows without such a slot are left out); NULL: to row t
+ *   counts  [batch] int32 or NULL: tokens in use. The rest is padding: zeros in
+ *           q_out (and in k_out, v_out where start is NULL), nothing in a cache
+ *   v, v_out: may be NULL (both)
+ *   strides [18]: q, k, v, q_out, k_out, v_out
+ * Outputs must not overlap inputs.
+ */
+int sfl_rotate(const void* q, const void* k, const void* v, const int32_t* positions, const float* cos,
+               const float* sin, const void* q_gain, const void* k_gain, const int32_t* start,
+               const int32_t* counts, void* q_out, void* k_out, void* v_out, const long* strides, int batch,
+               int tokens, int q_heads, int kv_heads, int head_dim, int rotary_dim, int table, int slots,
+               int half_layout, int gain_dtype, float eps, int dtype, void* stream);
+
+/*
+ * Attention of `tokens` (at most 128) drafts of each sequence: draft t sees the keys
+ * of slots [0, lengths[b]) and those of slots lengths[b] + j, j < counts[b], with
+ * mask[b, t, j] != 0. out = softmax(q k^T scale) v, lse = log sum exp(q k^T scale)
+ * (natural, fp32 [batch, q_heads, tokens]); a draft that sees nothing or lies past
+ * counts[b] has a zero row and lse -inf. Keys that a draft does not see have no part
+ * in its row, whatever their rows hold.
+ *   q, out [batch, q_heads, tokens] rows, Hq/Hkv in {1, 2, 4, 8}
+ *   mask   uint8, strides {batch, t, j} (0 for a shared one); counts [batch] or NULL
+ *   partial_max, partial_sum  batch * q_heads * tokens * splits fp32 values, partial_out
+ *   head_dim times as many: scratch, unused (may be NULL) with splits == 1
+ *   strides [15]: q, k, v, out, mask. q, k, v, out 16-byte aligned, their strides
+ *   multiples of 16 bytes
+ * Every sum in fp32. Results do not vary from call to call.
+ */
+int sfl_tree_attention(const void* q, const void* k, const void* v, const int32_t* lengths, const uint8_t* mask,
+                       const int32_t* counts, float* partial_max, float* partial_sum, float* partial_out,
+                       void* out, float* lse, const long* strides, int batch, int q_heads, int kv_heads,
+                       int capacity, int tokens, int head_dim, int splits, float scale, int dtype, void* stream);
+
+/*
+ * weights[b, h, slot] += sum of exp(q k^T scale - lse) over the drafts with rows[b, t]
+ * (uint8 [batch, tokens], NULL: all in use) and the query heads of KV head h, for the
+ * slots each draft sees; weights fp32 [batch, kv_heads, capacity]. The other
+ * arguments as for sfl_tree_attention (strides [15]: v's and out's are not used).
+ */
+int sfl_tree_weights(const void* q, const void* k, const float* lse, float* weights, const int32_t* lengths,
+                     const uint8_t* mask, const int32_t* counts, const uint8_t* rows, const long* strides,
+                     int batch, int q_heads, int kv_heads, int capacity, int tokens, int head_dim, float scale,
+                     int dtype, void* stream);
+
+/*
+ * Commits an accepted path: slot lengths[b] + j takes the rows (k, v, and weights and
+ * positions [batch, kv_heads, capacity] where not NULL) that slot lengths[b] + path[b, j]
+ * held before the call, for j < accepted[b]; new_lengths[b] = lengths[b] + accepted[b].
+ * The weights of the slots of the other drafts become 0. path [batch, tokens] int32,
+ * tokens at most 128; entries outside [0, tokens) or the cache move nothing. accepted is
+ * clamped to [0, tokens] and to what the cache holds. new_lengths is not lengths.
+ * strides [6]: k, v, multiples of 16 bytes, k and v 16-byte aligned.
+ */
+int sfl_accept_path(void* k, void* v, float* weights, int32_t* positions, const int32_t* lengths,
+                    const int32_t* path, const int32_t* accepted, int32_t* new_lengths, const long* strides,
+                    int batch, int kv_heads, int capacity, int tokens, int head_dim, int dtype, void* stream);
+
+#define SFL_SELECT_MAX_SLOTS 262144
+
+/*
+ * Which slots stay when each KV head keeps `keep` of them: first the recent ones (those
+ * whose position is above the row's largest minus `recent`, the lowest slots where they
+ * share positions and are more than keep; positions [batch, kv_heads, capacity] int32,
+ * NULL: a slot's index), then the others by weight (fp32 [batch,
+ * kv_heads, capacity], NaN below every number), ties to the lowest slot. kept [batch,
+ * kv_heads, keep] int32: i itself where slot i < keep stays; the places of the others,
+ * ascending, take the slots >= keep that stay, ascending. A sequence of at most keep
+ * slots keeps them all, and -1 follows. new_lengths[b] = min(lengths[b], keep).
+ * capacity at most SFL_SELECT_MAX_SLOTS.
+ */
+int sfl_select_slots(const float* weights, const int32_t* lengths, const int32_t* positions, int32_t* kept,
+                     int32_t* new_lengths, int batch, int kv_heads, int capacity, int keep, int recent,
+                     void* stream);
+
+/*
+ * Slot i of k and v (and of weights and positions where not NULL) takes what slot
+ * kept[b, h, i] held, where kept is from sfl_select_slots: entries >= keep move, all
+ * others stay. The weights of slots from keep on become 0. strides [6]: k, v, multiples
+ * of 16 bytes, k and v 16-byte aligned.
+ */
+int sfl_compact_slots(void* k, void* v, float* weights, int32_t* positions, const int32_t* kept,
+                      const long* strides, int batch, int kv_heads, int capacity, int keep, int head_dim,
+                      int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,486 @@
+// Rows of a KV cache: new tokens' q, k and v normed, rotated and written into it,
+// an accepted path moved behind the committed rows, and the rows of an eviction's
+// kept slots moved into the places that become free. All of it moves bytes: the
+// bound is memory, and below a few hundred KB the launch.
+#include "common.hpp"
+
+namespace sfl {
+namespace {
+
+struct RotateArgs {
+  const void *q, *k, *v;
+  const int32_t* positions;
+  const float *cos, *sin;
+  const void *q_gain, *k_gain;
+  const int32_t *start, *counts;
+  void *q_out, *k_out, *v_out;
+  long st[6][3];  // strides in elements (batch, head, token) of q, k, v, q_out, k_out, v_out
+  int batch, tokens, q_heads, kv_heads, half, table, slots, gain_f32;
+  float eps;
+};
+
+// One row of the launch: token t of sequence b, head h of q, then k, then v.
+struct RotateRow {
+  const void* in;
+  void* out;
+  const void* gain;
+  bool turn;   // q and k; v is copied
+  bool store;  // whether the row has a place
+  bool zero;   // padding of an output that is not a cache
+};
+template <typename T>
+__device__ __forceinline__ RotateRow rotate_row(const RotateArgs& a, int b, int t, int h) {
+  const int which = h < a.q_heads ? 0 : h < a.q_heads + a.kv_heads ? 1 : 2;
+  const int head = which == 0 ? h : which == 1 ? h - a.q_heads : h - a.q_heads - a.kv_heads;
+  const bool used = !a.counts || t < a.counts[b];
+  // q goes to token t of its output; k and v to slot start + t of the cache, where it has that slot.
+  const long slot = which && a.start ? long(a.start[b]) + t : t;
+  RotateRow r;
+  r.in = static_cast<const T*>(which == 0 ? a.q : which == 1 ? a.k : a.v) + b * a.st[which][0] + head * a.st[which][1] +
+         t * a.st[which][2];
+  r.out = static_cast<T*>(which == 0 ? a.q_out : which == 1 ? a.k_out : a.v_out) + b * a.st[3 + which][0] +
+          head * a.st[3 + which][1] + slot * a.st[3 + which][2];
+  r.gain = which == 0 ? a.q_gain : which == 1 ? a.k_gain : nullptr;
+  r.turn = which < 2;
+  r.zero = !used;
+  r.store = which == 0 || !a.start || (used && slot >= 0 && slot < a.slots);
+  return r;
+}
+
+__device__ __forceinline__ float gain_at(const RotateArgs& a, const void* gain, int d, float) {
+  return static_cast<const float*>(gain)[d];
+}
+template <typename T>
+__device__ __forceinline__ float gain_at(const RotateArgs& a, const void* gain, int d, T) {
+  return a.gain_f32 ? static_cast<const float*>(gain)[d] : load_scalar<T>(static_cast<const T*>(gain) + d);
+}
+
+// One wave per row, a row staged in LDS as fp32: any layout, rotated part and alignment.
+template <typename T, bool kHalfLayout>
+__global__ __launch_bounds__(256) void rotate_any_kernel(const RotateArgs a, int dim, long rows, int heads) {
+  __shared__ float stage[4][128];
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+  const long at = long(blockIdx.x) * 4 + wave;
+  const bool on = at < rows;
+  const long token = (on ? at : 0) / heads;
+  const int h = int((on ? at : 0) - token * heads), b = int(token / a.tokens), t = int(token - long(b) * a.tokens);
+  const RotateRow r = rotate_row<T>(a, b, t, h);
+  float x[2], sq = 0.f;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int d = lane + kWave * e;
+    x[e] = d < dim ? load_scalar<T>(static_cast<const T*>(r.in) + d) : 0.f;
+    sq = fmaf(x[e], x[e], sq);
+  }
+  if (r.gain) {
+    const float scale = 1.f / sqrtf(wave_sum(sq) / float(dim) + a.eps);
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      if (lane + kWave * e < dim) x[e] *= scale * gain_at(a, r.gain, lane + kWave * e, T{});
+  }
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+    if (lane + kWave * e < dim) stage[wave][lane + kWave * e] = x[e];
+  __syncthreads();
+  if (!on || !r.store) return;
+  const int pos = a.positions[long(b) * a.tokens + t];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int d = lane + kWave * e;
+    if (d >= dim) continue;
+    float y = x[e];
+    if (r.turn && d < 2 * a.half) {
+      const int i = kHalfLayout ? d % a.half : d / 2;
+      const bool second = kHalfLayout ? d >= a.half : d & 1;
+      const float other = stage[wave][kHalfLayout ? (second ? d - a.half : d + a.half) : d ^ 1];
+      const bool known = pos >= 0 && pos < a.table;
+      const float c = known ? a.cos[long(pos) * a.half + i] : NAN, s = known ? a.sin[long(pos) * a.half + i] : NAN;
+      y = second ? fmaf(other, s, y * c) : fmaf(-other, s, y * c);
+    }
+    store_scalar<T>(static_cast<T*>(r.out) + d, r.zero ? 0.f : y);
+  }
+}
+
+// ---- accepted path --------------------------------------------------------------
+
+constexpr int kMaxPath = 128;
+
+// Row len + j of a sequence's cache takes what row len + path[j] held, j < accepted.
+// One workgroup has all the rows of a (sequence, KV head) in one tensor and reads
+// every one before it writes any, so chains of rows that move are safe. Blocks in
+// z: k, v, the slot values (which also lose the rejected drafts' weights).
+struct AcceptArgs {
+  void *k, *v;
+  float* weights;
+  int32_t* positions;
+  const int32_t *lengths, *path, *accepted;
+  int32_t* new_lengths;
+  long ks[3], vs[3];
+  int kv_heads, cap, tokens, row_pieces;  // 16-byte pieces of a row
+  int elem_bytes;
+};
+__global__ __launch_bounds__(256) void accept_kernel(const AcceptArgs a) {
+  const int b = int(blockIdx.x) / a.kv_heads, hk = int(blockIdx.x) - b * a.kv_heads;
+  const int len = a.lengths[b];
+  const int count = len < 0 || len > a.cap ? 0 : min(min(max(a.accepted[b], 0), a.tokens), a.cap - len);
+  const int32_t* path = a.path + long(b) * a.tokens;
+  const auto source = [&](int j) {  // the slot that moves to len + j, -1 for none
+    const int from = path[j];
+    return from >= 0 && from < a.tokens && len + from < a.cap ? len + from : -1;
+  };
+  if (blockIdx.y == 2) {
+    const int j = threadIdx.x;
+    const long base = (long(b) * a.kv_heads + hk) * a.cap;
+    if (hk == 0 && j == 0) a.new_lengths[b] = len + count;
+    const int from = j < count ? source(j) : -1;
+    float w = 0.f;
+    int32_t p = 0;
+    if (from >= 0 && a.weights) w = a.weights[base + from];
+    if (from >= 0 && a.positions) p = a.positions[base + from];
+    __syncthreads();
+    if (len < 0 || j >= a.tokens || len + j >= a.cap) return;
+    if (a.weights && (from >= 0 || j >= count)) a.weights[base + len + j] = w;
+    if (a.positions && from >= 0) a.positions[base + len + j] = p;
+    return;
+  }
+  unsigned char* rows = static_cast<unsigned char*>(blockIdx.y ? a.v : a.k);
+  const long* st = blockIdx.y ? a.vs : a.ks;
+  rows += (b * st[0] + hk * st[1]) * a.elem_bytes;
+  constexpr int kPieces = kMaxPath * 32 / 256;  // of 16 bytes, per thread: 128 rows of 512 bytes
+  uint4 held[kPieces];
+#pragma unroll
+  for (int i = 0; i < kPieces; ++i) {
+    const int at = int(threadIdx.x) + 256 * i, j = at / a.row_pieces;
+    const int from = j < count ? source(j) : -1;
+    if (from >= 0) held[i] = load16(rows + from * st[2] * a.elem_bytes + 16 * (at - j * a.row_pieces));
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kPieces; ++i) {
+    const int at = int(threadIdx.x) + 256 * i, j = at / a.row_pieces;
+    if (j < count && source(j) >= 0)
+      *reinterpret_cast<uint4*>(rows + (len + j) * st[2] * a.elem_bytes + 16 * (at - j * a.row_pieces)) = held[i];
+  }
+}
+
+// ---- eviction -------------------------------------------------------------------
+
+// Weights as unsigned numbers in the same order: -0 as 0, NaN below every number,
+// and above them all the slots that stay because they are recent.
+__device__ __forceinline__ uint32_t weight_key(float w) {
+  if (w != w) return 0u;
+  const uint32_t u = __float_as_uint(w + 0.f);
+  return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
+}
+
+struct SelectArgs {
+  const float* weights;
+  const int32_t *lengths, *positions;
+  int32_t *kept, *new_lengths;
+  int kv_heads, cap, keep, recent;
+};
+
+constexpr int kSelectThreads = 1024;
+constexpr int kSelectWaves = kSelectThreads / kWave;
+
+// Sum over the workgroup of what the threads before this one have; *total: all of them.
+__device__ __forceinline__ int block_exclusive(int v, int* scratch, int* total) {
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  int incl = v;
+  for (int d = 1; d < kWave; d <<= 1) {
+    const int up = __shfl_up(incl, d);
+    if (lane >= d) incl += up;
+  }
+  __syncthreads();  // scratch may still be read
+  if (lane == kWave - 1) scratch[wave] = incl;
+  __syncthreads();
+  int before = 0, all = 0;
+  for (int w = 0; w < kSelectWaves; ++w) {
+    if (w < wave) before += scratch[w];
+    all += scratch[w];
+  }
+  *total = all;
+  return before + incl - v;
+}
+
+// kept[b, h, i]: the slot whose rows belong into slot i. A radix selection, 8 bits at
+// a time, finds the key of the last slot that stays; slots with that very key stay
+// from the lowest on. Bits of the slots that stay go to LDS, with the count before
+// each word, so that the r-th that stays above keep finds the r-th hole below it.
+__global__ __launch_bounds__(kSelectThreads) void select_kernel(const SelectArgs a) {
+  extern __shared__ __align__(16) unsigned char dynamic[];
+  __shared__ int hist[256];
+  __shared__ int scratch[kSelectWaves];
+  __shared__ uint32_t found[3];  // the digit, what is needed of its keys, newest
+  const int b = int(blockIdx.x) / a.kv_heads, hk = int(blockIdx.x) - b * a.kv_heads;
+  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+  const int n = min(max(a.lengths[b], 0), a.cap);
+  int32_t* kept = a.kept + long(blockIdx.x) * a.keep;
+  if (hk == 0 && tid == 0) a.new_lengths[b] = min(n, a.keep);
+  if (n <= a.keep) {
+    for (int i = tid; i < a.keep; i += kSelectThreads) kept[i] = i < n ? i : -1;
+    return;
+  }
+  const float* weights = a.weights + long(blockIdx.x) * a.cap;
+  const int32_t* positions = a.positions ? a.positions + long(blockIdx.x) * a.cap : nullptr;
+  int newest = n - 1;
+  if (positions) {
+    newest = positions[0];
+    for (int i = tid; i < n; i += kSelectThreads) newest = max(newest, positions[i]);
+    for (int m = 32; m >= 1; m >>= 1) newest = max(newest, lane_xor(newest, m));
+    if (lane == 0) scratch[wave] = newest;
+    __syncthreads();
+    for (int w = 0; w < kSelectWaves; ++w) newest = max(newest, scratch[w]);
+  }
+  const long since = long(newest) - a.recent;
+  const auto key_of = [&](int i) -> uint32_t {
+    return long(positions ? positions[i] : i) > since ? 0xffffffffu : weight_key(weights[i]);
+  };
+
+  uint32_t prefix = 0;
+  int need = a.keep;
+  for (int shift = 24; shift >= 0; shift -= 8) {
+    if (tid < 256) hist[tid] = 0;
+    __syncthreads();
+    for (int i = tid; i < n; i += kSelectThreads) {
+      const uint32_t key = key_of(i);
+      if (shift == 24 || key >> (shift + 8) == prefix >> (shift + 8)) atomicAdd(&hist[key >> shift & 255], 1);
+    }
+    __syncthreads();
+    if (tid < 256) {  // keys above this digit
+      int above = 0;
+      for (int d = tid + 1; d < 256; ++d) above += hist[d];
+      if (above < need && above + hist[tid] >= need) {
+        found[0] = uint32_t(tid);
+        found[1] = uint32_t(need - above);
+      }
+    }
+    __syncthreads();
+    prefix |= found[0] << shift;
+    need = int(found[1]);
+    __syncthreads();
+  }
+
+  // Words of 64 slots, one wave each: who is above the last key, who has it.
+  const int words = (n + 63) / 64;
+  uint64_t* stays = reinterpret_cast<uint64_t*>(dynamic);
+  int* before = reinterpret_cast<int*>(stays + words);
+  for (int w = wave; w < words; w += kSelectWaves) {
+    const int i = 64 * w + lane;
+    const bool equal = i < n && key_of(i) == prefix;
+    const int c = __builtin_popcountll(__ballot(equal));
+    if (lane == 0) before[w] = c;
+  }
+  __syncthreads();
+  const int per = (words + kSelectThreads - 1) / kSelectThreads;
+  const int first = min(tid * per, words), last = min(first + per, words);
+  const auto scan = [&]() {
+    int sum = 0, total;
+    for (int w = first; w < last; ++w) sum += before[w];
+    int run = block_exclusive(sum, scratch, &total);
+    for (int w = first; w < last; ++w) {
+      const int c = before[w];
+      before[w] = run;
+      run += c;
+    }
+    __syncthreads();
+  };
+  scan();
+  for (int w = wave; w < words; w += kSelectWaves) {
+    const int i = 64 * w + lane;
+    const uint32_t key = i < n ? key_of(i) : 0u;
+    const uint64_t equal = __ballot(i < n && key == prefix);
+    const int rank = before[w] + __builtin_popcountll(equal & ((1ull << lane) - 1));
+    const uint64_t bits = __ballot(i < n && (key > prefix || (key == prefix && rank < need)));
+    if (lane == 0) {
+      stays[w] = bits;
+      before[w] = __builtin_popcountll(bits);
+    }
+  }
+  __syncthreads();
+  scan();
+
+  const int edge = a.keep / 64;
+  const int below = before[edge] + __builtin_popcountll(stays[edge] & ((1ull << (a.keep % 64)) - 1));
+  for (int i = tid; i < n; i += kSelectThreads) {
+    const int w = i / 64;
+    const uint64_t bit = 1ull << (i % 64);
+    if (!(stays[w] & bit)) continue;
+    if (i < a.keep) {
+      kept[i] = i;
+      continue;
+    }
+    // The r-th that stays from keep on: into the r-th hole, in the last word with at most r holes before it.
+    const int r = before[w] + __builtin_popcountll(stays[w] & (bit - 1)) - below;
+    int lo = 0, hi = edge;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) / 2;
+      if (64 * mid - before[mid] <= r) lo = mid;
+      else hi = mid - 1;
+    }
+    uint64_t holes = ~stays[lo];
+    for (int skip = r - (64 * lo - before[lo]); skip > 0; --skip) holes &= holes - 1;
+    kept[64 * lo + __builtin_ctzll(holes)] = i;
+  }
+}
+
+// Slot i takes what slot kept[i] held where that lies at or above keep: what is read is
+// never written, so nothing has to wait. Blocks in y: k, v.
+struct CompactArgs {
+  void *k, *v;
+  float* weights;
+  int32_t* positions;
+  const int32_t* kept;
+  long ks[3], vs[3];
+  int kv_heads, cap, keep, row_pieces, elem_bytes, blocks;
+};
+__global__ __launch_bounds__(256) void compact_rows_kernel(const CompactArgs a) {
+  const int group = int(blockIdx.x) / a.blocks, part = int(blockIdx.x) - group * a.blocks;
+  const int b = group / a.kv_heads, hk = group - b * a.kv_heads;
+  unsigned char* rows = static_cast<unsigned char*>(blockIdx.y ? a.v : a.k);
+  const long* st = blockIdx.y ? a.vs : a.ks;
+  rows += (b * st[0] + hk * st[1]) * a.elem_bytes;
+  const int lanes = a.row_pieces, per = 256 / lanes;  // rows of a pass
+  const int piece = int(threadIdx.x) % lanes;
+  for (int i = part * per + int(threadIdx.x) / lanes; i < a.keep; i += a.blocks * per) {
+    const int from = a.kept[long(group) * a.keep + i];
+    if (from < a.keep || from >= a.cap) continue;
+    *reinterpret_cast<uint4*>(rows + i * st[2] * a.elem_bytes + 16 * piece) =
+        load16(rows + from * st[2] * a.elem_bytes + 16 * piece);
+  }
+}
+// Weights and positions by slot; the weights of slots from keep on are cleared once all have moved.
+__global__ __launch_bounds__(1024) void compact_values_kernel(const CompactArgs a) {
+  const long base = long(blockIdx.x) * a.cap;
+  for (int i = threadIdx.x; i < a.keep; i += 1024) {
+    const int from = a.kept[long(blockIdx.x) * a.keep + i];
+    if (from < a.keep || from >= a.cap) continue;
+    if (a.weights) a.weights[base + i] = a.weights[base + from];
+    if (a.positions) a.positions[base + i] = a.positions[base + from];
+  }
+  if (!a.weights) return;
+  __syncthreads();
+  for (int i = a.keep + int(threadIdx.x); i < a.cap; i += 1024) a.weights[base + i] = 0.f;
+}
+
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+int elem_size(int dtype) { return dtype == SFL_DTYPE_F32 ? 4 : dtype == SFL_DTYPE_BF16 || dtype == SFL_DTYPE_F16 ? 2 : 0; }
+
+// Cache rows that are moved in 16-byte pieces.
+int check_rows(const char* what, const void* k, const void* v, const long* strides, int batch, int kv_heads, int capacity,
+               int head_dim, int dtype) {
+  if (!k || !v || !strides) return set_error(SFL_ERR_INVALID, "%s: null pointer argument", what);
+  if (batch <= 0 || kv_heads <= 0 || capacity <= 0)
+    return set_error(SFL_ERR_INVALID, "%s: batch, heads and capacity must be positive", what);
+  if (long(batch) * kv_heads > (1L << 24)) return set_error(SFL_ERR_UNSUPPORTED, "%s: too many KV heads", what);
+  const int es = elem_size(dtype);
+  if (!es) return set_error(SFL_ERR_UNSUPPORTED, "%s: dtype must be F32, BF16 or F16", what);
+  if (head_dim != 16 && head_dim != 32 && head_dim != 64 && head_dim != 128)
+    return set_error(SFL_ERR_UNSUPPORTED, "%s: unsupported head dim %d", what, head_dim);
+  if (!aligned16(k) || !aligned16(v)) return set_error(SFL_ERR_INVALID, "%s: tensors must be 16-byte aligned", what);
+  for (int i = 0; i < 6; ++i)
+    if (strides[i] * es % 16) return set_error(SFL_ERR_INVALID, "%s: strides must be multiples of 16 bytes", what);
+  return SFL_OK;
+}
+
+}  // namespace
+}  // namespace sfl
+
+extern "C" int sfl_rotate(const void* q, const void* k, const void* v, const int32_t* positions, const float* cos,
+                          const float* sin, const void* q_gain, const void* k_gain, const int32_t* start,
+                          const int32_t* counts, void* q_out, void* k_out, void* v_out, const long* strides, int batch,
+                          int tokens, int q_heads, int kv_heads, int head_dim, int rotary_dim, int table, int slots,
+                          int half_layout, int gain_dtype, float eps, int dtype, void* stream) {
+  using namespace sfl;
+  const char* what = "rotate";
+  if (!q || !k || !positions || !cos || !sin || !q_out || !k_out || !strides || (v && !v_out))
+    return set_error(SFL_ERR_INVALID, "%s: null pointer argument", what);
+  if (batch <= 0 || tokens <= 0 || q_heads <= 0 || kv_heads <= 0 || table <= 0 || slots <= 0)
+    return set_error(SFL_ERR_INVALID, "%s: batch, tokens, heads, table and slots must be positive", what);
+  const int es = elem_size(dtype);
+  if (!es) return set_error(SFL_ERR_UNSUPPORTED, "%s: dtype must be F32, BF16 or F16", what);
+  if (head_dim != 16 && head_dim != 32 && head_dim != 64 && head_dim != 128)
+    return set_error(SFL_ERR_UNSUPPORTED, "%s: unsupported head dim %d", what, head_dim);
+  if (rotary_dim < 2 || rotary_dim > head_dim || rotary_dim % 2)
+    return set_error(SFL_ERR_INVALID, "%s: rotary dim must be even and in [2, head dim]", what);
+  if (gain_dtype != dtype && gain_dtype != SFL_DTYPE_F32)
+    return set_error(SFL_ERR_UNSUPPORTED, "%s: gains must have the dtype of q or F32", what);
+  if (!(eps >= 0.f) || !__builtin_isfinite(eps)) return set_error(SFL_ERR_INVALID, "%s: eps must be finite and not negative", what);
+  RotateArgs a{q, k, v, positions, cos, sin, q_gain, k_gain, start, counts, q_out, k_out, v_out};
+  for (int i = 0; i < 18; ++i) a.st[i / 3][i % 3] = strides[i];
+  a.batch = batch, a.tokens = tokens, a.q_heads = q_heads, a.kv_heads = kv_heads, a.half = rotary_dim / 2;
+  a.table = table, a.slots = slots, a.gain_f32 = gain_dtype == SFL_DTYPE_F32, a.eps = eps;
+  const int heads = q_heads + kv_heads * (v ? 2 : 1);
+  const long rows = long(batch) * tokens * heads;
+  if ((rows + 3) / 4 > 0x7fffffffL) return set_error(SFL_ERR_UNSUPPORTED, "%s: too many rows", what);
+  const auto run = [&](auto t) {
+    using T = decltype(t);
+    const dim3 grid(unsigned((rows + 3) / 4));
+    if (half_layout)
+      hipLaunchKernelGGL((rotate_any_kernel<T, true>), grid, dim3(256), 0, static_cast<hipStream_t>(stream), a, head_dim, rows, heads);
+    else
+      hipLaunchKernelGGL((rotate_any_kernel<T, false>), grid, dim3(256), 0, static_cast<hipStream_t>(stream), a, head_dim, rows, heads);
+    return check_launch(what);
+  };
+  if (dtype == SFL_DTYPE_F32) return run(float{});
+  return dtype == SFL_DTYPE_BF16 ? run(bf16_t{}) : run(f16_t{});
+}
+
+extern "C" int sfl_accept_path(void* k, void* v, float* weights, int32_t* positions, const int32_t* lengths,
+                               const int32_t* path, const int32_t* accepted, int32_t* new_lengths, const long* strides,
+                               int batch, int kv_heads, int capacity, int tokens, int head_dim, int dtype, void* stream) {
+  using namespace sfl;
+  const char* what = "accept_path";
+  if (int rc = check_rows(what, k, v, strides, batch, kv_heads, capacity, head_dim, dtype)) return rc;
+  if (!lengths || !path || !accepted || !new_lengths) return set_error(SFL_ERR_INVALID, "%s: null pointer argument", what);
+  if (tokens < 1 || tokens > kMaxPath)
+    return set_error(SFL_ERR_UNSUPPORTED, "%s: between 1 and %d drafted tokens", what, kMaxPath);
+  AcceptArgs a{k, v, weights, positions, lengths, path, accepted, new_lengths};
+  for (int i = 0; i < 3; ++i) a.ks[i] = strides[i], a.vs[i] = strides[3 + i];
+  a.kv_heads = kv_heads, a.cap = capacity, a.tokens = tokens, a.elem_bytes = elem_size(dtype);
+  a.row_pieces = head_dim * a.elem_bytes / 16;
+  hipLaunchKernelGGL(accept_kernel, dim3(unsigned(batch * kv_heads), 3), dim3(256), 0, static_cast<hipStream_t>(stream), a);
+  return check_launch(what);
+}
+
+extern "C" int sfl_select_slots(const float* weights, const int32_t* lengths, const int32_t* positions, int32_t* kept,
+                                int32_t* new_lengths, int batch, int kv_heads, int capacity, int keep, int recent,
+                                void* stream) {
+  using namespace sfl;
+  const char* what = "select_slots";
+  if (!weights || !lengths || !kept || !new_lengths) return set_error(SFL_ERR_INVALID, "%s: null pointer argument", what);
+  if (batch <= 0 || kv_heads <= 0 || capacity <= 0)
+    return set_error(SFL_ERR_INVALID, "%s: batch, heads and capacity must be positive", what);
+  if (capacity > SFL_SELECT_MAX_SLOTS)
+    return set_error(SFL_ERR_UNSUPPORTED, "%s: at most %d slots", what, SFL_SELECT_MAX_SLOTS);
+  if (keep < 1 || keep > capacity || recent < 0 || recent > keep)
+    return set_error(SFL_ERR_INVALID, "%s: keep must be in [1, capacity] and recent in [0, keep]", what);
+  if (long(batch) * kv_heads > (1L << 24)) return set_error(SFL_ERR_UNSUPPORTED, "%s: too many KV heads", what);
+  const SelectArgs a{weights, lengths, positions, kept, new_lengths, kv_heads, capacity, keep, recent};
+  const unsigned bytes = unsigned((capacity + 63) / 64) * 12u;
+  hipLaunchKernelGGL(select_kernel, dim3(unsigned(batch * kv_heads)), dim3(kSelectThreads), bytes, static_cast<hipStream_t>(stream), a);
+  return check_launch(what);
+}
+
+extern "C" int sfl_compact_slots(void* k, void* v, float* weights, int32_t* positions, const int32_t* kept,
+                                 const long* strides, int batch, int kv_heads, int capacity, int keep, int head_dim,
+                                 int dtype, void* stream) {
+  using namespace sfl;
+  const char* what = "compact_slots";
+  if (int rc = check_rows(what, k, v, strides, batch, kv_heads, capacity, head_dim, dtype)) return rc;
+  if (!kept) return set_error(SFL_ERR_INVALID, "%s: null pointer argument", what);
+  if (keep < 1 || keep > capacity) return set_error(SFL_ERR_INVALID, "%s: keep must be in [1, capacity]", what);
+  CompactArgs a{k, v, weights, positions, kept};
+  for (int i = 0; i < 3; ++i) a.ks[i] = strides[i], a.vs[i] = strides[3 + i];
+  a.kv_heads = kv_heads, a.cap = capacity, a.keep = keep, a.elem_bytes = elem_size(dtype);
+  a.row_pieces = head_dim * a.elem_bytes / 16;
+  const int per = 256 / a.row_pieces;
+  a.blocks = (keep + 4 * per - 1) / (4 * per);  // four passes of a workgroup
+  if (long(batch) * kv_heads * a.blocks > 0x7fffffffL) return set_error(SFL_ERR_UNSUPPORTED, "%s: too many workgroups", what);
+  hipLaunchKernelGGL(compact_rows_kernel, dim3(unsigned(batch * kv_heads * a.blocks), 2), dim3(256), 0,
+                     static_cast<hipStream_t>(stream), a);
+  if (int rc = check_launch(what)) return rc;
+  if (!weights && !positions) return SFL_OK;
+  hipLaunchKernelGGL(compact_values_kernel, dim3(unsigned(batch * kv_heads)), dim3(1024), 0, static_cast<hipStream_t>(stream), a);
+  return check_launch(what);
+}

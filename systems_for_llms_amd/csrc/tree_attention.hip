@@ -1,0 +1,644 @@
+// Attention of drafted tokens over a KV cache, and the attention weights by slot.
+//
+// A sequence has len committed keys in slots [0, len) of its cache and its count
+// drafted tokens' keys in slots [len, len + count). Draft t sees every committed
+// key and the drafts j with mask[t, j]:
+//
+//   s = scale q . k over the keys in sight,  o = sum exp(s - m) v / l,
+//   m = max s,  l = sum exp(s - m),  lse = m + log l        (one pass, m and l running)
+//   weights[slot] += sum over counted drafts and the group's heads of exp(s - lse)
+//
+// The G query heads that share a KV head, times the T drafts, are one block of
+// R = T G query rows (row r = t G + g) over the same keys, so a key is read once
+// for all of them and the products are matrix products: 16 rows to a tile.
+#include <type_traits>
+
+#include "attn_mfma.hpp"
+
+namespace sfl {
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kTreeWaves = 4;
+constexpr int kTreeTile = 32;  // keys of a wave's tile: two MFMA tiles of 16
+constexpr int kMaxDrafts = 128;
+constexpr float kLn2 = 0.6931471805599453f;
+
+struct TreeArgs {
+  const void *q, *k, *v;
+  const int32_t *lengths, *counts;
+  const uint8_t* mask;
+  float *pmax, *psum, *pout;
+  void* out;
+  float* lse;
+  long qs[3], ks[3], vs[3], os[3];  // strides in elements: batch, head, row
+  long ms[3];                       // mask: batch, draft, key draft
+  int kv_heads, cap, tokens, group_log2, splits, row_blocks, groups;
+  float cs;  // scale * log2(e): scores are kept in base 2
+};
+
+// What a sequence has: committed keys, drafts in use, keys in all (inside the cache).
+struct TreeRow {
+  int len, count, total;
+};
+__device__ __forceinline__ TreeRow tree_row(const int32_t* lengths, const int32_t* counts, int b, int cap, int tokens) {
+  TreeRow r;
+  r.len = min(max(lengths[b], 0), cap);
+  r.count = counts ? min(max(counts[b], 0), tokens) : tokens;
+  r.total = min(r.len + r.count, cap);
+  return r;
+}
+
+// Keys of one split: whole rounds of the workgroup's waves, so that a row's keys are
+// shared evenly among the splits whatever its length.
+__device__ __forceinline__ int split_chunk(int total, int splits) {
+  constexpr int kRound = kTreeTile * kTreeWaves;
+  return ((total + splits - 1) / splits + kRound - 1) / kRound * kRound;
+}
+
+__device__ __forceinline__ bool draft_sees(const TreeArgs& a, int b, const TreeRow& row, int t, int key) {
+  if (key < row.len) return true;
+  return key < row.total && a.mask[b * a.ms[0] + t * a.ms[1] + (key - row.len) * a.ms[2]] != 0;
+}
+
+// Operand registers of a wave's tile of 32 keys. MFMA tile h (0, 1) holds keys
+// 16 h .. 16 h + 15; lane = 16 g + n. Scores S^T = K Q^T come out with lane
+// (g, n) holding keys 16 h + 4 g + i (i < 4) of query row n, which is also how
+// O^T += V^T P^T takes P (k-slot (g, 4 h + i) of a 16-bit MFMA, k-slot g of the
+// fp32 MFMA (h, i)), so probabilities never leave their lane. For V^T, lane
+// (g, n) loads dims kVec n .. kVec n + kVec - 1 of its 8 keys: accumulator f
+// holds dims kVec m + f for m = 0..15, and the 16-bit pairs are put together
+// from two keys' words in registers.
+template <typename T, int D>
+struct TreeOps {
+  static constexpr bool kF32 = std::is_same<T, float>::value;
+  static constexpr int kVec = D / 16;                            // dims of V per lane and key
+  static constexpr int kSteps = kF32 ? D / 16 : (D + 31) / 32;   // 16-byte pieces of a K or Q row per lane
+  static constexpr int kWords = kF32 ? kVec : (kVec + 1) / 2;    // 32-bit words of V per lane and key
+
+  // One row's operand: step s, lane group g takes dims (fp32) 16 s + 4 g .. + 3 or
+  // (16-bit) 32 s + 8 g .. + 7; head dim 16 fills half of a 16-bit step.
+  static __device__ __forceinline__ void load_row(const T* row, int g, u32x4 (&r)[kSteps]) {
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      if constexpr (kF32) {
+        r[s] = *reinterpret_cast<const u32x4*>(row + 16 * s + 4 * g);
+      } else if constexpr (D == 16) {
+        r[s] = *reinterpret_cast<const u32x4*>(row + 8 * (g & 1));
+        if (g > 1) r[s] = u32x4{0u, 0u, 0u, 0u};
+      } else {
+        r[s] = *reinterpret_cast<const u32x4*>(row + 32 * s + 8 * g);
+      }
+    }
+  }
+
+  static __device__ __forceinline__ f32x4 dot(const u32x4& k, const u32x4& q, f32x4 c) {
+    if constexpr (kF32) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[e]), __uint_as_float(q[e]), c, 0, 0, 0);
+      return c;
+    } else if constexpr (std::is_same<T, bf16_t>::value) {
+      return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k), __builtin_bit_cast(bf16x8, q), c, 0, 0, 0);
+    } else {
+      return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, k), __builtin_bit_cast(f16x8, q), c, 0, 0, 0);
+    }
+  }
+
+  static __device__ __forceinline__ void load_v(const T* row, int n, uint32_t (&w)[kWords]) {
+    const T* p = row + kVec * n;
+    if constexpr (!kF32 && kVec == 1) {
+      w[0] = p->bits;
+    } else if constexpr (kWords == 1) {
+      w[0] = *reinterpret_cast<const uint32_t*>(p);
+    } else if constexpr (kWords == 2) {
+      const uint2 r = *reinterpret_cast<const uint2*>(p);
+      w[0] = r.x, w[1] = r.y;
+    } else {
+#pragma unroll
+      for (int j = 0; j < kWords / 4; ++j) {
+        const u32x4 r = reinterpret_cast<const u32x4*>(p)[j];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[4 * j + e] = r[e];
+      }
+    }
+  }
+
+  static __device__ __forceinline__ float v_value(const uint32_t (&w)[kWords], int f) {
+    if constexpr (kF32) return __uint_as_float(w[f]);
+    const uint32_t bits = (f & 1) ? w[f / 2] >> 16 : w[f / 2] & 0xffffu;
+    if constexpr (std::is_same<T, bf16_t>::value) return __uint_as_float(bits << 16);
+    return f16_bits_to_f32(uint16_t(bits));
+  }
+  static __device__ __forceinline__ void zero_value(uint32_t (&w)[kWords], int f) {
+    if constexpr (kF32) w[f] = 0u;
+    else w[f / 2] &= (f & 1) ? 0x0000ffffu : 0xffff0000u;
+  }
+
+  // acc[f] += V^T P^T for the tile; p[h][i] the lane's probabilities. 16-bit types round
+  // them to the type of V, half a step (2^-9 of bf16's own 2^-8 spacing at most) each and
+  // of either sign, as the products of the matrix cores ask; l sums them unrounded.
+  static __device__ __forceinline__ void add_pv(const uint32_t (&v)[8][kWords], const float (&p)[2][4], f32x4 (&acc)[kVec]) {
+    if constexpr (kF32) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int f = 0; f < kVec; ++f)
+          acc[f] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v[j][f]), p[j / 4][j % 4], acc[f], 0, 0, 0);
+    } else {
+      u32x4 pk;
+#pragma unroll
+      for (int a = 0; a < 4; ++a) pk[a] = pack2<T>(p[a / 2][2 * (a % 2)], p[a / 2][2 * (a % 2) + 1]);
+#pragma unroll
+      for (int f = 0; f < kVec; ++f) acc[f] = dot(v_operand(v, f), pk, acc[f]);
+    }
+  }
+  static __device__ __forceinline__ u32x4 v_operand(const uint32_t (&v)[8][kWords], int f) {
+    u32x4 r;
+#pragma unroll
+    for (int a = 0; a < 4; ++a)
+      r[a] = __builtin_amdgcn_perm(v[2 * a + 1][f / 2], v[2 * a][f / 2], (f & 1) ? 0x07060302u : 0x05040100u);
+    return r;
+  }
+};
+
+// A draft that does not see a key takes nothing from it, also where the key's
+// value is infinite or NaN, which a product with a probability of 0 would spread
+// over every row of the MFMA tile. Tiles with drafts in them take such values
+// out of the operand and add them here, row by row, to those that see the key.
+template <typename T, int D, int RT>
+__device__ __noinline__ void add_nonfinite(const uint32_t (&v)[8][TreeOps<T, D>::kWords], const float (&p)[RT][2][4],
+                                           uint32_t sees, f32x4 (&acc)[RT][TreeOps<T, D>::kVec]) {
+  using O = TreeOps<T, D>;
+  const int lane = threadIdx.x % kWave, g = lane / 16, n = lane % 16;
+  for (int j = 0; j < 8; ++j) {
+    for (int f = 0; f < O::kVec; ++f) {
+      const float mine = O::v_value(v[j], f);
+      const bool bad = !(fabsf(mine) < INFINITY);
+      if (!__ballot(bad)) continue;
+      for (int src = 0; src < 4; ++src) {  // the lane group that holds the key
+        for (int i = 0; i < 4; ++i) {
+          const float value = __shfl(mine, 16 * src + 4 * g + i);
+          const bool add = !(fabsf(value) < INFINITY);
+          for (int rt = 0; rt < RT; ++rt) {
+            const float pv = __shfl(p[rt][j / 4][j % 4], 16 * src + n);
+            const uint32_t seen = __shfl(int(sees), 16 * src + n);
+            if (add && (seen >> (8 * rt + j) & 1u)) acc[rt][f][i] += pv * value;
+          }
+        }
+      }
+    }
+  }
+}
+
+// Workgroup -> (KV head of a sequence, split, row block). Workgroups go to the 8
+// XCDs in turn; the row blocks that read the same keys take consecutive places
+// of one XCD, so that all but the first find them in its L2.
+struct TreeBlock {
+  int group, split, rb;
+};
+__device__ __forceinline__ TreeBlock tree_block(const TreeArgs& a) {
+  const int work = a.groups * a.splits;
+  const int x = int(blockIdx.x) % kXcds, y = int(blockIdx.x) / kXcds;
+  const int unit = (y / a.row_blocks) * kXcds + x;
+  TreeBlock t;
+  t.rb = y % a.row_blocks;
+  t.group = unit < work ? unit / a.splits : -1;
+  t.split = unit - t.group * a.splits;
+  return t;
+}
+
+template <typename T, int D, int RT>
+__global__ __launch_bounds__(kTreeWaves * kWave) void tree_attention_kernel(const TreeArgs a) {
+  using O = TreeOps<T, D>;
+  constexpr int W = kTreeWaves, BT = kTreeTile, VEC = O::kVec;
+  constexpr int kState = RT * (4 * VEC + 2);  // a lane's registers of a wave's state
+  static_assert(RT <= 4, "add_nonfinite's bits");
+  __shared__ float sm[2][kState][kWave];
+  const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave);
+  const int lane = threadIdx.x % kWave, g = lane / 16, n = lane % 16;
+  const TreeBlock blk = tree_block(a);
+  if (blk.group < 0) return;
+  const int b = blk.group / a.kv_heads, hk = blk.group - b * a.kv_heads;
+  const TreeRow row = tree_row(a.lengths, a.counts, b, a.cap, a.tokens);
+  const int G = 1 << a.group_log2, rows = a.tokens << a.group_log2;
+  const int row0 = blk.rb * 16 * RT;
+  const int chunk = split_chunk(row.total, a.splits);
+  const int begin = blk.split * chunk, end = min(row.total, begin + chunk);
+  const bool idle = row0 >= row.count << a.group_log2;  // drafts not in use, whose rows are zeros
+  if (a.splits > 1 && (begin >= end || idle)) return;   // the merge does not read these
+
+  u32x4 q[RT][O::kSteps];
+  int draft[RT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const int r = min(row0 + 16 * rt + n, rows - 1);  // rows past the last repeat it and are not stored
+    draft[rt] = r >> a.group_log2;
+    O::load_row(static_cast<const T*>(a.q) + b * a.qs[0] + long((hk << a.group_log2) + (r & (G - 1))) * a.qs[1] +
+                    draft[rt] * a.qs[2], g, q[rt]);
+  }
+  const T* kp = static_cast<const T*>(a.k) + b * a.ks[0] + hk * a.ks[1];
+  const T* vp = static_cast<const T*>(a.v) + b * a.vs[0] + hk * a.vs[1];
+
+  float m[RT], l[RT];
+  f32x4 acc[RT][VEC];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    m[rt] = -INFINITY;
+    l[rt] = 0.f;
+#pragma unroll
+    for (int f = 0; f < VEC; ++f) acc[rt][f] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  if (!idle) {
+    for (int t0 = begin + BT * wave; t0 < end; t0 += BT * W) {
+      // Keys past the last one of the row are its last one again: nothing outside is read.
+      u32x4 k[2][O::kSteps];
+      uint32_t v[8][O::kWords];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) O::load_row(kp + long(min(t0 + 16 * h + n, end - 1)) * a.ks[2], g, k[h]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        O::load_v(vp + long(min(t0 + 16 * (j / 4) + 4 * g + j % 4, end - 1)) * a.vs[2], n, v[j]);
+      const bool masked = t0 + BT > min(row.len, end);
+
+      float p[RT][2][4];
+      uint32_t sees = 0;
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        f32x4 s[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          s[h] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int st = 0; st < O::kSteps; ++st) s[h] = O::dot(k[h][st], q[rt][st], s[h]);
+        }
+        if (masked) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int key = t0 + 16 * (j / 4) + 4 * g + j % 4;
+            const bool ok = key < end && draft_sees(a, b, row, draft[rt], key);
+            s[j / 4][j % 4] = ok ? s[j / 4][j % 4] : -INFINITY;
+            sees |= uint32_t(ok) << (8 * rt + j);
+          }
+        }
+        float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                         fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+        mx = fmaxf(mx, lane_xor(mx, 16));
+        mx = fmaxf(mx, lane_xor(mx, 32));
+        // Lazy maximum: m moves only when the tile's is larger by kLazyMax, so that
+        // probabilities stay below 2^kLazyMax and the sums are rescaled seldom.
+        const bool grow = mx * a.cs > m[rt] + kLazyMax;
+        if (__ballot(grow)) {
+          const float mn = grow ? mx * a.cs : m[rt];
+          const float alpha = grow ? __builtin_amdgcn_exp2f(m[rt] - mn) : 1.f;
+          m[rt] = mn;
+          l[rt] *= alpha;
+#pragma unroll
+          for (int f = 0; f < VEC; ++f) acc[rt][f] *= alpha;
+        }
+        const float ms = m[rt] == -INFINITY ? 0.f : m[rt];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            p[rt][h][i] = __builtin_amdgcn_exp2f(fmaf(s[h][i], a.cs, -ms));
+            l[rt] += p[rt][h][i];
+          }
+      }
+      if (masked) {
+        bool bad = false;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+          for (int f = 0; f < VEC; ++f) bad |= !(fabsf(O::v_value(v[j], f)) < INFINITY);
+        if (__ballot(bad)) {
+          // Copies, so that the call leaves the state itself in registers.
+          uint32_t vt[8][O::kWords];
+          float pt[RT][2][4];
+          f32x4 at[RT][VEC];
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int w = 0; w < O::kWords; ++w) vt[j][w] = v[j][w];
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) pt[rt][j / 4][j % 4] = p[rt][j / 4][j % 4];
+#pragma unroll
+            for (int f = 0; f < VEC; ++f) at[rt][f] = acc[rt][f];
+          }
+          add_nonfinite<T, D, RT>(vt, pt, sees, at);
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+            for (int f = 0; f < VEC; ++f) acc[rt][f] = at[rt][f];
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int f = 0; f < VEC; ++f)
+              if (!(fabsf(O::v_value(v[j], f)) < INFINITY)) O::zero_value(v[j], f);
+        }
+      }
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) O::add_pv(v, p[rt], acc[rt]);
+    }
+  }
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    l[rt] += lane_xor(l[rt], 16);
+    l[rt] += lane_xor(l[rt], 32);
+  }
+
+  // Merge the waves' states in two rounds: the upper half of the waves hand theirs over.
+#pragma unroll
+  for (int half = W / 2; half >= 1; half /= 2) {
+    if (wave >= half && wave < 2 * half) {
+      float(*to)[kWave] = sm[wave - half];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        to[rt][lane] = m[rt];
+        to[RT + rt][lane] = l[rt];
+#pragma unroll
+        for (int f = 0; f < VEC; ++f)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) to[2 * RT + (rt * VEC + f) * 4 + i][lane] = acc[rt][f][i];
+      }
+    }
+    __syncthreads();
+    if (wave < half) {
+      float(*from)[kWave] = sm[wave];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        const float mo = from[rt][lane], top = fmaxf(m[rt], mo);
+        const float ca = m[rt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[rt] - top);
+        const float cb = mo == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mo - top);
+        m[rt] = top;
+        l[rt] = ca * l[rt] + cb * from[RT + rt][lane];
+#pragma unroll
+        for (int f = 0; f < VEC; ++f)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            acc[rt][f][i] = ca * acc[rt][f][i] + cb * from[2 * RT + (rt * VEC + f) * 4 + i][lane];
+      }
+    }
+    __syncthreads();
+  }
+  if (wave) return;
+
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const int r = row0 + 16 * rt + n;
+    if (r >= rows) continue;
+    if (a.splits > 1) {
+      const long part = (long(blk.group) * a.splits + blk.split) * rows + r;
+      if (g == 0) {
+        a.pmax[part] = m[rt];
+        a.psum[part] = l[rt];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int f = 0; f < VEC; ++f) a.pout[part * D + VEC * (4 * g + i) + f] = acc[rt][f][i];
+      continue;
+    }
+    const int t = r >> a.group_log2, head = (hk << a.group_log2) + (r & (G - 1));
+    const bool empty = t >= row.count || l[rt] == 0.f;
+    const float inv = empty ? 0.f : 1.f / l[rt];
+    T* o = static_cast<T*>(a.out) + b * a.os[0] + head * a.os[1] + t * a.os[2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int f = 0; f < VEC; ++f) store_scalar<T>(o + VEC * (4 * g + i) + f, empty ? 0.f : acc[rt][f][i] * inv);
+    if (g == 0)
+      a.lse[(long(b) * a.kv_heads * G + head) * a.tokens + t] = empty ? -INFINITY : (m[rt] + __builtin_log2f(l[rt])) * kLn2;
+  }
+}
+
+// One wave per query row: the splits' states in one, then the output and lse.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void tree_merge_kernel(const TreeArgs a) {
+  constexpr int DPL = (D + kWave - 1) / kWave;
+  const int lane = threadIdx.x % kWave;
+  const int rows = a.tokens << a.group_log2, G = 1 << a.group_log2;
+  const long at = long(blockIdx.x) * 4 + threadIdx.x / kWave;
+  if (at >= long(a.groups) * rows) return;
+  const int group = int(at / rows), r = int(at - long(group) * rows);
+  const int b = group / a.kv_heads, hk = group - b * a.kv_heads;
+  const TreeRow row = tree_row(a.lengths, a.counts, b, a.cap, a.tokens);
+  const int t = r >> a.group_log2, head = (hk << a.group_log2) + (r & (G - 1));
+  float top = -INFINITY, den = 0.f, num[DPL] = {};
+  if (t < row.count && row.total > 0) {
+    const int chunk = split_chunk(row.total, a.splits);
+    const int n = (row.total + chunk - 1) / chunk;
+    for (int s = 0; s < n; ++s) {
+      const long part = (long(group) * a.splits + s) * rows + r;
+      const float ms = a.pmax[part], mn = fmaxf(top, ms);
+      const float ca = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - mn);
+      const float cb = ms == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ms - mn);
+      den = ca * den + cb * a.psum[part];
+#pragma unroll
+      for (int i = 0; i < DPL; ++i)
+        num[i] = ca * num[i] + cb * a.pout[part * D + min(lane + i * kWave, D - 1)];
+      top = mn;
+    }
+  }
+  const bool empty = den == 0.f;
+  T* o = static_cast<T*>(a.out) + b * a.os[0] + head * a.os[1] + t * a.os[2];
+#pragma unroll
+  for (int i = 0; i < DPL; ++i)
+    if (lane + i * kWave < D) store_scalar<T>(o + lane + i * kWave, empty ? 0.f : num[i] / den);
+  if (lane == 0)
+    a.lse[(long(b) * a.kv_heads * G + head) * a.tokens + t] = empty ? -INFINITY : (top + __builtin_log2f(den)) * kLn2;
+}
+
+// weights[b, hk, slot] += sum over the counted drafts and the group's heads of
+// exp(s - lse). A wave keeps the K operands of its keys and walks the counted
+// rows, 16 at a time, scores as above; every slot has one writer.
+template <typename T, int D>
+__global__ __launch_bounds__(kTreeWaves * kWave) void tree_weights_kernel(const TreeArgs a, const uint8_t* __restrict__ counted,
+                                                                          float* __restrict__ weights) {
+  using O = TreeOps<T, D>;
+  constexpr int BT = kTreeTile, W = kTreeWaves;
+  __shared__ short list[kMaxDrafts];
+  const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave);
+  const int lane = threadIdx.x % kWave, g = lane / 16, n = lane % 16;
+  const int group = int(blockIdx.x) / a.splits, part = int(blockIdx.x) - group * a.splits;
+  const int b = group / a.kv_heads, hk = group - b * a.kv_heads;
+  const TreeRow row = tree_row(a.lengths, a.counts, b, a.cap, a.tokens);
+  const int G = 1 << a.group_log2;
+  if (part * BT * W >= row.total) return;
+
+  // The counted drafts, in order.
+  int drafts = 0;
+#pragma unroll
+  for (int w = 0; w < kMaxDrafts / kWave; ++w) {
+    const int t = kWave * w + lane;
+    const bool on = t < row.count && (!counted || counted[long(b) * a.tokens + t]);
+    const uint64_t bits = __ballot(on);
+    if (on && wave == 0) list[drafts + __builtin_popcountll(bits & ((1ull << lane) - 1))] = short(t);
+    drafts += __builtin_popcountll(bits);
+  }
+  __syncthreads();
+
+  const T* kp = static_cast<const T*>(a.k) + b * a.ks[0] + hk * a.ks[1];
+  const int rows = drafts << a.group_log2;
+  const int t0 = (part * W + wave) * BT;
+  if (t0 >= row.total) return;
+  u32x4 k[2][O::kSteps];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) O::load_row(kp + long(min(t0 + 16 * h + n, row.total - 1)) * a.ks[2], g, k[h]);
+  const bool masked = t0 + BT > row.len;
+  float sum[8] = {};
+  for (int r0 = 0; r0 < rows; r0 += 16) {
+    const int r = min(r0 + n, rows - 1);
+    const int t = list[r >> a.group_log2], head = (hk << a.group_log2) + (r & (G - 1));
+    u32x4 q[O::kSteps];
+    O::load_row(static_cast<const T*>(a.q) + b * a.qs[0] + head * a.qs[1] + t * a.qs[2], g, q);
+    const float lse = a.lse[(long(b) * a.kv_heads * G + head) * a.tokens + t];
+    // Rows past the last and rows that see nothing add exp2(-inf) = 0.
+    const float base = r0 + n < rows && lse != -INFINITY ? lse * kLog2e : INFINITY;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      f32x4 s = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int st = 0; st < O::kSteps; ++st) s = O::dot(k[h][st], q[st], s);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float p = __builtin_amdgcn_exp2f(fmaf(s[i], a.cs, -base));
+        if (base == INFINITY) p = 0.f;
+        if (masked && !draft_sees(a, b, row, t, t0 + 16 * h + 4 * g + i)) p = 0.f;
+        sum[4 * h + i] += p;
+      }
+    }
+  }
+  float* to = weights + (long(b) * a.kv_heads + hk) * a.cap;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float total = group_sum<16>(sum[j]);
+    const int key = t0 + 16 * (j / 4) + 4 * g + j % 4;
+    if (n == 0 && key < row.total) to[key] += total;
+  }
+}
+
+template <typename T, int D, int RT>
+int launch_rows(TreeArgs& a, hipStream_t stream) {
+  const int rows = a.tokens << a.group_log2;
+  a.row_blocks = (rows + 16 * RT - 1) / (16 * RT);
+  const long units = (long(a.groups) * a.splits + kXcds - 1) / kXcds * kXcds;
+  if (units * a.row_blocks > 0x7fffffffL) return set_error(SFL_ERR_UNSUPPORTED, "tree_attention: too many workgroups");
+  hipLaunchKernelGGL((tree_attention_kernel<T, D, RT>), dim3(unsigned(units * a.row_blocks)), dim3(kTreeWaves * kWave), 0, stream, a);
+  if (int rc = check_launch("tree_attention")) return rc;
+  if (a.splits == 1) return SFL_OK;
+  const long merged = long(a.groups) * rows;
+  hipLaunchKernelGGL((tree_merge_kernel<T, D>), dim3(unsigned((merged + 3) / 4)), dim3(256), 0, stream, a);
+  return check_launch("tree_attention");
+}
+
+template <typename T, int D>
+int launch_tree(TreeArgs& a, hipStream_t stream) {
+  const int rows = a.tokens << a.group_log2;
+  if (rows <= 16) return launch_rows<T, D, 1>(a, stream);
+  if (rows <= 32 || std::is_same<T, float>::value) return launch_rows<T, D, 2>(a, stream);
+  return launch_rows<T, D, std::is_same<T, float>::value ? 2 : 4>(a, stream);
+}
+
+template <typename T, int D>
+int launch_weights(TreeArgs& a, const uint8_t* counted, float* weights, hipStream_t stream) {
+  a.splits = (a.cap + kTreeTile * kTreeWaves - 1) / (kTreeTile * kTreeWaves);
+  if (long(a.groups) * a.splits > 0x7fffffffL) return set_error(SFL_ERR_UNSUPPORTED, "tree_weights: too many workgroups");
+  hipLaunchKernelGGL((tree_weights_kernel<T, D>), dim3(unsigned(a.groups * a.splits)), dim3(kTreeWaves * kWave), 0,
+                     stream, a, counted, weights);
+  return check_launch("tree_weights");
+}
+
+template <typename T, typename F>
+int tree_dims(int dim, F&& f) {
+  switch (dim) {
+    case 16: return f(T{}, std::integral_constant<int, 16>{});
+    case 32: return f(T{}, std::integral_constant<int, 32>{});
+    case 64: return f(T{}, std::integral_constant<int, 64>{});
+    default: return f(T{}, std::integral_constant<int, 128>{});
+  }
+}
+template <typename F>
+int tree_types(int dtype, int dim, F&& f) {
+  switch (dtype) {
+    case SFL_DTYPE_F32: return tree_dims<float>(dim, f);
+    case SFL_DTYPE_BF16: return tree_dims<bf16_t>(dim, f);
+    default: return tree_dims<f16_t>(dim, f);
+  }
+}
+
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+// What both entry points check, and the arguments they share.
+int fill(TreeArgs& a, const char* what, const void* q, const void* k, const int32_t* lengths, const uint8_t* mask,
+         const int32_t* counts, float* lse, const long* strides, int batch, int q_heads, int kv_heads, int capacity,
+         int tokens, int head_dim, float scale, int dtype) {
+  if (!q || !k || !lengths || !mask || !lse || !strides) return set_error(SFL_ERR_INVALID, "%s: null pointer argument", what);
+  if (batch <= 0 || q_heads <= 0 || kv_heads <= 0 || capacity <= 0 || tokens <= 0)
+    return set_error(SFL_ERR_INVALID, "%s: batch, heads, capacity and tokens must be positive", what);
+  if (tokens > kMaxDrafts) return set_error(SFL_ERR_UNSUPPORTED, "%s: at most %d drafted tokens", what, kMaxDrafts);
+  if (q_heads % kv_heads) return set_error(SFL_ERR_INVALID, "%s: query heads must be divisible by KV heads", what);
+  const int group = q_heads / kv_heads;
+  if (group != 1 && group != 2 && group != 4 && group != 8)
+    return set_error(SFL_ERR_UNSUPPORTED, "%s: unsupported GQA ratio %d", what, group);
+  if (head_dim != 16 && head_dim != 32 && head_dim != 64 && head_dim != 128)
+    return set_error(SFL_ERR_UNSUPPORTED, "%s: unsupported head dim %d", what, head_dim);
+  if (dtype != SFL_DTYPE_F32 && dtype != SFL_DTYPE_BF16 && dtype != SFL_DTYPE_F16)
+    return set_error(SFL_ERR_UNSUPPORTED, "%s: dtype must be F32, BF16 or F16", what);
+  if (!(scale > 0.f) || !__builtin_isfinite(scale)) return set_error(SFL_ERR_INVALID, "%s: scale must be finite and positive", what);
+  if (long(batch) * kv_heads > (1L << 24)) return set_error(SFL_ERR_UNSUPPORTED, "%s: too many KV heads", what);
+  const int piece = dtype == SFL_DTYPE_F32 ? 4 : 8;
+  if (!aligned16(q) || !aligned16(k)) return set_error(SFL_ERR_INVALID, "%s: tensors must be 16-byte aligned", what);
+  for (int i = 0; i < 12; ++i)
+    if (strides[i] % piece) return set_error(SFL_ERR_INVALID, "%s: strides must be multiples of 16 bytes", what);
+  a.q = q, a.k = k, a.lengths = lengths, a.mask = mask, a.counts = counts, a.lse = lse;
+  for (int i = 0; i < 3; ++i)
+    a.qs[i] = strides[i], a.ks[i] = strides[3 + i], a.vs[i] = strides[6 + i], a.os[i] = strides[9 + i], a.ms[i] = strides[12 + i];
+  a.kv_heads = kv_heads, a.cap = capacity, a.tokens = tokens, a.groups = batch * kv_heads;
+  a.group_log2 = group == 8 ? 3 : group / 2;
+  a.cs = scale * kLog2e;
+  return SFL_OK;
+}
+
+}  // namespace
+}  // namespace sfl
+
+extern "C" int sfl_tree_attention(const void* q, const void* k, const void* v, const int32_t* lengths,
+                                  const uint8_t* mask, const int32_t* counts, float* partial_max, float* partial_sum,
+                                  float* partial_out, void* out, float* lse, const long* strides, int batch,
+                                  int q_heads, int kv_heads, int capacity, int tokens, int head_dim, int splits,
+                                  float scale, int dtype, void* stream) {
+  using namespace sfl;
+  const char* what = "tree_attention";
+  TreeArgs a{};
+  if (int rc = fill(a, what, q, k, lengths, mask, counts, lse, strides, batch, q_heads, kv_heads, capacity, tokens,
+                    head_dim, scale, dtype))
+    return rc;
+  if (!v || !out) return set_error(SFL_ERR_INVALID, "%s: null pointer argument", what);
+  if (splits < 1 || splits > 1024) return set_error(SFL_ERR_INVALID, "%s: splits must be in [1, 1024]", what);
+  if (splits > 1 && (!partial_max || !partial_sum || !partial_out))
+    return set_error(SFL_ERR_INVALID, "%s: null pointer argument", what);
+  if (!aligned16(v) || !aligned16(out)) return set_error(SFL_ERR_INVALID, "%s: tensors must be 16-byte aligned", what);
+  a.v = v, a.out = out, a.pmax = partial_max, a.psum = partial_sum, a.pout = partial_out, a.splits = splits;
+  return tree_types(dtype, head_dim, [&](auto t, auto d) {
+    return launch_tree<decltype(t), decltype(d)::value>(a, static_cast<hipStream_t>(stream));
+  });
+}
+
+extern "C" int sfl_tree_weights(const void* q, const void* k, const float* lse, float* weights, const int32_t* lengths,
+                                const uint8_t* mask, const int32_t* counts, const uint8_t* rows, const long* strides,
+                                int batch, int q_heads, int kv_heads, int capacity, int tokens, int head_dim,
+                                float scale, int dtype, void* stream) {
+  using namespace sfl;
+  TreeArgs a{};
+  if (int rc = fill(a, "tree_weights", q, k, lengths, mask, counts, const_cast<float*>(lse), strides, batch, q_heads,
+                    kv_heads, capacity, tokens, head_dim, scale, dtype))
+    return rc;
+  if (!weights) return set_error(SFL_ERR_INVALID, "tree_weights: null pointer argument");
+  return tree_types(dtype, head_dim, [&](auto t, auto d) {
+    return launch_weights<decltype(t), decltype(d)::value>(a, rows, weights, static_cast<hipStream_t>(stream));
+  });
+}

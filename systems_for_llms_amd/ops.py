@@ -117,8 +117,107 @@ def _masked_attention_fake(q, k, v, out, lse, scale, causal, window_left, window
     return None
 
 
+def _all_strides(*tensors: torch.Tensor | None):
+    """Batch, head and row strides of each tensor in one array (zeros for an absent one)."""
+    return (ctypes.c_long * (3 * len(tensors)))(
+        *[s for t in tensors for s in ((0, 0, 0) if t is None else t.stride()[:3])])
+
+
+def _call(device: torch.device, name: str, *args) -> None:
+    """The entry point on ``device``'s current stream, with that device current."""
+    stream = _lib.stream_handle(device)
+    if device.index == torch.cuda.current_device():
+        _lib.call(name, *args, stream)
+        return
+    with torch.cuda.device(device):
+        _lib.call(name, *args, stream)
+
+
+def launch_rotate(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor | None, positions: torch.Tensor,
+                  cos: torch.Tensor, sin: torch.Tensor, q_norm: torch.Tensor | None, k_norm: torch.Tensor | None,
+                  start: torch.Tensor | None, counts: torch.Tensor | None, q_out: torch.Tensor, k_out: torch.Tensor,
+                  v_out: torch.Tensor | None, half_layout: bool, eps: float) -> None:
+    """Norm and rotation of q and k rows; k and v into a cache where ``start`` says so (``sfl_rotate``)."""
+    batch, heads, tokens, dim = q.shape
+    gain = q.dtype if q_norm is None and k_norm is None else (k_norm if q_norm is None else q_norm).dtype
+    _call(q.device, "sfl_rotate", q.data_ptr(), k.data_ptr(), _ptr(v), positions.data_ptr(), cos.data_ptr(),
+          sin.data_ptr(), _ptr(q_norm), _ptr(k_norm), _ptr(start), _ptr(counts), q_out.data_ptr(), k_out.data_ptr(),
+          _ptr(v_out), _all_strides(q, k, v, q_out, k_out, v_out), batch, tokens, heads, k.shape[1], dim,
+          2 * cos.shape[1], cos.shape[0], k_out.shape[2], int(half_layout), _lib.dtype_code(gain), eps,
+          _lib.dtype_code(q.dtype))
+
+
+def launch_tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: torch.Tensor,
+                          mask: torch.Tensor, counts: torch.Tensor | None, partial_max: torch.Tensor,
+                          partial_sum: torch.Tensor, partial_output: torch.Tensor, out: torch.Tensor,
+                          lse: torch.Tensor, splits: int, scale: float) -> None:
+    """Attention of drafted tokens over a cache into ``out`` and ``lse`` (``sfl_tree_attention``).
+
+    ``mask`` is [B, T, T] (an expanded [T, T] has a batch stride of 0).
+    """
+    batch, heads, tokens, dim = q.shape
+    _call(q.device, "sfl_tree_attention", q.data_ptr(), k.data_ptr(), v.data_ptr(), lengths.data_ptr(),
+          mask.data_ptr(), _ptr(counts), partial_max.data_ptr(), partial_sum.data_ptr(), partial_output.data_ptr(),
+          out.data_ptr(), lse.data_ptr(), _all_strides(q, k, v, out, mask), batch, heads, k.shape[1], k.shape[2],
+          tokens, dim, splits, scale, _lib.dtype_code(q.dtype))
+
+
+def launch_tree_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, lengths: torch.Tensor,
+                        mask: torch.Tensor, counts: torch.Tensor | None, rows: torch.Tensor | None,
+                        weights: torch.Tensor, scale: float) -> None:
+    """Attention weights of the counted drafts added to ``weights`` by slot (``sfl_tree_weights``)."""
+    batch, heads, tokens, dim = q.shape
+    _call(q.device, "sfl_tree_weights", q.data_ptr(), k.data_ptr(), lse.data_ptr(), weights.data_ptr(),
+          lengths.data_ptr(), mask.data_ptr(), _ptr(counts), _ptr(rows), _all_strides(q, k, None, None, mask), batch,
+          heads, k.shape[1], k.shape[2], tokens, dim, scale, _lib.dtype_code(q.dtype))
+
+
+def launch_accept_path(lengths: torch.Tensor, path: torch.Tensor, accepted: torch.Tensor, k: torch.Tensor,
+                       v: torch.Tensor, weights: torch.Tensor | None, positions: torch.Tensor | None,
+                       new_lengths: torch.Tensor) -> None:
+    """The accepted path's rows moved behind the committed ones (``sfl_accept_path``)."""
+    batch, heads, capacity, dim = k.shape
+    _call(k.device, "sfl_accept_path", k.data_ptr(), v.data_ptr(), _ptr(weights), _ptr(positions),
+          lengths.data_ptr(), path.data_ptr(), accepted.data_ptr(), new_lengths.data_ptr(), _all_strides(k, v), batch,
+          heads, capacity, path.shape[1], dim, _lib.dtype_code(k.dtype))
+
+
+def launch_select_slots(weights: torch.Tensor, lengths: torch.Tensor, positions: torch.Tensor | None,
+                        kept: torch.Tensor, new_lengths: torch.Tensor, recent: int) -> None:
+    """The slots that stay, into ``kept`` (``sfl_select_slots``)."""
+    batch, heads, capacity = weights.shape
+    _call(weights.device, "sfl_select_slots", weights.data_ptr(), lengths.data_ptr(), _ptr(positions),
+          kept.data_ptr(), new_lengths.data_ptr(), batch, heads, capacity, kept.shape[2], recent)
+
+
+def launch_compact_slots(kept: torch.Tensor, k: torch.Tensor, v: torch.Tensor, weights: torch.Tensor | None,
+                         positions: torch.Tensor | None) -> None:
+    """Kept rows moved into the free places below them (``sfl_compact_slots``)."""
+    batch, heads, capacity, dim = k.shape
+    _call(k.device, "sfl_compact_slots", k.data_ptr(), v.data_ptr(), _ptr(weights), _ptr(positions), kept.data_ptr(),
+          _all_strides(k, v), batch, heads, capacity, kept.shape[2], dim, _lib.dtype_code(k.dtype))
+
+
+def _nothing(*args):
+    return None
+
+
+_CACHE_OPS = {
+    "rotate": (launch_rotate, ("q_out", "k_out", "v_out")),
+    "tree_attention": (launch_tree_attention, ("partial_max", "partial_sum", "partial_output", "out", "lse")),
+    "tree_weights": (launch_tree_weights, ("weights",)),
+    "accept_path": (launch_accept_path, ("k", "v", "weights", "positions", "new_lengths")),
+    "select_slots": (launch_select_slots, ("kept", "new_lengths")),
+    "compact_slots": (launch_compact_slots, ("k", "v", "weights", "positions")),
+}
+for _name, (_launch, _written) in _CACHE_OPS.items():
+    torch.library.custom_op(f"sfl::{_name}", mutates_args=_written)(_launch).register_fake(_nothing)
+
+
 # The same launches as kernels of the GPU's dispatch key: the wrapper a custom op
 # puts around its function for every device is another 3.6 us of a call.
 _gpu_kernels = torch.library.Library("sfl", "FRAGMENT")
 _gpu_kernels.impl("decode_attention", launch_decode_attention, "CUDA")
 _gpu_kernels.impl("masked_attention", launch_masked_attention, "CUDA")
+for _name, (_launch, _) in _CACHE_OPS.items():
+    _gpu_kernels.impl(_name, _launch, "CUDA")

@@ -1,0 +1,711 @@
+"""GPU parity of the KV-cache operators with their float64 forms (``oracle/cache.py``).
+
+Error bounds count what the kernels do: a stored result is rounded once, by half a
+step (``finfo.eps / 2`` of the value); probabilities are rounded to 16 bits before the
+products with V (half a step each of p |v|); scores are fp32 sums of D products, off by
+at most (D + 8) 2^-24 of sum |q k| and a few roundings of the scaled value, which enter
+exp as a relative error; sums over n keys are off by at most n 2^-24 of sum |terms|.
+"""
+
+import pytest
+import torch
+
+from oracle import cache as oc
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
+TINY = {BF16: 1e-38, FP16: 2.0 ** -25, FP32: 1e-38}  # half a step of the smallest numbers
+
+
+def half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def randn(g, *shape, dtype=FP32, scale=1.0):
+    return (torch.randn(shape, generator=g) * scale).to(dtype)
+
+
+def within(got, want, bound, what=""):
+    got, want = got.double().cpu(), want.double()
+    assert got.shape == want.shape, what
+    same = (got == want) | (got.isnan() & want.isnan())
+    off = torch.where(same, 0.0, (got - want).abs())
+    assert not bool((off.isnan() | (off > bound)).any()), f"{what}: {(off / bound).nan_to_num(9e9).max()} of the bound"
+
+
+# ---- rotation ---------------------------------------------------------------------
+
+
+def rotate_bound(dtype, want, size):
+    # The norm: a sum of up to 128 squares, a root, a division, two products; the turn: three roundings.
+    return half_step(dtype) * want.abs() + 40 * U * size + TINY[dtype]
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("dim, rotary", [(128, 128), (128, 64), (128, 48), (128, 6), (64, 64), (64, 16), (32, 32),
+                                         (32, 20), (16, 16), (16, 2)])
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_rotate_and_append(dtype, dim, rotary, layout):
+    from systems_for_llms_amd import rotary as rt
+
+    g = torch.Generator().manual_seed(dim * 1000 + rotary)
+    for batch, heads, kv_heads, tokens, gains in ((1, 1, 1, 1, None), (3, 6, 2, 5, dtype), (2, 4, 4, 3, FP32)):
+        cos, sin = rt.rotary_tables(rotary, 70000)
+        qkv = randn(g, batch, tokens, heads + 2 * kv_heads, dim, dtype=dtype).transpose(1, 2)
+        q, k, v = qkv.split([heads, kv_heads, kv_heads], 1)
+        positions = torch.randint(0, 70000, (batch, tokens), generator=g, dtype=torch.int32)
+        lengths = torch.randint(0, 4, (batch,), generator=g, dtype=torch.int32)
+        counts = torch.tensor([tokens, 0, 2][:batch], dtype=torch.int32) if batch == 3 else None
+        gq, gk = (None, None) if gains is None else (1 + randn(g, dim, scale=0.3).to(gains), randn(g, dim).to(gains))
+        cache = randn(g, 2, batch, kv_heads, 4 + tokens, dim, dtype=dtype)
+        gpu = [None if x is None else x.cuda() for x in (positions, cos, sin, lengths, counts, gq, gk)]
+        moved = qkv.transpose(1, 2).contiguous().cuda().transpose(1, 2).split([heads, kv_heads, kv_heads], 1)
+        kc, vc = cache.cuda()
+        q_out = rt.rotate_append(*moved, *gpu[:3], kc, vc, gpu[3], counts=gpu[4], layout=layout, q_norm=gpu[5],
+                                 k_norm=gpu[6], eps=1e-5)
+        only = rt.rotate(*moved[:2], *gpu[:3], counts=gpu[4], layout=layout, q_norm=gpu[5], k_norm=gpu[6])
+        wq, sq = oc.rotate(q, positions, cos, sin, layout, gq)
+        wk, sk = oc.rotate(k, positions, cos, sin, layout, gk)
+        want_k, want_v, bound_k = cache[0].double(), cache[1].double(), torch.zeros(cache[0].shape, dtype=torch.float64)
+        bk = rotate_bound(dtype, wk, sk)
+        for b in range(batch):
+            used, n = tokens if counts is None else int(counts[b]), int(lengths[b])
+            wq[b, :, used:] = 0
+            want_k[b, :, n:n + used], want_v[b, :, n:n + used] = wk[b, :, :used], v[b, :, :used].double()
+            bound_k[b, :, n:n + used] = bk[b, :, :used]
+            wk[b, :, used:] = 0
+        within(q_out, wq, rotate_bound(dtype, wq, sq), "q")
+        within(kc, want_k, bound_k, "k cache")
+        within(vc, want_v, 0.0, "v cache")
+        within(only[0], wq, rotate_bound(dtype, wq, sq), "rotate q")
+        within(only[1], wk, bk, "rotate k")
+
+
+def test_rotate_is_the_models_rotation():
+    """Interleaved pairs over the whole head with the model's tables."""
+    from systems_for_llms_amd import rotary as rt
+    from systems_for_llms_amd.model import rope_tables
+
+    g = torch.Generator().manual_seed(5)
+    q, k = randn(g, 2, 3, 9, 64), randn(g, 2, 3, 9, 64)
+    cos, sin = rope_tables(10000.0, 64, 9)
+    positions = torch.arange(9, dtype=torch.int32).expand(2, 9).contiguous()
+    got, _ = rt.rotate(q.cuda(), k.cuda(), positions.cuda(), cos.cuda(), sin.cuda())
+    want, size = oc.rotate(q, positions, cos, sin, "interleaved")
+    within(got, want, rotate_bound(FP32, want, size))
+
+
+def test_rotate_positions_and_slots_out_of_range():
+    """A position outside the tables gives NaN where the head turns; a slot outside the cache is left out."""
+    from systems_for_llms_amd import rotary as rt
+
+    g = torch.Generator().manual_seed(6)
+    cos, sin = rt.rotary_tables(16, 8)
+    positions = torch.tensor([[7, 8, -1]], dtype=torch.int32)
+    q, k, v = (randn(g, 1, 2, 3, 32) for _ in range(3))
+    cache = torch.ones(2, 1, 2, 5, 32).cuda()
+    for layout in ("half", "interleaved"):
+        kc, vc = cache.clone()
+        out = rt.rotate_append(q.cuda(), k.cuda(), v.cuda(), positions.cuda(), cos.cuda(), sin.cuda(), kc, vc,
+                               torch.tensor([3], dtype=torch.int32).cuda(), layout=layout).cpu()
+        assert out[:, :, 0].isfinite().all() and out[:, :, 1:, :16].isnan().all()
+        assert torch.equal(out[:, :, 1:, 16:], q[:, :, 1:, 16:])
+        assert torch.equal(vc.cpu()[:, :, 3:], v[:, :, :2]) and (vc[:, :, :3] == 1).all() and (kc[:, :, :3] == 1).all()
+        for start in (-7, 5, 2 ** 31 - 1):
+            kc, vc = cache.clone()
+            rt.rotate_append(q.cuda(), k.cuda(), v.cuda(), positions.cuda(), cos.cuda(), sin.cuda(), kc, vc,
+                             torch.tensor([start], dtype=torch.int32).cuda(), layout=layout)
+            assert (kc == 1).all() and (vc == 1).all()
+
+
+def test_rotate_rows_at_any_alignment():
+    from systems_for_llms_amd import rotary as rt
+
+    g = torch.Generator().manual_seed(7)
+    cos, sin = rt.rotary_tables(64, 50)
+    positions = torch.randint(0, 50, (2, 7), generator=g, dtype=torch.int32)
+    wide = randn(g, 2, 4, 7, 64 + 3, dtype=BF16)
+    q, k = wide[:, :2, :, 3:], wide[:, 2:, :, 1:65]
+    gpu = wide.cuda()
+    for layout in ("half", "interleaved"):
+        got = rt.rotate(gpu[:, :2, :, 3:], gpu[:, 2:, :, 1:65], positions.cuda(), cos.cuda(), sin.cuda(), layout=layout)
+        for x, y in zip((q, k), got):
+            want, size = oc.rotate(x, positions, cos, sin, layout)
+            within(y, want, rotate_bound(BF16, want, size), layout)
+
+
+# ---- attention of drafts ----------------------------------------------------------
+
+
+def random_mask(g, batch, tokens):
+    from systems_for_llms_amd.tree import ancestor_mask
+
+    parents = torch.stack([torch.randint(-1, t, (batch,), generator=g) if t else torch.full((batch,), -1)
+                           for t in range(tokens)], 1)
+    return ancestor_mask(parents)
+
+
+def score_error(dim, size, scale_of_lse):
+    return (dim + 8) * U * size + 6 * U * scale_of_lse + 4 * U
+
+
+def tree_bounds(dtype, dim, keys, out, lse, spread, size):
+    ds = score_error(dim, size, size + lse.abs().nan_to_num(0, 0, 0))
+    p = 0.0 if dtype == FP32 else half_step(dtype)
+    out_bound = half_step(dtype) * out.abs() + spread * ((p + 2 * ds + 2 * (keys + 8) * U)[..., None]) + TINY[dtype]
+    return out_bound * 1.01, ds + (keys + 8) * U + 4 * U * lse.abs().nan_to_num(0, 0, 0)
+
+
+def check_tree(q, k, v, lengths, mask, counts=None, splits=None, scale=None, got=None):
+    from systems_for_llms_amd import tree
+
+    if got is None:
+        args = [None if x is None else x.cuda() for x in (q, k, v, lengths, mask, counts)]
+        got = tree.attend(*args[:5], counts=args[5], splits=splits, scale=scale)
+    full = torch.ones(q.shape[2], q.shape[2], dtype=torch.bool).tril() if mask is None else mask
+    out, lse, spread, size = oc.tree_attention(q, k, v, lengths, full, counts, scale)
+    bound, lse_bound = tree_bounds(q.dtype, q.shape[3], k.shape[2], out, lse, spread, size)
+    within(got[1], lse, lse_bound, "lse")
+    within(got[0], out, bound, "out")
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("dim", [16, 32, 64, 128])
+@pytest.mark.parametrize("group", [1, 2, 4, 8])
+def test_tree_attention(dtype, dim, group):
+    g = torch.Generator().manual_seed(dim + group)
+    for tokens, keys in ((1, 1), (1, 33), (3, 70), (16, 200), (17, 31), (9, 700)):
+        batch = 3
+        q = randn(g, batch, 2 * group, tokens, dim, dtype=dtype, scale=1.5)
+        k, v = (randn(g, batch, 2, keys + tokens, dim, dtype=dtype) for _ in range(2))
+        lengths = torch.tensor([keys, 0, keys // 2], dtype=torch.int32)
+        counts = torch.tensor([tokens, (tokens + 1) // 2, 0 if tokens % 2 else tokens], dtype=torch.int32)
+        mask = random_mask(g, batch, tokens)
+        for splits in (1, 3, None):
+            check_tree(q, k, v, lengths, mask, counts, splits)
+    check_tree(q, k, v, lengths, None, None, 2, scale=0.21)
+
+
+@pytest.mark.parametrize("tokens, group", [(32, 2), (64, 1), (128, 1), (65, 8), (128, 8)])
+def test_tree_attention_wide(tokens, group):
+    g = torch.Generator().manual_seed(tokens)
+    q = randn(g, 1, group, tokens, 64, dtype=BF16)
+    k, v = (randn(g, 1, 1, 300 + tokens, 64, dtype=BF16) for _ in range(2))
+    check_tree(q, k, v, torch.tensor([300], dtype=torch.int32), random_mask(g, 1, tokens), None, None)
+    check_tree(q, k, v, torch.tensor([7], dtype=torch.int32), random_mask(g, 1, tokens),
+               torch.tensor([tokens - 31], dtype=torch.int32), 2)
+
+
+def test_tree_attention_masks_that_leave_rows_empty():
+    g = torch.Generator().manual_seed(3)
+    q, k, v = randn(g, 2, 2, 4, 64, dtype=FP16), randn(g, 2, 1, 12, 64, dtype=FP16), randn(g, 2, 1, 12, 64, dtype=FP16)
+    mask = torch.zeros(2, 4, 4, dtype=torch.bool)
+    mask[0, 1, 3] = mask[1, 2, 2] = True
+    lengths = torch.tensor([0, 0], dtype=torch.int32)
+    for splits in (1, 2):
+        check_tree(q, k, v, lengths, mask, None, splits)
+        check_tree(q, k, v, torch.tensor([8, 0], dtype=torch.int32), mask, None, splits)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("dim", [16, 32, 64, 128])
+@pytest.mark.parametrize("tokens", [6, 20])
+def test_tree_attention_ignores_what_it_does_not_see(dtype, dim, tokens):
+    """NaN and infinities in rows past the drafts and in drafts that only some rows see."""
+    g = torch.Generator().manual_seed(dim + tokens)
+    batch, n = 2, 37
+    q = randn(g, batch, 4, tokens, dim, dtype=dtype)
+    k, v = (randn(g, batch, 2, 100, dim, dtype=dtype) for _ in range(2))
+    lengths = torch.tensor([n, 61], dtype=torch.int32)
+    counts = torch.tensor([tokens, tokens - 2], dtype=torch.int32)
+    mask = random_mask(g, batch, tokens)
+    mask[:, :, 3] = False
+    mask[:, 3, 3] = True  # only draft 3 sees itself
+    mask[:, :, 2] = False  # and nobody draft 2
+    mask[0, :, 1] = False
+    mask[0, 1, 1] = mask[0, 5, 1] = True
+    for b in range(batch):
+        end = int(lengths[b] + counts[b])
+        k[b, :, end:] = float("nan")
+        v[b, :, end:] = float("inf")
+        v[b, :, int(lengths[b]) + 3, ::3] = float("nan")
+        k[b, :, int(lengths[b]) + 2], v[b, :, int(lengths[b]) + 2, 1] = float("nan"), float("inf")
+    v[0, 1, n + 1, 5] = float("-inf")
+    v[0, 1, n + 1, 2] = float("inf")
+    for splits in (1, 2):
+        check_tree(q, k, v, lengths, mask, counts, splits)
+
+
+def test_tree_attention_strided_views_and_long_rows():
+    """q as a projection leaves it, k and v as one interleaved cache, a shared mask; rows far apart."""
+    g = torch.Generator().manual_seed(11)
+    q = randn(g, 2, 5, 8, 64, dtype=BF16).transpose(1, 2)
+    kv = randn(g, 2, 90, 2, 2, 64, dtype=BF16)
+    k, v = kv[..., 0, :].transpose(1, 2), kv[..., 1, :].transpose(1, 2)
+    lengths = torch.tensor([85, 40], dtype=torch.int32)
+    mask = random_mask(g, 1, 5)[0]
+    from systems_for_llms_amd import tree
+
+    gkv, gq = kv.cuda(), q.transpose(1, 2).contiguous().cuda().transpose(1, 2)
+    got = tree.attend(gq, gkv[..., 0, :].transpose(1, 2), gkv[..., 1, :].transpose(1, 2), lengths.cuda(), mask.cuda())
+    assert got[0].stride() == gq.stride()
+    check_tree(q, k, v, lengths, mask, got=got)
+
+
+def test_tree_attention_offsets_past_32_bits():
+    """Rows of a cache that lie more than 2^32 bytes from its start."""
+    from systems_for_llms_amd import tree
+
+    g = torch.Generator().manual_seed(12)
+    keys, tokens, dim, stride = 200, 3, 64, 64 * 300000  # 38 MB between rows: 7.7 GB in all
+    block = torch.zeros(keys * stride, dtype=BF16, device="cuda")
+    k = block.as_strided((1, 1, keys, dim), (keys * stride, keys * stride, stride, 1))
+    v = block[64:].as_strided((1, 1, keys, dim), (keys * stride, keys * stride, stride, 1))
+    small = [randn(g, 1, 1, keys, dim, dtype=BF16) for _ in range(2)]
+    k.copy_(small[0])
+    v.copy_(small[1])
+    q, lengths = randn(g, 1, 4, tokens, dim, dtype=BF16), torch.tensor([keys - tokens], dtype=torch.int32)
+    got = tree.attend(q.cuda(), k, v, lengths.cuda())
+    check_tree(q, *small, lengths, None, got=got)
+    weights = torch.zeros(1, 1, keys, device="cuda")
+    tree.accumulate(q.cuda(), k, got[1], weights, lengths.cuda())
+    check_weights(q, small[0], got[1].cpu(), torch.zeros(1, 1, keys), lengths, None, got=weights)
+
+
+def test_tree_prepare_refuses_lengths_outside_the_cache():
+    from systems_for_llms_amd import tree
+
+    q, k = torch.zeros(2, 2, 3, 64, device="cuda"), torch.zeros(2, 2, 10, 64, device="cuda")
+    for lengths in ([8, 0], [0, -1]):
+        with pytest.raises(ValueError, match="each length"):
+            tree.prepare(q, k, k, torch.tensor(lengths, dtype=torch.int32).cuda())
+    lengths = torch.zeros(2, dtype=torch.int32).cuda()
+    with pytest.raises(ValueError, match="each count"):
+        tree.prepare(q, k, k, lengths, counts=lengths + 4)
+    for change, message in ((dict(mask=torch.ones(2, 3, device="cuda", dtype=torch.bool)), "mask"),
+                            (dict(mask=torch.ones(3, 3, device="cuda")), "mask"),
+                            (dict(lengths=lengths.long()), "lengths"), (dict(k=k[:, :, :, ::2]), "contiguous last"),
+                            (dict(k=k[..., :32], v=k[..., :32]), "head dimension"), (dict(v=k[:, :, :9]), "same"),
+                            (dict(q=q[:, :1].expand(2, 3, 3, 64)), "divisible"), (dict(scale=0.0), "scale"),
+                            (dict(q=q[:, :1].expand(2, 6, 3, 64)), "GQA"),
+                            (dict(q=torch.zeros(2, 2, 129, 64, device="cuda")), "at most 128")):
+        with pytest.raises(ValueError, match=message):
+            tree.prepare(**{**dict(q=q, k=k, v=k, lengths=lengths), **change})
+
+
+def test_tree_lengths_changed_past_the_cache_stay_inside():
+    """After prepare lengths are only clamped: keys the cache has not are not there."""
+    from systems_for_llms_amd import tree
+
+    g = torch.Generator().manual_seed(13)
+    q, k, v = randn(g, 1, 2, 3, 64, dtype=BF16), *(randn(g, 1, 2, 40, 64, dtype=BF16) for _ in range(2))
+    lengths = torch.zeros(1, dtype=torch.int32, device="cuda")
+    op = tree.prepare(q.cuda(), k.cuda(), v.cuda(), lengths)
+    for n in (39, 40, 1000, -5):
+        lengths.fill_(n)
+        check_tree(q, k, v, torch.tensor([min(max(n, 0), 40)], dtype=torch.int32), None, got=(op(), op.lse))
+
+
+# ---- weights by slot --------------------------------------------------------------
+
+
+def check_weights(q, k, lse, weights, lengths, mask, counts=None, rows=None, scale=None, got=None):
+    from systems_for_llms_amd import tree
+
+    if got is None:
+        gpu = [None if x is None else x.cuda() for x in (q, k, lse, weights, lengths, mask, counts, rows)]
+        got = tree.accumulate(*gpu[:6], counts=gpu[6], rows=gpu[7], scale=scale)
+        assert got.data_ptr() == gpu[3].data_ptr()
+    full = torch.ones(q.shape[2], q.shape[2], dtype=torch.bool).tril() if mask is None else mask
+    want, size = oc.tree_weights(q, k, lse, weights, lengths, full, counts, rows, scale)
+    reach = size + lse.double().abs().nan_to_num(0, 0, 0).amax()
+    terms = q.shape[1] // k.shape[1] * q.shape[2]
+    bound = (want - weights.double()) * (score_error(q.shape[3], size, reach) + (terms + 4) * U) + U * want.abs()
+    within(got, want, bound * 1.01 + 1e-38, "weights")
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("dim", [16, 32, 64, 128])
+@pytest.mark.parametrize("group", [1, 2, 4, 8])
+def test_weights_by_slot(dtype, dim, group):
+    g = torch.Generator().manual_seed(dim * 10 + group)
+    for tokens, keys in ((1, 1), (1, 200), (5, 33), (23, 300)):
+        q = randn(g, 3, 2 * group, tokens, dim, dtype=dtype)
+        k = randn(g, 3, 2, keys + tokens, dim, dtype=dtype)
+        lengths = torch.tensor([keys, 0, keys // 2], dtype=torch.int32)
+        counts = torch.tensor([tokens, (tokens + 1) // 2, tokens], dtype=torch.int32)
+        mask = random_mask(g, 3, tokens)
+        for b in range(3):  # what nobody sees holds anything
+            k[b, :, int(lengths[b] + counts[b]):] = float("nan")
+        _, lse, _, _ = oc.tree_attention(q, k, k, lengths, mask, counts)
+        weights = torch.rand(3, 2, keys + tokens, generator=g)
+        rows = torch.rand(3, tokens, generator=g) < 0.5
+        rows[1] = False
+        check_weights(q, k, lse.float(), weights, lengths, mask, counts, rows)
+        check_weights(q, k, lse.float(), weights, lengths, mask, counts)
+
+
+def test_weights_of_wide_trees_and_empty_rows():
+    g = torch.Generator().manual_seed(21)
+    q, k = randn(g, 1, 8, 128, 64, dtype=FP16), randn(g, 1, 1, 400, 64, dtype=FP16)
+    lengths, mask = torch.tensor([270], dtype=torch.int32), random_mask(g, 1, 128)
+    lse = oc.tree_attention(q, k, k, lengths, mask)[1].float()
+    check_weights(q, k, lse, torch.zeros(1, 1, 400), lengths, mask)
+    nothing = torch.zeros(1, 128, 128, dtype=torch.bool)
+    lse = torch.full_like(lse, float("-inf"))
+    check_weights(q, k, lse, torch.ones(1, 1, 400), torch.tensor([0], dtype=torch.int32), nothing)
+
+
+def test_prepared_weights_sum_to_the_rows():
+    """Each counted row's weights add up to one by KV head."""
+    from systems_for_llms_amd import tree
+
+    g = torch.Generator().manual_seed(22)
+    q, k = randn(g, 2, 8, 6, 64, dtype=BF16).cuda(), randn(g, 2, 2, 700, 64, dtype=BF16).cuda()
+    op = tree.prepare(q, k, k, torch.tensor([690, 13], dtype=torch.int32).cuda())
+    op()
+    weights = torch.zeros(2, 2, 700, device="cuda")
+    rows = torch.tensor([[1, 0, 1, 1, 0, 0], [0, 0, 0, 0, 0, 1]], dtype=torch.bool)
+    op.accumulate(weights, rows.cuda())
+    total = weights.double().sum(-1).cpu()
+    want = rows.sum(1, keepdim=True).double() * 4
+    # Scores and lse err alike in the two kernels: a few hundred roundings of each exp.
+    within(total, want.expand(2, 2), 1e-4 * want)
+
+
+# ---- accepted paths ---------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("dim", [16, 32, 64, 128])
+@pytest.mark.parametrize("tokens", [1, 5, 128])
+def test_accept(dtype, dim, tokens):
+    from systems_for_llms_amd import tree
+
+    g = torch.Generator().manual_seed(dim + tokens)
+    batch, heads, keys = 4, 3, tokens + 9
+    k, v = (randn(g, batch, heads, keys, dim, dtype=dtype) for _ in range(2))
+    weights = torch.rand(batch, heads, keys, generator=g)
+    positions = torch.randint(0, 999, (batch, heads, keys), generator=g, dtype=torch.int32)
+    lengths = torch.tensor([0, 9, 4, 7], dtype=torch.int32)
+    accepted = torch.tensor([tokens, tokens // 2, 0, (tokens + 1) // 2], dtype=torch.int32)
+    path = torch.stack([torch.randperm(tokens, generator=g) for _ in range(batch)]).to(torch.int32)
+    for b in range(1, batch):  # ascending, as in a tree; the first row in any order
+        path[b, : accepted[b]] = path[b, : accepted[b]].sort().values
+    (wk, wv, ww, wp), want_lengths = oc.accept([k, v, weights, positions], lengths, path, accepted, weights)
+    for with_values in (True, False):
+        gk, gv, gw, gp = (x.cuda() for x in (k, v, weights, positions))
+        got = tree.accept(gk, gv, lengths.cuda(), path.cuda(), accepted.cuda(),
+                          **(dict(weights=gw, positions=gp) if with_values else {}))
+        assert torch.equal(got.cpu(), want_lengths) and torch.equal(gk.cpu(), wk) and torch.equal(gv.cpu(), wv)
+        if with_values:
+            assert torch.equal(gw.cpu(), ww) and torch.equal(gp.cpu(), wp)
+        else:
+            assert torch.equal(gw.cpu(), weights)
+
+
+def test_accept_entries_out_of_range():
+    from systems_for_llms_amd import tree
+
+    g = torch.Generator().manual_seed(31)
+    k = randn(g, 3, 1, 6, 32)
+    lengths = torch.tensor([3, 5, 7], dtype=torch.int32)
+    path = torch.tensor([[-1, 4, 1], [0, 1, 2], [0, 1, 2]], dtype=torch.int32)
+    accepted = torch.tensor([9, 3, 2], dtype=torch.int32)
+    gk, gv = k.cuda(), k.cuda()
+    got = tree.accept(gk, gv, lengths.cuda(), path.cuda(), accepted.cuda())
+    want = k.clone()
+    want[0, :, 5] = k[0, :, 4]
+    assert torch.equal(gk.cpu(), want) and torch.equal(gv.cpu(), want)
+    assert got.tolist() == [6, 6, 7]
+
+
+def test_writes_into_expanded_caches_are_refused():
+    from systems_for_llms_amd import evict, tree
+
+    k = torch.zeros(1, 1, 8, 32, device="cuda").expand(2, 1, 8, 32)
+    n = torch.zeros(2, dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError, match="expanded"):
+        tree.accept(k, k.clone(), n, n[:, None].contiguous(), n)
+    with pytest.raises(ValueError, match="expanded"):
+        evict.compact(torch.zeros(2, 1, 4, dtype=torch.int32, device="cuda"), k.clone(), k)
+
+
+# ---- eviction ---------------------------------------------------------------------
+
+
+def weights_of_kind(g, kind, *shape):
+    u = torch.rand(shape, generator=g)
+    if kind == "ties":
+        return (u * 6).floor()
+    if kind == "equal":
+        return torch.full(shape, 0.25)
+    if kind == "odd":
+        w = torch.randn(shape, generator=g)
+        w[u < 0.1], w[(u > 0.1) & (u < 0.15)], w[(u > 0.15) & (u < 0.2)] = float("nan"), float("inf"), float("-inf")
+        w[(u > 0.2) & (u < 0.3)], w[(u > 0.3) & (u < 0.4)] = 0.0, -0.0
+        return w
+    return u.pow(8) * 100
+
+
+@pytest.mark.parametrize("kind", ["heavy", "ties", "equal", "odd"])
+@pytest.mark.parametrize("keys, keep, recent", [(1, 1, 1), (70, 1, 0), (64, 63, 63), (200, 64, 10), (1000, 700, 100),
+                                                (2049, 128, 127), (5000, 4096, 0), (40000, 1000, 300)])
+def test_select(kind, keys, keep, recent):
+    from systems_for_llms_amd import evict
+
+    g = torch.Generator().manual_seed(keys)
+    batch, heads = 4, 2
+    weights = weights_of_kind(g, kind, batch, heads, keys + 3)
+    lengths = torch.tensor([keys, keep, max(0, keep - 1), (keys + keep) // 2], dtype=torch.int32)
+    positions = torch.rand(batch, heads, keys + 3, generator=g).argsort(-1).to(torch.int32) * 3
+    for p in (None, positions):
+        kept, new = evict.select(weights.cuda(), lengths.cuda(), keep, recent=recent,
+                                 positions=None if p is None else p.cuda())
+        want, want_new = oc.select(weights, lengths, keep, recent, p)
+        assert torch.equal(new.cpu(), want_new) and torch.equal(kept.cpu(), want)
+
+
+def test_select_recent_slots_that_share_positions():
+    from systems_for_llms_amd import evict
+
+    g = torch.Generator().manual_seed(41)
+    weights = torch.rand(2, 2, 300, generator=g)
+    positions = torch.randint(0, 20, (2, 2, 300), generator=g, dtype=torch.int32)
+    lengths = torch.tensor([300, 250], dtype=torch.int32)
+    for keep, recent in ((40, 10), (40, 40), (5, 5)):  # more recent slots than places, too
+        kept, _ = evict.select(weights.cuda(), lengths.cuda(), keep, recent=recent, positions=positions.cuda())
+        assert torch.equal(kept.cpu(), oc.select(weights, lengths, keep, recent, positions)[0])
+
+
+def test_select_clamps_lengths():
+    from systems_for_llms_amd import evict
+
+    weights = torch.rand(2, 1, 50)
+    kept, new = evict.select(weights.cuda(), torch.tensor([80, -3], dtype=torch.int32).cuda(), 20)
+    want, _ = oc.select(weights, torch.tensor([50, 0], dtype=torch.int32), 20)
+    assert torch.equal(kept.cpu(), want) and new.tolist() == [20, 0]
+
+
+def test_select_largest_cache():
+    from systems_for_llms_amd import evict
+
+    g = torch.Generator().manual_seed(42)
+    weights = weights_of_kind(g, "heavy", 1, 2, evict.MAX_SLOTS)
+    lengths = torch.tensor([evict.MAX_SLOTS], dtype=torch.int32)
+    kept, _ = evict.select(weights.cuda(), lengths.cuda(), 100001, recent=77)
+    assert torch.equal(kept.cpu(), oc.select(weights, lengths, 100001, 77)[0])
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("dim", [16, 32, 64, 128])
+def test_evict_moves_everything(dtype, dim):
+    from systems_for_llms_amd import evict
+
+    g = torch.Generator().manual_seed(dim)
+    for keys, keep in ((130, 100), (700, 33), (20, 20)):
+        k, v = (randn(g, 2, 3, keys, dim, dtype=dtype) for _ in range(2))
+        weights = weights_of_kind(g, "ties", 2, 3, keys)
+        positions = torch.rand(2, 3, keys, generator=g).argsort(-1).to(torch.int32)
+        lengths = torch.tensor([keys, keys - 9], dtype=torch.int32)
+        kept, new = oc.select(weights, lengths, keep, 7, positions)
+        want = oc.compact([k, v, weights, positions], kept, weights)
+        gpu = [x.cuda() for x in (k, v, weights, positions)]
+        got = evict.evict(gpu[0], gpu[1], gpu[2], lengths.cuda(), keep, recent=7, positions=gpu[3])
+        assert torch.equal(got[0].cpu(), kept) and torch.equal(got[1].cpu(), new)
+        for x, y in zip(gpu, want):
+            assert torch.equal(x.cpu(), y)
+        views = torch.zeros(2, keys, 2, 3, dim, dtype=dtype, device="cuda")  # k and v side by side, rows first
+        gk, gv = (views[:, :, i].transpose(1, 2) for i in range(2))
+        gk.copy_(k)
+        gv.copy_(v)
+        evict.compact(kept.cuda(), gk, gv)
+        assert torch.equal(gk.cpu(), want[0]) and torch.equal(gv.cpu(), want[1])
+
+
+# ---- together, as a serving program uses them ---------------------------------------
+
+
+class Server:
+    """Speculative steps on a bounded cache, on the GPU or in float64 with the caches' rounding."""
+
+    def __init__(self, seed, batch, heads, kv_heads, tokens, capacity, dim, dtype):
+        self.g = torch.Generator().manual_seed(seed)
+        self.batch, self.heads, self.kv_heads, self.tokens, self.dim, self.dtype = batch, heads, kv_heads, tokens, dim, dtype
+        self.k, self.v = (torch.zeros(batch, kv_heads, capacity, dim, dtype=dtype) for _ in range(2))
+        self.weights = torch.zeros(batch, kv_heads, capacity)
+        self.positions = torch.zeros(batch, kv_heads, capacity, dtype=torch.int32)
+        self.lengths = torch.zeros(batch, dtype=torch.int32)
+        self.next = torch.zeros(batch, dtype=torch.int32)  # the next token's position
+
+    def draw(self):
+        """The next step's q, k, v, tree, path: depths give the positions."""
+        t = self.tokens
+        parents = torch.stack([torch.randint(-1, i, (self.batch,), generator=self.g) if i else torch.full((self.batch,), -1)
+                               for i in range(t)], 1)
+        from systems_for_llms_amd.tree import ancestor_mask
+
+        mask = ancestor_mask(parents)
+        depth = mask.sum(-1) - 1
+        path = torch.zeros(self.batch, t, dtype=torch.int32)
+        accepted = torch.zeros(self.batch, dtype=torch.int32)
+        rows = torch.zeros(self.batch, t, dtype=torch.bool)
+        for b in range(self.batch):
+            leaf = int(torch.randint(0, t, (1,), generator=self.g))
+            chain = mask[b, leaf].nonzero()[:, 0]
+            path[b, : len(chain)] = chain.to(torch.int32)
+            accepted[b] = len(chain)
+            rows[b, chain] = True
+        shape = (self.batch, t, self.heads + 2 * self.kv_heads, self.dim)
+        qkv = randn(self.g, *shape, dtype=self.dtype)
+        return qkv, mask, depth.to(torch.int32), path, accepted, rows
+
+
+def test_speculative_steps_on_a_bounded_cache():
+    from systems_for_llms_amd import evict, rotary, tree
+
+    s = Server(51, 2, 8, 2, 6, 64, 64, BF16)
+    cos, sin = rotary.rotary_tables(64, 512)
+    gain = 1 + randn(s.g, 64, scale=0.2).to(BF16)
+    k, v, weights, positions, lengths = (x.cuda() for x in (s.k, s.v, s.weights, s.positions, s.lengths))
+    q_buffer = torch.zeros(2, 6, 8, 64, dtype=BF16, device="cuda").transpose(1, 2)
+    mask_buffer = torch.zeros(2, 6, 6, dtype=torch.bool, device="cuda")
+    op = tree.prepare(q_buffer, k, v, lengths, mask_buffer, splits=2)
+    evictions = 0
+    for step in range(40):
+        qkv, mask, depth, path, accepted, rows = s.draw()
+        at = s.next[:, None] + depth
+        before = [x.cpu() for x in (k, v, weights, positions, lengths)]
+        parts = qkv.cuda().transpose(1, 2).split([8, 2, 2], 1)
+        q = rotary.rotate_append(*parts, at.cuda(), cos.cuda(), sin.cuda(), k, v, lengths, layout="half",
+                                 q_norm=gain.cuda(), k_norm=gain.cuda())
+        slots = (lengths.long()[:, None] + torch.arange(6, device="cuda"))[:, None].expand(2, 2, 6)
+        positions.scatter_(2, slots, at.cuda()[:, None].expand(2, 2, 6))
+        q_buffer.copy_(q)
+        mask_buffer.copy_(mask)
+        op()
+        # Each operator against its float64 form on what the GPU's caches hold.
+        wk, sk = oc.rotate(qkv.transpose(1, 2)[:, 8:10], at, cos, sin, "half", gain)
+        for b in range(2):
+            n = int(before[4][b])
+            within(k[b, :, n:n + 6], wk[b], rotate_bound(BF16, wk[b], sk[b]), f"step {step}: k")
+        check_tree(q.cpu(), k.cpu(), v.cpu(), before[4], mask, got=(op.output, op.lse))
+        held = weights.cpu()
+        op.accumulate(weights, rows.cuda())
+        check_weights(q.cpu(), k.cpu(), op.lse.cpu(), held, before[4], mask, None, rows, got=weights)
+        state = [x.cpu() for x in (k, v, weights, positions)]
+        moved, n = oc.accept(state, before[4], path, accepted, state[2])
+        lengths.copy_(tree.accept(k, v, lengths, path.cuda(), accepted.cuda(), weights=weights, positions=positions))
+        assert torch.equal(lengths.cpu(), n)
+        for x, y in zip((k, v, weights, positions), moved):
+            assert torch.equal(x.cpu(), y)
+        s.next += accepted
+        if int(lengths.max()) + 6 > 40:
+            state = [x.cpu() for x in (k, v, weights, positions)]
+            want, n = oc.select(state[2], lengths.cpu(), 24, 8, state[3])
+            moved = oc.compact(state, want, state[2])
+            kept, new = evict.evict(k, v, weights, lengths, 24, recent=8, positions=positions)
+            assert torch.equal(kept.cpu(), want) and torch.equal(new.cpu(), n)
+            for x, y in zip((k, v, weights, positions), moved):
+                assert torch.equal(x.cpu(), y)
+            lengths.copy_(new)
+            evictions += 1
+    assert evictions > 1
+
+
+def test_captured_step_replays():
+    """The calls of a step in one HIP graph, replayed with eager work of the same kind in between."""
+    from systems_for_llms_amd import evict, rotary, tree
+
+    g = torch.Generator().manual_seed(61)
+    cos, sin = (x.cuda() for x in rotary.rotary_tables(64, 4096))
+    static = {"qkv": torch.zeros(2, 4, 12, 64, dtype=FP16, device="cuda"),
+              "at": torch.zeros(2, 4, dtype=torch.int32, device="cuda"),
+              "lengths": torch.zeros(2, dtype=torch.int32, device="cuda"),
+              "path": torch.zeros(2, 4, dtype=torch.int32, device="cuda"),
+              "accepted": torch.zeros(2, dtype=torch.int32, device="cuda"),
+              "k": torch.zeros(2, 2, 600, 64, dtype=FP16, device="cuda"),
+              "v": torch.zeros(2, 2, 600, 64, dtype=FP16, device="cuda"),
+              "weights": torch.zeros(2, 2, 600, device="cuda")}
+
+    def step(s, op):
+        q = rotary.rotate_append(*s["qkv"].transpose(1, 2).split([8, 2, 2], 1), s["at"], cos, sin, s["k"], s["v"],
+                                 s["lengths"])
+        op.q.copy_(q)
+        op()
+        op.accumulate(s["weights"])
+        n = tree.accept(s["k"], s["v"], s["lengths"], s["path"], s["accepted"], weights=s["weights"])
+        kept, n = evict.evict(s["k"], s["v"], s["weights"], n, 300, recent=20)
+        return op.output, op.lse, kept, n
+
+    def fresh(s):
+        for name, shape in (("qkv", (2, 4, 12, 64)), ("k", (2, 2, 600, 64)), ("v", (2, 2, 600, 64))):
+            s[name].copy_(randn(g, *shape, dtype=FP16))
+        s["at"].copy_(torch.randint(0, 4096, (2, 4), generator=g))
+        s["lengths"].copy_(torch.randint(0, 590, (2,), generator=g))
+        s["path"].copy_(torch.randperm(4, generator=g).sort().values.expand(2, 4))
+        s["accepted"].copy_(torch.randint(0, 5, (2,), generator=g))
+        s["weights"].copy_(torch.rand(2, 2, 600, generator=g))
+
+    def prepared(s):
+        return tree.prepare(torch.zeros(2, 8, 4, 64, dtype=FP16, device="cuda"), s["k"], s["v"], s["lengths"], splits=2)
+
+    op = prepared(static)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step(static, op)
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step(static, op)
+    for _ in range(4):
+        fresh(static)
+        eager = {name: x.clone() for name, x in static.items()}
+        graph.replay()
+        want = step(eager, prepared(eager))
+        torch.cuda.synchronize()
+        for x, y in zip(captured, want):
+            assert torch.equal(x, y)
+        for name in ("k", "v", "weights"):
+            assert torch.equal(static[name], eager[name]), name
+
+
+def test_calls_on_two_streams_at_once():
+    from systems_for_llms_amd import tree
+
+    g = torch.Generator().manual_seed(71)
+    ops, cpu = [], []
+    for i in range(2):
+        q, k, v = randn(g, 2, 8, 5, 64, dtype=BF16), *(randn(g, 2, 2, 3000, 64, dtype=BF16) for _ in range(2))
+        lengths = torch.tensor([2990, 1500 + i], dtype=torch.int32)
+        cpu.append((q, k, v, lengths))
+        ops.append(tree.prepare(*(x.cuda() for x in (q, k, v, lengths)), splits=4))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(3):
+        for op, stream in zip(ops, streams):
+            with torch.cuda.stream(stream):
+                op()
+    torch.cuda.synchronize()
+    for op, (q, k, v, lengths) in zip(ops, cpu):
+        want, lse, spread, size = (x for x in oc.tree_attention(q, k, v, lengths, torch.ones(5, 5, dtype=torch.bool).tril()))
+        bound, lse_bound = tree_bounds(BF16, 64, 3000, want, lse, spread, size)
+        within(op.output, want, bound)
+        within(op.lse, lse, lse_bound)
+
+
+def test_results_repeat_bit_for_bit():
+    from systems_for_llms_amd import tree
+
+    g = torch.Generator().manual_seed(81)
+    q, k, v = randn(g, 1, 8, 20, 128, dtype=FP16).cuda(), *(randn(g, 1, 2, 4000, 128, dtype=FP16).cuda() for _ in range(2))
+    op = tree.prepare(q, k, v, torch.tensor([3980], dtype=torch.int32).cuda(), splits=7)
+    first, lse = op().clone(), op.lse.clone()
+    weights = [torch.zeros(1, 2, 4000, device="cuda") for _ in range(2)]
+    for w in weights:
+        assert torch.equal(op(), first) and torch.equal(op.lse, lse)
+        op.accumulate(w)
+    assert torch.equal(*weights)
