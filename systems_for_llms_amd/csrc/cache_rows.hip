@@ -2,7 +2,10 @@
 // an accepted path moved behind the committed rows, and the rows of an eviction's
 // kept slots moved into the places that become free. All of it moves bytes: the
 // bound is memory, and below a few hundred KB the launch.
-#include "common.hpp"
+#include <algorithm>
+#include <type_traits>
+
+#include "attn_mfma.hpp"
 
 namespace sfl {
 namespace {
@@ -99,6 +102,138 @@ __global__ __launch_bounds__(256) void rotate_any_kernel(const RotateArgs a, int
     }
     store_scalar<T>(static_cast<T*>(r.out) + d, r.zero ? 0.f : y);
   }
+}
+
+// The same for rows of 16-byte pieces: a lane holds one piece, LPR lanes a row. A
+// group of LPR lanes takes every GH-th head of one token, so its angles and gains are
+// loaded once, and the loads of kRows heads are issued before the first is used. In
+// the half layout a lane also loads the piece its own is paired with (from the cache,
+// as its neighbour just did), which costs no exchange between lanes.
+template <typename T, int D, bool kHalfLayout>
+__global__ __launch_bounds__(256) void rotate_rows_kernel(const RotateArgs a, int heads, int gh_log2, bool norm) {
+  constexpr int VEC = vec_elems<T>(), LPR = D / VEC, kRows = 3;
+  const int group = int(threadIdx.x) / LPR, piece = int(threadIdx.x) % LPR;
+  const int gh = 1 << gh_log2;
+  const unsigned token = blockIdx.x * unsigned((256 / LPR) >> gh_log2) + unsigned(group >> gh_log2);
+  const unsigned tokens = unsigned(a.batch) * unsigned(a.tokens);
+  const bool on = token < tokens;
+  const int b = int((on ? token : 0u) / unsigned(a.tokens)), t = int((on ? token : 0u) - unsigned(b) * unsigned(a.tokens));
+  const int d0 = piece * VEC;
+  const bool turned = d0 < 2 * a.half;
+  const bool second = kHalfLayout && d0 >= a.half;
+  const int d1 = !kHalfLayout || !turned ? d0 : second ? d0 - a.half : d0 + a.half;  // the paired piece
+
+  // Angles of the lane's elements (interleaved: of its pairs); 1 and 0 where nothing turns.
+  constexpr int ANGLES = kHalfLayout ? VEC : VEC / 2;
+  float c[ANGLES], sn[ANGLES];
+  const int pos = a.positions[long(b) * a.tokens + t];
+  const bool known = pos >= 0 && pos < a.table;
+  const int i0 = kHalfLayout ? (second ? d0 - a.half : d0) : d0 / 2;
+#pragma unroll
+  for (int i = 0; i < ANGLES; ++i) {
+    const bool turns = i0 + i < a.half;
+    const long at = long(known ? pos : 0) * a.half + (turns ? i0 + i : 0);
+    const float cv = a.cos[at], sv = a.sin[at];
+    c[i] = !turns ? 1.f : known ? cv : NAN;
+    sn[i] = !turns ? 0.f : known ? sv : NAN;
+  }
+  const auto gains = [&](const void* gain, int d, float (&g)[VEC]) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) g[e] = gain ? gain_at(a, gain, d + e, T{}) : 1.f;
+  };
+  float gq[VEC], gk[VEC], pq[VEC], pk[VEC];
+  gains(a.q_gain, d0, gq);
+  gains(a.k_gain, d0, gk);
+  if constexpr (kHalfLayout) {
+    gains(a.q_gain, d1, pq);
+    gains(a.k_gain, d1, pk);
+  }
+
+  const int step = gh * int(gridDim.y);
+  for (int h0 = int(blockIdx.y) * gh; h0 < heads; h0 += kRows * step) {  // uniform over the workgroup
+    uint4 x[kRows], xp[kRows];
+    RotateRow row[kRows];
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      const int h = h0 + r * step + (group & (gh - 1));
+      row[r] = rotate_row<T>(a, b, t, min(h, heads - 1));
+      row[r].store = row[r].store && on && h < heads;
+      x[r] = load16(static_cast<const T*>(row[r].in) + d0);
+      if constexpr (kHalfLayout) xp[r] = load16(static_cast<const T*>(row[r].in) + d1);
+    }
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      float v[VEC], w[VEC];
+      unpack16<T>(x[r], v);
+      if constexpr (kHalfLayout) unpack16<T>(xp[r], w);
+      const bool is_q = row[r].gain == a.q_gain;
+      if (norm) {
+        float sq = 0.f;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) sq = fmaf(v[e], v[e], sq);
+        const float scale = 1.f / sqrtf(group_sum<LPR>(sq) / float(D) + a.eps);
+        if (row[r].gain) {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) {
+            v[e] *= scale * (is_q ? gq[e] : gk[e]);
+            if constexpr (kHalfLayout) w[e] *= scale * (is_q ? pq[e] : pk[e]);
+          }
+        }
+      }
+      if (row[r].turn && turned) {
+        if constexpr (kHalfLayout) {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) v[e] = fmaf(second ? w[e] : -w[e], sn[e], v[e] * c[e]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < VEC; e += 2) {
+            const float u = v[e], o = v[e + 1];
+            v[e] = fmaf(-o, sn[e / 2], u * c[e / 2]);
+            v[e + 1] = fmaf(u, sn[e / 2], o * c[e / 2]);
+          }
+        }
+      }
+      if (!row[r].store) continue;
+      uint4 y;
+      if constexpr (std::is_same<T, float>::value)
+        y = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+      else
+        y = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+      if (!row[r].turn) y = x[r];
+      if (row[r].zero) y = make_uint4(0u, 0u, 0u, 0u);
+      *reinterpret_cast<uint4*>(static_cast<T*>(row[r].out) + d0) = y;
+    }
+  }
+}
+
+// Whether the rows come in 16-byte pieces, the paired ones too.
+bool rotate_in_pieces(const RotateArgs& a, int es, bool half_layout) {
+  const void* p[6] = {a.q, a.k, a.v, a.q_out, a.k_out, a.v_out};
+  for (int i = 0; i < 6; ++i) {
+    if (reinterpret_cast<uintptr_t>(p[i]) % 16) return false;
+    for (int j = 0; j < 3; ++j)
+      if (p[i] && a.st[i][j] * es % 16) return false;
+  }
+  return (!half_layout || a.half * es % 16 == 0) && long(a.batch) * a.tokens < (1L << 31);
+}
+
+template <typename T, int D>
+int launch_rotate_rows(const RotateArgs& a, int heads, bool half_layout, hipStream_t stream) {
+  constexpr int kGroups = 256 / (D / vec_elems<T>());
+  int gh_log2 = 0;
+  while ((1 << gh_log2) < heads && (1 << gh_log2) < kGroups) ++gh_log2;
+  const int per_block = kGroups >> gh_log2;
+  const long blocks = (long(a.batch) * a.tokens + per_block - 1) / per_block;
+  // Few tokens: their heads on several workgroups, until there are about two for each CU.
+  const int rounds = (heads + (1 << gh_log2) - 1) >> gh_log2;
+  const int share = int(std::max(1L, std::min(long(rounds), 512 / blocks)));
+  const dim3 grid{unsigned(blocks), unsigned(share), 1u};
+  const bool norm = a.q_gain || a.k_gain;
+  if (half_layout)
+    hipLaunchKernelGGL((rotate_rows_kernel<T, D, true>), grid, dim3(256), 0, stream, a, heads, gh_log2, norm);
+  else
+    hipLaunchKernelGGL((rotate_rows_kernel<T, D, false>), grid, dim3(256), 0, stream, a, heads, gh_log2, norm);
+  return check_launch("rotate");
 }
 
 // ---- accepted path --------------------------------------------------------------
@@ -415,6 +550,15 @@ extern "C" int sfl_rotate(const void* q, const void* k, const void* v, const int
   if ((rows + 3) / 4 > 0x7fffffffL) return set_error(SFL_ERR_UNSUPPORTED, "%s: too many rows", what);
   const auto run = [&](auto t) {
     using T = decltype(t);
+    if (rotate_in_pieces(a, es, half_layout)) {
+      const hipStream_t on = static_cast<hipStream_t>(stream);
+      switch (head_dim) {
+        case 16: return launch_rotate_rows<T, 16>(a, heads, half_layout, on);
+        case 32: return launch_rotate_rows<T, 32>(a, heads, half_layout, on);
+        case 64: return launch_rotate_rows<T, 64>(a, heads, half_layout, on);
+        default: return launch_rotate_rows<T, 128>(a, heads, half_layout, on);
+      }
+    }
     const dim3 grid(unsigned((rows + 3) / 4));
     if (half_layout)
       hipLaunchKernelGGL((rotate_any_kernel<T, true>), grid, dim3(256), 0, static_cast<hipStream_t>(stream), a, head_dim, rows, heads);
