@@ -39,10 +39,14 @@ __device__ __forceinline__ RotateRow rotate_row(const RotateArgs& a, int b, int 
   // q goes to token t of its output; k and v to slot start + t of the cache, where it has that slot.
   const long slot = which && a.start ? long(a.start[b]) + t : t;
   RotateRow r;
-  r.in = static_cast<const T*>(which == 0 ? a.q : which == 1 ? a.k : a.v) + b * a.st[which][0] + head * a.st[which][1] +
-         t * a.st[which][2];
-  r.out = static_cast<T*>(which == 0 ? a.q_out : which == 1 ? a.k_out : a.v_out) + b * a.st[3 + which][0] +
-          head * a.st[3 + which][1] + slot * a.st[3 + which][2];
+  // Strides by selection: an index that is not a constant would put the arguments into scratch memory.
+  const auto at = [&](int first, long row, int i) {
+    return b * a.st[first + i][0] + head * a.st[first + i][1] + row * a.st[first + i][2];
+  };
+  r.in = which == 0 ? static_cast<const T*>(a.q) + at(0, t, 0)
+         : which == 1 ? static_cast<const T*>(a.k) + at(0, t, 1) : static_cast<const T*>(a.v) + at(0, t, 2);
+  r.out = which == 0 ? static_cast<T*>(a.q_out) + at(3, slot, 0)
+          : which == 1 ? static_cast<T*>(a.k_out) + at(3, slot, 1) : static_cast<T*>(a.v_out) + at(3, slot, 2);
   r.gain = which == 0 ? a.q_gain : which == 1 ? a.k_gain : nullptr;
   r.turn = which < 2;
   r.zero = !used;
@@ -60,13 +64,14 @@ __device__ __forceinline__ float gain_at(const RotateArgs& a, const void* gain, 
 
 // One wave per row, a row staged in LDS as fp32: any layout, rotated part and alignment.
 template <typename T, bool kHalfLayout>
-__global__ __launch_bounds__(256) void rotate_any_kernel(const RotateArgs a, int dim, long rows, int heads) {
+__global__ __launch_bounds__(256) void rotate_any_kernel(const RotateArgs a, int dim, unsigned rows, unsigned heads) {
   __shared__ float stage[4][128];
-  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
-  const long at = long(blockIdx.x) * 4 + wave;
+  const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave), lane = threadIdx.x % kWave;
+  const unsigned at = blockIdx.x * 4 + unsigned(wave);
   const bool on = at < rows;
-  const long token = (on ? at : 0) / heads;
-  const int h = int((on ? at : 0) - token * heads), b = int(token / a.tokens), t = int(token - long(b) * a.tokens);
+  const unsigned token = (on ? at : 0u) / heads;
+  const int h = int((on ? at : 0u) - token * heads), b = int(token / unsigned(a.tokens));
+  const int t = int(token - unsigned(b) * unsigned(a.tokens));
   const RotateRow r = rotate_row<T>(a, b, t, h);
   float x[2], sq = 0.f;
 #pragma unroll
@@ -104,42 +109,45 @@ __global__ __launch_bounds__(256) void rotate_any_kernel(const RotateArgs a, int
   }
 }
 
+// N values (8, 16 or 32 bytes) as fp32.
+template <typename T, int N>
+__device__ __forceinline__ void load_values(const T* p, float (&v)[N]) {
+  if constexpr (std::is_same<T, float>::value && N == 2) {
+    const float2 r = *reinterpret_cast<const float2*>(p);
+    v[0] = r.x, v[1] = r.y;
+  } else {
+    constexpr int E = vec_elems<T>();
+#pragma unroll
+    for (int i = 0; i < N / E; ++i) unpack16<T>(load16(p + i * E), &v[i * E]);
+  }
+}
+
 // The same for rows of 16-byte pieces: a lane holds one piece, LPR lanes a row. A
-// group of LPR lanes takes every GH-th head of one token, so its angles and gains are
-// loaded once, and the loads of kRows heads are issued before the first is used. In
-// the half layout a lane also loads the piece its own is paired with (from the cache,
-// as its neighbour just did), which costs no exchange between lanes.
+// group of LPR lanes walks tokens, every GH-th head of each: the gains are loaded once,
+// a token's angles once, and the rows of kRows heads before the first is used. In the
+// half layout a lane also loads the piece its own is paired with (from the cache, as
+// its neighbour just did), which costs no exchange between lanes.
 template <typename T, int D, bool kHalfLayout>
 __global__ __launch_bounds__(256) void rotate_rows_kernel(const RotateArgs a, int heads, int gh_log2, bool norm) {
   constexpr int VEC = vec_elems<T>(), LPR = D / VEC, kRows = 3;
+  constexpr int ANGLES = kHalfLayout ? VEC : VEC / 2;
   const int group = int(threadIdx.x) / LPR, piece = int(threadIdx.x) % LPR;
-  const int gh = 1 << gh_log2;
-  const unsigned token = blockIdx.x * unsigned((256 / LPR) >> gh_log2) + unsigned(group >> gh_log2);
-  const unsigned tokens = unsigned(a.batch) * unsigned(a.tokens);
-  const bool on = token < tokens;
-  const int b = int((on ? token : 0u) / unsigned(a.tokens)), t = int((on ? token : 0u) - unsigned(b) * unsigned(a.tokens));
+  const int gh = 1 << gh_log2, per_block = (256 / LPR) >> gh_log2;
   const int d0 = piece * VEC;
   const bool turned = d0 < 2 * a.half;
   const bool second = kHalfLayout && d0 >= a.half;
   const int d1 = !kHalfLayout || !turned ? d0 : second ? d0 - a.half : d0 + a.half;  // the paired piece
+  const int i0 = !turned ? 0 : kHalfLayout ? (second ? d1 : d0) : d0 / 2;            // the first angle
 
-  // Angles of the lane's elements (interleaved: of its pairs); 1 and 0 where nothing turns.
-  constexpr int ANGLES = kHalfLayout ? VEC : VEC / 2;
-  float c[ANGLES], sn[ANGLES];
-  const int pos = a.positions[long(b) * a.tokens + t];
-  const bool known = pos >= 0 && pos < a.table;
-  const int i0 = kHalfLayout ? (second ? d0 - a.half : d0) : d0 / 2;
-#pragma unroll
-  for (int i = 0; i < ANGLES; ++i) {
-    const bool turns = i0 + i < a.half;
-    const long at = long(known ? pos : 0) * a.half + (turns ? i0 + i : 0);
-    const float cv = a.cos[at], sv = a.sin[at];
-    c[i] = !turns ? 1.f : known ? cv : NAN;
-    sn[i] = !turns ? 0.f : known ? sv : NAN;
-  }
   const auto gains = [&](const void* gain, int d, float (&g)[VEC]) {
+    if (!gain) {
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) g[e] = gain ? gain_at(a, gain, d + e, T{}) : 1.f;
+      for (int e = 0; e < VEC; ++e) g[e] = 1.f;
+    } else if (a.gain_f32) {
+      load_values<float, VEC>(static_cast<const float*>(gain) + d, g);
+    } else {
+      load_values<T, VEC>(static_cast<const T*>(gain) + d, g);
+    }
   };
   float gq[VEC], gk[VEC], pq[VEC], pk[VEC];
   gains(a.q_gain, d0, gq);
@@ -149,64 +157,99 @@ __global__ __launch_bounds__(256) void rotate_rows_kernel(const RotateArgs a, in
     gains(a.k_gain, d1, pk);
   }
 
-  const int step = gh * int(gridDim.y);
-  for (int h0 = int(blockIdx.y) * gh; h0 < heads; h0 += kRows * step) {  // uniform over the workgroup
-    uint4 x[kRows], xp[kRows];
-    RotateRow row[kRows];
+  const unsigned tokens = unsigned(a.batch) * unsigned(a.tokens);
+  const int step = gh * int(gridDim.y), first = int(blockIdx.y) * gh;
+  for (unsigned tok0 = blockIdx.x * unsigned(per_block); tok0 < tokens; tok0 += gridDim.x * unsigned(per_block)) {
+    const unsigned token = tok0 + unsigned(group >> gh_log2);
+    const bool on = token < tokens;  // the lanes of the last workgroup's missing tokens repeat the last one
+    const unsigned at = on ? token : tokens - 1;
+    const int b = int(at / unsigned(a.tokens)), t = int(at - unsigned(b) * unsigned(a.tokens));
+    const bool used = !a.counts || t < a.counts[b];
+    const long slot = a.start ? long(a.start[b]) + t : t;
+    const bool kv_store = on && (!a.start || (used && slot >= 0 && slot < a.slots));
+    const int pos = a.positions[at];
+    const bool known = pos >= 0 && pos < a.table;
+    float c[ANGLES], sn[ANGLES];
+    const long angle = long(known ? pos : 0) * a.half + i0;
+    load_values<float, ANGLES>(a.cos + angle, c);
+    load_values<float, ANGLES>(a.sin + angle, sn);
 #pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-      const int h = h0 + r * step + (group & (gh - 1));
-      row[r] = rotate_row<T>(a, b, t, min(h, heads - 1));
-      row[r].store = row[r].store && on && h < heads;
-      x[r] = load16(static_cast<const T*>(row[r].in) + d0);
-      if constexpr (kHalfLayout) xp[r] = load16(static_cast<const T*>(row[r].in) + d1);
+    for (int i = 0; i < ANGLES; ++i) {
+      c[i] = !turned ? 1.f : known ? c[i] : NAN;
+      sn[i] = !turned ? 0.f : known ? sn[i] : NAN;
     }
+    // Where head 0 of the launch's order (q, k, v) would be in each tensor.
+    const T* in[3];
+    T* out[3];
+    const int before[3] = {0, a.q_heads, a.q_heads + a.kv_heads};
 #pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-      float v[VEC], w[VEC];
-      unpack16<T>(x[r], v);
-      if constexpr (kHalfLayout) unpack16<T>(xp[r], w);
-      const bool is_q = row[r].gain == a.q_gain;
-      if (norm) {
-        float sq = 0.f;
+    for (int w = 0; w < 3; ++w) {
+      in[w] = static_cast<const T*>(w == 0 ? a.q : w == 1 ? a.k : a.v) + b * a.st[w][0] + t * a.st[w][2] -
+              before[w] * a.st[w][1];
+      out[w] = static_cast<T*>(w == 0 ? a.q_out : w == 1 ? a.k_out : a.v_out) + b * a.st[3 + w][0] +
+               (w == 0 ? t : slot) * a.st[3 + w][2] - before[w] * a.st[3 + w][1];
+    }
+
+    for (int h0 = first; h0 < heads; h0 += kRows * step) {  // uniform over the workgroup
+      uint4 x[kRows], xp[kRows];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) sq = fmaf(v[e], v[e], sq);
-        const float scale = 1.f / sqrtf(group_sum<LPR>(sq) / float(D) + a.eps);
-        if (row[r].gain) {
+      for (int r = 0; r < kRows; ++r) {
+        const int h = min(h0 + r * step + (group & (gh - 1)), heads - 1);
+        const int w = h < before[1] ? 0 : h < before[2] ? 1 : 2;
+        const T* p = (w == 0 ? in[0] : w == 1 ? in[1] : in[2]) + h * (w == 0 ? a.st[0][1] : w == 1 ? a.st[1][1] : a.st[2][1]);
+        x[r] = load16(p + d0);
+        if constexpr (kHalfLayout) xp[r] = load16(p + d1);
+      }
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+        const int h = h0 + r * step + (group & (gh - 1));
+        const int w = h < before[1] ? 0 : h < before[2] ? 1 : 2;
+        float v[VEC], o[VEC];
+        unpack16<T>(x[r], v);
+        if constexpr (kHalfLayout) unpack16<T>(xp[r], o);
+        const bool is_q = w == 0;
+        if (norm) {
+          float sq = 0.f;
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) sq = fmaf(v[e], v[e], sq);
+          const float rms = 1.f / sqrtf(group_sum<LPR>(sq) / float(D) + a.eps);
+          const float scale = (is_q ? a.q_gain : a.k_gain) ? rms : 1.f;
 #pragma unroll
           for (int e = 0; e < VEC; ++e) {
             v[e] *= scale * (is_q ? gq[e] : gk[e]);
-            if constexpr (kHalfLayout) w[e] *= scale * (is_q ? pq[e] : pk[e]);
+            if constexpr (kHalfLayout) o[e] *= scale * (is_q ? pq[e] : pk[e]);
           }
         }
-      }
-      if (row[r].turn && turned) {
-        if constexpr (kHalfLayout) {
+        if (turned) {
+          if constexpr (kHalfLayout) {
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) v[e] = fmaf(second ? w[e] : -w[e], sn[e], v[e] * c[e]);
-        } else {
+            for (int e = 0; e < VEC; ++e) v[e] = fmaf(second ? o[e] : -o[e], sn[e], v[e] * c[e]);
+          } else {
 #pragma unroll
-          for (int e = 0; e < VEC; e += 2) {
-            const float u = v[e], o = v[e + 1];
-            v[e] = fmaf(-o, sn[e / 2], u * c[e / 2]);
-            v[e + 1] = fmaf(u, sn[e / 2], o * c[e / 2]);
+            for (int e = 0; e < VEC; e += 2) {
+              const float u = v[e], n = v[e + 1];
+              v[e] = fmaf(-n, sn[e / 2], u * c[e / 2]);
+              v[e + 1] = fmaf(u, sn[e / 2], n * c[e / 2]);
+            }
           }
         }
+        uint4 y;
+        if constexpr (std::is_same<T, float>::value)
+          y = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+        else
+          y = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+        if (w == 2) y = x[r];
+        if (!used) y = make_uint4(0u, 0u, 0u, 0u);
+        if (h < heads && (w == 0 ? on : kv_store)) {
+          T* p = (w == 0 ? out[0] : w == 1 ? out[1] : out[2]) + h * (w == 0 ? a.st[3][1] : w == 1 ? a.st[4][1] : a.st[5][1]);
+          *reinterpret_cast<uint4*>(p + d0) = y;
+        }
       }
-      if (!row[r].store) continue;
-      uint4 y;
-      if constexpr (std::is_same<T, float>::value)
-        y = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
-      else
-        y = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
-      if (!row[r].turn) y = x[r];
-      if (row[r].zero) y = make_uint4(0u, 0u, 0u, 0u);
-      *reinterpret_cast<uint4*>(static_cast<T*>(row[r].out) + d0) = y;
     }
   }
 }
 
-// Whether the rows come in 16-byte pieces, the paired ones too.
+// Whether the rows come in 16-byte pieces, the paired ones, the angles and the gains too.
 bool rotate_in_pieces(const RotateArgs& a, int es, bool half_layout) {
   const void* p[6] = {a.q, a.k, a.v, a.q_out, a.k_out, a.v_out};
   for (int i = 0; i < 6; ++i) {
@@ -214,7 +257,10 @@ bool rotate_in_pieces(const RotateArgs& a, int es, bool half_layout) {
     for (int j = 0; j < 3; ++j)
       if (p[i] && a.st[i][j] * es % 16) return false;
   }
-  return (!half_layout || a.half * es % 16 == 0) && long(a.batch) * a.tokens < (1L << 31);
+  const void* f[4] = {a.cos, a.sin, a.q_gain, a.k_gain};
+  for (const void* g : f)
+    if (reinterpret_cast<uintptr_t>(g) % 16) return false;
+  return (half_layout ? a.half : 2 * a.half) * es % 16 == 0;
 }
 
 template <typename T, int D>
@@ -227,7 +273,8 @@ int launch_rotate_rows(const RotateArgs& a, int heads, bool half_layout, hipStre
   // Few tokens: their heads on several workgroups, until there are about two for each CU.
   const int rounds = (heads + (1 << gh_log2) - 1) >> gh_log2;
   const int share = int(std::max(1L, std::min(long(rounds), 512 / blocks)));
-  const dim3 grid{unsigned(blocks), unsigned(share), 1u};
+  // Many tokens: eight workgroups to a CU, which walk them.
+  const dim3 grid{unsigned(std::min(blocks, 2048L)), unsigned(share), 1u};
   const bool norm = a.q_gain || a.k_gain;
   if (half_layout)
     hipLaunchKernelGGL((rotate_rows_kernel<T, D, true>), grid, dim3(256), 0, stream, a, heads, gh_log2, norm);
@@ -279,22 +326,22 @@ __global__ __launch_bounds__(256) void accept_kernel(const AcceptArgs a) {
     return;
   }
   unsigned char* rows = static_cast<unsigned char*>(blockIdx.y ? a.v : a.k);
-  const long* st = blockIdx.y ? a.vs : a.ks;
-  rows += (b * st[0] + hk * st[1]) * a.elem_bytes;
+  const long stride = (blockIdx.y ? a.vs[2] : a.ks[2]) * a.elem_bytes;
+  rows += (blockIdx.y ? b * a.vs[0] + hk * a.vs[1] : b * a.ks[0] + hk * a.ks[1]) * a.elem_bytes;
   constexpr int kPieces = kMaxPath * 32 / 256;  // of 16 bytes, per thread: 128 rows of 512 bytes
   uint4 held[kPieces];
 #pragma unroll
   for (int i = 0; i < kPieces; ++i) {
     const int at = int(threadIdx.x) + 256 * i, j = at / a.row_pieces;
     const int from = j < count ? source(j) : -1;
-    if (from >= 0) held[i] = load16(rows + from * st[2] * a.elem_bytes + 16 * (at - j * a.row_pieces));
+    if (from >= 0) held[i] = load16(rows + from * stride + 16 * (at - j * a.row_pieces));
   }
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kPieces; ++i) {
     const int at = int(threadIdx.x) + 256 * i, j = at / a.row_pieces;
     if (j < count && source(j) >= 0)
-      *reinterpret_cast<uint4*>(rows + (len + j) * st[2] * a.elem_bytes + 16 * (at - j * a.row_pieces)) = held[i];
+      *reinterpret_cast<uint4*>(rows + (len + j) * stride + 16 * (at - j * a.row_pieces)) = held[i];
   }
 }
 
@@ -473,15 +520,15 @@ __global__ __launch_bounds__(256) void compact_rows_kernel(const CompactArgs a) 
   const int group = int(blockIdx.x) / a.blocks, part = int(blockIdx.x) - group * a.blocks;
   const int b = group / a.kv_heads, hk = group - b * a.kv_heads;
   unsigned char* rows = static_cast<unsigned char*>(blockIdx.y ? a.v : a.k);
-  const long* st = blockIdx.y ? a.vs : a.ks;
-  rows += (b * st[0] + hk * st[1]) * a.elem_bytes;
+  const long stride = (blockIdx.y ? a.vs[2] : a.ks[2]) * a.elem_bytes;
+  rows += (blockIdx.y ? b * a.vs[0] + hk * a.vs[1] : b * a.ks[0] + hk * a.ks[1]) * a.elem_bytes;
   const int lanes = a.row_pieces, per = 256 / lanes;  // rows of a pass
   const int piece = int(threadIdx.x) % lanes;
   for (int i = part * per + int(threadIdx.x) / lanes; i < a.keep; i += a.blocks * per) {
     const int from = a.kept[long(group) * a.keep + i];
     if (from < a.keep || from >= a.cap) continue;
-    *reinterpret_cast<uint4*>(rows + i * st[2] * a.elem_bytes + 16 * piece) =
-        load16(rows + from * st[2] * a.elem_bytes + 16 * piece);
+    *reinterpret_cast<uint4*>(rows + i * stride + 16 * piece) =
+        load16(rows + from * stride + 16 * piece);
   }
 }
 // Weights and positions by slot; the weights of slots from keep on are cleared once all have moved.
@@ -547,7 +594,7 @@ extern "C" int sfl_rotate(const void* q, const void* k, const void* v, const int
   a.table = table, a.slots = slots, a.gain_f32 = gain_dtype == SFL_DTYPE_F32, a.eps = eps;
   const int heads = q_heads + kv_heads * (v ? 2 : 1);
   const long rows = long(batch) * tokens * heads;
-  if ((rows + 3) / 4 > 0x7fffffffL) return set_error(SFL_ERR_UNSUPPORTED, "%s: too many rows", what);
+  if (rows > 0x7fffffffL) return set_error(SFL_ERR_UNSUPPORTED, "%s: too many rows", what);
   const auto run = [&](auto t) {
     using T = decltype(t);
     if (rotate_in_pieces(a, es, half_layout)) {
@@ -561,9 +608,9 @@ extern "C" int sfl_rotate(const void* q, const void* k, const void* v, const int
     }
     const dim3 grid(unsigned((rows + 3) / 4));
     if (half_layout)
-      hipLaunchKernelGGL((rotate_any_kernel<T, true>), grid, dim3(256), 0, static_cast<hipStream_t>(stream), a, head_dim, rows, heads);
+      hipLaunchKernelGGL((rotate_any_kernel<T, true>), grid, dim3(256), 0, static_cast<hipStream_t>(stream), a, head_dim, unsigned(rows), unsigned(heads));
     else
-      hipLaunchKernelGGL((rotate_any_kernel<T, false>), grid, dim3(256), 0, static_cast<hipStream_t>(stream), a, head_dim, rows, heads);
+      hipLaunchKernelGGL((rotate_any_kernel<T, false>), grid, dim3(256), 0, static_cast<hipStream_t>(stream), a, head_dim, unsigned(rows), unsigned(heads));
     return check_launch(what);
   };
   if (dtype == SFL_DTYPE_F32) return run(float{});
