@@ -11,9 +11,11 @@
 // The G query heads that share a KV head, times the T drafts, are one block of
 // R = T G query rows (row r = t G + g) over the same keys, so a key is read once
 // for all of them and the products are matrix products: 16 rows to a tile.
+#include <algorithm>
 #include <type_traits>
 
 #include "attn_mfma.hpp"
+#include "lds_dma.hpp"
 
 namespace sfl {
 namespace {
@@ -38,14 +40,14 @@ struct TreeArgs {
   float cs;  // scale * log2(e): scores are kept in base 2
 };
 
-// What a sequence has: committed keys, drafts in use, keys in all (inside the cache).
+// What a sequence (the same for a whole wave) has: committed keys, drafts in use, keys in all inside the cache.
 struct TreeRow {
   int len, count, total;
 };
 __device__ __forceinline__ TreeRow tree_row(const int32_t* lengths, const int32_t* counts, int b, int cap, int tokens) {
   TreeRow r;
-  r.len = min(max(lengths[b], 0), cap);
-  r.count = counts ? min(max(counts[b], 0), tokens) : tokens;
+  r.len = min(max(__builtin_amdgcn_readfirstlane(lengths[b]), 0), cap);
+  r.count = counts ? min(max(__builtin_amdgcn_readfirstlane(counts[b]), 0), tokens) : tokens;
   r.total = min(r.len + r.count, cap);
   return r;
 }
@@ -54,7 +56,7 @@ __device__ __forceinline__ TreeRow tree_row(const int32_t* lengths, const int32_
 // shared evenly among the splits whatever its length.
 __device__ __forceinline__ int split_chunk(int total, int splits) {
   constexpr int kRound = kTreeTile * kTreeWaves;
-  return ((total + splits - 1) / splits + kRound - 1) / kRound * kRound;
+  return (__builtin_amdgcn_readfirstlane((total + splits - 1) / splits) + kRound - 1) / kRound * kRound;
 }
 
 __device__ __forceinline__ bool draft_sees(const TreeArgs& a, int b, const TreeRow& row, int t, int key) {
@@ -130,6 +132,10 @@ struct TreeOps {
     if constexpr (std::is_same<T, bf16_t>::value) return __uint_as_float(bits << 16);
     return f16_bits_to_f32(uint16_t(bits));
   }
+  static __device__ __forceinline__ void set_one(uint32_t (&w)[kWords], int f) {
+    if constexpr (kF32) w[f] = 0x3f800000u;
+    else w[f / 2] |= (std::is_same<T, bf16_t>::value ? 0x3f80u : 0x3c00u) << (f & 1 ? 16 : 0);
+  }
   static __device__ __forceinline__ void zero_value(uint32_t (&w)[kWords], int f) {
     if constexpr (kF32) w[f] = 0u;
     else w[f / 2] &= (f & 1) ? 0x0000ffffu : 0xffff0000u;
@@ -162,34 +168,21 @@ struct TreeOps {
   }
 };
 
-// A draft that does not see a key takes nothing from it, also where the key's
-// value is infinite or NaN, which a product with a probability of 0 would spread
-// over every row of the MFMA tile. Tiles with drafts in them take such values
-// out of the operand and add them here, row by row, to those that see the key.
-template <typename T, int D, int RT>
-__device__ __noinline__ void add_nonfinite(const uint32_t (&v)[8][TreeOps<T, D>::kWords], const float (&p)[RT][2][4],
-                                           uint32_t sees, f32x4 (&acc)[RT][TreeOps<T, D>::kVec]) {
-  using O = TreeOps<T, D>;
-  const int lane = threadIdx.x % kWave, g = lane / 16, n = lane % 16;
-  for (int j = 0; j < 8; ++j) {
-    for (int f = 0; f < O::kVec; ++f) {
-      const float mine = O::v_value(v[j], f);
-      const bool bad = !(fabsf(mine) < INFINITY);
-      if (!__ballot(bad)) continue;
-      for (int src = 0; src < 4; ++src) {  // the lane group that holds the key
-        for (int i = 0; i < 4; ++i) {
-          const float value = __shfl(mine, 16 * src + 4 * g + i);
-          const bool add = !(fabsf(value) < INFINITY);
-          for (int rt = 0; rt < RT; ++rt) {
-            const float pv = __shfl(p[rt][j / 4][j % 4], 16 * src + n);
-            const uint32_t seen = __shfl(int(sees), 16 * src + n);
-            if (add && (seen >> (8 * rt + j) & 1u)) acc[rt][f][i] += pv * value;
-          }
-        }
-      }
-    }
-  }
+// A draft that does not see a key takes nothing from it, also where the key's value
+// is infinite or NaN, which a product with a probability of 0 would spread over
+// every row of the MFMA tile. Tiles with drafts in them therefore take such values
+// out of the products; where there are any, products of 0s and 1s say which rows
+// reach one (by kind), and those rows get it added:
+//   0: +inf times p > 0    1: -inf times p > 0    2: NaN    3: an infinity times p = 0
+constexpr int kKinds = 4;
+__device__ __forceinline__ float kind_adds(int kind) { return kind == 0 ? INFINITY : kind == 1 ? -INFINITY : NAN; }
+__device__ __forceinline__ bool kind_has(int kind, float v) {
+  return kind == 0 ? v == INFINITY : kind == 1 ? v == -INFINITY : kind == 2 ? v != v : fabsf(v) == INFINITY;
 }
+__device__ __forceinline__ float kind_takes(int kind, bool sees, float p) {
+  return sees && (kind == 2 || (kind == 3 ? p == 0.f : p > 0.f)) ? 1.f : 0.f;
+}
+__device__ __forceinline__ bool finite(float v) { return fabsf(v) < INFINITY; }
 
 // Workgroup -> (KV head of a sequence, split, row block). Workgroups go to the 8
 // XCDs in turn; the row blocks that read the same keys take consecutive places
@@ -200,12 +193,339 @@ struct TreeBlock {
 __device__ __forceinline__ TreeBlock tree_block(const TreeArgs& a) {
   const int work = a.groups * a.splits;
   const int x = int(blockIdx.x) % kXcds, y = int(blockIdx.x) / kXcds;
-  const int unit = (y / a.row_blocks) * kXcds + x;
+  // (Quotients of scalars are formed on the vector unit; readfirstlane takes them back.)
+  const int q = __builtin_amdgcn_readfirstlane(y / a.row_blocks), unit = q * kXcds + x;
   TreeBlock t;
-  t.rb = y % a.row_blocks;
-  t.group = unit < work ? unit / a.splits : -1;
+  t.rb = y - q * a.row_blocks;
+  t.group = unit < work ? __builtin_amdgcn_readfirstlane(unit / a.splits) : -1;
   t.split = unit - t.group * a.splits;
   return t;
+}
+
+// The 32-row form for 16-bit types and head dims 64 and 128: 32x32x16 MFMAs on
+// 32 keys x 32 query rows, S^T = K Q^T and O^T += V^T P^T as in the masked prefill
+// attention, keys and values staged in LDS by DMA (K rows swizzled for the operand
+// reads, V rows laid out for the transpose reads). WR of the 4 waves share a tile of
+// 32 keys, each with 32 query rows of its own, and the 4 / WR groups of waves take
+// tiles in turn. A key costs 4 D operations a row: with few rows the launch streams
+// the cache (WR = 1: the waves' tiles are their own, no barrier), with 128 rows to a
+// workgroup the products bound it, and a tile is read from memory once for all.
+template <int D, int WR>
+struct TileShape {
+  static constexpr int WK = kTreeWaves / WR;      // tiles of a round
+  static constexpr int NB = WR == 4 ? 4 : 2;      // rounds of tiles in LDS
+  static constexpr int SL = D / 8;                // 16-byte slots of a row
+  static constexpr int RPL = kWave / SL;          // rows one DMA load moves
+  static constexpr int NLD = kTreeTile / RPL;     // loads of a tile and operand
+  static constexpr int L = 2 * NLD / WR;          // a wave's loads of a round
+  static constexpr int kTiles = NB * WK * 2 * kTreeTile * SL * 16, kMerge = WK > 1 ? WK * 32 * WR * (D + 2) * 4 : 0;
+  static constexpr int kBytes = kTiles > kMerge ? kTiles : kMerge;
+  static constexpr int kGroups = kBytes > 80 * 1024 ? 1 : 2;  // workgroups a CU holds, at least
+};
+
+// One tile: scores, running maximum and sum, products with V. kMask: the tile holds
+// keys past the committed ones; sees: which of the lane's keys its row sees.
+template <typename T, int D, bool kMask>
+__device__ __forceinline__ void tile_step(const uint4 (*kt)[D / 8], const uint4 (*vt)[D / 8], const u32x4 (&q)[D / 16],
+                                          f32x16 (&acc)[D / 32], float& m, float& l, int c, int h, uint32_t sees,
+                                          bool bad, float cs, const unsigned (&vlane)[D / 32]) {
+  f32x16 s;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) s[j] = 0.f;
+#pragma unroll
+  for (int ks = 0; ks < D / 16; ++ks) {
+    const uint4 r = kt[c][(D / 16 * h + ks) ^ k_swizzle<D>(c)];
+    s = mfma32<T>(u32x4{r.x, r.y, r.z, r.w}, q[ks], s);
+  }
+  if constexpr (kMask) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) s[j] = sees >> j & 1u ? s[j] : -INFINITY;
+  }
+  float mx = fmaxf(s[0], s[1]);
+#pragma unroll
+  for (int j = 2; j < 16; j += 2) mx = fmaxf(fmaxf(mx, s[j]), s[j + 1]);
+  mx = fmaxf(mx, lane_xor(mx, 32));
+  const bool grow = mx * cs > m + kLazyMax;  // the lazy maximum, as below
+  if (__ballot(grow)) {
+    const float mn = grow ? mx * cs : m;
+    const float alpha = grow ? __builtin_amdgcn_exp2f(m - mn) : 1.f;
+    m = mn;
+    l *= alpha;
+#pragma unroll
+    for (int t = 0; t < D / 32; ++t) acc[t] *= alpha;
+  }
+  const unsigned vbase = lds_offset(&vt[0][0]);
+  const auto v_operand = [&](int s2, int t) {
+    const unsigned off = vbase + vlane[t] + 32u * D * unsigned(s2);
+    const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)(size_t)(off));
+    const i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)(size_t)(off + 16u * D));
+    const uint2 a = __builtin_bit_cast(uint2, lo), b = __builtin_bit_cast(uint2, hi);
+    return u32x4{a.x, a.y, b.x, b.y};
+  };
+  const float ms = m == -INFINITY ? 0.f : m;
+  float p[16], sum[2] = {0.f, 0.f};
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    p[j] = __builtin_amdgcn_exp2f(fmaf(s[j], cs, -ms));
+    sum[j & 1] += p[j];
+  }
+  l += sum[0] + sum[1];
+  // Probabilities in the type of V for the products, half a step each and of either
+  // sign; l sums them unrounded.
+  const auto pack8 = [](const float* x) {
+    return u32x4{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7])};
+  };
+  u32x4 pk[2] = {pack8(p), pack8(p + 8)};
+  // Each 16-bit value of an operand through f(bits) -> bits.
+  const auto each = [](u32x4 w, auto&& f) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = f(w[e] & 0xffffu) | f(w[e] >> 16) << 16;
+    return w;
+  };
+  constexpr uint32_t kExp = std::is_same<T, bf16_t>::value ? 0x7f80u : 0x7c00u;
+  constexpr uint32_t kOne = std::is_same<T, bf16_t>::value ? 0x3f80u : 0x3c00u;
+#pragma unroll
+  for (int s2 = 0; s2 < 2; ++s2) {
+#pragma unroll
+    for (int t = 0; t < D / 32; ++t) {
+      u32x4 v = v_operand(s2, t);
+      if constexpr (kMask) {
+        if (bad) v = each(v, [](uint32_t x) { return (x & kExp) == kExp ? 0u : x; });
+      }
+      acc[t] = mfma32<T>(v, pk[s2], acc[t]);
+    }
+  }
+  if constexpr (kMask) {
+    if (!bad) return;
+#pragma unroll 1
+    for (int kind = 0; kind < kKinds; ++kind) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) s[j] = kind_takes(kind, sees >> j & 1u, p[j]);
+      float x[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) x[j] = s[j];
+      const u32x4 takes[2] = {pack8(x), pack8(x + 8)};
+#pragma unroll
+      for (int t = 0; t < D / 32; ++t) {
+        f32x16 hit;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) hit[j] = 0.f;
+#pragma unroll
+        for (int s2 = 0; s2 < 2; ++s2)
+          hit = mfma32<T>(each(v_operand(s2, t), [&](uint32_t b) {
+                            const bool top = (b & kExp) == kExp, inf = top && !(b & 0x7fffu & ~kExp), neg = b & 0x8000u;
+                            return (kind == 0 ? inf && !neg : kind == 1 ? inf && neg : kind == 2 ? top && !inf : inf) ? kOne : 0u;
+                          }), takes[s2], hit);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) acc[t][j] += hit[j] > 0.f ? kind_adds(kind) : 0.f;
+      }
+    }
+  }
+}
+
+template <typename T, int D, int WR>
+__global__ __launch_bounds__(kTreeWaves * kWave, (TileShape<D, WR>::kGroups)) void tree_tile_kernel(const TreeArgs a) {
+  using S = TileShape<D, WR>;
+  constexpr int WK = S::WK, NB = S::NB, SL = S::SL, RPL = S::RPL, BT = kTreeTile, BK = BT * WK;
+  __shared__ __align__(16) unsigned char lds[S::kBytes];
+  typedef uint4 Tile[BT][SL];
+  Tile* tiles = reinterpret_cast<Tile*>(lds);  // [buffer][tile of the round][K, V]
+  const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave);
+  const int lane = threadIdx.x % kWave, c = lane % 32, h = lane / 32;
+  const int wk = wave / WR, wr = wave % WR;
+  const TreeBlock blk = tree_block(a);
+  if (blk.group < 0) return;
+  const int b = __builtin_amdgcn_readfirstlane(blk.group / a.kv_heads), hk = blk.group - b * a.kv_heads;
+  const TreeRow row = tree_row(a.lengths, a.counts, b, a.cap, a.tokens);
+  const int G = 1 << a.group_log2, rows = a.tokens << a.group_log2, used = row.count << a.group_log2;
+  const int block0 = blk.rb * 32 * WR, row0 = block0 + 32 * wr;
+  const int chunk = split_chunk(row.total, a.splits);
+  const int begin = blk.split * chunk, end = min(row.total, begin + chunk);
+  if (a.splits > 1 && (begin >= end || block0 >= used)) return;  // the merge does not read these
+
+  const int r = min(row0 + c, rows - 1);  // rows past the last repeat it and are not stored
+  const int draft = r >> a.group_log2;
+  u32x4 q[D / 16];
+  {
+    const T* qp = static_cast<const T*>(a.q) + b * a.qs[0] + long((hk << a.group_log2) + (r & (G - 1))) * a.qs[1] +
+                  draft * a.qs[2] + D / 2 * h;
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) q[ks] = *reinterpret_cast<const u32x4*>(qp + 8 * ks);
+    // Landed before the tiles' loads are issued: the compiler would wait for them where
+    // they are used first, in the loop, and there for every tile in flight with them.
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) asm volatile("" : "+v"(q[ks]));
+  }
+
+  // The split's keys as buffers whose range ends with its last key: rows past it read as zeros.
+  const unsigned krow = unsigned(a.ks[2]) * 2u, vrow = unsigned(a.vs[2]) * 2u;
+  const int keys = __builtin_amdgcn_readfirstlane(block0 < used ? max(end - begin, 0) : 0);
+  const auto scalar = [](i32x4_t r) {  // 64-bit products are formed on the vector unit, too
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r[e] = __builtin_amdgcn_readfirstlane(r[e]);
+    return r;
+  };
+  const i32x4_t krsrc = scalar(buffer_rsrc(static_cast<const T*>(a.k) + b * a.ks[0] + hk * a.ks[1] + long(begin) * a.ks[2],
+                                           keys ? unsigned(keys - 1) * krow + 2u * D : 0u));
+  const i32x4_t vrsrc = scalar(buffer_rsrc(static_cast<const T*>(a.v) + b * a.vs[0] + hk * a.vs[1] + long(begin) * a.vs[2],
+                                           keys ? unsigned(keys - 1) * vrow + 2u * D : 0u));
+  // A wave's share of its tile's loads (load j moves rows RPL j .. RPL j + RPL - 1):
+  // all of K and V where the tile is its own, else a part of K or a part of V.
+  const int lrr = lane / SL, lpp = lane % SL;
+  const auto slot = [&](bool values, int j) {  // 16-byte slot that lands in physical slot lpp of row RPL j + lrr
+    return values ? 2u * ((unsigned(lpp) >> 1) ^ (unsigned(lrr) & 3u)) + (unsigned(lpp) & 1u)
+                  : unsigned(lpp ^ k_swizzle<D>(RPL * j + lrr));
+  };
+  const auto offset = [&](bool values, unsigned stride, int j) {
+    return unsigned(RPL * j + lrr) * stride + 16u * slot(values, j);
+  };
+  constexpr int kOwn = WR == 1 ? S::NLD : 1;
+  unsigned koff[kOwn], off[S::L];  // V's, or those of the wave's part
+  const bool values = WR == 1 || wr >= WR / 2;
+  const i32x4_t mine = scalar(values ? vrsrc : krsrc);
+  const unsigned mrow = values ? vrow : krow;
+  constexpr int kLoads = WR == 1 ? S::NLD : S::L;
+  const int j0 = WR == 1 ? 0 : (wr % std::max(WR / 2, 1)) * S::L;
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) off[i] = offset(values, mrow, j0 + i);
+  if constexpr (WR == 1) {
+#pragma unroll
+    for (int i = 0; i < S::NLD; ++i) koff[i] = offset(false, krow, i);
+  }
+  const auto issue = [&](int round) {
+    Tile* to = tiles + ((round % NB) * WK + wk) * 2;
+    const unsigned first = unsigned(round * BK + wk * BT);
+    const unsigned kfirst = first * krow, mfirst = first * mrow;
+    const unsigned at = lds_offset(&to[values][RPL * j0][0]);
+    if constexpr (WR == 1) {
+      const unsigned kat = lds_offset(&to[0][0][0]);
+#pragma unroll
+      for (int i = 0; i < S::NLD; ++i) lds_load16(krsrc, kat + 1024u * unsigned(i), koff[i], kfirst);
+    }
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) lds_load16(mine, at + 1024u * unsigned(i), off[i], mfirst);
+  };
+  unsigned vlane[D / 32];
+#pragma unroll
+  for (int t = 0; t < D / 32; ++t) vlane[t] = vt_lane_offset<D>(lane, t);
+
+  float m = -INFINITY, l = 0.f;
+  f32x16 acc[D / 32];
+#pragma unroll
+  for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) acc[t][j] = 0.f;
+
+  const int rounds = (keys + BK - 1) / BK;
+  for (int i = 0; i < NB - 1 && i < rounds; ++i) issue(i);
+  const auto arrive = [&](int i) {
+    if constexpr (WR == 1) {
+      // The tiles are the wave's own: it refills the one it has read and waits for this one.
+      wait_lds_reads();
+      if (i + 1 < rounds) issue(i + 1);
+      wait_younger<1, S::L>(min(1, rounds - 1 - i));
+    } else {
+      // Every wave's part of this round has landed, and everyone has read the round
+      // before, whose place the load after the barrier takes.
+      wait_younger<NB - 2, S::L>(min(NB - 2, rounds - 1 - i));
+      wait_lds_reads();
+      __syncthreads();
+      if (i + NB - 1 < rounds) issue(i + NB - 1);
+    }
+    return tiles + ((i % NB) * WK + wk) * 2;
+  };
+  const bool busy = row0 < used;  // uniform over the wave
+  // Rounds of committed keys alone, then those with drafts or the end in them (two
+  // loops: with a choice inside one, the accumulators are copied in every round).
+  const int full = min(rounds, max(0, min(row.len, end) - begin) / BK);
+  for (int i = 0; i < full; ++i) {
+    const Tile* tile = arrive(i);
+    if (busy) tile_step<T, D, false>(tile[0], tile[1], q, acc, m, l, c, h, 0u, false, a.cs, vlane);
+  }
+  for (int i = full; i < rounds; ++i) {
+    const Tile* tile = arrive(i);
+    const int t0 = begin + i * BK + wk * BT;
+    if (!busy || t0 >= end) continue;
+    uint32_t sees = 0;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const int key = t0 + 8 * (j / 4) + 4 * h + j % 4;
+      sees |= uint32_t(key < end && draft_sees(a, b, row, draft, key)) << j;
+    }
+    bool bad = false;
+    constexpr uint32_t kExp = std::is_same<T, bf16_t>::value ? 0x7f80u : 0x7c00u;
+#pragma unroll
+    for (int x = 0; x < BT * SL / kWave; ++x) {
+      const uint4 w = (&tile[1][0][0])[x * kWave + lane];
+      const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) bad |= (u[e] & kExp) == kExp || (u[e] >> 16 & kExp) == kExp;
+    }
+    tile_step<T, D, true>(tile[0], tile[1], q, acc, m, l, c, h, sees, __ballot(bad) != 0, a.cs, vlane);
+  }
+  l += lane_xor(l, 32);
+
+  const auto store = [&](int at, int d0, const float(&num)[4], float top, float den) {  // four dims of query row at
+    if (a.splits > 1) {
+      const long part = (long(blk.group) * a.splits + blk.split) * rows + at;
+      *reinterpret_cast<float4*>(a.pout + part * D + d0) = make_float4(num[0], num[1], num[2], num[3]);
+      if (d0 == 0) {
+        a.pmax[part] = top;
+        a.psum[part] = den;
+      }
+      return;
+    }
+    const int t = at >> a.group_log2, head = (hk << a.group_log2) + (at & (G - 1));
+    const bool empty = t >= row.count || den == 0.f;
+    const float inv = empty ? 0.f : 1.f / den;
+    uint2 w = make_uint2(pack2<T>(num[0] * inv, num[1] * inv), pack2<T>(num[2] * inv, num[3] * inv));
+    if (empty) w = make_uint2(0u, 0u);
+    *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + b * a.os[0] + head * a.os[1] + t * a.os[2] + d0) = w;
+    if (d0 == 0)
+      a.lse[(long(b) * a.kv_heads * G + head) * a.tokens + t] = empty ? -INFINITY : (top + __builtin_log2f(den)) * kLn2;
+  };
+  if constexpr (WK == 1) {
+    if (row0 + c < rows) {
+#pragma unroll
+      for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+        for (int j = 0; j < 16; j += 4) {
+          const float num[4] = {acc[t][j], acc[t][j + 1], acc[t][j + 2], acc[t][j + 3]};
+          store(row0 + c, 32 * t + 2 * j + 4 * h, num, m, l);
+        }
+    }
+  } else {
+    // The groups' states through LDS, then four dims of a row by each thread.
+    typedef float MergeRow[32 * WR][D + 2];
+    MergeRow* sm = reinterpret_cast<MergeRow*>(lds);
+    __syncthreads();  // everyone is done with the tiles
+#pragma unroll
+    for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) sm[wk][32 * wr + c][32 * t + 8 * (j / 4) + 4 * h + j % 4] = acc[t][j];
+    if (h == 0) {
+      sm[wk][32 * wr + c][D] = m;
+      sm[wk][32 * wr + c][D + 1] = l;
+    }
+    __syncthreads();
+    for (int x = threadIdx.x; x < 32 * WR * D / 4; x += kTreeWaves * kWave) {
+      const int at = x / (D / 4), d0 = 4 * (x % (D / 4));
+      if (block0 + at >= rows) break;
+      float top = sm[0][at][D];
+#pragma unroll
+      for (int w = 1; w < WK; ++w) top = fmaxf(top, sm[w][at][D]);
+      float den = 0.f, num[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < WK; ++w) {
+        const float mw = sm[w][at][D];
+        const float f = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - top);
+        den = fmaf(f, sm[w][at][D + 1], den);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) num[e] = fmaf(f, sm[w][at][d0 + e], num[e]);
+      }
+      store(block0 + at, d0, num, top, den);
+    }
+  }
 }
 
 template <typename T, int D, int RT>
@@ -213,13 +533,13 @@ __global__ __launch_bounds__(kTreeWaves * kWave) void tree_attention_kernel(cons
   using O = TreeOps<T, D>;
   constexpr int W = kTreeWaves, BT = kTreeTile, VEC = O::kVec;
   constexpr int kState = RT * (4 * VEC + 2);  // a lane's registers of a wave's state
-  static_assert(RT <= 4, "add_nonfinite's bits");
+  static_assert(RT <= 4, "bits of sees");
   __shared__ float sm[2][kState][kWave];
   const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave);
   const int lane = threadIdx.x % kWave, g = lane / 16, n = lane % 16;
   const TreeBlock blk = tree_block(a);
   if (blk.group < 0) return;
-  const int b = blk.group / a.kv_heads, hk = blk.group - b * a.kv_heads;
+  const int b = __builtin_amdgcn_readfirstlane(blk.group / a.kv_heads), hk = blk.group - b * a.kv_heads;
   const TreeRow row = tree_row(a.lengths, a.counts, b, a.cap, a.tokens);
   const int G = 1 << a.group_log2, rows = a.tokens << a.group_log2;
   const int row0 = blk.rb * 16 * RT;
@@ -311,33 +631,39 @@ __global__ __launch_bounds__(kTreeWaves * kWave) void tree_attention_kernel(cons
 #pragma unroll
         for (int j = 0; j < 8; ++j)
 #pragma unroll
-          for (int f = 0; f < VEC; ++f) bad |= !(fabsf(O::v_value(v[j], f)) < INFINITY);
+          for (int f = 0; f < VEC; ++f) bad |= !finite(O::v_value(v[j], f));
         if (__ballot(bad)) {
-          // Copies, so that the call leaves the state itself in registers.
-          uint32_t vt[8][O::kWords];
-          float pt[RT][2][4];
-          f32x4 at[RT][VEC];
+#pragma unroll 1
+          for (int kind = 0; kind < kKinds; ++kind) {
+            uint32_t has[8][O::kWords];
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
+            for (int j = 0; j < 8; ++j) {
 #pragma unroll
-            for (int w = 0; w < O::kWords; ++w) vt[j][w] = v[j][w];
+              for (int w = 0; w < O::kWords; ++w) has[j][w] = 0u;
 #pragma unroll
-          for (int rt = 0; rt < RT; ++rt) {
+              for (int f = 0; f < VEC; ++f)
+                if (kind_has(kind, O::v_value(v[j], f))) O::set_one(has[j], f);
+            }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) pt[rt][j / 4][j % 4] = p[rt][j / 4][j % 4];
+            for (int rt = 0; rt < RT; ++rt) {
+              float takes[2][4];
 #pragma unroll
-            for (int f = 0; f < VEC; ++f) at[rt][f] = acc[rt][f];
+              for (int j = 0; j < 8; ++j) takes[j / 4][j % 4] = kind_takes(kind, sees >> (8 * rt + j) & 1u, p[rt][j / 4][j % 4]);
+              f32x4 hit[VEC];
+#pragma unroll
+              for (int f = 0; f < VEC; ++f) hit[f] = f32x4{0.f, 0.f, 0.f, 0.f};
+              O::add_pv(has, takes, hit);
+#pragma unroll
+              for (int f = 0; f < VEC; ++f)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[rt][f][i] += hit[f][i] > 0.f ? kind_adds(kind) : 0.f;
+            }
           }
-          add_nonfinite<T, D, RT>(vt, pt, sees, at);
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-            for (int f = 0; f < VEC; ++f) acc[rt][f] = at[rt][f];
 #pragma unroll
           for (int j = 0; j < 8; ++j)
 #pragma unroll
             for (int f = 0; f < VEC; ++f)
-              if (!(fabsf(O::v_value(v[j], f)) < INFINITY)) O::zero_value(v[j], f);
+              if (!finite(O::v_value(v[j], f))) O::zero_value(v[j], f);
         }
       }
 #pragma unroll
@@ -521,13 +847,14 @@ __global__ __launch_bounds__(kTreeWaves * kWave) void tree_weights_kernel(const 
   }
 }
 
-template <typename T, int D, int RT>
-int launch_rows(TreeArgs& a, hipStream_t stream) {
+// The launch of `kernel` on row blocks of `block` rows, and the merge of its splits.
+template <typename T, int D>
+int launch_blocks(void (*kernel)(TreeArgs), int block, TreeArgs& a, hipStream_t stream) {
   const int rows = a.tokens << a.group_log2;
-  a.row_blocks = (rows + 16 * RT - 1) / (16 * RT);
+  a.row_blocks = (rows + block - 1) / block;
   const long units = (long(a.groups) * a.splits + kXcds - 1) / kXcds * kXcds;
   if (units * a.row_blocks > 0x7fffffffL) return set_error(SFL_ERR_UNSUPPORTED, "tree_attention: too many workgroups");
-  hipLaunchKernelGGL((tree_attention_kernel<T, D, RT>), dim3(unsigned(units * a.row_blocks)), dim3(kTreeWaves * kWave), 0, stream, a);
+  hipLaunchKernelGGL(kernel, dim3(unsigned(units * a.row_blocks)), dim3(kTreeWaves * kWave), 0, stream, a);
   if (int rc = check_launch("tree_attention")) return rc;
   if (a.splits == 1) return SFL_OK;
   const long merged = long(a.groups) * rows;
@@ -538,9 +865,20 @@ int launch_rows(TreeArgs& a, hipStream_t stream) {
 template <typename T, int D>
 int launch_tree(TreeArgs& a, hipStream_t stream) {
   const int rows = a.tokens << a.group_log2;
-  if (rows <= 16) return launch_rows<T, D, 1>(a, stream);
-  if (rows <= 32 || std::is_same<T, float>::value) return launch_rows<T, D, 2>(a, stream);
-  return launch_rows<T, D, std::is_same<T, float>::value ? 2 : 4>(a, stream);
+  constexpr bool kF32 = std::is_same<T, float>::value;
+  if constexpr (!kF32 && D >= 64) {
+    // Buffer offsets are 32 bits; caches of 2 GiB a head and more take the kernel below.
+    if (long(a.cap) * std::max(a.ks[2], a.vs[2]) * 2 < (1L << 31)) {
+      if (rows <= 32) return launch_blocks<T, D>(tree_tile_kernel<T, D, 1>, 32, a, stream);
+      if (rows <= 64) return launch_blocks<T, D>(tree_tile_kernel<T, D, 2>, 64, a, stream);
+      return launch_blocks<T, D>(tree_tile_kernel<T, D, 4>, 128, a, stream);
+    }
+    return launch_blocks<T, D>(tree_attention_kernel<T, D, 1>, 16, a, stream);
+  } else {
+    if (rows <= 16) return launch_blocks<T, D>(tree_attention_kernel<T, D, 1>, 16, a, stream);
+    if (kF32 || rows <= 32) return launch_blocks<T, D>(tree_attention_kernel<T, D, 2>, 32, a, stream);
+    return launch_blocks<T, D>(tree_attention_kernel<T, D, kF32 ? 2 : 4>, kF32 ? 32 : 64, a, stream);
+  }
 }
 
 template <typename T, int D>
