@@ -59,9 +59,12 @@ __device__ __forceinline__ int split_chunk(int total, int splits) {
   return (__builtin_amdgcn_readfirstlane((total + splits - 1) / splits) + kRound - 1) / kRound * kRound;
 }
 
+// Without branches (the mask is read for every key, from a clamped place): the loads
+// of a tile's keys go out together.
 __device__ __forceinline__ bool draft_sees(const TreeArgs& a, int b, const TreeRow& row, int t, int key) {
-  if (key < row.len) return true;
-  return key < row.total && a.mask[b * a.ms[0] + t * a.ms[1] + (key - row.len) * a.ms[2]] != 0;
+  const int j = min(max(key - row.len, 0), a.tokens - 1);
+  const bool on = a.mask[b * a.ms[0] + t * a.ms[1] + j * a.ms[2]] != 0;
+  return (key < row.len) | (on & (key < row.total));
 }
 
 // Operand registers of a wave's tile of 32 keys. MFMA tile h (0, 1) holds keys
@@ -132,10 +135,6 @@ struct TreeOps {
     if constexpr (std::is_same<T, bf16_t>::value) return __uint_as_float(bits << 16);
     return f16_bits_to_f32(uint16_t(bits));
   }
-  static __device__ __forceinline__ void set_one(uint32_t (&w)[kWords], int f) {
-    if constexpr (kF32) w[f] = 0x3f800000u;
-    else w[f / 2] |= (std::is_same<T, bf16_t>::value ? 0x3f80u : 0x3c00u) << (f & 1 ? 16 : 0);
-  }
   static __device__ __forceinline__ void zero_value(uint32_t (&w)[kWords], int f) {
     if constexpr (kF32) w[f] = 0u;
     else w[f / 2] &= (f & 1) ? 0x0000ffffu : 0xffff0000u;
@@ -168,21 +167,25 @@ struct TreeOps {
   }
 };
 
+__device__ __forceinline__ bool finite(float v) { return fabsf(v) < INFINITY; }
+
 // A draft that does not see a key takes nothing from it, also where the key's value
 // is infinite or NaN, which a product with a probability of 0 would spread over
-// every row of the MFMA tile. Tiles with drafts in them therefore take such values
-// out of the products; where there are any, products of 0s and 1s say which rows
-// reach one (by kind), and those rows get it added:
-//   0: +inf times p > 0    1: -inf times p > 0    2: NaN    3: an infinity times p = 0
-constexpr int kKinds = 4;
-__device__ __forceinline__ float kind_adds(int kind) { return kind == 0 ? INFINITY : kind == 1 ? -INFINITY : NAN; }
-__device__ __forceinline__ bool kind_has(int kind, float v) {
-  return kind == 0 ? v == INFINITY : kind == 1 ? v == -INFINITY : kind == 2 ? v != v : fabsf(v) == INFINITY;
+// every row of an MFMA tile. Tiles with drafts in them therefore lose such values
+// before the products, and where there were any, the wave adds them here, key by key
+// and row by row, to those that see them: add(p, value row) with p = exp2(s - m), of
+// which only the sign matters there. (Apart from the tiles' loop, whose registers
+// decide how many waves a SIMD holds.)
+template <typename T, int D, typename Add>
+__device__ __forceinline__ void add_nonfinite(const T* q, const T* k, const T* v, float m, float cs, bool sees, Add&& add) {
+  bool bad = false;
+  for (int d = int(threadIdx.x) % kWave; d < D; d += kWave) bad |= !finite(load_scalar<T>(v + d));
+  if (!__ballot(bad)) return;
+  float s = 0.f;
+#pragma unroll 1
+  for (int d = 0; d < D; ++d) s = fmaf(load_scalar<T>(q + d), load_scalar<T>(k + d), s);
+  if (sees) add(__builtin_amdgcn_exp2f(fmaf(s, cs, -m)), v);
 }
-__device__ __forceinline__ float kind_takes(int kind, bool sees, float p) {
-  return sees && (kind == 2 || (kind == 3 ? p == 0.f : p > 0.f)) ? 1.f : 0.f;
-}
-__device__ __forceinline__ bool finite(float v) { return fabsf(v) < INFINITY; }
 
 // Workgroup -> (KV head of a sequence, split, row block). Workgroups go to the 8
 // XCDs in turn; the row blocks that read the same keys take consecutive places
@@ -212,13 +215,14 @@ __device__ __forceinline__ TreeBlock tree_block(const TreeArgs& a) {
 // workgroup the products bound it, and a tile is read from memory once for all.
 template <int D, int WR>
 struct TileShape {
-  static constexpr int WK = kTreeWaves / WR;      // tiles of a round
-  static constexpr int NB = WR == 4 ? 4 : 2;      // rounds of tiles in LDS
+  static constexpr int WK = kTreeWaves / WR;      // tiles taken side by side
+  static constexpr int TP = WR == 4 ? 2 : 1;      // tiles a wave takes in a round (a barrier's worth)
+  static constexpr int NB = 2;                    // rounds of tiles in LDS
   static constexpr int SL = D / 8;                // 16-byte slots of a row
   static constexpr int RPL = kWave / SL;          // rows one DMA load moves
   static constexpr int NLD = kTreeTile / RPL;     // loads of a tile and operand
-  static constexpr int L = 2 * NLD / WR;          // a wave's loads of a round
-  static constexpr int kTiles = NB * WK * 2 * kTreeTile * SL * 16, kMerge = WK > 1 ? WK * 32 * WR * (D + 2) * 4 : 0;
+  static constexpr int L = 2 * NLD / WR;          // a wave's loads of a tile
+  static constexpr int kTiles = NB * WK * TP * 2 * kTreeTile * SL * 16, kMerge = WK > 1 ? WK * 32 * WR * (D + 2) * 4 : 0;
   static constexpr int kBytes = kTiles > kMerge ? kTiles : kMerge;
   static constexpr int kGroups = kBytes > 80 * 1024 ? 1 : 2;  // workgroups a CU holds, at least
 };
@@ -283,7 +287,6 @@ __device__ __forceinline__ void tile_step(const uint4 (*kt)[D / 8], const uint4 
     return w;
   };
   constexpr uint32_t kExp = std::is_same<T, bf16_t>::value ? 0x7f80u : 0x7c00u;
-  constexpr uint32_t kOne = std::is_same<T, bf16_t>::value ? 0x3f80u : 0x3c00u;
 #pragma unroll
   for (int s2 = 0; s2 < 2; ++s2) {
 #pragma unroll
@@ -295,41 +298,15 @@ __device__ __forceinline__ void tile_step(const uint4 (*kt)[D / 8], const uint4 
       acc[t] = mfma32<T>(v, pk[s2], acc[t]);
     }
   }
-  if constexpr (kMask) {
-    if (!bad) return;
-#pragma unroll 1
-    for (int kind = 0; kind < kKinds; ++kind) {
-#pragma unroll
-      for (int j = 0; j < 16; ++j) s[j] = kind_takes(kind, sees >> j & 1u, p[j]);
-      float x[16];
-#pragma unroll
-      for (int j = 0; j < 16; ++j) x[j] = s[j];
-      const u32x4 takes[2] = {pack8(x), pack8(x + 8)};
-#pragma unroll
-      for (int t = 0; t < D / 32; ++t) {
-        f32x16 hit;
-#pragma unroll
-        for (int j = 0; j < 16; ++j) hit[j] = 0.f;
-#pragma unroll
-        for (int s2 = 0; s2 < 2; ++s2)
-          hit = mfma32<T>(each(v_operand(s2, t), [&](uint32_t b) {
-                            const bool top = (b & kExp) == kExp, inf = top && !(b & 0x7fffu & ~kExp), neg = b & 0x8000u;
-                            return (kind == 0 ? inf && !neg : kind == 1 ? inf && neg : kind == 2 ? top && !inf : inf) ? kOne : 0u;
-                          }), takes[s2], hit);
-#pragma unroll
-        for (int j = 0; j < 16; ++j) acc[t][j] += hit[j] > 0.f ? kind_adds(kind) : 0.f;
-      }
-    }
-  }
 }
 
 template <typename T, int D, int WR>
 __global__ __launch_bounds__(kTreeWaves * kWave, (TileShape<D, WR>::kGroups)) void tree_tile_kernel(const TreeArgs a) {
   using S = TileShape<D, WR>;
-  constexpr int WK = S::WK, NB = S::NB, SL = S::SL, RPL = S::RPL, BT = kTreeTile, BK = BT * WK;
+  constexpr int WK = S::WK, TP = S::TP, NB = S::NB, SL = S::SL, RPL = S::RPL, BT = kTreeTile, BK = BT * WK * TP;
   __shared__ __align__(16) unsigned char lds[S::kBytes];
   typedef uint4 Tile[BT][SL];
-  Tile* tiles = reinterpret_cast<Tile*>(lds);  // [buffer][tile of the round][K, V]
+  Tile* tiles = reinterpret_cast<Tile*>(lds);  // [buffer][tile of the round, TP of each wave][K, V]
   const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave);
   const int lane = threadIdx.x % kWave, c = lane % 32, h = lane / 32;
   const int wk = wave / WR, wr = wave % WR;
@@ -345,12 +322,11 @@ __global__ __launch_bounds__(kTreeWaves * kWave, (TileShape<D, WR>::kGroups)) vo
 
   const int r = min(row0 + c, rows - 1);  // rows past the last repeat it and are not stored
   const int draft = r >> a.group_log2;
+  const T* q_row = static_cast<const T*>(a.q) + b * a.qs[0] + long((hk << a.group_log2) + (r & (G - 1))) * a.qs[1] + draft * a.qs[2];
   u32x4 q[D / 16];
   {
-    const T* qp = static_cast<const T*>(a.q) + b * a.qs[0] + long((hk << a.group_log2) + (r & (G - 1))) * a.qs[1] +
-                  draft * a.qs[2] + D / 2 * h;
 #pragma unroll
-    for (int ks = 0; ks < D / 16; ++ks) q[ks] = *reinterpret_cast<const u32x4*>(qp + 8 * ks);
+    for (int ks = 0; ks < D / 16; ++ks) q[ks] = *reinterpret_cast<const u32x4*>(q_row + D / 2 * h + 8 * ks);
     // Landed before the tiles' loads are issued: the compiler would wait for them where
     // they are used first, in the loop, and there for every tile in flight with them.
 #pragma unroll
@@ -393,17 +369,20 @@ __global__ __launch_bounds__(kTreeWaves * kWave, (TileShape<D, WR>::kGroups)) vo
     for (int i = 0; i < S::NLD; ++i) koff[i] = offset(false, krow, i);
   }
   const auto issue = [&](int round) {
-    Tile* to = tiles + ((round % NB) * WK + wk) * 2;
-    const unsigned first = unsigned(round * BK + wk * BT);
-    const unsigned kfirst = first * krow, mfirst = first * mrow;
-    const unsigned at = lds_offset(&to[values][RPL * j0][0]);
-    if constexpr (WR == 1) {
-      const unsigned kat = lds_offset(&to[0][0][0]);
 #pragma unroll
-      for (int i = 0; i < S::NLD; ++i) lds_load16(krsrc, kat + 1024u * unsigned(i), koff[i], kfirst);
+    for (int tp = 0; tp < TP; ++tp) {
+      Tile* to = tiles + (((round % NB) * WK + wk) * TP + tp) * 2;
+      const unsigned first = unsigned(round * BK + (wk * TP + tp) * BT);
+      const unsigned kfirst = first * krow, mfirst = first * mrow;
+      const unsigned at = lds_offset(&to[values][RPL * j0][0]);
+      if constexpr (WR == 1) {
+        const unsigned kat = lds_offset(&to[0][0][0]);
+#pragma unroll
+        for (int i = 0; i < S::NLD; ++i) lds_load16(krsrc, kat + 1024u * unsigned(i), koff[i], kfirst);
+      }
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) lds_load16(mine, at + 1024u * unsigned(i), off[i], mfirst);
     }
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) lds_load16(mine, at + 1024u * unsigned(i), off[i], mfirst);
   };
   unsigned vlane[D / 32];
 #pragma unroll
@@ -423,16 +402,16 @@ __global__ __launch_bounds__(kTreeWaves * kWave, (TileShape<D, WR>::kGroups)) vo
       // The tiles are the wave's own: it refills the one it has read and waits for this one.
       wait_lds_reads();
       if (i + 1 < rounds) issue(i + 1);
-      wait_younger<1, S::L>(min(1, rounds - 1 - i));
+      wait_younger<1, S::L * TP>(min(1, rounds - 1 - i));
     } else {
       // Every wave's part of this round has landed, and everyone has read the round
       // before, whose place the load after the barrier takes.
-      wait_younger<NB - 2, S::L>(min(NB - 2, rounds - 1 - i));
+      wait_younger<NB - 2, S::L * TP>(min(NB - 2, rounds - 1 - i));
       wait_lds_reads();
       __syncthreads();
       if (i + NB - 1 < rounds) issue(i + NB - 1);
     }
-    return tiles + ((i % NB) * WK + wk) * 2;
+    return tiles + ((i % NB) * WK + wk) * TP * 2;
   };
   const bool busy = row0 < used;  // uniform over the wave
   // Rounds of committed keys alone, then those with drafts or the end in them (two
@@ -440,28 +419,53 @@ __global__ __launch_bounds__(kTreeWaves * kWave, (TileShape<D, WR>::kGroups)) vo
   const int full = min(rounds, max(0, min(row.len, end) - begin) / BK);
   for (int i = 0; i < full; ++i) {
     const Tile* tile = arrive(i);
-    if (busy) tile_step<T, D, false>(tile[0], tile[1], q, acc, m, l, c, h, 0u, false, a.cs, vlane);
+    if (!busy) continue;
+#pragma unroll
+    for (int tp = 0; tp < TP; ++tp)
+      tile_step<T, D, false>(tile[2 * tp], tile[2 * tp + 1], q, acc, m, l, c, h, 0u, false, a.cs, vlane);
   }
+  bool lost = false;  // values left out of the products
   for (int i = full; i < rounds; ++i) {
     const Tile* tile = arrive(i);
-    const int t0 = begin + i * BK + wk * BT;
-    if (!busy || t0 >= end) continue;
-    uint32_t sees = 0;
+#pragma unroll 1
+    for (int tp = 0; tp < TP; ++tp, tile += 2) {
+      const int t0 = begin + i * BK + (wk * TP + tp) * BT;
+      if (!busy || t0 >= end) break;
+      uint32_t sees = 0;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const int key = t0 + 8 * (j / 4) + 4 * h + j % 4;
-      sees |= uint32_t(key < end && draft_sees(a, b, row, draft, key)) << j;
+      for (int j = 0; j < 16; ++j) {
+        const int key = t0 + 8 * (j / 4) + 4 * h + j % 4;
+        sees |= uint32_t((key < end) & draft_sees(a, b, row, draft, key)) << j;
+      }
+      bool bad = false;
+      constexpr uint32_t kExp = std::is_same<T, bf16_t>::value ? 0x7f80u : 0x7c00u;
+#pragma unroll
+      for (int x = 0; x < BT * SL / kWave; ++x) {
+        const uint4 w = (&tile[1][0][0])[x * kWave + lane];
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) bad |= (u[e] & kExp) == kExp || (u[e] >> 16 & kExp) == kExp;
+      }
+      bad = __ballot(bad) != 0;
+      lost |= bad;
+      tile_step<T, D, true>(tile[0], tile[1], q, acc, m, l, c, h, sees, bad, a.cs, vlane);
     }
-    bool bad = false;
-    constexpr uint32_t kExp = std::is_same<T, bf16_t>::value ? 0x7f80u : 0x7c00u;
+  }
+  if (lost) {
+    const T* kp = static_cast<const T*>(a.k) + b * a.ks[0] + hk * a.ks[1];
+    const T* vp = static_cast<const T*>(a.v) + b * a.vs[0] + hk * a.vs[1];
+    for (int t0 = begin + full * BK + wk * BT * TP; t0 < end; t0 += BK)
+      for (int key = t0; key < min(t0 + BT * TP, end); ++key)
+        add_nonfinite<T, D>(q_row, kp + key * a.ks[2], vp + key * a.vs[2], m, a.cs, draft_sees(a, b, row, draft, key),
+                            [&](float p, const T* value) {
 #pragma unroll
-    for (int x = 0; x < BT * SL / kWave; ++x) {
-      const uint4 w = (&tile[1][0][0])[x * kWave + lane];
-      const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+                              for (int t = 0; t < D / 32; ++t)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) bad |= (u[e] & kExp) == kExp || (u[e] >> 16 & kExp) == kExp;
-    }
-    tile_step<T, D, true>(tile[0], tile[1], q, acc, m, l, c, h, sees, __ballot(bad) != 0, a.cs, vlane);
+                                for (int j = 0; j < 16; ++j) {
+                                  const float x = load_scalar<T>(value + 32 * t + 8 * (j / 4) + 4 * h + j % 4);
+                                  if (!finite(x)) acc[t][j] += p * x;
+                                }
+                            });
   }
   l += lane_xor(l, 32);
 
@@ -533,7 +537,6 @@ __global__ __launch_bounds__(kTreeWaves * kWave) void tree_attention_kernel(cons
   using O = TreeOps<T, D>;
   constexpr int W = kTreeWaves, BT = kTreeTile, VEC = O::kVec;
   constexpr int kState = RT * (4 * VEC + 2);  // a lane's registers of a wave's state
-  static_assert(RT <= 4, "bits of sees");
   __shared__ float sm[2][kState][kWave];
   const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave);
   const int lane = threadIdx.x % kWave, g = lane / 16, n = lane % 16;
@@ -548,14 +551,17 @@ __global__ __launch_bounds__(kTreeWaves * kWave) void tree_attention_kernel(cons
   const bool idle = row0 >= row.count << a.group_log2;  // drafts not in use, whose rows are zeros
   if (a.splits > 1 && (begin >= end || idle)) return;   // the merge does not read these
 
+  const auto q_row = [&](int rt) {  // rows past the last repeat it and are not stored
+    const int r = min(row0 + 16 * rt + n, rows - 1);
+    return static_cast<const T*>(a.q) + b * a.qs[0] + long((hk << a.group_log2) + (r & (G - 1))) * a.qs[1] +
+           (r >> a.group_log2) * a.qs[2];
+  };
   u32x4 q[RT][O::kSteps];
   int draft[RT];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    const int r = min(row0 + 16 * rt + n, rows - 1);  // rows past the last repeat it and are not stored
-    draft[rt] = r >> a.group_log2;
-    O::load_row(static_cast<const T*>(a.q) + b * a.qs[0] + long((hk << a.group_log2) + (r & (G - 1))) * a.qs[1] +
-                    draft[rt] * a.qs[2], g, q[rt]);
+    draft[rt] = min(row0 + 16 * rt + n, rows - 1) >> a.group_log2;
+    O::load_row(q_row(rt), g, q[rt]);
   }
   const T* kp = static_cast<const T*>(a.k) + b * a.ks[0] + hk * a.ks[1];
   const T* vp = static_cast<const T*>(a.v) + b * a.vs[0] + hk * a.vs[1];
@@ -570,6 +576,7 @@ __global__ __launch_bounds__(kTreeWaves * kWave) void tree_attention_kernel(cons
     for (int f = 0; f < VEC; ++f) acc[rt][f] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
+  bool lost = false;  // values left out of the products
   if (!idle) {
     for (int t0 = begin + BT * wave; t0 < end; t0 += BT * W) {
       // Keys past the last one of the row are its last one again: nothing outside is read.
@@ -583,7 +590,6 @@ __global__ __launch_bounds__(kTreeWaves * kWave) void tree_attention_kernel(cons
       const bool masked = t0 + BT > min(row.len, end);
 
       float p[RT][2][4];
-      uint32_t sees = 0;
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
         f32x4 s[2];
@@ -594,13 +600,14 @@ __global__ __launch_bounds__(kTreeWaves * kWave) void tree_attention_kernel(cons
           for (int st = 0; st < O::kSteps; ++st) s[h] = O::dot(k[h][st], q[rt][st], s[h]);
         }
         if (masked) {
+          uint32_t sees = 0;
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             const int key = t0 + 16 * (j / 4) + 4 * g + j % 4;
-            const bool ok = key < end && draft_sees(a, b, row, draft[rt], key);
-            s[j / 4][j % 4] = ok ? s[j / 4][j % 4] : -INFINITY;
-            sees |= uint32_t(ok) << (8 * rt + j);
+            sees |= uint32_t((key < end) & draft_sees(a, b, row, draft[rt], key)) << j;
           }
+#pragma unroll
+          for (int j = 0; j < 8; ++j) s[j / 4][j % 4] = sees >> j & 1u ? s[j / 4][j % 4] : -INFINITY;
         }
         float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
                          fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
@@ -633,32 +640,7 @@ __global__ __launch_bounds__(kTreeWaves * kWave) void tree_attention_kernel(cons
 #pragma unroll
           for (int f = 0; f < VEC; ++f) bad |= !finite(O::v_value(v[j], f));
         if (__ballot(bad)) {
-#pragma unroll 1
-          for (int kind = 0; kind < kKinds; ++kind) {
-            uint32_t has[8][O::kWords];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-#pragma unroll
-              for (int w = 0; w < O::kWords; ++w) has[j][w] = 0u;
-#pragma unroll
-              for (int f = 0; f < VEC; ++f)
-                if (kind_has(kind, O::v_value(v[j], f))) O::set_one(has[j], f);
-            }
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-              float takes[2][4];
-#pragma unroll
-              for (int j = 0; j < 8; ++j) takes[j / 4][j % 4] = kind_takes(kind, sees >> (8 * rt + j) & 1u, p[rt][j / 4][j % 4]);
-              f32x4 hit[VEC];
-#pragma unroll
-              for (int f = 0; f < VEC; ++f) hit[f] = f32x4{0.f, 0.f, 0.f, 0.f};
-              O::add_pv(has, takes, hit);
-#pragma unroll
-              for (int f = 0; f < VEC; ++f)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) acc[rt][f][i] += hit[f][i] > 0.f ? kind_adds(kind) : 0.f;
-            }
-          }
+          lost = true;
 #pragma unroll
           for (int j = 0; j < 8; ++j)
 #pragma unroll
@@ -668,6 +650,25 @@ __global__ __launch_bounds__(kTreeWaves * kWave) void tree_attention_kernel(cons
       }
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) O::add_pv(v, p[rt], acc[rt]);
+    }
+  }
+  if (lost) {
+    for (int t0 = begin + BT * wave; t0 < end; t0 += BT * W) {
+      if (t0 + BT <= min(row.len, end)) continue;
+      for (int key = t0; key < min(t0 + BT, end); ++key) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+          add_nonfinite<T, D>(q_row(rt), kp + key * a.ks[2], vp + key * a.vs[2], m[rt], a.cs, draft_sees(a, b, row, draft[rt], key),
+                              [&](float p, const T* value) {
+#pragma unroll
+                                for (int f = 0; f < VEC; ++f)
+#pragma unroll
+                                  for (int i = 0; i < 4; ++i) {
+                                    const float x = load_scalar<T>(value + VEC * (4 * g + i) + f);
+                                    if (!finite(x)) acc[rt][f][i] += p * x;
+                                  }
+                              });
+      }
     }
   }
 #pragma unroll
