@@ -46,8 +46,10 @@ struct TreeRow {
 };
 __device__ __forceinline__ TreeRow tree_row(const int32_t* lengths, const int32_t* counts, int b, int cap, int tokens) {
   TreeRow r;
-  r.len = min(max(__builtin_amdgcn_readfirstlane(lengths[b]), 0), cap);
-  r.count = counts ? min(max(__builtin_amdgcn_readfirstlane(counts[b]), 0), tokens) : tokens;
+  typedef const __attribute__((address_space(4))) int32_t* Constant;  // read by scalar loads
+  b = __builtin_amdgcn_readfirstlane(b);
+  r.len = min(max(Constant(lengths)[b], 0), cap);
+  r.count = counts ? min(max(Constant(counts)[b], 0), tokens) : tokens;
   r.total = min(r.len + r.count, cap);
   return r;
 }
@@ -320,19 +322,6 @@ __global__ __launch_bounds__(kTreeWaves * kWave, (TileShape<D, WR>::kGroups)) vo
   const int begin = blk.split * chunk, end = min(row.total, begin + chunk);
   if (a.splits > 1 && (begin >= end || block0 >= used)) return;  // the merge does not read these
 
-  const int r = min(row0 + c, rows - 1);  // rows past the last repeat it and are not stored
-  const int draft = r >> a.group_log2;
-  const T* q_row = static_cast<const T*>(a.q) + b * a.qs[0] + long((hk << a.group_log2) + (r & (G - 1))) * a.qs[1] + draft * a.qs[2];
-  u32x4 q[D / 16];
-  {
-#pragma unroll
-    for (int ks = 0; ks < D / 16; ++ks) q[ks] = *reinterpret_cast<const u32x4*>(q_row + D / 2 * h + 8 * ks);
-    // Landed before the tiles' loads are issued: the compiler would wait for them where
-    // they are used first, in the loop, and there for every tile in flight with them.
-#pragma unroll
-    for (int ks = 0; ks < D / 16; ++ks) asm volatile("" : "+v"(q[ks]));
-  }
-
   // The split's keys as buffers whose range ends with its last key: rows past it read as zeros.
   const unsigned krow = unsigned(a.ks[2]) * 2u, vrow = unsigned(a.vs[2]) * 2u;
   const int keys = __builtin_amdgcn_readfirstlane(block0 < used ? max(end - begin, 0) : 0);
@@ -396,7 +385,21 @@ __global__ __launch_bounds__(kTreeWaves * kWave, (TileShape<D, WR>::kGroups)) vo
     for (int j = 0; j < 16; ++j) acc[t][j] = 0.f;
 
   const int rounds = (keys + BK - 1) / BK;
-  for (int i = 0; i < NB - 1 && i < rounds; ++i) issue(i);
+  if (rounds > 0) issue(0);
+
+  const int r = min(row0 + c, rows - 1);  // rows past the last repeat it and are not stored
+  const int draft = r >> a.group_log2;
+  const T* q_row = static_cast<const T*>(a.q) + b * a.qs[0] + long((hk << a.group_log2) + (r & (G - 1))) * a.qs[1] + draft * a.qs[2];
+  u32x4 q[D / 16];
+  {
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) q[ks] = *reinterpret_cast<const u32x4*>(q_row + D / 2 * h + 8 * ks);
+    // Waited for here, with the first tiles: the compiler would wait for them where they
+    // are used first, in the loop, and there for every tile in flight.
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) asm volatile("" : "+v"(q[ks]));
+  }
+
   const auto arrive = [&](int i) {
     if constexpr (WR == 1) {
       // The tiles are the wave's own: it refills the one it has read and waits for this one.
@@ -406,10 +409,10 @@ __global__ __launch_bounds__(kTreeWaves * kWave, (TileShape<D, WR>::kGroups)) vo
     } else {
       // Every wave's part of this round has landed, and everyone has read the round
       // before, whose place the load after the barrier takes.
-      wait_younger<NB - 2, S::L * TP>(min(NB - 2, rounds - 1 - i));
+      wait_younger<0, S::L * TP>(0);
       wait_lds_reads();
       __syncthreads();
-      if (i + NB - 1 < rounds) issue(i + NB - 1);
+      if (i + 1 < rounds) issue(i + 1);
     }
     return tiles + ((i % NB) * WK + wk) * TP * 2;
   };
@@ -743,7 +746,7 @@ __global__ __launch_bounds__(kTreeWaves * kWave) void tree_attention_kernel(cons
 }
 
 // One wave per query row: the splits' states in one, then the output and lse.
-template <typename T, int D>
+template <typename T, int D, int kRound>
 __global__ __launch_bounds__(256) void tree_merge_kernel(const TreeArgs a) {
   constexpr int DPL = (D + kWave - 1) / kWave;
   const int lane = threadIdx.x % kWave;
@@ -758,15 +761,31 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(const TreeArgs a) {
   if (t < row.count && row.total > 0) {
     const int chunk = split_chunk(row.total, a.splits);
     const int n = (row.total + chunk - 1) / chunk;
-    for (int s = 0; s < n; ++s) {
-      const long part = (long(group) * a.splits + s) * rows + r;
-      const float ms = a.pmax[part], mn = fmaxf(top, ms);
-      const float ca = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - mn);
-      const float cb = ms == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ms - mn);
-      den = ca * den + cb * a.psum[part];
+    // kRound splits at a time, all their loads before the first use (one after another
+    // they took 7 us for 16 splits of 32 rows, together 3). Lane s holds the maximum and
+    // the sum of split s.
+    for (int s0 = 0; s0 < n; s0 += kRound) {
+      const auto part = [&](int s) { return (long(group) * a.splits + min(s0 + s, n - 1)) * rows + r; };
+      const float mine = a.pmax[part(lane % kRound)], sum = a.psum[part(lane % kRound)];
+      float x[kRound][DPL];
 #pragma unroll
-      for (int i = 0; i < DPL; ++i)
-        num[i] = ca * num[i] + cb * a.pout[part * D + min(lane + i * kWave, D - 1)];
+      for (int s = 0; s < kRound; ++s)
+#pragma unroll
+        for (int i = 0; i < DPL; ++i) x[s][i] = a.pout[part(s) * D + min(lane + i * kWave, D - 1)];
+      const bool on = lane < kRound && s0 + lane < n;
+      const float mn = fmaxf(top, wave_max(on ? mine : -INFINITY));
+      const float base = mn == -INFINITY ? 0.f : mn;
+      const float keep = __builtin_amdgcn_exp2f(top - base);
+      const float w = on ? __builtin_amdgcn_exp2f(mine - base) : 0.f;
+      den = den * keep + wave_sum(on ? w * sum : 0.f);
+#pragma unroll
+      for (int i = 0; i < DPL; ++i) num[i] *= keep;
+#pragma unroll
+      for (int s = 0; s < kRound; ++s) {
+        const float ws = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), s));
+#pragma unroll
+        for (int i = 0; i < DPL; ++i) num[i] = fmaf(ws, s0 + s < n ? x[s][i] : 0.f, num[i]);
+      }
       top = mn;
     }
   }
@@ -859,7 +878,8 @@ int launch_blocks(void (*kernel)(TreeArgs), int block, TreeArgs& a, hipStream_t 
   if (int rc = check_launch("tree_attention")) return rc;
   if (a.splits == 1) return SFL_OK;
   const long merged = long(a.groups) * rows;
-  hipLaunchKernelGGL((tree_merge_kernel<T, D>), dim3(unsigned((merged + 3) / 4)), dim3(256), 0, stream, a);
+  const auto merge = a.splits <= 4 ? tree_merge_kernel<T, D, 4> : a.splits <= 8 ? tree_merge_kernel<T, D, 8> : tree_merge_kernel<T, D, 16>;
+  hipLaunchKernelGGL(merge, dim3(unsigned((merged + 3) / 4)), dim3(256), 0, stream, a);
   return check_launch("tree_attention");
 }
 

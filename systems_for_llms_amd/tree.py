@@ -79,10 +79,22 @@ def _scale(scale, dim):
     return float(scale)
 
 
-def auto_splits(batch: int, kv_heads: int, capacity: int, rows: int) -> int:
-    """Workgroups that share a KV head's keys: about two to a CU, none with under 512 keys."""
-    blocks = batch * kv_heads * math.ceil(rows / 64)
-    return max(1, min(MAX_SPLITS, math.ceil(512 / blocks), math.ceil(capacity / 512)))
+def auto_splits(batch: int, kv_heads: int, capacity: int, rows: int, dim: int, dtype: torch.dtype) -> int:
+    """Workgroups that share a KV head's keys, for ``rows`` query rows over each (drafts times
+    query heads of the KV head).
+
+    16-bit heads of 64 and 128 run up to 128 rows to a workgroup, other 16-bit heads 64,
+    fp32 32. About 256 workgroups (one to a CU) where the launch streams the cache, 512
+    where the products take longer (many rows, short heads), at most 32 splits, as the
+    merge reads them all, of at least 128 keys. Measured, us at 8 / 16 / 32 / 64 splits:
+    B=1 Hkv=4 N=65536 512 rows 155 / 100 / 93 / 107; B=4 Hkv=4 D=64 N=16384 64 rows
+    26 / 20 / 22 / 27; B=1 Hkv=4 N=8192 32 rows 19 / 16 / 16 / 18; B=8 Hkv=8 N=8191 108
+    rows 71 / 86 / 112 / 163.
+    """
+    tiled = dtype != torch.float32 and dim >= 64
+    blocks = batch * kv_heads * math.ceil(rows / (128 if tiled else 32 if dtype == torch.float32 else 64))
+    target = 512 if rows > 64 or (dtype != torch.float32 and not tiled) else 256
+    return max(1, min(32, math.ceil(target / blocks), math.ceil(capacity / 128)))
 
 
 @dataclass
@@ -146,7 +158,7 @@ def prepare(q, k, v, lengths, mask=None, *, counts=None, splits=None, scale=None
         raise ValueError("each length must be in [0, cache capacity - drafts]")
     _lib.lib()  # fail here, before allocation, if the library is not built
     if splits is None:
-        splits = auto_splits(batch, kv_heads, capacity, tokens * (heads // kv_heads))
+        splits = auto_splits(batch, kv_heads, capacity, tokens * (heads // kv_heads), dim, q.dtype)
     maximum = torch.empty((batch, heads, tokens, splits if splits > 1 else 0), device=q.device, dtype=torch.float32)
     numerator = torch.empty((*maximum.shape, dim), device=q.device, dtype=torch.float32)
     lse = torch.empty((batch, heads, tokens), device=q.device, dtype=torch.float32)
