@@ -364,11 +364,14 @@ struct SelectArgs {
 
 constexpr int kSelectThreads = 1024;
 constexpr int kSelectWaves = kSelectThreads / kWave;
+constexpr int kBins = 2048;          // 11 bits of a key
+constexpr int kMoverList = 8192;     // movers placed at a time
 
 // Sum over the workgroup of what the threads before this one have; *total: all of them.
 __device__ __forceinline__ int block_exclusive(int v, int* scratch, int* total) {
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
   int incl = v;
+#pragma unroll
   for (int d = 1; d < kWave; d <<= 1) {
     const int up = __shfl_up(incl, d);
     if (lane >= d) incl += up;
@@ -377,23 +380,30 @@ __device__ __forceinline__ int block_exclusive(int v, int* scratch, int* total) 
   if (lane == kWave - 1) scratch[wave] = incl;
   __syncthreads();
   int before = 0, all = 0;
+#pragma unroll
   for (int w = 0; w < kSelectWaves; ++w) {
-    if (w < wave) before += scratch[w];
-    all += scratch[w];
+    const int c = scratch[w];
+    before += w < wave ? c : 0;
+    all += c;
   }
   *total = all;
   return before + incl - v;
 }
 
-// kept[b, h, i]: the slot whose rows belong into slot i. A radix selection, 8 bits at
-// a time, finds the key of the last slot that stays; slots with that very key stay
-// from the lowest on. Bits of the slots that stay go to LDS, with the count before
-// each word, so that the r-th that stays above keep finds the r-th hole below it.
+// kept[b, h, i]: the slot whose rows belong into slot i; one workgroup for a head. A
+// radix selection, 11 bits of the keys at a time, finds the key of the last slot that
+// stays; slots with that very key stay from the lowest on. (Weights share few
+// exponents: with 8 bits at a time most of a wave counted in the same few bins, one
+// lane after another.) The slots that stay are then counted by words of 64, the r-th
+// of them from keep on goes through a list in LDS, and the r-th hole below keep takes
+// it. Bound by its chain of barriers and by one CU's LDS: n slots of 1024 threads.
+// KPT: the keys stay in registers, up to KPT a thread; 0: any number, read again.
+template <int KPT>
 __global__ __launch_bounds__(kSelectThreads) void select_kernel(const SelectArgs a) {
-  extern __shared__ __align__(16) unsigned char dynamic[];
-  __shared__ int hist[256];
+  extern __shared__ __align__(16) unsigned char dynamic[];  // [words] bits that stay, [words] counts before
+  __shared__ int bins[kMoverList > kBins ? kMoverList : kBins];  // of the radix passes, then the movers
   __shared__ int scratch[kSelectWaves];
-  __shared__ uint32_t found[3];  // the digit, what is needed of its keys, newest
+  __shared__ int found[3];  // the digit, how many of its keys are needed, how many there are
   const int b = int(blockIdx.x) / a.kv_heads, hk = int(blockIdx.x) - b * a.kv_heads;
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
   const int n = min(max(a.lengths[b], 0), a.cap);
@@ -405,8 +415,38 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(const SelectArgs
   }
   const float* weights = a.weights + long(blockIdx.x) * a.cap;
   const int32_t* positions = a.positions ? a.positions + long(blockIdx.x) * a.cap : nullptr;
+
+  // Round r of the workgroup: slots 1024 r .. 1024 r + 1023. f(round, slot, key), for all
+  // threads of a round (slots from n on have no key of their own).
+  const int rounds = (n + kSelectThreads - 1) / kSelectThreads;
+  uint32_t held[KPT ? KPT : 1];
   int newest = n - 1;
-  if (positions) {
+  if constexpr (KPT > 0) {
+    int age[KPT];
+#pragma unroll
+    for (int r = 0; r < KPT; ++r)
+      if (r < rounds) {
+        const int i = min(r * kSelectThreads + tid, n - 1);
+        held[r] = weight_key(weights[i]);
+        age[r] = positions ? positions[i] : i;
+      }
+    if (positions) {
+      newest = age[0];
+#pragma unroll
+      for (int r = 1; r < KPT; ++r)
+        if (r < rounds) newest = max(newest, age[r]);
+    }
+    if (positions) {
+      for (int m = 32; m >= 1; m >>= 1) newest = max(newest, lane_xor(newest, m));
+      if (lane == 0) scratch[wave] = newest;
+      __syncthreads();
+      for (int w = 0; w < kSelectWaves; ++w) newest = max(newest, scratch[w]);
+    }
+    const long since = long(newest) - a.recent;
+#pragma unroll
+    for (int r = 0; r < KPT; ++r)
+      if (r < rounds && age[r] > since) held[r] = 0xffffffffu;
+  } else if (positions) {
     newest = positions[0];
     for (int i = tid; i < n; i += kSelectThreads) newest = max(newest, positions[i]);
     for (int m = 32; m >= 1; m >>= 1) newest = max(newest, lane_xor(newest, m));
@@ -415,94 +455,113 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(const SelectArgs
     for (int w = 0; w < kSelectWaves; ++w) newest = max(newest, scratch[w]);
   }
   const long since = long(newest) - a.recent;
-  const auto key_of = [&](int i) -> uint32_t {
-    return long(positions ? positions[i] : i) > since ? 0xffffffffu : weight_key(weights[i]);
-  };
-
-  uint32_t prefix = 0;
-  int need = a.keep;
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    if (tid < 256) hist[tid] = 0;
-    __syncthreads();
-    for (int i = tid; i < n; i += kSelectThreads) {
-      const uint32_t key = key_of(i);
-      if (shift == 24 || key >> (shift + 8) == prefix >> (shift + 8)) atomicAdd(&hist[key >> shift & 255], 1);
-    }
-    __syncthreads();
-    if (tid < 256) {  // keys above this digit
-      int above = 0;
-      for (int d = tid + 1; d < 256; ++d) above += hist[d];
-      if (above < need && above + hist[tid] >= need) {
-        found[0] = uint32_t(tid);
-        found[1] = uint32_t(need - above);
+  const auto each = [&](auto&& f) {
+    if constexpr (KPT > 0) {
+#pragma unroll
+      for (int r = 0; r < KPT; ++r)
+        if (r < rounds) f(r, r * kSelectThreads + tid, held[r]);
+    } else {
+      for (int r = 0; r < rounds; ++r) {
+        const int i = r * kSelectThreads + tid, at = min(i, n - 1);
+        const uint32_t key = weight_key(weights[at]);
+        f(r, i, long(positions ? positions[at] : at) > since ? 0xffffffffu : key);
       }
     }
-    __syncthreads();
-    prefix |= found[0] << shift;
-    need = int(found[1]);
-    __syncthreads();
-  }
+  };
 
-  // Words of 64 slots, one wave each: who is above the last key, who has it.
+  uint32_t last = 0;  // the key of the last slot that stays, as far as it is known
+  int need = a.keep, equal = n, shift = 32;
+  while (shift > 0 && need < equal) {  // done as soon as every key that begins like this stays
+    const int top = shift, width = shift > 10 ? 11 : 10;
+    shift -= width;
+    for (int i = tid; i < kBins; i += kSelectThreads) bins[i] = 0;
+    __syncthreads();
+    each([&](int, int i, uint32_t key) {
+      if (i < n && (top == 32 || key >> top == last >> top)) atomicAdd(&bins[key >> shift & ((1u << width) - 1)], 1);
+    });
+    __syncthreads();
+    // Thread t has bins 2 t' and 2 t' + 1 counted from the highest.
+    const int high = (1 << width) - 1 - 2 * tid;
+    const int c0 = high >= 0 ? bins[high] : 0, c1 = high >= 1 ? bins[high - 1] : 0;
+    int all;
+    const int above = block_exclusive(c0 + c1, scratch, &all);
+    if (above < need && need <= above + c0 + c1) {
+      const bool first = need <= above + c0;
+      found[0] = first ? high : high - 1;
+      found[1] = need - above - (first ? 0 : c0);
+      found[2] = first ? c0 : c1;
+    }
+    __syncthreads();
+    last |= uint32_t(found[0]) << shift;
+    need = found[1];
+    equal = found[2];
+  }
+  // Stays: a key above the last one's known bits, or with those bits and among the first `need` of them.
+  const auto above_last = [&](uint32_t key) { return shift < 32 && key >> shift > last >> shift; };
+  const auto like_last = [&](uint32_t key) { return shift == 32 || key >> shift == last >> shift; };
+
   const int words = (n + 63) / 64;
   uint64_t* stays = reinterpret_cast<uint64_t*>(dynamic);
   int* before = reinterpret_cast<int*>(stays + words);
-  for (int w = wave; w < words; w += kSelectWaves) {
-    const int i = 64 * w + lane;
-    const bool equal = i < n && key_of(i) == prefix;
-    const int c = __builtin_popcountll(__ballot(equal));
-    if (lane == 0) before[w] = c;
-  }
-  __syncthreads();
   const int per = (words + kSelectThreads - 1) / kSelectThreads;
-  const int first = min(tid * per, words), last = min(first + per, words);
-  const auto scan = [&]() {
+  const int first = min(tid * per, words), end = min(first + per, words);
+  const auto scan = [&]() {  // counts of words to the counts before them
+    __syncthreads();
     int sum = 0, total;
-    for (int w = first; w < last; ++w) sum += before[w];
+    for (int w = first; w < end; ++w) sum += before[w];
     int run = block_exclusive(sum, scratch, &total);
-    for (int w = first; w < last; ++w) {
+    for (int w = first; w < end; ++w) {
       const int c = before[w];
       before[w] = run;
       run += c;
     }
     __syncthreads();
   };
-  scan();
-  for (int w = wave; w < words; w += kSelectWaves) {
-    const int i = 64 * w + lane;
-    const uint32_t key = i < n ? key_of(i) : 0u;
-    const uint64_t equal = __ballot(i < n && key == prefix);
-    const int rank = before[w] + __builtin_popcountll(equal & ((1ull << lane) - 1));
-    const uint64_t bits = __ballot(i < n && (key > prefix || (key == prefix && rank < need)));
-    if (lane == 0) {
-      stays[w] = bits;
-      before[w] = __builtin_popcountll(bits);
-    }
+  const bool ties = need < equal;
+  if (ties) {
+    each([&](int r, int i, uint32_t key) {
+      const uint64_t bits = __ballot(i < n && like_last(key));
+      if (lane == 0 && r * kSelectWaves + wave < words) before[r * kSelectWaves + wave] = __builtin_popcountll(bits);
+    });
+    scan();
   }
-  __syncthreads();
+  each([&](int r, int i, uint32_t key) {
+    const int w = r * kSelectWaves + wave;
+    const bool like = i < n && like_last(key);
+    bool in = like;
+    if (ties) {
+      const uint64_t bits = __ballot(like);
+      in = like && before[min(w, words - 1)] + __builtin_popcountll(bits & ((1ull << lane) - 1)) < need;
+    }
+    const uint64_t bits = __ballot(in || (i < n && above_last(key)));
+    if (lane == 0 && w < words) {
+      stays[w] = bits;
+      before[w] = __builtin_popcountll(bits);  // this wave alone reads and writes the word's entry
+    }
+  });
   scan();
 
   const int edge = a.keep / 64;
   const int below = before[edge] + __builtin_popcountll(stays[edge] & ((1ull << (a.keep % 64)) - 1));
-  for (int i = tid; i < n; i += kSelectThreads) {
-    const int w = i / 64;
-    const uint64_t bit = 1ull << (i % 64);
-    if (!(stays[w] & bit)) continue;
-    if (i < a.keep) {
-      kept[i] = i;
-      continue;
+  const int movers = a.keep - below;
+  for (int base = 0; base == 0 || base < movers; base += kMoverList) {
+    for (int r = 0; r < rounds; ++r) {
+      const int i = r * kSelectThreads + tid, w = i / 64;
+      if (i < a.keep || i >= n || !(stays[w] >> lane & 1)) continue;
+      const int rank = before[w] + __builtin_popcountll(stays[w] & ((1ull << lane) - 1)) - below - base;
+      if (rank >= 0 && rank < kMoverList) bins[rank] = i;
     }
-    // The r-th that stays from keep on: into the r-th hole, in the last word with at most r holes before it.
-    const int r = before[w] + __builtin_popcountll(stays[w] & (bit - 1)) - below;
-    int lo = 0, hi = edge;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) / 2;
-      if (64 * mid - before[mid] <= r) lo = mid;
-      else hi = mid - 1;
+    __syncthreads();
+    for (int i = tid; i < a.keep; i += kSelectThreads) {
+      const int w = i / 64;
+      const int holes = i - before[w] - __builtin_popcountll(stays[w] & ((1ull << lane) - 1)) - base;  // below slot i
+      if (stays[w] >> lane & 1) {
+        if (base == 0) kept[i] = i;
+      } else if (holes >= 0 && holes < kMoverList) {
+        kept[i] = bins[holes];
+      }
     }
-    uint64_t holes = ~stays[lo];
-    for (int skip = r - (64 * lo - before[lo]); skip > 0; --skip) holes &= holes - 1;
-    kept[64 * lo + __builtin_ctzll(holes)] = i;
+    __syncthreads();
   }
 }
 
@@ -649,7 +708,10 @@ extern "C" int sfl_select_slots(const float* weights, const int32_t* lengths, co
   if (long(batch) * kv_heads > (1L << 24)) return set_error(SFL_ERR_UNSUPPORTED, "%s: too many KV heads", what);
   const SelectArgs a{weights, lengths, positions, kept, new_lengths, kv_heads, capacity, keep, recent};
   const unsigned bytes = unsigned((capacity + 63) / 64) * 12u;
-  hipLaunchKernelGGL(select_kernel, dim3(unsigned(batch * kv_heads)), dim3(kSelectThreads), bytes, static_cast<hipStream_t>(stream), a);
+  const auto kernel = capacity <= 8 * kSelectThreads    ? select_kernel<8>
+                      : capacity <= 24 * kSelectThreads ? select_kernel<24>
+                                                        : select_kernel<0>;
+  hipLaunchKernelGGL(kernel, dim3(unsigned(batch * kv_heads)), dim3(kSelectThreads), bytes, static_cast<hipStream_t>(stream), a);
   return check_launch(what);
 }
 
