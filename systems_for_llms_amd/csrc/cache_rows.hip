@@ -566,28 +566,59 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(const SelectArgs
 }
 
 // Slot i takes what slot kept[i] held where that lies at or above keep: what is read is
-// never written, so nothing has to wait. Blocks in y: k, v.
+// never written, so nothing has to wait. A workgroup looks at 256 places, lists those
+// that take another slot's rows, and moves the pieces of k and v of all of them
+// together, kPieces loads of a thread in flight: few or many, the threads stay busy.
 struct CompactArgs {
   void *k, *v;
   float* weights;
   int32_t* positions;
   const int32_t* kept;
   long ks[3], vs[3];
-  int kv_heads, cap, keep, row_pieces, elem_bytes, blocks;
+  int kv_heads, cap, keep, pieces_log2, elem_bytes, blocks;
 };
 __global__ __launch_bounds__(256) void compact_rows_kernel(const CompactArgs a) {
+  constexpr int kPieces = 8;
+  __shared__ int2 moves[256];
+  __shared__ int counts[4];
   const int group = int(blockIdx.x) / a.blocks, part = int(blockIdx.x) - group * a.blocks;
   const int b = group / a.kv_heads, hk = group - b * a.kv_heads;
-  unsigned char* rows = static_cast<unsigned char*>(blockIdx.y ? a.v : a.k);
-  const long stride = (blockIdx.y ? a.vs[2] : a.ks[2]) * a.elem_bytes;
-  rows += (blockIdx.y ? b * a.vs[0] + hk * a.vs[1] : b * a.ks[0] + hk * a.ks[1]) * a.elem_bytes;
-  const int lanes = a.row_pieces, per = 256 / lanes;  // rows of a pass
-  const int piece = int(threadIdx.x) % lanes;
-  for (int i = part * per + int(threadIdx.x) / lanes; i < a.keep; i += a.blocks * per) {
-    const int from = a.kept[long(group) * a.keep + i];
-    if (from < a.keep || from >= a.cap) continue;
-    *reinterpret_cast<uint4*>(rows + i * stride + 16 * piece) =
-        load16(rows + from * stride + 16 * piece);
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int i = part * 256 + int(threadIdx.x);
+  const int from = i < a.keep ? a.kept[long(group) * a.keep + i] : -1;
+  const bool move = from >= a.keep && from < a.cap;
+  const uint64_t bits = __ballot(move);
+  if (lane == 0) counts[wave] = __builtin_popcountll(bits);
+  __syncthreads();
+  int before = 0, total = 0;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    before += w < wave ? counts[w] : 0;
+    total += counts[w];
+  }
+  if (move) moves[before + __builtin_popcountll(bits & ((1ull << lane) - 1))] = make_int2(i, from);
+  __syncthreads();
+
+  unsigned char* k = static_cast<unsigned char*>(a.k) + (b * a.ks[0] + hk * a.ks[1]) * a.elem_bytes;
+  unsigned char* v = static_cast<unsigned char*>(a.v) + (b * a.vs[0] + hk * a.vs[1]) * a.elem_bytes;
+  const long kstride = a.ks[2] * a.elem_bytes, vstride = a.vs[2] * a.elem_bytes;
+  const int items = total << (a.pieces_log2 + 1);  // (row, k or v, piece)
+  for (int x0 = threadIdx.x; x0 < items; x0 += 256 * kPieces) {
+    uint4 held[kPieces];
+    unsigned char* to[kPieces];
+#pragma unroll
+    for (int e = 0; e < kPieces; ++e) {
+      const int x = min(x0 + 256 * e, items - 1), y = x >> a.pieces_log2;
+      const int2 m = moves[y >> 1];
+      const int piece = x & ((1 << a.pieces_log2) - 1);
+      unsigned char* rows = (y & 1 ? v : k) + 16 * piece;
+      const long stride = y & 1 ? vstride : kstride;
+      to[e] = rows + m.x * stride;
+      held[e] = load16(rows + m.y * stride);
+    }
+#pragma unroll
+    for (int e = 0; e < kPieces; ++e)
+      if (x0 + 256 * e < items) *reinterpret_cast<uint4*>(to[e]) = held[e];
   }
 }
 // Weights and positions by slot; the weights of slots from keep on are cleared once all have moved.
@@ -726,11 +757,10 @@ extern "C" int sfl_compact_slots(void* k, void* v, float* weights, int32_t* posi
   CompactArgs a{k, v, weights, positions, kept};
   for (int i = 0; i < 3; ++i) a.ks[i] = strides[i], a.vs[i] = strides[3 + i];
   a.kv_heads = kv_heads, a.cap = capacity, a.keep = keep, a.elem_bytes = elem_size(dtype);
-  a.row_pieces = head_dim * a.elem_bytes / 16;
-  const int per = 256 / a.row_pieces;
-  a.blocks = (keep + 4 * per - 1) / (4 * per);  // four passes of a workgroup
+  while ((16 << a.pieces_log2) < head_dim * a.elem_bytes) ++a.pieces_log2;
+  a.blocks = (keep + 255) / 256;
   if (long(batch) * kv_heads * a.blocks > 0x7fffffffL) return set_error(SFL_ERR_UNSUPPORTED, "%s: too many workgroups", what);
-  hipLaunchKernelGGL(compact_rows_kernel, dim3(unsigned(batch * kv_heads * a.blocks), 2), dim3(256), 0,
+  hipLaunchKernelGGL(compact_rows_kernel, dim3(unsigned(batch * kv_heads * a.blocks)), dim3(256), 0,
                      static_cast<hipStream_t>(stream), a);
   if (int rc = check_launch(what)) return rc;
   if (!weights && !positions) return SFL_OK;

@@ -799,9 +799,12 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(const TreeArgs a) {
 }
 
 // weights[b, hk, slot] += sum over the counted drafts and the group's heads of
-// exp(s - lse). A wave keeps the K operands of its keys and walks the counted
-// rows, 16 at a time, scores as above; every slot has one writer.
-template <typename T, int D>
+// exp(s - lse), scores as in the kernels above. A workgroup has a share of a head's
+// keys, its waves tiles of 32 in turn; up to NT tiles of 16 counted rows stay in
+// registers while K streams by, the next tile's keys and weights loaded ahead (more
+// rows: another pass over the share, whose keys then come from L2). Bound by reading
+// K. Every slot has one writer, and its terms one order.
+template <typename T, int D, int NT>
 __global__ __launch_bounds__(kTreeWaves * kWave) void tree_weights_kernel(const TreeArgs a, const uint8_t* __restrict__ counted,
                                                                           float* __restrict__ weights) {
   using O = TreeOps<T, D>;
@@ -809,11 +812,26 @@ __global__ __launch_bounds__(kTreeWaves * kWave) void tree_weights_kernel(const 
   __shared__ short list[kMaxDrafts];
   const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave);
   const int lane = threadIdx.x % kWave, g = lane / 16, n = lane % 16;
-  const int group = int(blockIdx.x) / a.splits, part = int(blockIdx.x) - group * a.splits;
-  const int b = group / a.kv_heads, hk = group - b * a.kv_heads;
+  const int group = __builtin_amdgcn_readfirstlane(int(blockIdx.x) / a.splits), part = int(blockIdx.x) - group * a.splits;
+  const int b = __builtin_amdgcn_readfirstlane(group / a.kv_heads), hk = group - b * a.kv_heads;
   const TreeRow row = tree_row(a.lengths, a.counts, b, a.cap, a.tokens);
   const int G = 1 << a.group_log2;
-  if (part * BT * W >= row.total) return;
+  const int chunk = split_chunk(row.total, a.splits), begin = part * chunk, end = min(row.total, begin + chunk);
+  if (begin >= end) return;
+
+  const T* kp = static_cast<const T*>(a.k) + b * a.ks[0] + hk * a.ks[1];
+  float* to = weights + (long(b) * a.kv_heads + hk) * a.cap;
+  // The lane whose sum a slot's terms end up in: of the 16 rows' lanes, n = 2 j for key j of the 8.
+  const int mine = 16 * (n >> 3) + 4 * g + (n >> 1 & 3);
+  u32x4 k[2][O::kSteps];
+  float old = 0.f;
+  const auto fetch = [&](int t0) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) O::load_row(kp + long(min(t0 + 16 * h + n, end - 1)) * a.ks[2], g, k[h]);
+    old = to[min(t0 + mine, end - 1)];
+  };
+  const int first = begin + BT * wave;
+  if (first < end) fetch(first);
 
   // The counted drafts, in order.
   int drafts = 0;
@@ -826,44 +844,67 @@ __global__ __launch_bounds__(kTreeWaves * kWave) void tree_weights_kernel(const 
     drafts += __builtin_popcountll(bits);
   }
   __syncthreads();
-
-  const T* kp = static_cast<const T*>(a.k) + b * a.ks[0] + hk * a.ks[1];
   const int rows = drafts << a.group_log2;
-  const int t0 = (part * W + wave) * BT;
-  if (t0 >= row.total) return;
-  u32x4 k[2][O::kSteps];
+
+  for (int r0 = 0; r0 < rows; r0 += 16 * NT) {
+    u32x4 q[NT][O::kSteps];
+    float base[NT];
+    int draft[NT];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) O::load_row(kp + long(min(t0 + 16 * h + n, row.total - 1)) * a.ks[2], g, k[h]);
-  const bool masked = t0 + BT > row.len;
-  float sum[8] = {};
-  for (int r0 = 0; r0 < rows; r0 += 16) {
-    const int r = min(r0 + n, rows - 1);
-    const int t = list[r >> a.group_log2], head = (hk << a.group_log2) + (r & (G - 1));
-    u32x4 q[O::kSteps];
-    O::load_row(static_cast<const T*>(a.q) + b * a.qs[0] + head * a.qs[1] + t * a.qs[2], g, q);
-    const float lse = a.lse[(long(b) * a.kv_heads * G + head) * a.tokens + t];
-    // Rows past the last and rows that see nothing add exp2(-inf) = 0.
-    const float base = r0 + n < rows && lse != -INFINITY ? lse * kLog2e : INFINITY;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      f32x4 s = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int st = 0; st < O::kSteps; ++st) s = O::dot(k[h][st], q[st], s);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float p = __builtin_amdgcn_exp2f(fmaf(s[i], a.cs, -base));
-        if (base == INFINITY) p = 0.f;
-        if (masked && !draft_sees(a, b, row, t, t0 + 16 * h + 4 * g + i)) p = 0.f;
-        sum[4 * h + i] += p;
-      }
+    for (int rt = 0; rt < NT; ++rt) {
+      const int at = r0 + 16 * rt + n, r = min(at, rows - 1);
+      draft[rt] = list[r >> a.group_log2];
+      const int head = (hk << a.group_log2) + (r & (G - 1));
+      O::load_row(static_cast<const T*>(a.q) + b * a.qs[0] + head * a.qs[1] + draft[rt] * a.qs[2], g, q[rt]);
+      const float lse = a.lse[(long(b) * a.kv_heads * G + head) * a.tokens + draft[rt]];
+      // Rows past the last and rows that see nothing add exp2(-inf) = 0.
+      base[rt] = at < rows && lse != -INFINITY ? lse * kLog2e : INFINITY;
     }
-  }
-  float* to = weights + (long(b) * a.kv_heads + hk) * a.cap;
+    if (r0 > 0 && first < end) fetch(first);
+    for (int t0 = first; t0 < end; t0 += BT * W) {
+      u32x4 now[2][O::kSteps];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float total = group_sum<16>(sum[j]);
-    const int key = t0 + 16 * (j / 4) + 4 * g + j % 4;
-    if (n == 0 && key < row.total) to[key] += total;
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int st = 0; st < O::kSteps; ++st) now[h][st] = k[h][st];
+      const float held = old;
+      if (t0 + BT * W < end) fetch(t0 + BT * W);
+      const bool masked = t0 + BT > row.len;
+      float sum[8] = {};
+#pragma unroll
+      for (int rt = 0; rt < NT; ++rt) {
+        if (r0 + 16 * rt >= rows) break;
+        uint32_t sees = ~0u;
+        if (masked) {
+          sees = 0;
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            sees |= uint32_t(draft_sees(a, b, row, draft[rt], t0 + 16 * (j / 4) + 4 * g + j % 4)) << j;
+        }
+        sees = base[rt] == INFINITY ? 0u : sees;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          f32x4 s = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int st = 0; st < O::kSteps; ++st) s = O::dot(now[h][st], q[rt][st], s);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float p = __builtin_amdgcn_exp2f(fmaf(s[i], a.cs, -base[rt]));
+            sum[4 * h + i] += sees >> (4 * h + i) & 1u ? p : 0.f;
+          }
+        }
+      }
+      // Over the 16 rows' lanes, each step handing half of the keys to the lane's partner.
+#pragma unroll
+      for (int m = 8, left = 4; m >= 2; m >>= 1, left >>= 1)
+#pragma unroll
+        for (int j = 0; j < left; ++j) {
+          const float give = n & m ? sum[j] : sum[j + left], keep = n & m ? sum[j + left] : sum[j];
+          sum[j] = keep + lane_xor(give, m);
+        }
+      const float total = sum[0] + lane_xor(sum[0], 1);
+      if (!(n & 1) && t0 + mine < end) to[t0 + mine] = held + total;
+    }
   }
 }
 
@@ -904,10 +945,14 @@ int launch_tree(TreeArgs& a, hipStream_t stream) {
 
 template <typename T, int D>
 int launch_weights(TreeArgs& a, const uint8_t* counted, float* weights, hipStream_t stream) {
-  a.splits = (a.cap + kTreeTile * kTreeWaves - 1) / (kTreeTile * kTreeWaves);
+  // About four workgroups to a CU, whose waves keep a tile or two of loads in flight each.
+  const int rounds = (a.cap + kTreeTile * kTreeWaves - 1) / (kTreeTile * kTreeWaves);
+  a.splits = std::max(1, std::min(rounds, (1024 + a.groups - 1) / a.groups));
   if (long(a.groups) * a.splits > 0x7fffffffL) return set_error(SFL_ERR_UNSUPPORTED, "tree_weights: too many workgroups");
-  hipLaunchKernelGGL((tree_weights_kernel<T, D>), dim3(unsigned(a.groups * a.splits)), dim3(kTreeWaves * kWave), 0,
-                     stream, a, counted, weights);
+  const int rows = a.tokens << a.group_log2;
+  constexpr int kMost = std::is_same<T, float>::value ? 2 : 4;
+  const auto kernel = rows <= 16 ? tree_weights_kernel<T, D, 1> : rows <= 32 ? tree_weights_kernel<T, D, 2> : tree_weights_kernel<T, D, kMost>;
+  hipLaunchKernelGGL(kernel, dim3(unsigned(a.groups * a.splits)), dim3(kTreeWaves * kWave), 0, stream, a, counted, weights);
   return check_launch("tree_weights");
 }
 
