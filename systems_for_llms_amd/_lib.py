@@ -64,12 +64,12 @@ SIGNATURES: dict[str, list] = {
     "sfl_prefill_layers": [P, P],
     "sfl_causal_attention_f32": [P, P, P, P, c_int, c_int, c_int, c_int, POINTER(c_long), POINTER(c_long),
                                  POINTER(c_long), POINTER(c_long), c_float, P],
-    "sfl_rotate": [P] * 13 + [POINTER(c_long)] + [c_int] * 10 + [c_float, c_int, P],
-    "sfl_tree_attention": [P] * 11 + [POINTER(c_long)] + [c_int] * 7 + [c_float, c_int, P],
-    "sfl_tree_weights": [P] * 8 + [POINTER(c_long)] + [c_int] * 6 + [c_float, c_int, P],
-    "sfl_accept_path": [P] * 8 + [POINTER(c_long)] + [c_int] * 6 + [P],
+    "sfl_rotate": [P] * 13 + [P] + [c_int] * 10 + [c_float, c_int, P],
+    "sfl_tree_attention": [P] * 11 + [P] + [c_int] * 7 + [c_float, c_int, P],
+    "sfl_tree_weights": [P] * 8 + [P] + [c_int] * 6 + [c_float, c_int, P],
+    "sfl_accept_path": [P] * 8 + [P] + [c_int] * 6 + [P],
     "sfl_select_slots": [P] * 5 + [c_int] * 5 + [P],
-    "sfl_compact_slots": [P] * 5 + [POINTER(c_long)] + [c_int] * 6 + [P],
+    "sfl_compact_slots": [P] * 5 + [P] + [c_int] * 6 + [P],
 }
 
 _LIB = None

@@ -34,28 +34,28 @@ def select(weights, lengths, keep, *, recent=0, positions=None):
     more than ``keep``; NaN counts below every number.
     ``new_lengths`` is ``min(lengths, keep)``.
     """
-    if weights.ndim != 3 or weights.dtype != torch.float32 or not weights.is_contiguous() or min(weights.shape) < 1:
-        raise ValueError("weights must be a contiguous float32 tensor [B, Hkv, N]")
-    if weights.requires_grad:
-        raise RuntimeError("select is forward-only; requires_grad inputs are unsupported")
-    batch, heads, capacity = weights.shape
+    if weights.ndim != 3 or 0 in weights.shape:
+        raise ValueError("weights must be [B, Hkv, N] and not empty")
+    batch, heads, capacity = shape = weights.shape
+    index = weights.get_device()
+    cache.check_vector("select", "weights", weights, torch.float32, shape, index)
     if capacity > MAX_SLOTS:
         raise ValueError(f"at most {MAX_SLOTS} slots are supported")
-    for name, value in (("keep", keep), ("recent", recent)):
-        if type(value) is not int:
-            raise TypeError(f"{name} must be an integer")
+    if type(keep) is not int or type(recent) is not int:
+        raise TypeError("keep and recent must be integers")
     if not 1 <= keep <= capacity:
         raise ValueError("keep must be in [1, cache capacity]")
     if not 0 <= recent <= keep:
         raise ValueError("recent must be in [0, keep]")
-    cache.check_vector("lengths", lengths, torch.int32, (batch,))
-    cache.check_vector("positions", positions, torch.int32, tuple(weights.shape))
-    cache.check_device(weights.device, {"lengths": lengths, "positions": positions})
+    cache.check_vector("select", "lengths", lengths, torch.int32, (batch,), index)
+    if positions is not None:
+        cache.check_vector("select", "positions", positions, torch.int32, shape, index)
+    cache.check_device(index)
     _lib.lib()  # fail here, before allocating, if the library is not built
     kept = torch.empty((batch, heads, keep), dtype=torch.int32, device=weights.device)
     new_lengths = torch.empty_like(lengths)
     ops.dispatch(torch.ops.sfl.select_slots, (weights, lengths, positions, kept, new_lengths), (kept, new_lengths),
-                 recent)
+                 recent, checked=True)
     return kept, new_lengths
 
 
@@ -65,28 +65,26 @@ def compact(kept, k, v, *, weights=None, positions=None):
     ``weights`` (fp32) and ``positions`` (int32), ``[B, Hkv, N]``, move with them, and the
     weights of the slots from ``keep`` on become 0.
     """
-    cache.check_rows("compact", {"k": k, "v": v})
+    index = cache.check_rows("compact", ("k", "v"), (k, v))
     cache.check_cache(k, v)
     batch, heads, capacity, _ = k.shape
     if kept.ndim != 3 or not 1 <= kept.shape[2] <= capacity:
         raise ValueError("kept must be [B, Hkv, keep] with keep in [1, cache capacity]")
-    cache.check_vector("kept", kept, torch.int32, (batch, heads, kept.shape[2]))
-    cache.check_vector("weights", weights, torch.float32, (batch, heads, capacity))
-    cache.check_vector("positions", positions, torch.int32, (batch, heads, capacity))
-    cache.check_device(k.device, {"kept": kept, "weights": weights, "positions": positions})
-    if weights is not None and weights.requires_grad:
-        raise RuntimeError("compact is forward-only; requires_grad inputs are unsupported")
+    cache.check_vector("compact", "kept", kept, torch.int32, (batch, heads, kept.shape[2]), index)
+    if weights is not None:
+        cache.check_vector("compact", "weights", weights, torch.float32, (batch, heads, capacity), index)
+    if positions is not None:
+        cache.check_vector("compact", "positions", positions, torch.int32, (batch, heads, capacity), index)
+    cache.check_device(index)
     written = (k, v, weights, positions)
-    ops.dispatch(torch.ops.sfl.compact_slots, (kept, *written), written)
+    ops.dispatch(torch.ops.sfl.compact_slots, (kept, *written), written, checked=True)
 
 
 def evict(k, v, weights, lengths, keep, *, recent=0, positions=None):
     """``select`` and ``compact`` with everything moved: returns ``(kept, new_lengths)``."""
-    cache.check_rows("evict", {"k": k, "v": v})
+    index = cache.check_rows("evict", ("k", "v"), (k, v))
     cache.check_cache(k, v)
-    if tuple(weights.shape) != tuple(k.shape[:3]):
-        raise ValueError("weights must be [B, Hkv, N] for caches [B, Hkv, N, D]")
-    cache.check_device(k.device, {"weights": weights})
+    cache.check_vector("evict", "weights", weights, torch.float32, k.shape[:3], index)
     kept, new_lengths = select(weights, lengths, keep, recent=recent, positions=positions)
     compact(kept, k, v, weights=weights, positions=positions)
     return kept, new_lengths

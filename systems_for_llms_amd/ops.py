@@ -13,6 +13,7 @@ implementation, and a missing library raises.
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import torch
 
@@ -23,7 +24,7 @@ from . import _lib
 _below_autograd = getattr(torch._C, "_AutoDispatchBelowADInplaceOrView", None)
 
 
-def dispatch(op, tensors: tuple, written: tuple, *rest) -> None:
+def dispatch(op, tensors: tuple, written: tuple, *rest, checked: bool = False) -> None:
     """``op(*tensors, *rest)``, below the custom op's autograd layers where they would do nothing.
 
     The op goes through the dispatcher either way, so whatever watches or
@@ -31,9 +32,10 @@ def dispatch(op, tensors: tuple, written: tuple, *rest) -> None:
     the profiler and its observers, lazily negated tensors) takes part. Its
     autograd and version-counting layers are Python, 10 of the 19 us of a call:
     where no tensor requires grad they only count the versions of the
-    ``written`` tensors, which is done here.
+    ``written`` tensors, which is done here. ``checked``: the caller has refused tensors
+    that require grad.
     """
-    if _below_autograd is None or torch.compiler.is_compiling() or _any_requires_grad(tensors):
+    if _below_autograd is None or torch.compiler.is_compiling() or not checked and _any_requires_grad(tensors):
         op(*tensors, *rest)
         return
     with _below_autograd():
@@ -117,20 +119,23 @@ def _masked_attention_fake(q, k, v, out, lse, scale, causal, window_left, window
     return None
 
 
-def _all_strides(*tensors: torch.Tensor | None):
-    """Batch, head and row strides of each tensor in one array (zeros for an absent one)."""
-    return (ctypes.c_long * (3 * len(tensors)))(
-        *[s for t in tensors for s in ((0, 0, 0) if t is None else t.stride()[:3])])
+_NO_STRIDES = (0, 0, 0)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # without building a Stream object
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _call(device: torch.device, name: str, *args) -> None:
     """The entry point on ``device``'s current stream, with that device current."""
-    stream = _lib.stream_handle(device)
-    if device.index == torch.cuda.current_device():
-        _lib.call(name, *args, stream)
+    index = device.index
+    if index != _current_device():
+        with torch.cuda.device(device):
+            _lib.call(name, *args, _lib.stream_handle(device))
         return
-    with torch.cuda.device(device):
-        _lib.call(name, *args, stream)
+    _lib.call(name, *args, _lib.stream_handle(device) if _raw_stream is None else _raw_stream(index))
+
+
+# Strides of several tensors {batch, head, row} as the array of longs the entry points take.
+_strides_2, _strides_5, _strides_6 = (struct.Struct(f"{3 * n}l").pack for n in (2, 5, 6))
 
 
 def launch_rotate(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor | None, positions: torch.Tensor,
@@ -139,10 +144,12 @@ def launch_rotate(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor | None, posi
                   v_out: torch.Tensor | None, half_layout: bool, eps: float) -> None:
     """Norm and rotation of q and k rows; k and v into a cache where ``start`` says so (``sfl_rotate``)."""
     batch, heads, tokens, dim = q.shape
+    strides = _strides_6(*q.stride()[:3], *k.stride()[:3], *(_NO_STRIDES if v is None else v.stride()[:3]),
+                         *q_out.stride()[:3], *k_out.stride()[:3], *(_NO_STRIDES if v is None else v_out.stride()[:3]))
     gain = q.dtype if q_norm is None and k_norm is None else (k_norm if q_norm is None else q_norm).dtype
     _call(q.device, "sfl_rotate", q.data_ptr(), k.data_ptr(), _ptr(v), positions.data_ptr(), cos.data_ptr(),
           sin.data_ptr(), _ptr(q_norm), _ptr(k_norm), _ptr(start), _ptr(counts), q_out.data_ptr(), k_out.data_ptr(),
-          _ptr(v_out), _all_strides(q, k, v, q_out, k_out, v_out), batch, tokens, heads, k.shape[1], dim,
+          _ptr(v_out), strides, batch, tokens, heads, k.shape[1], dim,
           2 * cos.shape[1], cos.shape[0], k_out.shape[2], int(half_layout), _lib.dtype_code(gain), eps,
           _lib.dtype_code(q.dtype))
 
@@ -158,7 +165,8 @@ def launch_tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, len
     batch, heads, tokens, dim = q.shape
     _call(q.device, "sfl_tree_attention", q.data_ptr(), k.data_ptr(), v.data_ptr(), lengths.data_ptr(),
           mask.data_ptr(), _ptr(counts), partial_max.data_ptr(), partial_sum.data_ptr(), partial_output.data_ptr(),
-          out.data_ptr(), lse.data_ptr(), _all_strides(q, k, v, out, mask), batch, heads, k.shape[1], k.shape[2],
+          out.data_ptr(), lse.data_ptr(),
+          _strides_5(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3], *mask.stride()), batch, heads, k.shape[1], k.shape[2],
           tokens, dim, splits, scale, _lib.dtype_code(q.dtype))
 
 
@@ -168,8 +176,8 @@ def launch_tree_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, len
     """Attention weights of the counted drafts added to ``weights`` by slot (``sfl_tree_weights``)."""
     batch, heads, tokens, dim = q.shape
     _call(q.device, "sfl_tree_weights", q.data_ptr(), k.data_ptr(), lse.data_ptr(), weights.data_ptr(),
-          lengths.data_ptr(), mask.data_ptr(), _ptr(counts), _ptr(rows), _all_strides(q, k, None, None, mask), batch,
-          heads, k.shape[1], k.shape[2], tokens, dim, scale, _lib.dtype_code(q.dtype))
+          lengths.data_ptr(), mask.data_ptr(), _ptr(counts), _ptr(rows),
+          _strides_5(*q.stride()[:3], *k.stride()[:3], *_NO_STRIDES, *_NO_STRIDES, *mask.stride()), batch, heads, k.shape[1], k.shape[2], tokens, dim, scale, _lib.dtype_code(q.dtype))
 
 
 def launch_accept_path(lengths: torch.Tensor, path: torch.Tensor, accepted: torch.Tensor, k: torch.Tensor,
@@ -178,8 +186,8 @@ def launch_accept_path(lengths: torch.Tensor, path: torch.Tensor, accepted: torc
     """The accepted path's rows moved behind the committed ones (``sfl_accept_path``)."""
     batch, heads, capacity, dim = k.shape
     _call(k.device, "sfl_accept_path", k.data_ptr(), v.data_ptr(), _ptr(weights), _ptr(positions),
-          lengths.data_ptr(), path.data_ptr(), accepted.data_ptr(), new_lengths.data_ptr(), _all_strides(k, v), batch,
-          heads, capacity, path.shape[1], dim, _lib.dtype_code(k.dtype))
+          lengths.data_ptr(), path.data_ptr(), accepted.data_ptr(), new_lengths.data_ptr(),
+          _strides_2(*k.stride()[:3], *v.stride()[:3]), batch, heads, capacity, path.shape[1], dim, _lib.dtype_code(k.dtype))
 
 
 def launch_select_slots(weights: torch.Tensor, lengths: torch.Tensor, positions: torch.Tensor | None,
@@ -195,7 +203,7 @@ def launch_compact_slots(kept: torch.Tensor, k: torch.Tensor, v: torch.Tensor, w
     """Kept rows moved into the free places below them (``sfl_compact_slots``)."""
     batch, heads, capacity, dim = k.shape
     _call(k.device, "sfl_compact_slots", k.data_ptr(), v.data_ptr(), _ptr(weights), _ptr(positions), kept.data_ptr(),
-          _all_strides(k, v), batch, heads, capacity, kept.shape[2], dim, _lib.dtype_code(k.dtype))
+          _strides_2(*k.stride()[:3], *v.stride()[:3]), batch, heads, capacity, kept.shape[2], dim, _lib.dtype_code(k.dtype))
 
 
 def _nothing(*args):

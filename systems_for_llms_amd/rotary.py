@@ -72,44 +72,35 @@ def rotary_tables(rotary_dim, positions, theta=10000.0, *, scaling=None, factor=
     return cos.to(device), sin.to(device)
 
 
-def _check(operator, named, q, k, positions, cos, sin, counts, layout, q_norm, k_norm, eps):
+def _check(operator, names, rows, positions, cos, sin, counts, layout, q_norm, k_norm, eps):
+    """What both calls ask of their arguments; rows are q, k and what else has the same dtype. Returns the device index."""
     if layout not in LAYOUTS:
         raise ValueError("layout must be 'interleaved' or 'half'")
     if not math.isfinite(eps) or eps < 0:
         raise ValueError("eps must be finite and not negative")
-    first = q
-    for name, t in named.items():
-        if t.ndim != 4:
-            raise ValueError(f"{name} must be [B, H, T, D]")
-        if t.requires_grad:
-            raise RuntimeError(f"{operator} is forward-only; requires_grad inputs are unsupported")
-        if t.dtype != first.dtype or t.dtype not in _lib.DTYPE_CODES:
-            raise TypeError(f"{operator}: all rows must have the same FP16, BF16 or FP32 dtype")
-        if min(t.shape) < 1:
-            raise ValueError(f"{name} must not be empty")
-        if t.stride(3) != 1:
-            raise ValueError(f"{name} must have a contiguous last dimension")
+    index = cache.check_rows(operator, names, rows, aligned=False)
+    q = rows[0]
     batch, _, tokens, dim = q.shape
-    if k.shape[0] != batch or k.shape[2] != tokens or k.shape[3] != dim:
+    kb, _, kt, kd = rows[1].shape
+    if kb != batch or kt != tokens or kd != dim:
         raise ValueError("q and k must agree in batch, tokens and head dimension")
-    if dim not in cache.SUPPORTED_DIMS:
-        raise ValueError("supported head dimensions are 16/32/64/128")
-    if cos.ndim != 2 or not 1 <= cos.shape[1] <= dim // 2 or cos.shape[0] < 1:
+    table = cos.shape
+    if len(table) != 2 or not 1 <= table[1] <= dim // 2 or table[0] < 1:
         raise ValueError("cos and sin must be [positions, rotary_dim / 2] with rotary_dim at most the head dimension")
-    cache.check_vector("cos", cos, torch.float32, cos.shape)
-    cache.check_vector("sin", sin, torch.float32, cos.shape)
-    cache.check_vector("positions", positions, torch.int32, (batch, tokens))
-    cache.check_vector("counts", counts, torch.int32, (batch,))
-    gains = [g for g in (q_norm, k_norm) if g is not None]
-    for g in gains:
-        if g.requires_grad:
-            raise RuntimeError(f"{operator} is forward-only; requires_grad inputs are unsupported")
-        if g.shape != (dim,) or not g.is_contiguous() or g.dtype not in (q.dtype, torch.float32):
+    cache.check_vector(operator, "cos", cos, torch.float32, table, index)
+    cache.check_vector(operator, "sin", sin, torch.float32, table, index)
+    cache.check_vector(operator, "positions", positions, torch.int32, (batch, tokens), index)
+    if counts is not None:
+        cache.check_vector(operator, "counts", counts, torch.int32, (batch,), index)
+    for gain in (q_norm, k_norm):
+        if gain is None:
+            continue
+        if gain.dtype not in (q.dtype, torch.float32):
             raise ValueError("q_norm and k_norm must be contiguous [D] gains in the dtype of q or float32")
-        if g.dtype != gains[0].dtype:
-            raise ValueError("q_norm and k_norm must have the same dtype")
-    cache.check_device(q.device, {**named, "cos": cos, "sin": sin, "positions": positions, "counts": counts,
-                                  "q_norm": q_norm, "k_norm": k_norm})
+        cache.check_vector(operator, "gains (q_norm and k_norm)", gain, gain.dtype, (dim,), index)
+    if q_norm is not None and k_norm is not None and q_norm.dtype != k_norm.dtype:
+        raise ValueError("q_norm and k_norm must have the same dtype")
+    return index
 
 
 def rotate(q, k, positions, cos, sin, *, counts=None, layout="interleaved", q_norm=None, k_norm=None, eps=1e-5):
@@ -120,7 +111,7 @@ def rotate(q, k, positions, cos, sin, *, counts=None, layout="interleaved", q_no
     ``(i, i + rotary_dim / 2)`` (``"half"``); the others keep their (normed) values.
     ``counts`` int32 ``[B]``: tokens in use; the rows of the others are zeros.
     """
-    _check("rotate", {"q": q, "k": k}, q, k, positions, cos, sin, counts, layout, q_norm, k_norm, eps)
+    cache.check_device(_check("rotate", ("q", "k"), (q, k), positions, cos, sin, counts, layout, q_norm, k_norm, eps))
     _lib.lib()  # fail here, before allocating, if the library is not built
     q_out, k_out = torch.empty_like(q), torch.empty_like(k)
     _launch((q, k, None, positions, cos, sin, q_norm, k_norm, None, counts, q_out, k_out, None), layout, eps)
@@ -137,14 +128,15 @@ def rotate_append(q, k, v, positions, cos, sin, k_cache, v_cache, lengths, *, co
     after an eviction a slot is not a position. Tokens from ``counts[b]`` on are padding:
     zero rows of q, and the cache stays as it was. ``lengths`` is not changed.
     """
-    _check("rotate_append", {"q": q, "k": k, "v": v, "k_cache": k_cache, "v_cache": v_cache}, q, k, positions, cos,
-           sin, counts, layout, q_norm, k_norm, eps)
-    batch, heads, _, dim = k.shape
-    if v.shape != k.shape or k_cache.shape[0] != batch or k_cache.shape[1] != heads or k_cache.shape[3] != dim:
+    index = _check("rotate_append", ("q", "k", "v", "k_cache", "v_cache"), (q, k, v, k_cache, v_cache), positions, cos,
+                   sin, counts, layout, q_norm, k_norm, eps)
+    batch, heads, _, dim = shape = k.shape
+    cb, ch, _, cd = k_cache.shape
+    if v.shape != shape or cb != batch or ch != heads or cd != dim:
         raise ValueError("k, v and the caches must agree in batch, heads and head dimension")
     cache.check_cache(k_cache, v_cache)
-    cache.check_vector("lengths", lengths, torch.int32, (batch,))
-    cache.check_device(q.device, {"lengths": lengths})
+    cache.check_vector("rotate_append", "lengths", lengths, torch.int32, (batch,), index)
+    cache.check_device(index)
     _lib.lib()
     q_out = torch.empty_like(q)
     _launch((q, k, v, positions, cos, sin, q_norm, k_norm, lengths, counts, q_out, k_cache, v_cache), layout, eps)
@@ -152,4 +144,4 @@ def rotate_append(q, k, v, positions, cos, sin, k_cache, v_cache, lengths, *, co
 
 
 def _launch(tensors, layout, eps):
-    ops.dispatch(torch.ops.sfl.rotate, tensors, tensors[-3:], layout == "half", float(eps))
+    ops.dispatch(torch.ops.sfl.rotate, tensors, tensors[-3:], layout == "half", float(eps), checked=True)

@@ -53,23 +53,27 @@ def ancestor_mask(parents: torch.Tensor) -> torch.Tensor:
     return mask
 
 
-def _check(operator, q, k, lengths, mask, counts, rows):
-    """Shapes of a call; returns the mask as [B, T, T]."""
-    cache.check_rows(operator, rows)
-    batch, heads, tokens, dim = q.shape
-    if k.shape[0] != batch or k.shape[3] != dim:
+def _check(operator, names, rows, lengths, mask, counts):
+    """What the calls on drafts ask of rows (q, k and, where it is read, v); returns the mask as [B, T, T] and the device index."""
+    index = cache.check_rows(operator, names, rows)
+    batch, heads, tokens, dim = rows[0].shape
+    kb, kv_heads, _, kd = rows[1].shape
+    if kb != batch or kd != dim:
         raise ValueError("q and k must agree in batch and head dimension")
-    cache.check_heads(heads, k.shape[1])
+    cache.check_heads(heads, kv_heads)
     if tokens > MAX_DRAFTS:
         raise ValueError(f"at most {MAX_DRAFTS} drafted tokens are supported")
-    cache.check_vector("lengths", lengths, torch.int32, (batch,))
-    cache.check_vector("counts", counts, torch.int32, (batch,))
+    cache.check_vector(operator, "lengths", lengths, torch.int32, (batch,), index)
+    if counts is not None:
+        cache.check_vector(operator, "counts", counts, torch.int32, (batch,), index)
     if mask is None:
-        mask = torch.ones(tokens, tokens, dtype=torch.bool, device=q.device).tril_()
-    if mask.dtype != torch.bool or mask.shape not in ((tokens, tokens), (batch, tokens, tokens)):
+        mask = torch.ones(tokens, tokens, dtype=torch.bool, device=rows[0].device).tril_()
+    shape = mask.shape
+    if mask.dtype is not torch.bool or shape != (batch, tokens, tokens) and shape != (tokens, tokens):
         raise ValueError("mask must be a bool tensor [T, T] or [B, T, T]")
-    cache.check_device(q.device, {"lengths": lengths, "counts": counts, "mask": mask})
-    return mask.expand(batch, tokens, tokens)
+    if mask.get_device() != index:
+        cache.check_device(-1)
+    return mask if len(shape) == 3 else mask.expand(batch, tokens, tokens), index
 
 
 def _scale(scale, dim):
@@ -118,7 +122,7 @@ class PreparedTree:
         written = (self.partial_max, self.partial_sum, self.partial_output, self.output, self.lse)
         ops.dispatch(torch.ops.sfl.tree_attention,
                      (self.q, self.k, self.v, self.lengths, self.mask, self.counts, *written), written, self.splits,
-                     self.scale)
+                     self.scale, checked=True)
         return self.output
 
     def accumulate(self, weights: torch.Tensor, rows: torch.Tensor | None = None) -> torch.Tensor:
@@ -145,12 +149,13 @@ def prepare(q, k, v, lengths, mask=None, *, counts=None, splits=None, scale=None
     """
     if splits is not None and (type(splits) is not int or not 1 <= splits <= MAX_SPLITS):
         raise ValueError("splits must be an integer in [1, 128]")
-    mask = _check("tree attention", q, k, lengths, mask, counts, {"q": q, "k": k, "v": v})
+    mask, index = _check("tree attention", ("q", "k", "v"), (q, k, v), lengths, mask, counts)
     batch, heads, tokens, dim = q.shape
     kv_heads, capacity = k.shape[1:3]
     if v.shape != k.shape:
         raise ValueError("k and v must have the same [B, Hkv, N, D] shape")
     scale = _scale(scale, dim)
+    cache.check_device(index)
     used = tokens if counts is None else counts
     if counts is not None and not bool(((counts >= 0) & (counts <= tokens)).all()):
         raise ValueError("each count must be in [0, T]")
@@ -180,21 +185,17 @@ def accumulate(q, k, lse, weights, lengths, mask=None, *, counts=None, rows=None
     bool ``[B, T]``: the drafts that count (default: all in use). Call it before ``accept``,
     which moves the slots.
     """
-    mask = _check("accumulate", q, k, lengths, mask, counts, {"q": q, "k": k})
+    mask, index = _check("accumulate", ("q", "k"), (q, k), lengths, mask, counts)
     batch, heads, tokens, dim = q.shape
-    cache.check_vector("lse", lse, torch.float32, (batch, heads, tokens))
-    cache.check_vector("weights", weights, torch.float32, tuple(k.shape[:3]))
-    cache.check_vector("rows", rows, torch.bool, (batch, tokens))
-    cache.check_device(q.device, {"lse": lse, "weights": weights, "rows": rows})
-    _check_no_grad("accumulate", lse, weights)
-    ops.dispatch(torch.ops.sfl.tree_weights, (q, k, lse, lengths, mask, counts, rows, weights), (weights,),
-                 _scale(scale, dim))
+    cache.check_vector("accumulate", "lse", lse, torch.float32, (batch, heads, tokens), index)
+    cache.check_vector("accumulate", "weights", weights, torch.float32, k.shape[:3], index)
+    if rows is not None:
+        cache.check_vector("accumulate", "rows", rows, torch.bool, (batch, tokens), index)
+    scale = _scale(scale, dim)
+    cache.check_device(index)
+    ops.dispatch(torch.ops.sfl.tree_weights, (q, k, lse, lengths, mask, counts, rows, weights), (weights,), scale,
+                 checked=True)
     return weights
-
-
-def _check_no_grad(operator, *tensors):
-    if any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{operator} is forward-only; requires_grad inputs are unsupported")
 
 
 def accept(k, v, lengths, path, accepted, *, weights=None, positions=None):
@@ -206,21 +207,21 @@ def accept(k, v, lengths, path, accepted, *, weights=None, positions=None):
     weights of the rejected drafts' slots become 0, as ``accumulate`` adds to them next time.
     Entries that name no draft or slot move nothing.
     """
-    cache.check_rows("accept", {"k": k, "v": v})
+    index = cache.check_rows("accept", ("k", "v"), (k, v))
     cache.check_cache(k, v)
     batch = k.shape[0]
     if path.ndim != 2 or not 1 <= path.shape[1] <= MAX_DRAFTS:
         raise ValueError(f"path must be [B, T] with T in [1, {MAX_DRAFTS}]")
-    cache.check_vector("lengths", lengths, torch.int32, (batch,))
-    cache.check_vector("path", path, torch.int32, (batch, path.shape[1]))
-    cache.check_vector("accepted", accepted, torch.int32, (batch,))
-    cache.check_vector("weights", weights, torch.float32, tuple(k.shape[:3]))
-    cache.check_vector("positions", positions, torch.int32, tuple(k.shape[:3]))
-    cache.check_device(k.device, {"lengths": lengths, "path": path, "accepted": accepted, "weights": weights,
-                                  "positions": positions})
-    _check_no_grad("accept", weights)
+    cache.check_vector("accept", "lengths", lengths, torch.int32, (batch,), index)
+    cache.check_vector("accept", "path", path, torch.int32, (batch, path.shape[1]), index)
+    cache.check_vector("accept", "accepted", accepted, torch.int32, (batch,), index)
+    if weights is not None:
+        cache.check_vector("accept", "weights", weights, torch.float32, k.shape[:3], index)
+    if positions is not None:
+        cache.check_vector("accept", "positions", positions, torch.int32, k.shape[:3], index)
+    cache.check_device(index)
     _lib.lib()
     new_lengths = torch.empty_like(lengths)
     written = (k, v, weights, positions, new_lengths)
-    ops.dispatch(torch.ops.sfl.accept_path, (lengths, path, accepted, *written), written)
+    ops.dispatch(torch.ops.sfl.accept_path, (lengths, path, accepted, *written), written, checked=True)
     return new_lengths
