@@ -157,53 +157,70 @@ __global__ __launch_bounds__(256) void rotate_rows_kernel(const RotateArgs a, in
     gains(a.k_gain, d1, pk);
   }
 
-  const unsigned tokens = unsigned(a.batch) * unsigned(a.tokens);
+  const unsigned tokens = unsigned(a.batch) * unsigned(a.tokens), stride = gridDim.x * unsigned(per_block);
   const int step = gh * int(gridDim.y), first = int(blockIdx.y) * gh;
-  for (unsigned tok0 = blockIdx.x * unsigned(per_block); tok0 < tokens; tok0 += gridDim.x * unsigned(per_block)) {
-    const unsigned token = tok0 + unsigned(group >> gh_log2);
-    const bool on = token < tokens;  // the lanes of the last workgroup's missing tokens repeat the last one
-    const unsigned at = on ? token : tokens - 1;
-    const int b = int(at / unsigned(a.tokens)), t = int(at - unsigned(b) * unsigned(a.tokens));
-    const bool used = !a.counts || t < a.counts[b];
-    const long slot = a.start ? long(a.start[b]) + t : t;
+  // What a token's rows depend on, loaded a token ahead.
+  struct Token {
+    int b, t, pos, start, count;
+  };
+  const auto look = [&](unsigned token) {
+    const unsigned at = min(token, tokens - 1);  // the lanes of missing tokens repeat the last one
+    Token k;
+    k.b = int(at / unsigned(a.tokens));
+    k.t = int(at - unsigned(k.b) * unsigned(a.tokens));
+    k.pos = a.positions[at];
+    k.start = a.start ? a.start[k.b] : 0;
+    k.count = a.counts ? a.counts[k.b] : a.tokens;
+    return k;
+  };
+  const unsigned lead = unsigned(group >> gh_log2);
+  Token next = look(blockIdx.x * unsigned(per_block) + lead);
+  for (unsigned tok0 = blockIdx.x * unsigned(per_block); tok0 < tokens; tok0 += stride) {
+    const bool on = tok0 + lead < tokens;
+    const int b = next.b, t = next.t, pos = next.pos;
+    const bool used = t < next.count;
+    const long slot = long(next.start) + t;
     const bool kv_store = on && (!a.start || (used && slot >= 0 && slot < a.slots));
-    const int pos = a.positions[at];
     const bool known = pos >= 0 && pos < a.table;
+    // Where head 0 of the launch's order (q, k, v) would be in each tensor.
+    const int k0 = a.q_heads, v0 = a.q_heads + a.kv_heads;
+    const auto from = [&](const void* p, int w, int h0) {
+      return static_cast<const T*>(p) + b * a.st[w][0] + t * a.st[w][2] - h0 * a.st[w][1];
+    };
+    const auto into = [&](void* p, int w, int h0, long row) {
+      return static_cast<T*>(p) + b * a.st[w][0] + row * a.st[w][2] - h0 * a.st[w][1];
+    };
+    const T *qi = from(a.q, 0, 0), *ki = from(a.k, 1, k0), *vi = from(a.v, 2, v0);
+    T *qo = into(a.q_out, 3, 0, t), *ko = into(a.k_out, 4, k0, slot), *vo = into(a.v_out, 5, v0, slot);
+    uint4 x[kRows], xp[kRows];
+    const auto load = [&](int h0) {
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+        const int h = min(h0 + r * step + (group & (gh - 1)), heads - 1);
+        const T* p = h < k0 ? qi + h * a.st[0][1] : h < v0 ? ki + h * a.st[1][1] : vi + h * a.st[2][1];
+        x[r] = load16(p + d0);
+        if constexpr (kHalfLayout) xp[r] = load16(p + d1);
+      }
+    };
+    // All of a token's loads before the first use: its rows, its angles, the next token's place.
     float c[ANGLES], sn[ANGLES];
     const long angle = long(known ? pos : 0) * a.half + i0;
     load_values<float, ANGLES>(a.cos + angle, c);
     load_values<float, ANGLES>(a.sin + angle, sn);
+    load(first);
+    next = look(tok0 + stride + lead);
 #pragma unroll
     for (int i = 0; i < ANGLES; ++i) {
       c[i] = !turned ? 1.f : known ? c[i] : NAN;
       sn[i] = !turned ? 0.f : known ? sn[i] : NAN;
     }
-    // Where head 0 of the launch's order (q, k, v) would be in each tensor.
-    const T* in[3];
-    T* out[3];
-    const int before[3] = {0, a.q_heads, a.q_heads + a.kv_heads};
-#pragma unroll
-    for (int w = 0; w < 3; ++w) {
-      in[w] = static_cast<const T*>(w == 0 ? a.q : w == 1 ? a.k : a.v) + b * a.st[w][0] + t * a.st[w][2] -
-              before[w] * a.st[w][1];
-      out[w] = static_cast<T*>(w == 0 ? a.q_out : w == 1 ? a.k_out : a.v_out) + b * a.st[3 + w][0] +
-               (w == 0 ? t : slot) * a.st[3 + w][2] - before[w] * a.st[3 + w][1];
-    }
 
     for (int h0 = first; h0 < heads; h0 += kRows * step) {  // uniform over the workgroup
-      uint4 x[kRows], xp[kRows];
-#pragma unroll
-      for (int r = 0; r < kRows; ++r) {
-        const int h = min(h0 + r * step + (group & (gh - 1)), heads - 1);
-        const int w = h < before[1] ? 0 : h < before[2] ? 1 : 2;
-        const T* p = (w == 0 ? in[0] : w == 1 ? in[1] : in[2]) + h * (w == 0 ? a.st[0][1] : w == 1 ? a.st[1][1] : a.st[2][1]);
-        x[r] = load16(p + d0);
-        if constexpr (kHalfLayout) xp[r] = load16(p + d1);
-      }
+      if (h0 > first) load(h0);
 #pragma unroll
       for (int r = 0; r < kRows; ++r) {
         const int h = h0 + r * step + (group & (gh - 1));
-        const int w = h < before[1] ? 0 : h < before[2] ? 1 : 2;
+        const int w = h < k0 ? 0 : h < v0 ? 1 : 2;
         float v[VEC], o[VEC];
         unpack16<T>(x[r], v);
         if constexpr (kHalfLayout) unpack16<T>(xp[r], o);
@@ -220,17 +237,17 @@ __global__ __launch_bounds__(256) void rotate_rows_kernel(const RotateArgs a, in
             if constexpr (kHalfLayout) o[e] *= scale * (is_q ? pq[e] : pk[e]);
           }
         }
-        if (turned) {
-          if constexpr (kHalfLayout) {
+        if constexpr (kHalfLayout) {
+          if (turned) {
 #pragma unroll
             for (int e = 0; e < VEC; ++e) v[e] = fmaf(second ? o[e] : -o[e], sn[e], v[e] * c[e]);
-          } else {
+          }
+        } else {
 #pragma unroll
-            for (int e = 0; e < VEC; e += 2) {
-              const float u = v[e], n = v[e + 1];
-              v[e] = fmaf(-n, sn[e / 2], u * c[e / 2]);
-              v[e + 1] = fmaf(u, sn[e / 2], n * c[e / 2]);
-            }
+          for (int e = 0; e < VEC; e += 2) {
+            const float u = v[e], n = v[e + 1];
+            v[e] = fmaf(-n, sn[e / 2], u * c[e / 2]);
+            v[e + 1] = fmaf(u, sn[e / 2], n * c[e / 2]);
           }
         }
         uint4 y;
@@ -241,7 +258,7 @@ __global__ __launch_bounds__(256) void rotate_rows_kernel(const RotateArgs a, in
         if (w == 2) y = x[r];
         if (!used) y = make_uint4(0u, 0u, 0u, 0u);
         if (h < heads && (w == 0 ? on : kv_store)) {
-          T* p = (w == 0 ? out[0] : w == 1 ? out[1] : out[2]) + h * (w == 0 ? a.st[3][1] : w == 1 ? a.st[4][1] : a.st[5][1]);
+          T* p = w == 0 ? qo + h * a.st[3][1] : w == 1 ? ko + h * a.st[4][1] : vo + h * a.st[5][1];
           *reinterpret_cast<uint4*>(p + d0) = y;
         }
       }
@@ -273,8 +290,8 @@ int launch_rotate_rows(const RotateArgs& a, int heads, bool half_layout, hipStre
   // Few tokens: their heads on several workgroups, until there are about two for each CU.
   const int rounds = (heads + (1 << gh_log2) - 1) >> gh_log2;
   const int share = int(std::max(1L, std::min(long(rounds), 512 / blocks)));
-  // Many tokens: eight workgroups to a CU, which walk them.
-  const dim3 grid{unsigned(std::min(blocks, 2048L)), unsigned(share), 1u};
+  // Many tokens: as many workgroups as the CUs hold at once, which walk them.
+  const dim3 grid{unsigned(std::min(blocks, 1024L)), unsigned(share), 1u};
   const bool norm = a.q_gain || a.k_gain;
   if (half_layout)
     hipLaunchKernelGGL((rotate_rows_kernel<T, D, true>), grid, dim3(256), 0, stream, a, heads, gh_log2, norm);
@@ -365,7 +382,7 @@ struct SelectArgs {
 constexpr int kSelectThreads = 1024;
 constexpr int kSelectWaves = kSelectThreads / kWave;
 constexpr int kBins = 2048;          // 11 bits of a key
-constexpr int kMoverList = 8192;     // movers placed at a time
+constexpr int kMoverList = 4096;     // movers placed at a time
 
 // Sum over the workgroup of what the threads before this one have; *total: all of them.
 __device__ __forceinline__ int block_exclusive(int v, int* scratch, int* total) {
@@ -396,11 +413,12 @@ __device__ __forceinline__ int block_exclusive(int v, int* scratch, int* total) 
 // exponents: with 8 bits at a time most of a wave counted in the same few bins, one
 // lane after another.) The slots that stay are then counted by words of 64, the r-th
 // of them from keep on goes through a list in LDS, and the r-th hole below keep takes
-// it. Bound by its chain of barriers and by one CU's LDS: n slots of 1024 threads.
-// KPT: the keys stay in registers, up to KPT a thread; 0: any number, read again.
-template <int KPT>
+// it. Bound by its chain of barriers and by one CU's LDS: of 21 us for 20011 slots the
+// loads take 3, the counting of 11 and 11 bits 5 and 3, the slots that stay 6, the
+// list 4. kHeld: the keys stay in LDS; else they are formed again in every pass.
+template <bool kHeld>
 __global__ __launch_bounds__(kSelectThreads) void select_kernel(const SelectArgs a) {
-  extern __shared__ __align__(16) unsigned char dynamic[];  // [words] bits that stay, [words] counts before
+  extern __shared__ __align__(16) unsigned char dynamic[];  // [words] bits that stay, [words] counts before, [n] keys
   __shared__ int bins[kMoverList > kBins ? kMoverList : kBins];  // of the radix passes, then the movers
   __shared__ int scratch[kSelectWaves];
   __shared__ int found[3];  // the digit, how many of its keys are needed, how many there are
@@ -416,37 +434,13 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(const SelectArgs
   const float* weights = a.weights + long(blockIdx.x) * a.cap;
   const int32_t* positions = a.positions ? a.positions + long(blockIdx.x) * a.cap : nullptr;
 
-  // Round r of the workgroup: slots 1024 r .. 1024 r + 1023. f(round, slot, key), for all
-  // threads of a round (slots from n on have no key of their own).
-  const int rounds = (n + kSelectThreads - 1) / kSelectThreads;
-  uint32_t held[KPT ? KPT : 1];
+  const int words = (n + 63) / 64;
+  uint64_t* stays = reinterpret_cast<uint64_t*>(dynamic);
+  int* before = reinterpret_cast<int*>(stays + words);
+  uint32_t* keys = reinterpret_cast<uint32_t*>(before + words);
+
   int newest = n - 1;
-  if constexpr (KPT > 0) {
-    int age[KPT];
-#pragma unroll
-    for (int r = 0; r < KPT; ++r)
-      if (r < rounds) {
-        const int i = min(r * kSelectThreads + tid, n - 1);
-        held[r] = weight_key(weights[i]);
-        age[r] = positions ? positions[i] : i;
-      }
-    if (positions) {
-      newest = age[0];
-#pragma unroll
-      for (int r = 1; r < KPT; ++r)
-        if (r < rounds) newest = max(newest, age[r]);
-    }
-    if (positions) {
-      for (int m = 32; m >= 1; m >>= 1) newest = max(newest, lane_xor(newest, m));
-      if (lane == 0) scratch[wave] = newest;
-      __syncthreads();
-      for (int w = 0; w < kSelectWaves; ++w) newest = max(newest, scratch[w]);
-    }
-    const long since = long(newest) - a.recent;
-#pragma unroll
-    for (int r = 0; r < KPT; ++r)
-      if (r < rounds && age[r] > since) held[r] = 0xffffffffu;
-  } else if (positions) {
+  if (positions) {
     newest = positions[0];
     for (int i = tid; i < n; i += kSelectThreads) newest = max(newest, positions[i]);
     for (int m = 32; m >= 1; m >>= 1) newest = max(newest, lane_xor(newest, m));
@@ -455,17 +449,22 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(const SelectArgs
     for (int w = 0; w < kSelectWaves; ++w) newest = max(newest, scratch[w]);
   }
   const long since = long(newest) - a.recent;
+  const auto form = [&](int i) {
+    const uint32_t key = weight_key(weights[i]);
+    return long(positions ? positions[i] : i) > since ? 0xffffffffu : key;
+  };
+  if constexpr (kHeld) {
+    for (int i = tid; i < n; i += kSelectThreads) keys[i] = form(i);  // its own thread's alone, in every pass
+  }
+  // Round r of the workgroup: slots 1024 r .. 1024 r + 1023. f(round, slot, key), for all
+  // threads of a round (slots from n on have the key 0).
+  const int rounds = (n + kSelectThreads - 1) / kSelectThreads;
   const auto each = [&](auto&& f) {
-    if constexpr (KPT > 0) {
-#pragma unroll
-      for (int r = 0; r < KPT; ++r)
-        if (r < rounds) f(r, r * kSelectThreads + tid, held[r]);
-    } else {
-      for (int r = 0; r < rounds; ++r) {
-        const int i = r * kSelectThreads + tid, at = min(i, n - 1);
-        const uint32_t key = weight_key(weights[at]);
-        f(r, i, long(positions ? positions[at] : at) > since ? 0xffffffffu : key);
-      }
+    for (int r = 0; r < rounds; ++r) {
+      const int i = r * kSelectThreads + tid;
+      uint32_t key = 0u;
+      if (i < n) key = kHeld ? keys[i] : form(i);
+      f(r, i, key);
     }
   };
 
@@ -500,9 +499,6 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(const SelectArgs
   const auto above_last = [&](uint32_t key) { return shift < 32 && key >> shift > last >> shift; };
   const auto like_last = [&](uint32_t key) { return shift == 32 || key >> shift == last >> shift; };
 
-  const int words = (n + 63) / 64;
-  uint64_t* stays = reinterpret_cast<uint64_t*>(dynamic);
-  int* before = reinterpret_cast<int*>(stays + words);
   const int per = (words + kSelectThreads - 1) / kSelectThreads;
   const int first = min(tid * per, words), end = min(first + per, words);
   const auto scan = [&]() {  // counts of words to the counts before them
@@ -738,10 +734,9 @@ extern "C" int sfl_select_slots(const float* weights, const int32_t* lengths, co
     return set_error(SFL_ERR_INVALID, "%s: keep must be in [1, capacity] and recent in [0, keep]", what);
   if (long(batch) * kv_heads > (1L << 24)) return set_error(SFL_ERR_UNSUPPORTED, "%s: too many KV heads", what);
   const SelectArgs a{weights, lengths, positions, kept, new_lengths, kv_heads, capacity, keep, recent};
-  const unsigned bytes = unsigned((capacity + 63) / 64) * 12u;
-  const auto kernel = capacity <= 8 * kSelectThreads    ? select_kernel<8>
-                      : capacity <= 24 * kSelectThreads ? select_kernel<24>
-                                                        : select_kernel<0>;
+  const bool held = capacity <= 24 * kSelectThreads;  // 96 KB of keys
+  const unsigned bytes = unsigned((capacity + 63) / 64) * 12u + (held ? 4u * unsigned(capacity) : 0u);
+  const auto kernel = held ? select_kernel<true> : select_kernel<false>;
   hipLaunchKernelGGL(kernel, dim3(unsigned(batch * kv_heads)), dim3(kSelectThreads), bytes, static_cast<hipStream_t>(stream), a);
   return check_launch(what);
 }
