@@ -2,6 +2,8 @@
 // an accepted path moved behind the committed rows, and the rows of an eviction's
 // kept slots moved into the places that become free. All of it moves bytes: the
 // bound is memory, and below a few hundred KB the launch.
+#include <limits.h>
+
 #include <algorithm>
 #include <type_traits>
 
@@ -439,32 +441,64 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(const SelectArgs
   int* before = reinterpret_cast<int*>(stays + words);
   uint32_t* keys = reinterpret_cast<uint32_t*>(before + words);
 
+  // f(slot, values of kBatch rounds' slots): the loads of kBatch rounds go out together.
+  constexpr int kBatch = 8;
+  const auto positions_of = [&](int i0, int (&p)[kBatch]) {
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const int i = min(i0 + u * kSelectThreads, n - 1);
+      p[u] = positions ? positions[i] : i;
+    }
+  };
   int newest = n - 1;
   if (positions) {
-    newest = positions[0];
-    for (int i = tid; i < n; i += kSelectThreads) newest = max(newest, positions[i]);
+    newest = INT_MIN;
+    for (int i0 = tid; i0 < n; i0 += kBatch * kSelectThreads) {
+      int p[kBatch];
+      positions_of(i0, p);
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) newest = max(newest, p[u]);
+    }
     for (int m = 32; m >= 1; m >>= 1) newest = max(newest, lane_xor(newest, m));
     if (lane == 0) scratch[wave] = newest;
     __syncthreads();
+#pragma unroll
     for (int w = 0; w < kSelectWaves; ++w) newest = max(newest, scratch[w]);
   }
   const long since = long(newest) - a.recent;
-  const auto form = [&](int i) {
-    const uint32_t key = weight_key(weights[i]);
-    return long(positions ? positions[i] : i) > since ? 0xffffffffu : key;
+  const auto keys_of = [&](int i0, uint32_t (&k)[kBatch]) {
+    int p[kBatch];
+    positions_of(i0, p);
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) k[u] = weight_key(weights[min(i0 + u * kSelectThreads, n - 1)]);
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u)
+      if (long(p[u]) > since) k[u] = 0xffffffffu;
   };
   if constexpr (kHeld) {
-    for (int i = tid; i < n; i += kSelectThreads) keys[i] = form(i);  // its own thread's alone, in every pass
+    for (int i0 = tid; i0 < n; i0 += kBatch * kSelectThreads) {
+      uint32_t k[kBatch];
+      keys_of(i0, k);
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u)
+        if (i0 + u * kSelectThreads < n) keys[i0 + u * kSelectThreads] = k[u];  // its own thread's alone, in every pass
+    }
   }
   // Round r of the workgroup: slots 1024 r .. 1024 r + 1023. f(round, slot, key), for all
-  // threads of a round (slots from n on have the key 0).
+  // threads of a round (slots from n on have some key).
   const int rounds = (n + kSelectThreads - 1) / kSelectThreads;
   const auto each = [&](auto&& f) {
-    for (int r = 0; r < rounds; ++r) {
-      const int i = r * kSelectThreads + tid;
-      uint32_t key = 0u;
-      if (i < n) key = kHeld ? keys[i] : form(i);
-      f(r, i, key);
+    for (int r0 = 0; r0 < rounds; r0 += kBatch) {
+      uint32_t k[kBatch];
+      if constexpr (kHeld) {
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) k[u] = keys[min((r0 + u) * kSelectThreads + tid, n - 1)];
+      } else {
+        keys_of(r0 * kSelectThreads + tid, k);
+      }
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u)
+        if (r0 + u < rounds) f(r0 + u, (r0 + u) * kSelectThreads + tid, k[u]);
     }
   };
 
@@ -498,6 +532,7 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(const SelectArgs
   // Stays: a key above the last one's known bits, or with those bits and among the first `need` of them.
   const auto above_last = [&](uint32_t key) { return shift < 32 && key >> shift > last >> shift; };
   const auto like_last = [&](uint32_t key) { return shift == 32 || key >> shift == last >> shift; };
+  const bool ties = need < equal;
 
   const int per = (words + kSelectThreads - 1) / kSelectThreads;
   const int first = min(tid * per, words), end = min(first + per, words);
@@ -513,7 +548,6 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(const SelectArgs
     }
     __syncthreads();
   };
-  const bool ties = need < equal;
   if (ties) {
     each([&](int r, int i, uint32_t key) {
       const uint64_t bits = __ballot(i < n && like_last(key));
@@ -541,11 +575,20 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(const SelectArgs
   const int below = before[edge] + __builtin_popcountll(stays[edge] & ((1ull << (a.keep % 64)) - 1));
   const int movers = a.keep - below;
   for (int base = 0; base == 0 || base < movers; base += kMoverList) {
-    for (int r = 0; r < rounds; ++r) {
-      const int i = r * kSelectThreads + tid, w = i / 64;
-      if (i < a.keep || i >= n || !(stays[w] >> lane & 1)) continue;
-      const int rank = before[w] + __builtin_popcountll(stays[w] & ((1ull << lane) - 1)) - below - base;
-      if (rank >= 0 && rank < kMoverList) bins[rank] = i;
+    for (int r0 = a.keep / kSelectThreads; r0 < rounds; r0 += kBatch) {
+      uint64_t bits[kBatch];
+      int rank[kBatch];
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        const int w = min((r0 + u) * kSelectWaves + wave, words - 1);
+        bits[u] = stays[w];
+        rank[u] = before[w] + __builtin_popcountll(bits[u] & ((1ull << lane) - 1)) - below - base;
+      }
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        const int i = (r0 + u) * kSelectThreads + tid;
+        if (i >= a.keep && i < n && (bits[u] >> lane & 1) && rank[u] >= 0 && rank[u] < kMoverList) bins[rank[u]] = i;
+      }
     }
     __syncthreads();
     for (int i = tid; i < a.keep; i += kSelectThreads) {
