@@ -937,7 +937,7 @@ int launch_tree(TreeArgs& a, hipStream_t stream) {
     }
     return launch_blocks<T, D>(tree_attention_kernel<T, D, 1>, 16, a, stream);
   } else {
-    if (rows <= 16) return launch_blocks<T, D>(tree_attention_kernel<T, D, 1>, 16, a, stream);
+    if (rows <= 16 || (kF32 && D == 128)) return launch_blocks<T, D>(tree_attention_kernel<T, D, 1>, 16, a, stream);
     if (kF32 || rows <= 32) return launch_blocks<T, D>(tree_attention_kernel<T, D, 2>, 32, a, stream);
     return launch_blocks<T, D>(tree_attention_kernel<T, D, kF32 ? 2 : 4>, kF32 ? 32 : 64, a, stream);
   }

@@ -87,18 +87,19 @@ def auto_splits(batch: int, kv_heads: int, capacity: int, rows: int, dim: int, d
     """Workgroups that share a KV head's keys, for ``rows`` query rows over each (drafts times
     query heads of the KV head).
 
-    16-bit heads of 64 and 128 run up to 128 rows to a workgroup, other 16-bit heads 64,
-    fp32 32. About 256 workgroups (one to a CU) where the launch streams the cache, 512
-    where the products take longer (many rows, short heads), at most 32 splits, as the
-    merge reads them all, of at least 128 keys. Measured, us at 8 / 16 / 32 / 64 splits:
-    B=1 Hkv=4 N=65536 512 rows 155 / 100 / 93 / 107; B=4 Hkv=4 D=64 N=16384 64 rows
-    26 / 20 / 22 / 27; B=1 Hkv=4 N=8192 32 rows 19 / 16 / 16 / 18; B=8 Hkv=8 N=8191 108
-    rows 71 / 86 / 112 / 163.
+    A workgroup takes up to 128 rows of 16-bit heads of 64 and 128, 64 of shorter ones, and
+    in fp32 32, or 16 of heads of 128. As many workgroups as run at once: 512, but 256 (one
+    to a CU, by LDS) for up to 64 rows of the first kind; at most 32 splits, as the merge
+    reads them all, of at least 128 keys. Measured, us at 8 / 16 / 32 / 64 splits: B=1 Hkv=4
+    N=65536 512 rows 155 / 98 / 94 / 110; B=4 Hkv=4 D=64 N=16384 64 rows 26 / 20 / 22 / 27;
+    B=1 Hkv=4 N=8192 32 rows 19 / 16 / 16 / 18; B=8 Hkv=8 N=8191 108 rows 71 / 87 / 112 /
+    164; fp32 B=2 Hkv=4 D=128 N=8192 64 rows 39 / 37 / 43 / 56.
     """
     tiled = dtype != torch.float32 and dim >= 64
-    blocks = batch * kv_heads * math.ceil(rows / (128 if tiled else 32 if dtype == torch.float32 else 64))
-    target = 512 if rows > 64 or (dtype != torch.float32 and not tiled) else 256
-    return max(1, min(32, math.ceil(target / blocks), math.ceil(capacity / 128)))
+    block = 128 if tiled else 64 if dtype != torch.float32 else 16 if dim == 128 else 32
+    blocks = batch * kv_heads * math.ceil(rows / block)
+    target = 256 if tiled and rows <= 64 else 512
+    return max(1, min(32, round(target / blocks), math.ceil(capacity / 128)))
 
 
 @dataclass

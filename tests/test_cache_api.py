@@ -153,7 +153,8 @@ def test_auto_splits_bounds():
     assert tree.auto_splits(1, 4, 65536, 512, 128, bf16) == 32  # 4 row blocks of 4 heads, 512 workgroups
     assert tree.auto_splits(8, 8, 8191, 108, 128, bf16) == 8
     assert tree.auto_splits(64, 16, 16384, 16, 64, bf16) == 1
-    assert tree.auto_splits(2, 4, 8192, 64, 128, fp32) == 16    # two row blocks in fp32
+    assert tree.auto_splits(2, 4, 8192, 64, 128, fp32) == 16    # four row blocks in fp32
+    assert tree.auto_splits(14, 4, 2735, 352, 64, bf16) == 3    # 168 row blocks: three rounds fit at once
     for args in ((1, 1, 1, 1), (1, 4, 65536, 512), (128, 16, 100, 1024), (1, 1, 1 << 20, 1)):
         for dim, dtype in ((16, bf16), (128, bf16), (128, fp32)):
             assert 1 <= tree.auto_splits(*args, dim, dtype) <= 32
