@@ -17,20 +17,16 @@ def rotate(x, positions, cos, sin, layout, gain=None, eps=1e-5):
     y = x.double().clone()
     if gain is not None:
         y = y / ((y * y).mean(-1, keepdim=True) + eps).sqrt() * gain.double()
-    size = y.abs()
     half, table = cos.shape[1], cos.shape[0]
-    out = y.clone()
-    for b in range(x.shape[0]):
-        for t in range(x.shape[2]):
-            p = int(positions[b, t])
-            c = cos[p].double() if 0 <= p < table else torch.full((half,), math.nan, dtype=torch.float64)
-            s = sin[p].double() if 0 <= p < table else c
-            for i in range(half):
-                first, second = (i, i + half) if layout == "half" else (2 * i, 2 * i + 1)
-                u, w = y[b, :, t, first], y[b, :, t, second]
-                out[b, :, t, first] = u * c[i] - w * s[i]
-                out[b, :, t, second] = w * c[i] + u * s[i]
-                size[b, :, t, first] = size[b, :, t, second] = torch.hypot(u, w)
+    known = ((positions >= 0) & (positions < table))[..., None]  # [B, T, 1]
+    at = positions.clamp(0, table - 1).long()
+    c, sn = (torch.where(known, x[at].double(), math.nan)[:, None] for x in (cos, sin))
+    first = torch.arange(half) if layout == "half" else 2 * torch.arange(half)
+    second = first + half if layout == "half" else first + 1
+    u, w = y[..., first], y[..., second]
+    out, size = y.clone(), y.abs()
+    out[..., first], out[..., second] = u * c - w * sn, w * c + u * sn
+    size[..., first] = size[..., second] = torch.hypot(u, w)
     return out, size
 
 

@@ -69,45 +69,45 @@ template <typename T, bool kHalfLayout>
 __global__ __launch_bounds__(256) void rotate_any_kernel(const RotateArgs a, int dim, unsigned rows, unsigned heads) {
   __shared__ float stage[4][128];
   const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave), lane = threadIdx.x % kWave;
-  const unsigned at = blockIdx.x * 4 + unsigned(wave);
-  const bool on = at < rows;
-  const unsigned token = (on ? at : 0u) / heads;
-  const int h = int((on ? at : 0u) - token * heads), b = int(token / unsigned(a.tokens));
-  const int t = int(token - unsigned(b) * unsigned(a.tokens));
-  const RotateRow r = rotate_row<T>(a, b, t, h);
-  float x[2], sq = 0.f;
+  for (unsigned row0 = blockIdx.x * 4; row0 < rows; row0 += gridDim.x * 4) {
+    const unsigned at = min(row0 + unsigned(wave), rows - 1);  // the last workgroup's missing rows repeat the last one
+    const unsigned token = at / heads;
+    const int h = int(at - token * heads), b = int(token / unsigned(a.tokens)), t = int(token - unsigned(b) * unsigned(a.tokens));
+    const RotateRow r = rotate_row<T>(a, b, t, h);
+    float x[2], sq = 0.f;
 #pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const int d = lane + kWave * e;
-    x[e] = d < dim ? load_scalar<T>(static_cast<const T*>(r.in) + d) : 0.f;
-    sq = fmaf(x[e], x[e], sq);
-  }
-  if (r.gain) {
-    const float scale = 1.f / sqrtf(wave_sum(sq) / float(dim) + a.eps);
+    for (int e = 0; e < 2; ++e) {
+      const int d = lane + kWave * e;
+      x[e] = d < dim ? load_scalar<T>(static_cast<const T*>(r.in) + d) : 0.f;
+      sq = fmaf(x[e], x[e], sq);
+    }
+    if (r.gain) {
+      const float scale = 1.f / sqrtf(wave_sum(sq) / float(dim) + a.eps);
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        if (lane + kWave * e < dim) x[e] *= scale * gain_at(a, r.gain, lane + kWave * e, T{});
+    }
 #pragma unroll
     for (int e = 0; e < 2; ++e)
-      if (lane + kWave * e < dim) x[e] *= scale * gain_at(a, r.gain, lane + kWave * e, T{});
-  }
+      if (lane + kWave * e < dim) stage[wave][lane + kWave * e] = x[e];
+    __syncthreads();
+    const int pos = a.positions[long(b) * a.tokens + t];
+    const bool known = pos >= 0 && pos < a.table;
 #pragma unroll
-  for (int e = 0; e < 2; ++e)
-    if (lane + kWave * e < dim) stage[wave][lane + kWave * e] = x[e];
-  __syncthreads();
-  if (!on || !r.store) return;
-  const int pos = a.positions[long(b) * a.tokens + t];
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const int d = lane + kWave * e;
-    if (d >= dim) continue;
-    float y = x[e];
-    if (r.turn && d < 2 * a.half) {
-      const int i = kHalfLayout ? d % a.half : d / 2;
-      const bool second = kHalfLayout ? d >= a.half : d & 1;
-      const float other = stage[wave][kHalfLayout ? (second ? d - a.half : d + a.half) : d ^ 1];
-      const bool known = pos >= 0 && pos < a.table;
-      const float c = known ? a.cos[long(pos) * a.half + i] : NAN, s = known ? a.sin[long(pos) * a.half + i] : NAN;
-      y = second ? fmaf(other, s, y * c) : fmaf(-other, s, y * c);
+    for (int e = 0; e < 2; ++e) {
+      const int d = lane + kWave * e;
+      if (d >= dim || !r.store) continue;
+      float y = x[e];
+      if (r.turn && d < 2 * a.half) {
+        const int i = kHalfLayout ? d % a.half : d / 2;
+        const bool second = kHalfLayout ? d >= a.half : d & 1;
+        const float other = stage[wave][kHalfLayout ? (second ? d - a.half : d + a.half) : d ^ 1];
+        const float c = known ? a.cos[long(pos) * a.half + i] : NAN, s = known ? a.sin[long(pos) * a.half + i] : NAN;
+        y = second ? fmaf(other, s, y * c) : fmaf(-other, s, y * c);
+      }
+      store_scalar<T>(static_cast<T*>(r.out) + d, r.zero ? 0.f : y);
     }
-    store_scalar<T>(static_cast<T*>(r.out) + d, r.zero ? 0.f : y);
+    __syncthreads();  // before the next rows' values
   }
 }
 
@@ -674,6 +674,8 @@ __global__ __launch_bounds__(1024) void compact_values_kernel(const CompactArgs 
   for (int i = a.keep + int(threadIdx.x); i < a.cap; i += 1024) a.weights[base + i] = 0.f;
 }
 
+constexpr long kMostHeads = 1L << 22;  // a launch holds fewer than 2^32 threads
+
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 int elem_size(int dtype) { return dtype == SFL_DTYPE_F32 ? 4 : dtype == SFL_DTYPE_BF16 || dtype == SFL_DTYPE_F16 ? 2 : 0; }
 
@@ -683,7 +685,7 @@ int check_rows(const char* what, const void* k, const void* v, const long* strid
   if (!k || !v || !strides) return set_error(SFL_ERR_INVALID, "%s: null pointer argument", what);
   if (batch <= 0 || kv_heads <= 0 || capacity <= 0)
     return set_error(SFL_ERR_INVALID, "%s: batch, heads and capacity must be positive", what);
-  if (long(batch) * kv_heads > (1L << 24)) return set_error(SFL_ERR_UNSUPPORTED, "%s: too many KV heads", what);
+  if (long(batch) * kv_heads >= kMostHeads) return set_error(SFL_ERR_UNSUPPORTED, "%s: too many KV heads", what);
   const int es = elem_size(dtype);
   if (!es) return set_error(SFL_ERR_UNSUPPORTED, "%s: dtype must be F32, BF16 or F16", what);
   if (head_dim != 16 && head_dim != 32 && head_dim != 64 && head_dim != 128)
@@ -723,7 +725,7 @@ extern "C" int sfl_rotate(const void* q, const void* k, const void* v, const int
   a.table = table, a.slots = slots, a.gain_f32 = gain_dtype == SFL_DTYPE_F32, a.eps = eps;
   const int heads = q_heads + kv_heads * (v ? 2 : 1);
   const long rows = long(batch) * tokens * heads;
-  if (rows > 0x7fffffffL) return set_error(SFL_ERR_UNSUPPORTED, "%s: too many rows", what);
+  if (rows >= (1L << 31)) return set_error(SFL_ERR_UNSUPPORTED, "%s: too many rows", what);
   const auto run = [&](auto t) {
     using T = decltype(t);
     if (rotate_in_pieces(a, es, half_layout)) {
@@ -735,7 +737,7 @@ extern "C" int sfl_rotate(const void* q, const void* k, const void* v, const int
         default: return launch_rotate_rows<T, 128>(a, heads, half_layout, on);
       }
     }
-    const dim3 grid(unsigned((rows + 3) / 4));
+    const dim3 grid(unsigned(std::min((rows + 3) / 4, 1L << 20)));
     if (half_layout)
       hipLaunchKernelGGL((rotate_any_kernel<T, true>), grid, dim3(256), 0, static_cast<hipStream_t>(stream), a, head_dim, unsigned(rows), unsigned(heads));
     else
@@ -775,7 +777,7 @@ extern "C" int sfl_select_slots(const float* weights, const int32_t* lengths, co
     return set_error(SFL_ERR_UNSUPPORTED, "%s: at most %d slots", what, SFL_SELECT_MAX_SLOTS);
   if (keep < 1 || keep > capacity || recent < 0 || recent > keep)
     return set_error(SFL_ERR_INVALID, "%s: keep must be in [1, capacity] and recent in [0, keep]", what);
-  if (long(batch) * kv_heads > (1L << 24)) return set_error(SFL_ERR_UNSUPPORTED, "%s: too many KV heads", what);
+  if (long(batch) * kv_heads >= kMostHeads) return set_error(SFL_ERR_UNSUPPORTED, "%s: too many KV heads", what);
   const SelectArgs a{weights, lengths, positions, kept, new_lengths, kv_heads, capacity, keep, recent};
   const bool held = capacity <= 24 * kSelectThreads;  // 96 KB of keys
   const unsigned bytes = unsigned((capacity + 63) / 64) * 12u + (held ? 4u * unsigned(capacity) : 0u);
@@ -797,7 +799,7 @@ extern "C" int sfl_compact_slots(void* k, void* v, float* weights, int32_t* posi
   a.kv_heads = kv_heads, a.cap = capacity, a.keep = keep, a.elem_bytes = elem_size(dtype);
   while ((16 << a.pieces_log2) < head_dim * a.elem_bytes) ++a.pieces_log2;
   a.blocks = (keep + 255) / 256;
-  if (long(batch) * kv_heads * a.blocks > 0x7fffffffL) return set_error(SFL_ERR_UNSUPPORTED, "%s: too many workgroups", what);
+  if (long(batch) * kv_heads * a.blocks >= (1L << 24)) return set_error(SFL_ERR_UNSUPPORTED, "%s: too many workgroups", what);
   hipLaunchKernelGGL(compact_rows_kernel, dim3(unsigned(batch * kv_heads * a.blocks)), dim3(256), 0,
                      static_cast<hipStream_t>(stream), a);
   if (int rc = check_launch(what)) return rc;

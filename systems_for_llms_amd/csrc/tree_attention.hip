@@ -908,17 +908,20 @@ __global__ __launch_bounds__(kTreeWaves * kWave) void tree_weights_kernel(const 
   }
 }
 
+constexpr long kMostGroups = 1L << 24;  // a launch holds fewer than 2^32 threads
+
 // The launch of `kernel` on row blocks of `block` rows, and the merge of its splits.
 template <typename T, int D>
 int launch_blocks(void (*kernel)(TreeArgs), int block, TreeArgs& a, hipStream_t stream) {
   const int rows = a.tokens << a.group_log2;
   a.row_blocks = (rows + block - 1) / block;
   const long units = (long(a.groups) * a.splits + kXcds - 1) / kXcds * kXcds;
-  if (units * a.row_blocks > 0x7fffffffL) return set_error(SFL_ERR_UNSUPPORTED, "tree_attention: too many workgroups");
+  const long merged = long(a.groups) * rows;
+  if (units * a.row_blocks >= kMostGroups || merged / 4 >= kMostGroups - 1)
+    return set_error(SFL_ERR_UNSUPPORTED, "tree_attention: too many workgroups");
   hipLaunchKernelGGL(kernel, dim3(unsigned(units * a.row_blocks)), dim3(kTreeWaves * kWave), 0, stream, a);
   if (int rc = check_launch("tree_attention")) return rc;
   if (a.splits == 1) return SFL_OK;
-  const long merged = long(a.groups) * rows;
   const auto merge = a.splits <= 4 ? tree_merge_kernel<T, D, 4> : a.splits <= 8 ? tree_merge_kernel<T, D, 8> : tree_merge_kernel<T, D, 16>;
   hipLaunchKernelGGL(merge, dim3(unsigned((merged + 3) / 4)), dim3(256), 0, stream, a);
   return check_launch("tree_attention");
@@ -937,9 +940,16 @@ int launch_tree(TreeArgs& a, hipStream_t stream) {
     }
     return launch_blocks<T, D>(tree_attention_kernel<T, D, 1>, 16, a, stream);
   } else {
-    if (rows <= 16 || (kF32 && D == 128)) return launch_blocks<T, D>(tree_attention_kernel<T, D, 1>, 16, a, stream);
-    if (kF32 || rows <= 32) return launch_blocks<T, D>(tree_attention_kernel<T, D, 2>, 32, a, stream);
-    return launch_blocks<T, D>(tree_attention_kernel<T, D, kF32 ? 2 : 4>, kF32 ? 32 : 64, a, stream);
+    if (rows <= 16) return launch_blocks<T, D>(tree_attention_kernel<T, D, 1>, 16, a, stream);
+    if constexpr (kF32) {
+      // Heads of 128 with 32 rows leave a SIMD one wave: 11 sequences of 88 rows over up to
+      // 8K keys 290 us, with 16 rows 168.
+      constexpr int RT = D == 128 ? 1 : 2;
+      return launch_blocks<T, D>(tree_attention_kernel<T, D, RT>, 16 * RT, a, stream);
+    } else {
+      if (rows <= 32) return launch_blocks<T, D>(tree_attention_kernel<T, D, 2>, 32, a, stream);
+      return launch_blocks<T, D>(tree_attention_kernel<T, D, 4>, 64, a, stream);
+    }
   }
 }
 
@@ -948,7 +958,7 @@ int launch_weights(TreeArgs& a, const uint8_t* counted, float* weights, hipStrea
   // About four workgroups to a CU, whose waves keep a tile or two of loads in flight each.
   const int rounds = (a.cap + kTreeTile * kTreeWaves - 1) / (kTreeTile * kTreeWaves);
   a.splits = std::max(1, std::min(rounds, (1024 + a.groups - 1) / a.groups));
-  if (long(a.groups) * a.splits > 0x7fffffffL) return set_error(SFL_ERR_UNSUPPORTED, "tree_weights: too many workgroups");
+  if (long(a.groups) * a.splits >= kMostGroups) return set_error(SFL_ERR_UNSUPPORTED, "tree_weights: too many workgroups");
   const int rows = a.tokens << a.group_log2;
   constexpr int kMost = std::is_same<T, float>::value ? 2 : 4;
   const auto kernel = rows <= 16 ? tree_weights_kernel<T, D, 1> : rows <= 32 ? tree_weights_kernel<T, D, 2> : tree_weights_kernel<T, D, kMost>;

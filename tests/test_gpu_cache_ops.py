@@ -83,6 +83,31 @@ def test_rotate_and_append(dtype, dim, rotary, layout):
         within(only[1], wk, bk, "rotate k")
 
 
+@pytest.mark.parametrize("dtype, dim, tokens, heads, kv_heads", [
+    (BF16, 128, 2501, 4, 2), (FP32, 64, 1500, 5, 1), (FP16, 32, 9000, 2, 2), (BF16, 128, 3, 64, 16), (FP32, 128, 2, 40, 8)])
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_rotate_many_tokens_and_many_heads(dtype, dim, tokens, heads, kv_heads, layout):
+    """More tokens than workgroups, which walk them, and more heads than a workgroup takes at once."""
+    from systems_for_llms_amd import rotary as rt
+
+    g = torch.Generator().manual_seed(tokens)
+    cos, sin = rt.rotary_tables(dim, 10000)
+    q, k, v = (randn(g, 2, n, tokens, dim, dtype=dtype) for n in (heads, kv_heads, kv_heads))
+    positions = torch.randint(0, 10000, (2, tokens), generator=g, dtype=torch.int32)
+    gain = 1 + randn(g, dim, scale=0.3)
+    lengths = torch.tensor([1, 0], dtype=torch.int32)
+    kc, vc = torch.zeros(2, 2, kv_heads, tokens + 1, dim, dtype=dtype, device="cuda")
+    got = rt.rotate_append(q.cuda(), k.cuda(), v.cuda(), positions.cuda(), cos.cuda(), sin.cuda(), kc, vc, lengths.cuda(),
+                           layout=layout, k_norm=gain.cuda())
+    want, size = oc.rotate(q, positions, cos, sin, layout)
+    within(got, want, rotate_bound(dtype, want, size), "q")
+    want, size = oc.rotate(k, positions, cos, sin, layout, gain)
+    for b, n in enumerate((1, 0)):
+        within(kc[b, :, n:n + tokens], want[b], rotate_bound(dtype, want[b], size[b]), "k")
+        assert torch.equal(vc[b, :, n:n + tokens].cpu(), v[b])
+    assert not kc[0, :, 0].any() and not kc[1, :, tokens].any()
+
+
 def test_rotate_is_the_models_rotation():
     """Interleaved pairs over the whole head with the model's tables."""
     from systems_for_llms_amd import rotary as rt
@@ -406,6 +431,24 @@ def test_accept(dtype, dim, tokens):
             assert torch.equal(gw.cpu(), weights)
 
 
+def test_accept_in_strided_caches():
+    """k and v side by side, rows before heads."""
+    from systems_for_llms_amd import tree
+
+    g = torch.Generator().manual_seed(32)
+    both = randn(g, 2, 20, 2, 3, 64, dtype=FP16)
+    k, v = (both[:, :, i].transpose(1, 2) for i in range(2))
+    lengths, accepted = torch.tensor([9, 3], dtype=torch.int32), torch.tensor([2, 3], dtype=torch.int32)
+    path = torch.tensor([[1, 4, 0, 0], [0, 2, 3, 0]], dtype=torch.int32)
+    path[0, 1] = 3
+    want, n = oc.accept([k, v], lengths, path, accepted)
+    gpu = both.cuda()
+    got = tree.accept(*(gpu[:, :, i].transpose(1, 2) for i in range(2)), lengths.cuda(), path.cuda(), accepted.cuda())
+    assert torch.equal(got.cpu(), n)
+    for i in range(2):
+        assert torch.equal(gpu[:, :, i].transpose(1, 2).cpu(), want[i])
+
+
 def test_accept_entries_out_of_range():
     from systems_for_llms_amd import tree
 
@@ -452,7 +495,7 @@ def weights_of_kind(g, kind, *shape):
 
 @pytest.mark.parametrize("kind", ["heavy", "ties", "equal", "odd"])
 @pytest.mark.parametrize("keys, keep, recent", [(1, 1, 1), (70, 1, 0), (64, 63, 63), (200, 64, 10), (1000, 700, 100),
-                                                (2049, 128, 127), (5000, 4096, 0), (40000, 1000, 300)])
+                                                (2049, 128, 127), (5000, 4096, 0), (24573, 9000, 5), (24574, 24000, 64), (40000, 1000, 300)])
 def test_select(kind, keys, keep, recent):
     from systems_for_llms_amd import evict
 
