@@ -24,4 +24,7 @@ Pinning (what fixes each function independently of its own formula):
   on explicitly repeated KV heads with a length mask, as the reference's tests do.
 * ``attention.masked_attention``: fp64 agreement with SDPA under the dense mask;
   the dense mask against the reference's known-answer schedule and brute force.
+* ``cache.*`` (the KV-cache operators, which the reference does not have): float64 and
+  row by row from the definitions; one draft of ``tree_attention`` equals
+  ``attention.decode_reference``, a row's ``tree_weights`` add up to one.
 """

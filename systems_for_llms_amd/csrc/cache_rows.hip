@@ -128,7 +128,9 @@ __device__ __forceinline__ void load_values(const T* p, float (&v)[N]) {
 // group of LPR lanes walks tokens, every GH-th head of each: the gains are loaded once,
 // a token's angles once, and the rows of kRows heads before the first is used. In the
 // half layout a lane also loads the piece its own is paired with (from the cache, as
-// its neighbour just did), which costs no exchange between lanes.
+// its neighbour just did), which costs no exchange between lanes. Bound by memory: 4 x
+// 4001 tokens of 48 heads of 128 (348 MB read and written) 84 us, 4.1 TB/s, where a copy
+// reaches 5.1; 32 tokens 5 us, one chain of position, angle and store.
 template <typename T, int D, bool kHalfLayout>
 __global__ __launch_bounds__(256) void rotate_rows_kernel(const RotateArgs a, int heads, int gh_log2, bool norm) {
   constexpr int VEC = vec_elems<T>(), LPR = D / VEC, kRows = 3;
@@ -309,7 +311,8 @@ constexpr int kMaxPath = 128;
 // Row len + j of a sequence's cache takes what row len + path[j] held, j < accepted.
 // One workgroup has all the rows of a (sequence, KV head) in one tensor and reads
 // every one before it writes any, so chains of rows that move are safe. Blocks in
-// z: k, v, the slot values (which also lose the rejected drafts' weights).
+// y: k, v, the slot values (which also lose the rejected drafts' weights). Bound by
+// latency: path, rows, stores (64 sequences, 9 MB: 6.5 us).
 struct AcceptArgs {
   void *k, *v;
   float* weights;
@@ -415,9 +418,10 @@ __device__ __forceinline__ int block_exclusive(int v, int* scratch, int* total) 
 // exponents: with 8 bits at a time most of a wave counted in the same few bins, one
 // lane after another.) The slots that stay are then counted by words of 64, the r-th
 // of them from keep on goes through a list in LDS, and the r-th hole below keep takes
-// it. Bound by its chain of barriers and by one CU's LDS: of 21 us for 20011 slots the
-// loads take 3, the counting of 11 and 11 bits 5 and 3, the slots that stay 6, the
-// list 4. kHeld: the keys stay in LDS; else they are formed again in every pass.
+// it. Bound by its chain of some 20 barriers and by one CU's LDS: 32 heads of 20011
+// slots 26 us (of 21 between the first and the last barrier the loads took 3, counting
+// 11 and 11 bits 5 and 3, who stays 6, the list 4), 128 heads of 4160 slots with
+// positions 18.6. kHeld: the keys stay in LDS; else they are formed again in every pass.
 template <bool kHeld>
 __global__ __launch_bounds__(kSelectThreads) void select_kernel(const SelectArgs a) {
   extern __shared__ __align__(16) unsigned char dynamic[];  // [words] bits that stay, [words] counts before, [n] keys
@@ -608,6 +612,8 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(const SelectArgs
 // never written, so nothing has to wait. A workgroup looks at 256 places, lists those
 // that take another slot's rows, and moves the pieces of k and v of all of them
 // together, kPieces loads of a thread in flight: few or many, the threads stay busy.
+// Bound by memory where many move (3300 of 4096 rows of 32 heads, 100 MB, 22 us), by the
+// launch and the list where few do (63 rows of 128 heads 8 us; without the list 12).
 struct CompactArgs {
   void *k, *v;
   float* weights;

@@ -143,8 +143,9 @@ struct TreeOps {
   }
 
   // acc[f] += V^T P^T for the tile; p[h][i] the lane's probabilities. 16-bit types round
-  // them to the type of V, half a step (2^-9 of bf16's own 2^-8 spacing at most) each and
-  // of either sign, as the products of the matrix cores ask; l sums them unrounded.
+  // them to the type of V, as the products of the matrix cores ask: each is off by at
+  // most half a step (bf16 2^-8, fp16 2^-11 of its value), of either sign, which over
+  // many keys stays near the rounding of the output itself; l sums them unrounded.
   static __device__ __forceinline__ void add_pv(const uint32_t (&v)[8][kWords], const float (&p)[2][4], f32x4 (&acc)[kVec]) {
     if constexpr (kF32) {
 #pragma unroll
@@ -214,7 +215,11 @@ __device__ __forceinline__ TreeBlock tree_block(const TreeArgs& a) {
 // 32 keys, each with 32 query rows of its own, and the 4 / WR groups of waves take
 // tiles in turn. A key costs 4 D operations a row: with few rows the launch streams
 // the cache (WR = 1: the waves' tiles are their own, no barrier), with 128 rows to a
-// workgroup the products bound it, and a tile is read from memory once for all.
+// workgroup a tile is read from memory once for all of them and the waves bound it:
+// for each tile 16 MFMAs (0.25 us), 102 VALU instructions, 16 of them exp (0.28), and
+// 24 LDS reads (0.23), of which two waves to a SIMD overlap little. Measured: 512 rows
+// over 65536 keys of 4 heads 87 us (789 TFLOP/s; the 16-row kernel 170), 8 sequences of
+// 108 rows over 1K to 8K keys of 8 heads 44 us (3.8 TB/s), 8 rows over 1024 keys 8 us.
 template <int D, int WR>
 struct TileShape {
   static constexpr int WK = kTreeWaves / WR;      // tiles taken side by side
@@ -344,12 +349,11 @@ __global__ __launch_bounds__(kTreeWaves * kWave, (TileShape<D, WR>::kGroups)) vo
   const auto offset = [&](bool values, unsigned stride, int j) {
     return unsigned(RPL * j + lrr) * stride + 16u * slot(values, j);
   };
-  constexpr int kOwn = WR == 1 ? S::NLD : 1;
-  unsigned koff[kOwn], off[S::L];  // V's, or those of the wave's part
+  constexpr int kLoads = WR == 1 ? S::NLD : S::L;
+  unsigned koff[WR == 1 ? S::NLD : 1], off[kLoads];  // K's where the tile is the wave's own; V's, or those of its part
   const bool values = WR == 1 || wr >= WR / 2;
   const i32x4_t mine = scalar(values ? vrsrc : krsrc);
   const unsigned mrow = values ? vrow : krow;
-  constexpr int kLoads = WR == 1 ? S::NLD : S::L;
   const int j0 = WR == 1 ? 0 : (wr % std::max(WR / 2, 1)) * S::L;
 #pragma unroll
   for (int i = 0; i < kLoads; ++i) off[i] = offset(values, mrow, j0 + i);
@@ -361,7 +365,9 @@ __global__ __launch_bounds__(kTreeWaves * kWave, (TileShape<D, WR>::kGroups)) vo
 #pragma unroll
     for (int tp = 0; tp < TP; ++tp) {
       Tile* to = tiles + (((round % NB) * WK + wk) * TP + tp) * 2;
-      const unsigned first = unsigned(round * BK + (wk * TP + tp) * BT);
+      // A tile past the keys (the round's last ones) starts at the last key: the range check
+      // of a load counts from its scalar offset, which has to lie inside.
+      const unsigned first = unsigned(min(round * BK + (wk * TP + tp) * BT, keys - 1));
       const unsigned kfirst = first * krow, mfirst = first * mrow;
       const unsigned at = lds_offset(&to[values][RPL * j0][0]);
       if constexpr (WR == 1) {
@@ -391,14 +397,12 @@ __global__ __launch_bounds__(kTreeWaves * kWave, (TileShape<D, WR>::kGroups)) vo
   const int draft = r >> a.group_log2;
   const T* q_row = static_cast<const T*>(a.q) + b * a.qs[0] + long((hk << a.group_log2) + (r & (G - 1))) * a.qs[1] + draft * a.qs[2];
   u32x4 q[D / 16];
-  {
 #pragma unroll
-    for (int ks = 0; ks < D / 16; ++ks) q[ks] = *reinterpret_cast<const u32x4*>(q_row + D / 2 * h + 8 * ks);
-    // Waited for here, with the first tiles: the compiler would wait for them where they
-    // are used first, in the loop, and there for every tile in flight.
+  for (int ks = 0; ks < D / 16; ++ks) q[ks] = *reinterpret_cast<const u32x4*>(q_row + D / 2 * h + 8 * ks);
+  // Waited for here, with the first tiles: the compiler would wait for them where they
+  // are used first, in the loop, and there for every tile in flight.
 #pragma unroll
-    for (int ks = 0; ks < D / 16; ++ks) asm volatile("" : "+v"(q[ks]));
-  }
+  for (int ks = 0; ks < D / 16; ++ks) asm volatile("" : "+v"(q[ks]));
 
   const auto arrive = [&](int i) {
     if constexpr (WR == 1) {
@@ -409,7 +413,7 @@ __global__ __launch_bounds__(kTreeWaves * kWave, (TileShape<D, WR>::kGroups)) vo
     } else {
       // Every wave's part of this round has landed, and everyone has read the round
       // before, whose place the load after the barrier takes.
-      wait_younger<0, S::L * TP>(0);
+      __builtin_amdgcn_s_waitcnt(sfl_vmcnt(0));
       wait_lds_reads();
       __syncthreads();
       if (i + 1 < rounds) issue(i + 1);
@@ -535,6 +539,13 @@ __global__ __launch_bounds__(kTreeWaves * kWave, (TileShape<D, WR>::kGroups)) vo
   }
 }
 
+// The 16-row form, for fp32, short heads and caches past 32-bit offsets: each wave has
+// tiles of 32 keys of its own, operands straight from memory (a lane's pieces of a row
+// are 16 bytes, so nothing goes through LDS), and RT tiles of 16 rows to use them for.
+// Bound by the fp32 MFMAs where there are many rows, else by the way from memory, as
+// the next tile's loads wait for this one's products. Measured with the merge: 20 rows
+// over 20000 16-bit keys of 32 heads of 32 20 us (4.0 TB/s), 64 fp32 rows over 8192 keys
+// of 8 heads of 128 37 us (57 TFLOP/s).
 template <typename T, int D, int RT>
 __global__ __launch_bounds__(kTreeWaves * kWave) void tree_attention_kernel(const TreeArgs a) {
   using O = TreeOps<T, D>;
@@ -745,7 +756,8 @@ __global__ __launch_bounds__(kTreeWaves * kWave) void tree_attention_kernel(cons
   }
 }
 
-// One wave per query row: the splits' states in one, then the output and lse.
+// One wave per query row: the splits' states in one, then the output and lse. Bound by
+// reading the partials (2048 rows of 32 splits, 34 MB, 8.6 us), below that by latency.
 template <typename T, int D, int kRound>
 __global__ __launch_bounds__(256) void tree_merge_kernel(const TreeArgs a) {
   constexpr int DPL = (D + kWave - 1) / kWave;
@@ -803,7 +815,9 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(const TreeArgs a) {
 // keys, its waves tiles of 32 in turn; up to NT tiles of 16 counted rows stay in
 // registers while K streams by, the next tile's keys and weights loaded ahead (more
 // rows: another pass over the share, whose keys then come from L2). Bound by reading
-// K. Every slot has one writer, and its terms one order.
+// K: 16 rows of up to 8K keys of 16 heads of 64, 169 MB, 40 us (4.2 TB/s; without the
+// loads ahead and with a workgroup for every 128 keys 60). Every slot has one writer,
+// and its terms one order.
 template <typename T, int D, int NT>
 __global__ __launch_bounds__(kTreeWaves * kWave) void tree_weights_kernel(const TreeArgs a, const uint8_t* __restrict__ counted,
                                                                           float* __restrict__ weights) {

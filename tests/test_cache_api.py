@@ -178,6 +178,25 @@ def test_schemas_and_meta_dispatch():
     torch.ops.sfl.select_slots(w, n, None, torch.empty(1, 2, 8, device="meta", dtype=torch.int32), n.clone(), 2)
 
 
+def test_float64_forms_agree_with_the_older_oracles():
+    """One draft that sees itself is decode attention over one key more; weights of a row add up to one."""
+    from oracle import cache as oc
+    from oracle.attention import decode_reference
+
+    g = torch.Generator().manual_seed(1)
+    q = torch.randn(3, 8, 1, 16, generator=g)
+    k, v = torch.randn(2, 3, 2, 20, 16, generator=g)
+    lengths = torch.tensor([0, 7, 19], dtype=torch.int32)
+    mask = torch.ones(1, 1, dtype=torch.bool)
+    out, lse, _, _ = oc.tree_attention(q, k, v, lengths, mask)
+    want = decode_reference(q[:, :, 0], k, v, lengths + 1)
+    assert (out[:, :, 0] - want).abs().max() < 1e-5  # the older one works in float32
+    weights, _ = oc.tree_weights(q, k, lse, torch.zeros(3, 2, 20), lengths, mask)
+    assert (weights.sum(-1) - 4).abs().max() < 1e-12
+    kept, _ = oc.select(torch.tensor([[[3.0, 1.0, 2.0, 2.0, 5.0]]]), torch.tensor([5]), 3, 1)
+    assert kept.tolist() == [[[0, 4, 2]]]
+
+
 INVALID, UNSUPPORTED = -1, -2
 
 
