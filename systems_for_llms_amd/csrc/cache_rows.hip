@@ -342,7 +342,8 @@ __global__ __launch_bounds__(256) void accept_kernel(const AcceptArgs a) {
     if (from >= 0 && a.weights) w = a.weights[base + from];
     if (from >= 0 && a.positions) p = a.positions[base + from];
     __syncthreads();
-    if (len < 0 || j >= a.tokens || len + j >= a.cap) return;
+    // No sum with a length that may be any number: near 2^31 it would wrap into range.
+    if (len < 0 || len >= a.cap || j >= a.tokens || j >= a.cap - len) return;
     if (a.weights && (from >= 0 || j >= count)) a.weights[base + len + j] = w;
     if (a.positions && from >= 0) a.positions[base + len + j] = p;
     return;

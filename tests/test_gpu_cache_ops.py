@@ -752,3 +752,28 @@ def test_results_repeat_bit_for_bit():
         assert torch.equal(op(), first) and torch.equal(op.lse, lse)
         op.accumulate(w)
     assert torch.equal(*weights)
+
+
+# ---- lengths that no cache has ------------------------------------------------------
+
+
+def test_accept_lengths_out_of_range():
+    """Below 0, at the capacity, past it, and where length + draft passes 2^31: nothing moves, nothing is cleared."""
+    from systems_for_llms_amd import tree
+
+    g = torch.Generator().manual_seed(33)
+    bad = [-1, -2 ** 31, 6, 7, 2 ** 31 - 1, 2 ** 31 - 2, 2 ** 31 - 128]
+    lengths = torch.tensor([*bad, 3], dtype=torch.int32)
+    k, v = (randn(g, 8, 2, 6, 32) for _ in range(2))
+    weights = torch.rand(8, 2, 6, generator=g)
+    positions = torch.randint(0, 99, (8, 2, 6), generator=g, dtype=torch.int32)
+    path = torch.tensor([[1, 2, 0, 3]] * 8, dtype=torch.int32)
+    for n in (0, 1, 2):
+        accepted = torch.full((8,), n, dtype=torch.int32)
+        gpu = [x.cuda() for x in (k, v, weights, positions)]
+        got = tree.accept(gpu[0], gpu[1], lengths.cuda(), path.cuda(), accepted.cuda(), weights=gpu[2], positions=gpu[3])
+        tensors = [x[7:] for x in (k, v, weights, positions)]
+        want, _ = oc.accept(tensors, lengths[7:], path[7:], accepted[7:], tensors[2])
+        assert got.tolist() == [*bad, 3 + n]
+        for x, y, z in zip(gpu, (k, v, weights, positions), want):
+            assert torch.equal(x[:7].cpu(), y[:7]) and torch.equal(x[7:].cpu(), z)
