@@ -160,7 +160,7 @@ def prepare(q, k, v, lengths, mask=None, *, counts=None, splits=None, scale=None
     used = tokens if counts is None else counts
     if counts is not None and not bool(((counts >= 0) & (counts <= tokens)).all()):
         raise ValueError("each count must be in [0, T]")
-    if not bool(((lengths >= 0) & (lengths + used <= capacity)).all()):
+    if not bool(((lengths >= 0) & (lengths <= capacity - used)).all()):
         raise ValueError("each length must be in [0, cache capacity - drafts]")
     _lib.lib()  # fail here, before allocation, if the library is not built
     if splits is None:

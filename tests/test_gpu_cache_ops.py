@@ -777,3 +777,16 @@ def test_accept_lengths_out_of_range():
         assert got.tolist() == [*bad, 3 + n]
         for x, y, z in zip(gpu, (k, v, weights, positions), want):
             assert torch.equal(x[:7].cpu(), y[:7]) and torch.equal(x[7:].cpu(), z)
+
+
+def test_tree_prepare_refuses_lengths_whose_sum_with_the_drafts_wraps():
+    from systems_for_llms_amd import tree
+
+    q, k = torch.zeros(2, 2, 3, 64, device="cuda"), torch.zeros(2, 2, 10, 64, device="cuda")
+    counts = torch.tensor([3, 1], dtype=torch.int32, device="cuda")
+    for n in (2 ** 31 - 1, 2 ** 31 - 3):
+        lengths = torch.tensor([n, 0], dtype=torch.int32, device="cuda")
+        for used in (None, counts):
+            with pytest.raises(ValueError, match="each length"):
+                tree.prepare(q, k, k, lengths, counts=used)
+    tree.prepare(q, k, k, torch.tensor([7, 9], dtype=torch.int32, device="cuda"), counts=counts)
