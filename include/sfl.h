@@ -477,11 +477,13 @@ int sfl_prefill_layers(const sfl_prefill_args* args, void* stream);
  * budget. A cache is k, v [batch, kv_heads, capacity, head_dim] of one dtype
  * (F32, BF16 or F16); sequence b has lengths[b] committed rows in slots
  * [0, lengths[b]) and its drafts' rows from slot lengths[b] on. head_dim 16, 32,
- * 64 or 128. `strides`: one array of strides in elements, per tensor {batch,
- * head, row}; the last dimension is contiguous. Lengths, counts, positions and
+ * 64 or 128, capacity at most SFL_CACHE_MAX_SLOTS. `strides`: one array of strides
+ * in elements, per tensor {batch, head, row}; the last dimension is contiguous. Lengths, counts, positions and
  * paths are read on the device: values outside their range are clamped or their
  * rows left out, never followed out of a buffer.
  */
+
+#define SFL_CACHE_MAX_SLOTS (1 << 30)
 
 /*
  * Norm, rotation and cache append of new tokens, in one pass:

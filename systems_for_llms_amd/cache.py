@@ -14,6 +14,7 @@ from . import _lib
 from .decode import SUPPORTED_DIMS, SUPPORTED_GROUPS
 
 MAX_DRAFTS = 128
+MAX_ROWS = 1 << 30  # of a tensor's [B, H, rows, D]: the kernels count slots in 32 bits, a step or two past the last
 _STEPS = {dtype: 16 // dtype.itemsize for dtype in _lib.DTYPE_CODES}  # elements of 16 bytes
 
 
@@ -36,6 +37,8 @@ def check_rows(operator: str, names: tuple, tensors: tuple, aligned: bool = True
             raise ValueError(f"{name} must not be empty")
         if shape[3] not in SUPPORTED_DIMS:
             raise ValueError("supported head dimensions are 16/32/64/128")
+        if shape[2] > MAX_ROWS:
+            raise ValueError(f"{name} must have at most {MAX_ROWS} rows")
         sb, sh, sr, sd = t.stride()
         if sd != 1:
             raise ValueError(f"{name} must have a contiguous last dimension")

@@ -693,6 +693,8 @@ int check_rows(const char* what, const void* k, const void* v, const long* strid
   if (batch <= 0 || kv_heads <= 0 || capacity <= 0)
     return set_error(SFL_ERR_INVALID, "%s: batch, heads and capacity must be positive", what);
   if (long(batch) * kv_heads >= kMostHeads) return set_error(SFL_ERR_UNSUPPORTED, "%s: too many KV heads", what);
+  if (capacity > SFL_CACHE_MAX_SLOTS)  // slots are counted in 32 bits, up to a workgroup's step past the last
+    return set_error(SFL_ERR_UNSUPPORTED, "%s: at most %d slots", what, SFL_CACHE_MAX_SLOTS);
   const int es = elem_size(dtype);
   if (!es) return set_error(SFL_ERR_UNSUPPORTED, "%s: dtype must be F32, BF16 or F16", what);
   if (head_dim != 16 && head_dim != 32 && head_dim != 64 && head_dim != 128)
@@ -717,6 +719,8 @@ extern "C" int sfl_rotate(const void* q, const void* k, const void* v, const int
     return set_error(SFL_ERR_INVALID, "%s: null pointer argument", what);
   if (batch <= 0 || tokens <= 0 || q_heads <= 0 || kv_heads <= 0 || table <= 0 || slots <= 0)
     return set_error(SFL_ERR_INVALID, "%s: batch, tokens, heads, table and slots must be positive", what);
+  if (slots > SFL_CACHE_MAX_SLOTS)
+    return set_error(SFL_ERR_UNSUPPORTED, "%s: at most %d slots", what, SFL_CACHE_MAX_SLOTS);
   const int es = elem_size(dtype);
   if (!es) return set_error(SFL_ERR_UNSUPPORTED, "%s: dtype must be F32, BF16 or F16", what);
   if (head_dim != 16 && head_dim != 32 && head_dim != 64 && head_dim != 128)

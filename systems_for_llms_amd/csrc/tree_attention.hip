@@ -1007,6 +1007,8 @@ int fill(TreeArgs& a, const char* what, const void* q, const void* k, const int3
   if (!q || !k || !lengths || !mask || !lse || !strides) return set_error(SFL_ERR_INVALID, "%s: null pointer argument", what);
   if (batch <= 0 || q_heads <= 0 || kv_heads <= 0 || capacity <= 0 || tokens <= 0)
     return set_error(SFL_ERR_INVALID, "%s: batch, heads, capacity and tokens must be positive", what);
+  if (capacity > SFL_CACHE_MAX_SLOTS)  // slots are counted in 32 bits, up to a workgroup's round past the last
+    return set_error(SFL_ERR_UNSUPPORTED, "%s: at most %d slots", what, SFL_CACHE_MAX_SLOTS);
   if (tokens > kMaxDrafts) return set_error(SFL_ERR_UNSUPPORTED, "%s: at most %d drafted tokens", what, kMaxDrafts);
   if (q_heads % kv_heads) return set_error(SFL_ERR_INVALID, "%s: query heads must be divisible by KV heads", what);
   const int group = q_heads / kv_heads;

@@ -258,3 +258,31 @@ def test_entry_points_refuse_before_any_launch():
     compact = [p] * 5 + [strides(6), 1, 2, 16, 4, 64, f, None]
     for change, value, code in ((4, None, INVALID), (9, 17, INVALID), (10, 24, UNSUPPORTED), (11, 5, UNSUPPORTED)):
         assert _status("sfl_compact_slots", *[value if i == change else x for i, x in enumerate(compact)]) == code, change
+
+
+def test_caches_of_more_slots_than_the_kernels_count_are_refused():
+    """2^30 rows: an expanded view has that many without holding them."""
+    from systems_for_llms_amd.cache import MAX_ROWS
+
+    t = _tree()
+    lengths, path = t["lengths"], torch.zeros(2, 3, dtype=torch.int32)
+    new = torch.zeros(2, 2, 3, 64, dtype=torch.float16)
+    cos, sin = rotary.rotary_tables(64, 16)
+    for rows in (MAX_ROWS + 1, 2 ** 31 - 1, 2 ** 32 + 40):
+        k = torch.zeros(1, 1, 1, 64, dtype=torch.float16).expand(2, 2, rows, 64)
+        for call in (lambda: tree.prepare(t["q"], k, k, lengths),
+                     lambda: tree.accumulate(t["q"], k, torch.zeros(2, 8, 3), torch.zeros(2, 2, 40), lengths),
+                     lambda: tree.accept(k, k, lengths, path, lengths),
+                     lambda: evict.compact(torch.zeros(2, 2, 8, dtype=torch.int32), k, k),
+                     lambda: rotary.rotate_append(t["q"], new, new, path, cos, sin, k, k, lengths)):
+            with pytest.raises(ValueError, match="rows"):
+                call()
+    if not _lib.LIB_PATH.exists():
+        pytest.skip("libsfl.so not built")
+    many, p, f = MAX_ROWS + 1, 64, 1
+    strides = (ctypes.c_long * 18)(*[64] * 18)
+    assert _status("sfl_tree_attention", *[p] * 11, strides, 1, 4, 2, many, 3, 64, 1, 0.125, f, None) == UNSUPPORTED
+    assert _status("sfl_tree_weights", *[p] * 8, strides, 1, 4, 2, many, 3, 64, 0.125, f, None) == UNSUPPORTED
+    assert _status("sfl_accept_path", *[p] * 8, strides, 1, 2, many, 3, 64, f, None) == UNSUPPORTED
+    assert _status("sfl_compact_slots", *[p] * 5, strides, 1, 2, many, 4, 64, f, None) == UNSUPPORTED
+    assert _status("sfl_rotate", *[p] * 13, strides, 1, 3, 4, 2, 64, 64, 16, many, 0, f, 1e-5, f, None) == UNSUPPORTED
