@@ -311,7 +311,8 @@ constexpr int kMaxPath = 128;
 // Row len + j of a sequence's cache takes what row len + path[j] held, j < accepted.
 // One workgroup has all the rows of a (sequence, KV head) in one tensor and reads
 // every one before it writes any, so chains of rows that move are safe. Blocks in
-// y: k, v, the slot values (which also lose the rejected drafts' weights). Bound by
+// y: k, v, the slot values (which also lose the rejected drafts' weights); where k and
+// v are one tensor its rows move once. Bound by
 // latency: path, rows, stores (64 sequences, 9 MB: 6.5 us).
 struct AcceptArgs {
   void *k, *v;
@@ -348,6 +349,7 @@ __global__ __launch_bounds__(256) void accept_kernel(const AcceptArgs a) {
     if (a.positions && from >= 0) a.positions[base + len + j] = p;
     return;
   }
+  if (blockIdx.y == 1 && a.v == a.k) return;
   unsigned char* rows = static_cast<unsigned char*>(blockIdx.y ? a.v : a.k);
   const long stride = (blockIdx.y ? a.vs[2] : a.ks[2]) * a.elem_bytes;
   rows += (blockIdx.y ? b * a.vs[0] + hk * a.vs[1] : b * a.ks[0] + hk * a.ks[1]) * a.elem_bytes;

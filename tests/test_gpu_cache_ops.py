@@ -790,3 +790,19 @@ def test_tree_prepare_refuses_lengths_whose_sum_with_the_drafts_wraps():
             with pytest.raises(ValueError, match="each length"):
                 tree.prepare(q, k, k, lengths, counts=used)
     tree.prepare(q, k, k, torch.tensor([7, 9], dtype=torch.int32, device="cuda"), counts=counts)
+
+
+@pytest.mark.parametrize("tokens", [4, 100])
+def test_accept_of_keys_that_are_the_values_too(tokens):
+    """k and v one tensor: a chain of rows that take each other's place moves once."""
+    from systems_for_llms_amd import tree
+
+    g = torch.Generator().manual_seed(34 + tokens)
+    k = randn(g, 16, 4, tokens + 5, 64, dtype=BF16)
+    lengths = torch.randint(0, 6, (16,), generator=g, dtype=torch.int32)
+    path = torch.stack([(torch.arange(tokens) + 1 + i) % tokens for i in range(16)]).to(torch.int32)
+    accepted = torch.full((16,), tokens, dtype=torch.int32)
+    (want,), n = oc.accept([k], lengths, path, accepted)
+    gpu = k.cuda()
+    got = tree.accept(gpu, gpu, lengths.cuda(), path.cuda(), accepted.cuda())
+    assert torch.equal(got.cpu(), n) and torch.equal(gpu.cpu(), want)
