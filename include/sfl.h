@@ -501,7 +501,7 @@ int sfl_prefill_layers(const sfl_prefill_args* args, void* stream);
  *           q_out (and in k_out, v_out where start is NULL), nothing in a cache
  *   v, v_out: may be NULL (both)
  *   strides [18]: q, k, v, q_out, k_out, v_out
- * Outputs must not overlap inputs.
+ * Outputs must not overlap inputs or each other.
  */
 int sfl_rotate(const void* q, const void* k, const void* v, const int32_t* positions, const float* cos,
                const float* sin, const void* q_gain, const void* k_gain, const int32_t* start,

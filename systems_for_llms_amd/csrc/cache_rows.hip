@@ -732,6 +732,7 @@ extern "C" int sfl_rotate(const void* q, const void* k, const void* v, const int
   if (gain_dtype != dtype && gain_dtype != SFL_DTYPE_F32)
     return set_error(SFL_ERR_UNSUPPORTED, "%s: gains must have the dtype of q or F32", what);
   if (!(eps >= 0.f) || !__builtin_isfinite(eps)) return set_error(SFL_ERR_INVALID, "%s: eps must be finite and not negative", what);
+  if (v && k_out == v_out) return set_error(SFL_ERR_INVALID, "%s: k_out and v_out must not be the same memory", what);
   RotateArgs a{q, k, v, positions, cos, sin, q_gain, k_gain, start, counts, q_out, k_out, v_out};
   for (int i = 0; i < 18; ++i) a.st[i / 3][i % 3] = strides[i];
   a.batch = batch, a.tokens = tokens, a.q_heads = q_heads, a.kv_heads = kv_heads, a.half = rotary_dim / 2;

@@ -126,7 +126,8 @@ def rotate_append(q, k, v, positions, cos, sin, k_cache, v_cache, lengths, *, co
     (``[B, Hkv, N, D]`` views; slots they do not have are left out), v unchanged.
     ``positions`` are independent of the slots: drafts of a tree share positions, and
     after an eviction a slot is not a position. Tokens from ``counts[b]`` on are padding:
-    zero rows of q, and the cache stays as it was. ``lengths`` is not changed.
+    zero rows of q, and the cache stays as it was. ``lengths`` is not changed. The caches
+    are two tensors and share no memory with q, k and v.
     """
     index = _check("rotate_append", ("q", "k", "v", "k_cache", "v_cache"), (q, k, v, k_cache, v_cache), positions, cos,
                    sin, counts, layout, q_norm, k_norm, eps)

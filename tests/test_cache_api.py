@@ -286,3 +286,12 @@ def test_caches_of_more_slots_than_the_kernels_count_are_refused():
     assert _status("sfl_accept_path", *[p] * 8, strides, 1, 2, many, 3, 64, f, None) == UNSUPPORTED
     assert _status("sfl_compact_slots", *[p] * 5, strides, 1, 2, many, 4, 64, f, None) == UNSUPPORTED
     assert _status("sfl_rotate", *[p] * 13, strides, 1, 3, 4, 2, 64, 64, 16, many, 0, f, 1e-5, f, None) == UNSUPPORTED
+
+
+def test_append_of_k_and_v_to_the_same_rows_is_refused():
+    if not _lib.LIB_PATH.exists():
+        pytest.skip("libsfl.so not built")
+    p, f = 64, 1
+    strides = (ctypes.c_long * 18)(*[64] * 18)
+    tail = (strides, 1, 3, 4, 2, 64, 64, 16, 16, 0, f, 1e-5, f, None)
+    assert _status("sfl_rotate", *[p] * 11, 4096, 4096, *tail) == INVALID
