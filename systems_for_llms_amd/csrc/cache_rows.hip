@@ -215,8 +215,8 @@ __global__ __launch_bounds__(256) void rotate_rows_kernel(const RotateArgs a, in
     next = look(tok0 + stride + lead);
 #pragma unroll
     for (int i = 0; i < ANGLES; ++i) {
-      c[i] = !turned ? 1.f : known ? c[i] : NAN;
-      sn[i] = !turned ? 0.f : known ? sn[i] : NAN;
+      c[i] = known ? c[i] : NAN;
+      sn[i] = known ? sn[i] : NAN;
     }
 
     for (int h0 = first; h0 < heads; h0 += kRows * step) {  // uniform over the workgroup
@@ -246,7 +246,7 @@ __global__ __launch_bounds__(256) void rotate_rows_kernel(const RotateArgs a, in
 #pragma unroll
             for (int e = 0; e < VEC; ++e) v[e] = fmaf(second ? o[e] : -o[e], sn[e], v[e] * c[e]);
           }
-        } else {
+        } else if (turned) {
 #pragma unroll
           for (int e = 0; e < VEC; e += 2) {
             const float u = v[e], n = v[e + 1];

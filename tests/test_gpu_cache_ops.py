@@ -806,3 +806,36 @@ def test_accept_of_keys_that_are_the_values_too(tokens):
     gpu = k.cuda()
     got = tree.accept(gpu, gpu, lengths.cuda(), path.cuda(), accepted.cuda())
     assert torch.equal(got.cpu(), n) and torch.equal(gpu.cpu(), want)
+
+
+# ---- values that are no numbers -----------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("dim, rotary", [(128, 64), (64, 16), (32, 16)])
+def test_rotate_keeps_unturned_dimensions_beside_infinities(dtype, layout, dim, rotary):
+    """Infinities and NaN past the rotated part stay in their own places, at any alignment of the rows."""
+    from systems_for_llms_amd import rotary as rt
+
+    g = torch.Generator().manual_seed(dim)
+    cos, sin = rt.rotary_tables(rotary, 50)
+    positions = torch.randint(0, 50, (2, 5), generator=g, dtype=torch.int32)
+    q, k = randn(g, 2, 4, 5, dim, dtype=dtype), randn(g, 2, 2, 5, dim, dtype=dtype)
+    for x in (q, k):
+        x[..., rotary + 3] = float("inf")
+        x[:, :, 1, rotary] = float("nan")
+        x[:, :, 2, dim - 1] = float("-inf")
+    for shift in (0, 1):  # rows of whole 16-byte pieces, and others
+        moved = []
+        for x in (q, k):
+            wide = torch.zeros(*x.shape[:3], dim + 8, dtype=dtype, device="cuda")
+            wide[..., shift:shift + dim] = x.cuda()
+            moved.append(wide[..., shift:shift + dim])
+        got = rt.rotate(*moved, positions.cuda(), cos.cuda(), sin.cuda(), layout=layout)
+        for x, y in zip((q, k), got):
+            want, size = oc.rotate(x, positions, cos, sin, layout)
+            assert want[..., :rotary].isfinite().all()
+            within(y, want, rotate_bound(dtype, want, size), f"shift {shift}")
+            kept, exact = y[..., rotary:].cpu(), x[..., rotary:]
+            assert torch.equal(kept.nan_to_num(7, 8, 9), exact.nan_to_num(7, 8, 9)) and torch.equal(kept.isnan(), exact.isnan())
