@@ -5,7 +5,7 @@
 // key and the drafts j with mask[t, j]:
 //
 //   s = scale q . k over the keys in sight,  o = sum exp(s - m) v / l,
-//   m = max s,  l = sum exp(s - m),  lse = m + log l        (one pass, m and l running)
+//   m near max s,  l = sum exp(s - m),  lse = m + log l     (one pass, m and l running)
 //   weights[slot] += sum over counted drafts and the group's heads of exp(s - lse)
 //
 // The G query heads that share a KV head, times the T drafts, are one block of
@@ -26,6 +26,19 @@ constexpr int kTreeWaves = 4;
 constexpr int kTreeTile = 32;  // keys of a wave's tile: two MFMA tiles of 16
 constexpr int kMaxDrafts = 128;
 constexpr float kLn2 = 0.6931471805599453f;
+
+// Probabilities are exp2(score - m) with a reference m that moves seldom: to kProbBase below
+// the running maximum when that has come to lie more than kProbTop above m. They are rounded
+// to the type of V for the products. bf16 has the exponents of fp32 (m is a maximum itself);
+// fp16 ends at 2^16 and has its full 11 bits down to 2^-14, so probabilities take the top of
+// its range: one of w (relative to the row's largest) is off by at most half a step, 2^-11 of
+// it, where w >= 2^-25, and by 2^-36 below. (With m at the maximum the tail behind one heavy
+// key was lost from 2^-14 on, while the sum kept it. Rescaled more often, 512 rows over
+// 65536 fp16 keys take 97.6 us instead of 95.4.)
+template <typename T>
+constexpr float kProbTop = std::is_same<T, f16_t>::value ? 15.f : kLazyMax;
+template <typename T>
+constexpr float kProbBase = std::is_same<T, f16_t>::value ? 11.f : 0.f;
 
 struct TreeArgs {
   const void *q, *k, *v;
@@ -144,8 +157,8 @@ struct TreeOps {
 
   // acc[f] += V^T P^T for the tile; p[h][i] the lane's probabilities. 16-bit types round
   // them to the type of V, as the products of the matrix cores ask: each is off by at
-  // most half a step (bf16 2^-8, fp16 2^-11 of its value), of either sign, which over
-  // many keys stays near the rounding of the output itself; l sums them unrounded.
+  // most half a step (bf16 2^-8, fp16 2^-11 of its value; kProbBase), of either sign, which
+  // over many keys stays near the rounding of the output itself; l sums them unrounded.
   static __device__ __forceinline__ void add_pv(const uint32_t (&v)[8][kWords], const float (&p)[2][4], f32x4 (&acc)[kVec]) {
     if constexpr (kF32) {
 #pragma unroll
@@ -256,9 +269,9 @@ __device__ __forceinline__ void tile_step(const uint4 (*kt)[D / 8], const uint4 
 #pragma unroll
   for (int j = 2; j < 16; j += 2) mx = fmaxf(fmaxf(mx, s[j]), s[j + 1]);
   mx = fmaxf(mx, lane_xor(mx, 32));
-  const bool grow = mx * cs > m + kLazyMax;  // the lazy maximum, as below
+  const bool grow = mx * cs > m + kProbTop<T>;  // seldom, as below
   if (__ballot(grow)) {
-    const float mn = grow ? mx * cs : m;
+    const float mn = grow ? mx * cs - kProbBase<T> : m;
     const float alpha = grow ? __builtin_amdgcn_exp2f(m - mn) : 1.f;
     m = mn;
     l *= alpha;
@@ -281,8 +294,8 @@ __device__ __forceinline__ void tile_step(const uint4 (*kt)[D / 8], const uint4 
     sum[j & 1] += p[j];
   }
   l += sum[0] + sum[1];
-  // Probabilities in the type of V for the products, half a step each and of either
-  // sign; l sums them unrounded.
+  // Probabilities in the type of V for the products, half a step each (kProbBase) and of
+  // either sign; l sums them unrounded.
   const auto pack8 = [](const float* x) {
     return u32x4{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7])};
   };
@@ -627,11 +640,11 @@ __global__ __launch_bounds__(kTreeWaves * kWave) void tree_attention_kernel(cons
                          fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
         mx = fmaxf(mx, lane_xor(mx, 16));
         mx = fmaxf(mx, lane_xor(mx, 32));
-        // Lazy maximum: m moves only when the tile's is larger by kLazyMax, so that
-        // probabilities stay below 2^kLazyMax and the sums are rescaled seldom.
-        const bool grow = mx * a.cs > m[rt] + kLazyMax;
+        // m moves only when the tile's maximum is more than kProbTop above it, so that
+        // probabilities stay below 2^kProbTop and the sums are rescaled seldom.
+        const bool grow = mx * a.cs > m[rt] + kProbTop<T>;
         if (__ballot(grow)) {
-          const float mn = grow ? mx * a.cs : m[rt];
+          const float mn = grow ? mx * a.cs - kProbBase<T> : m[rt];
           const float alpha = grow ? __builtin_amdgcn_exp2f(m[rt] - mn) : 1.f;
           m[rt] = mn;
           l[rt] *= alpha;

@@ -839,3 +839,54 @@ def test_rotate_keeps_unturned_dimensions_beside_infinities(dtype, layout, dim, 
             within(y, want, rotate_bound(dtype, want, size), f"shift {shift}")
             kept, exact = y[..., rotary:].cpu(), x[..., rotary:]
             assert torch.equal(kept.nan_to_num(7, 8, 9), exact.nan_to_num(7, 8, 9)) and torch.equal(kept.isnan(), exact.isnan())
+
+
+# ---- light keys behind a heavy one --------------------------------------------------
+
+
+def far_rows(x, elements):
+    """The rows of x [1, 1, N, D] as a view of rows ``elements`` apart."""
+    rows, dim = x.shape[2:]
+    block = torch.zeros(rows * elements, dtype=x.dtype, device="cuda")
+    view = block.as_strided((1, 1, rows, dim), (rows * elements, rows * elements, elements, 1))
+    view.copy_(x)
+    return view
+
+
+@pytest.mark.parametrize("dtype, dim, group, tokens, far", [
+    (FP16, 64, 1, 1, False), (FP16, 128, 8, 4, False), (FP16, 64, 8, 7, False), (FP16, 128, 8, 9, False),
+    (FP16, 64, 8, 17, False), (FP16, 32, 2, 3, False), (FP16, 16, 8, 3, False), (FP16, 32, 8, 9, False),
+    (FP16, 128, 4, 5, True), (BF16, 128, 8, 9, False), (BF16, 32, 8, 3, False), (FP32, 128, 4, 3, False)])
+@pytest.mark.parametrize("heavy", [0, 9001, 17999])
+def test_tree_attention_keeps_the_tail_behind_a_heavy_key(dtype, dim, group, tokens, far, heavy):
+    """One key with a value of 0 takes nearly all of the weight, and 18000 of 2^-18 to 2^-30 of it make the output.
+
+    A probability w (relative to the largest) is rounded by half a step where it is at least
+    2^-25 and by at most 2^-36 below (2^11 w is then an fp16 number under 2^-14, whose half step is 2^-25).
+    """
+    from systems_for_llms_amd import tree
+
+    g = torch.Generator().manual_seed(dim + group + heavy)
+    n = 18000
+    k, v = torch.zeros(2, 1, 1, n + tokens, dim).unbind(0)
+    k[:, :, heavy, 0] = 4
+    v[...] = 1 + 0.25 * torch.randn(v.shape, generator=g)
+    v[:, :, heavy] = 0
+    q = torch.zeros(1, group, tokens, dim)
+    rows = group * tokens
+    bits = torch.linspace(18, 30, rows)[torch.randperm(rows, generator=g)] if rows > 1 else torch.tensor([24.4])
+    q[..., 0] = (bits / 32).reshape(1, group, tokens)  # a score of bits / 8 for the heavy key
+    scale = 8 * 0.6931471805599453
+    q, k, v = (x.to(dtype) for x in (q, k, v))
+    lengths = torch.tensor([n], dtype=torch.int32)
+    mask = torch.ones(tokens, tokens, dtype=torch.bool).tril()
+    out, lse, spread, size = oc.tree_attention(q, k, v, lengths, mask, None, scale)
+    bound, lse_bound = tree_bounds(dtype, dim, n + tokens, out, lse, spread, size)
+    if dtype == FP16:
+        bound = bound + (n + tokens) * 2.0 ** -36 * float(v.abs().max())
+    stride = 62000  # 62000 * 2 * 18005 bytes pass 2^31
+    gk, gv = (far_rows(x, stride) if far else x.cuda() for x in (k, v))
+    for splits in (1, 5):
+        got = tree.attend(q.cuda(), gk, gv, lengths.cuda(), mask.cuda(), splits=splits, scale=scale)
+        within(got[1], lse, lse_bound, f"lse, {splits} splits")
+        within(got[0], out, bound, f"out, {splits} splits")
