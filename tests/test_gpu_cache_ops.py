@@ -890,3 +890,89 @@ def test_tree_attention_keeps_the_tail_behind_a_heavy_key(dtype, dim, group, tok
         got = tree.attend(q.cuda(), gk, gv, lengths.cuda(), mask.cuda(), splits=splits, scale=scale)
         within(got[1], lse, lse_bound, f"lse, {splits} splits")
         within(got[0], out, bound, f"out, {splits} splits")
+
+
+# ---- more splits, tiles and passes than the cases above reach ------------------------
+
+
+@pytest.mark.parametrize("dtype, dim, group, tokens", [(BF16, 128, 8, 1), (FP16, 64, 4, 3), (FP32, 64, 2, 3), (BF16, 32, 2, 2)])
+@pytest.mark.parametrize("splits", [9, 17, 33, 128])
+def test_tree_attention_of_many_splits(dtype, dim, group, tokens, splits):
+    """Rounds of splits in the merge whose maxima rise, fall and do both."""
+    g = torch.Generator().manual_seed(splits)
+    keys = 128 * splits + 70
+    place = torch.linspace(0, 1, keys)
+    size = torch.stack([0.3 + 1.5 * place, 1.8 - 1.5 * place, 1 + 0.8 * torch.sin(40 * place)])
+    q = randn(g, 3, group, tokens, dim, dtype=dtype, scale=1.5)
+    k = (torch.randn(3, 1, keys, dim, generator=g) * size[:, None, :, None]).to(dtype)
+    v = randn(g, 3, 1, keys, dim, dtype=dtype)
+    lengths = torch.tensor([keys - tokens, keys - 61, keys // 2], dtype=torch.int32)
+    check_tree(q, k, v, lengths, None, None, splits)
+
+
+@pytest.mark.parametrize("dtype, dim, group, tokens, keys", [
+    (BF16, 128, 8, 16, 5000), (FP16, 128, 4, 50, 2100), (BF16, 128, 8, 7, 5000), (BF16, 64, 8, 20, 3001), (FP32, 128, 8, 5, 2500),
+    (FP32, 32, 4, 30, 2500), (BF16, 16, 8, 20, 4000)])
+def test_tree_attention_of_many_rows_and_keys(dtype, dim, group, tokens, keys):
+    """Each row form over many tiles of committed keys, alone and shared by splits."""
+    g = torch.Generator().manual_seed(keys + tokens)
+    q = randn(g, 1, group, tokens, dim, dtype=dtype, scale=1.5)
+    k, v = (randn(g, 1, 1, keys + tokens, dim, dtype=dtype) for _ in range(2))
+    for splits in (1, None):
+        check_tree(q, k, v, torch.tensor([keys], dtype=torch.int32), random_mask(g, 1, tokens), None, splits)
+
+
+def test_tree_attention_of_many_rows_over_rows_far_apart():
+    """72 query rows over a head's cache of more than 2 GiB."""
+    from systems_for_llms_amd import tree
+
+    g = torch.Generator().manual_seed(91)
+    keys, tokens = 700, 9
+    q = randn(g, 1, 8, tokens, 64, dtype=BF16)
+    k, v = (randn(g, 1, 1, keys, 64, dtype=BF16) for _ in range(2))
+    lengths, mask = torch.tensor([keys - tokens], dtype=torch.int32), random_mask(g, 1, tokens)
+    gk, gv = (far_rows(x, 64 * 25000) for x in (k, v))
+    for splits in (1, 3):
+        check_tree(q, k, v, lengths, mask, got=tree.attend(q.cuda(), gk, gv, lengths.cuda(), mask.cuda(), splits=splits))
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("dim", [16, 64, 128])
+@pytest.mark.parametrize("tokens, group", [(3, 2), (9, 8)])
+def test_tree_attention_of_committed_infinities(dtype, dim, tokens, group):
+    """Infinite and NaN values of committed keys reach every row that sees them, in their own dimension only."""
+    g = torch.Generator().manual_seed(dim + tokens)
+    n = 400
+    q = randn(g, 2, group, tokens, dim, dtype=dtype)
+    k, v = (randn(g, 2, 1, n + tokens, dim, dtype=dtype) for _ in range(2))
+    lengths = torch.tensor([n, n - 101], dtype=torch.int32)
+    v[:, :, 5, 1] = float("inf")
+    v[0, :, 250, 2] = float("-inf")
+    v[0, :, 40, 3] = v[1, :, n - 102, 3] = float("inf")
+    v[0, :, 350, 3] = float("-inf")
+    v[:, :, 130, 4] = float("nan")
+    for splits in (1, 3):
+        check_tree(q, k, v, lengths, random_mask(g, 2, tokens), None, splits)
+    k[1, :, 77, 7] = float("nan")  # every score of the sequence's rows with this key
+    check_tree(q, k, v, lengths, random_mask(g, 2, tokens), None, 2)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("batch, kv_heads, group, tokens, keys, dim", [(64, 16, 2, 40, 400, 16), (64, 16, 1, 4, 700, 32),
+                                                                        (32, 16, 1, 5, 900, 128), (20, 16, 4, 3, 1500, 64)])
+def test_weights_of_many_tiles(dtype, batch, kv_heads, group, tokens, keys, dim):
+    """Shares of several tiles for each wave, in the first case walked once for every 64 (fp32: 32) counted rows."""
+    g = torch.Generator().manual_seed(batch + keys)
+    q = randn(g, batch, kv_heads * group, tokens, dim, dtype=dtype)
+    k = randn(g, batch, kv_heads, keys + tokens, dim, dtype=dtype)
+    lengths = torch.randint(keys // 2, keys + 1, (batch,), generator=g, dtype=torch.int32)
+    lengths[0] = keys
+    counts = torch.randint(1, tokens + 1, (batch,), generator=g, dtype=torch.int32)
+    counts[0] = tokens
+    mask = random_mask(g, batch, tokens)
+    # Any reference that keeps the weights near 1 will do for lse.
+    lse = torch.full((batch, kv_heads * group, tokens), 5.0) + torch.rand(batch, kv_heads * group, tokens, generator=g)
+    weights = torch.rand(batch, kv_heads, keys + tokens, generator=g)
+    rows = torch.rand(batch, tokens, generator=g) < 0.9
+    rows[0] = True
+    check_weights(q, k, lse, weights, lengths, mask, counts, rows)
