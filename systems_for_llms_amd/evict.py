@@ -7,7 +7,8 @@ slots ``[0, keep)``. A slot that stays and lies there already does not move: the
 that stay above ``keep`` fill the holes below it, so an eviction moves no more rows than
 it must (attention does not care for the order of its keys, whose rotation is in them).
 Slots are then no longer in the order of their tokens; ``positions`` keeps track of that
-for the next ``select``. Both calls only touch the device and can be captured.
+for the next ``select``: the program writes a token's position into its slot, for every KV
+head, when it appends it, and ``tree.accept`` and ``compact`` move it with the row. Both calls only touch the device and can be captured.
 """
 
 from __future__ import annotations
@@ -29,7 +30,8 @@ def select(weights, lengths, keep, *, recent=0, positions=None):
     places, in ascending order, take the slots from ``keep`` on that stay, in ascending
     order. A sequence of at most ``keep`` slots keeps them all, followed by -1.
     ``recent``: a slot stays before all others when its position is above its head's largest
-    minus ``recent``; ``positions`` int32 ``[B, Hkv, N]`` (default: a slot's index). Equal
+    minus ``recent``; ``positions`` int32 ``[B, Hkv, N]``, written by the program for each
+    token it appends (default: a slot's index, the age until slots have moved). Equal
     weights stay from the lowest slot on, as do recent slots that share positions and are
     more than ``keep``; NaN counts below every number.
     ``new_lengths`` is ``min(lengths, keep)``.

@@ -206,6 +206,7 @@ def accept(k, v, lengths, path, accepted, *, weights=None, positions=None):
     first ``accepted[b]`` entries of ``path`` (int32 ``[B, T]``, drafts by index, T at most 128).
     ``weights`` (fp32) and ``positions`` (int32), ``[B, Hkv, N]``, move with them, and the
     weights of the rejected drafts' slots become 0, as ``accumulate`` adds to them next time.
+    The positions of the drafts' slots are the program's to write before the call.
     Entries that name no draft or slot move nothing.
     """
     index = cache.check_rows("accept", ("k", "v"), (k, v))

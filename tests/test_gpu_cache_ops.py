@@ -976,3 +976,53 @@ def test_weights_of_many_tiles(dtype, batch, kv_heads, group, tokens, keys, dim)
     rows = torch.rand(batch, tokens, generator=g) < 0.9
     rows[0] = True
     check_weights(q, k, lse, weights, lengths, mask, counts, rows)
+
+
+def test_steps_that_write_their_positions_by_slot():
+    """Padded drafts at the end of a full cache too: evictions keep the newest tokens and the heaviest others."""
+    from systems_for_llms_amd import evict, tree
+
+    g = torch.Generator().manual_seed(95)
+    B, Hkv, N, T = 2, 3, 26, 4
+    k, v = torch.zeros(2, B, Hkv, N, 32, device="cuda").unbind(0)
+    weights = torch.zeros(B, Hkv, N, device="cuda")
+    positions = torch.zeros(B, Hkv, N, dtype=torch.int32, device="cuda")
+    slots = torch.arange(N, dtype=torch.int32, device="cuda")
+    lengths = torch.zeros(B, dtype=torch.int32, device="cuda")
+    written = torch.zeros(B, dtype=torch.int64)  # tokens committed so far
+    evictions = 0
+    for step in range(30):
+        counts = torch.randint(1, T + 1, (B,), generator=g, dtype=torch.int32)
+        token_positions = (written[:, None] + torch.arange(T)).to(torch.int32)
+        at = lengths.tolist()
+        before, new_positions, new_counts = positions.clone(), token_positions.cuda(), counts.cuda()
+        draft = slots - lengths[:, None]
+        new = ((draft >= 0) & (draft < new_counts[:, None]))[:, None]
+        positions.copy_(torch.where(new, new_positions.gather(1, draft.clamp(0, T - 1).long())[:, None], positions))
+        want = before.cpu()
+        for b in range(B):
+            for j in range(int(counts[b])):
+                if at[b] + j < N:
+                    want[b, :, at[b] + j] = token_positions[b, j]
+        assert torch.equal(positions.cpu(), want)
+        weights += torch.rand(B, Hkv, N, generator=g).cuda() * (slots < (lengths + new_counts)[:, None])[:, None]
+        accepted = torch.minimum(torch.randint(0, T + 1, (B,), generator=g, dtype=torch.int32), counts)
+        accepted = torch.minimum(accepted, torch.tensor([N - n for n in at], dtype=torch.int32))
+        path = torch.arange(T, dtype=torch.int32).expand(B, T).contiguous()
+        lengths.copy_(tree.accept(k, v, lengths, path.cuda(), accepted.cuda(), weights=weights, positions=positions))
+        written += accepted
+        if int(lengths.max()) == N or step % 9 == 8:
+            held, heavy, used = positions.cpu(), weights.cpu(), lengths.cpu()
+            _, n = evict.evict(k, v, weights, lengths, 15, recent=6, positions=positions)
+            lengths.copy_(n)
+            for b in range(B):
+                for h in range(Hkv):
+                    stay = set(positions[b, h, : int(n[b])].tolist())
+                    assert len(stay) == int(n[b])
+                    newest = held[b, h, : int(used[b])].sort().values[-6:].tolist()
+                    assert newest == list(range(int(written[b]) - len(newest), int(written[b]))) and stay >= set(newest)
+                    others = [i for i in range(int(used[b])) if int(held[b, h, i]) not in newest]
+                    others.sort(key=lambda i: -float(heavy[b, h, i]))
+                    assert stay == set(newest) | {int(held[b, h, i]) for i in others[: int(n[b]) - len(newest)]}
+            evictions += 1
+    assert evictions > 2
