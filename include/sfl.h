@@ -544,8 +544,8 @@ int sfl_tree_weights(const void* q, const void* k, const float* lse, float* weig
  * Commits an accepted path: slot lengths[b] + j takes the rows (k, v, and weights and
  * positions [batch, kv_heads, capacity] where not NULL) that slot lengths[b] + path[b, j]
  * held before the call, for j < accepted[b]; new_lengths[b] = lengths[b] + accepted[b].
- * The weights of the slots of the other drafts become 0. path [batch, tokens] int32,
- * tokens at most 128; entries outside [0, tokens) or the cache move nothing. accepted is
+ * The weights of the slots of the other drafts become 0. path [batch, tokens] int32 for
+ * the `tokens` drafts of the step, at most 128; entries outside [0, tokens) or the cache move nothing. accepted is
  * clamped to [0, tokens] and to what the cache holds. new_lengths is not lengths.
  * strides [6]: k, v, multiples of 16 bytes, k and v 16-byte aligned.
  */

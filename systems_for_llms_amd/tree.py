@@ -37,7 +37,9 @@ def ancestor_mask(parents: torch.Tensor) -> torch.Tensor:
     """The bool mask ``[..., T, T]`` of token trees: draft t sees itself and its ancestors.
 
     ``parents`` ``[..., T]`` holds each draft's parent draft, -1 for those that follow the
-    committed text; a parent comes before its children.
+    committed text; a parent comes before its children. The check of that is read back
+    (so the call stays outside graph captures), and the rows are formed one after another
+    by elementary operations, some ten a draft.
     """
     if parents.ndim < 1 or parents.dtype not in (torch.int32, torch.int64):
         raise ValueError("parents must be an integer tensor [..., T]")
@@ -173,7 +175,7 @@ def prepare(q, k, v, lengths, mask=None, *, counts=None, splits=None, scale=None
 
 
 def attend(q, k, v, lengths, mask=None, *, counts=None, splits=None, scale=None):
-    """Allocate scratch and compute once on the current stream: ``(out, lse)``."""
+    """``prepare`` and compute once on the current stream, outside captures: ``(out, lse)``."""
     op = prepare(q, k, v, lengths, mask, counts=counts, splits=splits, scale=scale)
     return op(), op.lse
 
@@ -183,8 +185,8 @@ def accumulate(q, k, lse, weights, lengths, mask=None, *, counts=None, rows=None
 
     Every slot gains ``exp(scale * q . k - lse)`` of each draft that sees it, over the query
     heads of its KV head; ``lse`` fp32 ``[B, Hq, T]`` is that of the attention call. ``rows``
-    bool ``[B, T]``: the drafts that count (default: all in use). Call it before ``accept``,
-    which moves the slots.
+    bool ``[B, T]``: the drafts that count (default: all in use). Without a ``mask`` one is
+    built by every call. Call it before ``accept``, which moves the slots.
     """
     mask, index = _check("accumulate", ("q", "k"), (q, k), lengths, mask, counts)
     batch, heads, tokens, dim = q.shape
@@ -203,11 +205,12 @@ def accept(k, v, lengths, path, accepted, *, weights=None, positions=None):
     """Commit an accepted path in place and return the new lengths (a new tensor).
 
     Slot ``lengths[b] + j`` takes the rows that slot ``lengths[b] + path[b, j]`` held, for the
-    first ``accepted[b]`` entries of ``path`` (int32 ``[B, T]``, drafts by index, T at most 128).
+    first ``accepted[b]`` entries of ``path`` (int32 ``[B, T]`` for the T drafts of the step, at
+    most 128, drafts by index; one may stand in several entries).
     ``weights`` (fp32) and ``positions`` (int32), ``[B, Hkv, N]``, move with them, and the
     weights of the rejected drafts' slots become 0, as ``accumulate`` adds to them next time.
     The positions of the drafts' slots are the program's to write before the call.
-    Entries that name no draft or slot move nothing.
+    Entries outside ``[0, T)`` or the cache move nothing.
     """
     index = cache.check_rows("accept", ("k", "v"), (k, v))
     cache.check_cache(k, v)
