@@ -65,6 +65,8 @@ __device__ __forceinline__ float gain_at(const RotateArgs& a, const void* gain, 
 }
 
 // One wave per row, a row staged in LDS as fp32: any layout, rotated part and alignment.
+// Bound by its scalar accesses: 4 x 4001 tokens of 48 fp16 heads of 128 390 us, in
+// 16-byte pieces (below) 82.
 template <typename T, bool kHalfLayout>
 __global__ __launch_bounds__(256) void rotate_any_kernel(const RotateArgs a, int dim, unsigned rows, unsigned heads) {
   __shared__ float stage[4][128];
@@ -793,6 +795,9 @@ extern "C" int sfl_select_slots(const float* weights, const int32_t* lengths, co
     return set_error(SFL_ERR_INVALID, "%s: keep must be in [1, capacity] and recent in [0, keep]", what);
   if (long(batch) * kv_heads >= kMostHeads) return set_error(SFL_ERR_UNSUPPORTED, "%s: too many KV heads", what);
   const SelectArgs a{weights, lengths, positions, kept, new_lengths, kv_heads, capacity, keep, recent};
+  // By the capacity, as the slots in use are known on the device only. Keys held / formed again,
+  // us with 8 and 32 heads: 24573 slots 23.7, 26.8 / 29.7, 30.2; 5000 slots in use 12.7 either way.
+  // Past that: 32768 slots 37, 131072 141 (32 heads 169), 262144 273.
   const bool held = capacity <= 24 * kSelectThreads;  // 96 KB of keys
   const unsigned bytes = unsigned((capacity + 63) / 64) * 12u + (held ? 4u * unsigned(capacity) : 0u);
   const auto kernel = held ? select_kernel<true> : select_kernel<false>;

@@ -231,7 +231,7 @@ __device__ __forceinline__ TreeBlock tree_block(const TreeArgs& a) {
 // workgroup a tile is read from memory once for all of them and the waves bound it:
 // for each tile 16 MFMAs (0.25 us), 102 VALU instructions, 16 of them exp (0.28), and
 // 24 LDS reads (0.23), of which two waves to a SIMD overlap little. Measured: 512 rows
-// over 65536 keys of 4 heads 87 us (789 TFLOP/s; the 16-row kernel 170), 8 sequences of
+// over 65536 fp16 keys of 4 heads 90 us (765 TFLOP/s; the 16-row kernel 170), 8 sequences of
 // 108 rows over 1K to 8K keys of 8 heads 44 us (3.8 TB/s), 8 rows over 1024 keys 8 us.
 template <int D, int WR>
 struct TileShape {
@@ -829,8 +829,10 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(const TreeArgs a) {
 // registers while K streams by, the next tile's keys and weights loaded ahead (more
 // rows: another pass over the share, whose keys then come from L2). Bound by reading
 // K: 16 rows of up to 8K keys of 16 heads of 64, 169 MB, 40 us (4.2 TB/s; without the
-// loads ahead and with a workgroup for every 128 keys 60). Every slot has one writer,
-// and its terms one order.
+// loads ahead and with a workgroup for every 128 keys 60); one row of 4 short sequences
+// (kernel 6.9 us for 2.3 of bytes) by the chain of length, rows, scores and store; many
+// rows by the passes: 512 rows over 32768 keys of 4 heads of 128 122 us in bf16 (141
+// TFLOP/s), 393 in fp32 (44). Every slot has one writer, and its terms one order.
 template <typename T, int D, int NT>
 __global__ __launch_bounds__(kTreeWaves * kWave) void tree_weights_kernel(const TreeArgs a, const uint8_t* __restrict__ counted,
                                                                           float* __restrict__ weights) {
@@ -959,7 +961,11 @@ int launch_tree(TreeArgs& a, hipStream_t stream) {
   const int rows = a.tokens << a.group_log2;
   constexpr bool kF32 = std::is_same<T, float>::value;
   if constexpr (!kF32 && D >= 64) {
-    // Buffer offsets are 32 bits; caches of 2 GiB a head and more take the kernel below.
+    // Buffer offsets are 32 bits; caches of 2 GiB a head and more take the kernel below (a call
+    // over 8192 keys of one such head: 8 rows 13.5 us, 128 rows 14.8).
+    // By rows, us with 1 / 2 / 4 waves to a tile, 64 heads of 4096 bf16 keys: D 128 32 rows
+    // 31.5 / 28.9 / 31.8, 64 rows 38.7 / 31.6 / 34.5, 128 rows 96 / 48 / 44; D 64 8 rows
+    // 18.2 / 18.1 / 22.7, 64 rows 21.1 / 20.2 / 25.8, 128 rows 43.2 / 29.3 / 29.4.
     if (long(a.cap) * std::max(a.ks[2], a.vs[2]) * 2 < (1L << 31)) {
       if (rows <= 32) return launch_blocks<T, D>(tree_tile_kernel<T, D, 1>, 32, a, stream);
       if (rows <= 64) return launch_blocks<T, D>(tree_tile_kernel<T, D, 2>, 64, a, stream);
@@ -967,10 +973,14 @@ int launch_tree(TreeArgs& a, hipStream_t stream) {
     }
     return launch_blocks<T, D>(tree_attention_kernel<T, D, 1>, 16, a, stream);
   } else {
+    // us with blocks of 16 / 32 / 64 rows, 64 heads of 4096 keys: bf16 D 32 16 rows 12.6 / 13.2 /
+    // 17.7, 32 rows 13.7 / 13.7 / 18.2, 64 rows 20.1 / 17.9 / 19.7, 128 rows 30.4 / 26.0 / 27.1;
+    // fp32 D 64 16 rows 26 / 33, 32 rows 37 / 33, 128 rows 102 / 90.
     if (rows <= 16) return launch_blocks<T, D>(tree_attention_kernel<T, D, 1>, 16, a, stream);
     if constexpr (kF32) {
       // Heads of 128 with 32 rows leave a SIMD one wave: 11 sequences of 88 rows over up to
-      // 8K keys 290 us, with 16 rows 168.
+      // 8K keys 290 us, with 16 rows 168; where a few workgroups do not decide the time, 16 rows
+      // lose to 32 (64 heads of 4096 keys: 32 rows 67 / 59 us, 128 rows 204 / 169).
       constexpr int RT = D == 128 ? 1 : 2;
       return launch_blocks<T, D>(tree_attention_kernel<T, D, RT>, 16 * RT, a, stream);
     } else {
@@ -986,6 +996,9 @@ int launch_weights(TreeArgs& a, const uint8_t* counted, float* weights, hipStrea
   const int rounds = (a.cap + kTreeTile * kTreeWaves - 1) / (kTreeTile * kTreeWaves);
   a.splits = std::max(1, std::min(rounds, (1024 + a.groups - 1) / a.groups));
   if (long(a.groups) * a.splits >= kMostGroups) return set_error(SFL_ERR_UNSUPPORTED, "tree_weights: too many workgroups");
+  // Rows held in registers, in tiles of 16: us with 1 / 2 / 4 tiles, 64 heads of 4096 keys of 128,
+  // bf16 16 rows 17.2 / 16.9 / 17.9, 32 rows 29.6 / 19.2 / 20.4, 64 rows 50 / 33 / 26; fp32 16 rows
+  // 30 / 39, 64 rows 96 / 93.
   const int rows = a.tokens << a.group_log2;
   constexpr int kMost = std::is_same<T, float>::value ? 2 : 4;
   const auto kernel = rows <= 16 ? tree_weights_kernel<T, D, 1> : rows <= 32 ? tree_weights_kernel<T, D, 2> : tree_weights_kernel<T, D, kMost>;

@@ -95,7 +95,10 @@ def auto_splits(batch: int, kv_heads: int, capacity: int, rows: int, dim: int, d
     reads them all, of at least 128 keys. Measured, us at 8 / 16 / 32 / 64 splits: B=1 Hkv=4
     N=65536 512 rows 155 / 98 / 94 / 110; B=4 Hkv=4 D=64 N=16384 64 rows 26 / 20 / 22 / 27;
     B=1 Hkv=4 N=8192 32 rows 19 / 16 / 16 / 18; B=8 Hkv=8 N=8191 108 rows 71 / 87 / 112 /
-    164; fp32 B=2 Hkv=4 D=128 N=8192 64 rows 39 / 37 / 43 / 56.
+    164; fp32 B=2 Hkv=4 D=128 N=8192 64 rows 39 / 37 / 43 / 56. A few rows over one long cache
+    (us at 16 / 32 / 64 / 128, 8 rows): Hkv=4 N=65536 40 / 29 / 32 / 38, N=131072 70 / 50 / 51 / 56;
+    Hkv=1 N=65536 40 / 27 / 22 / 22, N=131072 69 / 41 / 29 / 27, so with one or two KV heads
+    ``splits=64`` is the better choice there.
     """
     tiled = dtype != torch.float32 and dim >= 64
     block = 128 if tiled else 64 if dtype != torch.float32 else 16 if dim == 128 else 32
@@ -147,8 +150,9 @@ def prepare(q, k, v, lengths, mask=None, *, counts=None, splits=None, scale=None
     ``[T, T]`` or ``[B, T, T]``: whether draft t sees draft j, itself included (default: all
     up to itself). ``counts`` int32 ``[B]``: drafts in use; the rows of the others are zeros
     with an ``lse`` of -inf, as are those of drafts that see nothing. What a draft does not
-    see has no part in its row, NaN included. ``splits``: workgroups that share a KV head's
-    keys, 1 to 128 (default by size).
+    see has no part in its row, NaN included; an infinite value that it sees with a weight too
+    small for the products (in fp16 below 2^-36 of the row's largest) can give NaN.
+    ``splits``: workgroups that share a KV head's keys, 1 to 128 (default by size).
     """
     if splits is not None and (type(splits) is not int or not 1 <= splits <= MAX_SPLITS):
         raise ValueError("splits must be an integer in [1, 128]")
