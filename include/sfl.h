@@ -478,9 +478,9 @@ int sfl_prefill_layers(const sfl_prefill_args* args, void* stream);
  * (F32, BF16 or F16); sequence b has lengths[b] committed rows in slots
  * [0, lengths[b]) and its drafts' rows from slot lengths[b] on. head_dim 16, 32,
  * 64 or 128, capacity at most SFL_CACHE_MAX_SLOTS. `strides`: one array of strides
- * in elements, per tensor {batch, head, row}; the last dimension is contiguous. Lengths, counts, positions and
- * paths are read on the device: values outside their range are clamped or their
- * rows left out, never followed out of a buffer.
+ * in elements, per tensor {batch, head, row}; the last dimension is contiguous.
+ * Lengths, counts, positions and paths are read on the device: values outside their
+ * range are clamped or their rows left out, never followed out of a buffer.
  */
 
 #define SFL_CACHE_MAX_SLOTS (1 << 30)
@@ -545,8 +545,9 @@ int sfl_tree_weights(const void* q, const void* k, const float* lse, float* weig
  * positions [batch, kv_heads, capacity] where not NULL) that slot lengths[b] + path[b, j]
  * held before the call, for j < accepted[b]; new_lengths[b] = lengths[b] + accepted[b].
  * The weights of the slots of the other drafts become 0. path [batch, tokens] int32 for
- * the `tokens` drafts of the step, at most 128; entries outside [0, tokens) or the cache move nothing. accepted is
- * clamped to [0, tokens] and to what the cache holds. new_lengths is not lengths.
+ * the `tokens` drafts of the step, at most 128; entries outside [0, tokens) or the cache
+ * move nothing. accepted is clamped to [0, tokens] and to what the cache holds.
+ * new_lengths is not lengths. k and v may be one tensor.
  * strides [6]: k, v, multiples of 16 bytes, k and v 16-byte aligned.
  */
 int sfl_accept_path(void* k, void* v, float* weights, int32_t* positions, const int32_t* lengths,

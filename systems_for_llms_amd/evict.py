@@ -8,7 +8,8 @@ that stay above ``keep`` fill the holes below it, so an eviction moves no more r
 it must (attention does not care for the order of its keys, whose rotation is in them).
 Slots are then no longer in the order of their tokens; ``positions`` keeps track of that
 for the next ``select``: the program writes a token's position into its slot, for every KV
-head, when it appends it, and ``tree.accept`` and ``compact`` move it with the row. Both calls only touch the device and can be captured.
+head, when it appends it, and ``tree.accept`` and ``compact`` move it with the row. Both
+calls only touch the device and can be captured.
 """
 
 from __future__ import annotations
