@@ -581,6 +581,89 @@ int sfl_compact_slots(void* k, void* v, float* weights, int32_t* positions, cons
                       const long* strides, int batch, int kv_heads, int capacity, int keep, int head_dim,
                       int dtype, void* stream);
 
+/* ---- a paged KV cache held in 8 bits --------------------------------------------
+ * No counterpart in the reference: a cache whose sequences share a pool of pages. A page
+ * holds page_size (16, 32, 64 or 128) tokens of every KV head of every layer as float8
+ * (e4m3) codes; a value is code * scale, with one power-of-two scale per page and head for
+ * the keys and one for the values.
+ *   k_codes  [layers, pages, kv_heads, page_size, head_dim]    uint8 codes
+ *   v_codes  [layers, pages, kv_heads, head_dim, page_size]
+ *   k_scale, v_scale [layers, pages, kv_heads] fp32
+ *   tables   [batch, places] int32: the page of a sequence's tokens place * page_size ..; -1: none
+ *   lengths  [batch] int32: committed tokens
+ *   refs     [pages] int32: in how many tables a page is; 0: free
+ * all contiguous. head_dim 16, 32, 64 or 128, places * page_size at most
+ * SFL_CACHE_MAX_SLOTS, pages at most SFL_PAGE_MAX_PAGES; the calls on tables as a whole take
+ * up to 1024 sequences. What is read on the device is clamped or left out where it is
+ * outside its range, never followed.
+ */
+
+#define SFL_PAGE_MAX_PAGES (1 << 24)
+
+/*
+ * New tokens into one layer's pages: token t < counts[b] (NULL: all) of sequence b goes to
+ * slot lengths[b] + t. For each page, head and tensor the scale becomes 2^e with the least
+ * e >= -100 such that the new tokens' finite values are at most 448 * 2^e, and not below
+ * the scale before where the page holds committed tokens, whose codes are then rounded
+ * again under it. Codes are rounded to nearest even; NaN and magnitudes from 2^127 on become
+ * the code of NaN. Tokens are left out whose page is missing or has refs != 1.
+ *   k, v [batch, kv_heads, tokens] rows of head_dim of dtype F32, BF16 or F16
+ *   strides [6]: k, v {batch, head, token}, multiples of 16 bytes
+ */
+int sfl_page_append(const void* k, const void* v, void* k_codes, void* v_codes, float* k_scale, float* v_scale,
+                    const int32_t* tables, const int32_t* lengths, const int32_t* counts, const int32_t* refs,
+                    const long* strides, int batch, int kv_heads, int tokens, int places, int pages,
+                    int page_size, int head_dim, int dtype, void* stream);
+
+/*
+ * Attention of `tokens` (at most 128) new tokens over one layer's pages: token t <
+ * counts[b] sees the slots in [0, lengths[b] + t] that have a page, with window_left >= 0
+ * only those from lengths[b] + t - window_left on. out = softmax(q k^T scale) v, lse = log
+ * sum exp(q k^T scale) (natural, fp32 [batch, q_heads, tokens]); a token that sees nothing,
+ * lies past counts[b] or has no slot has a zero row and lse -inf. What a token does not see
+ * has no part in its row, NaN codes included.
+ *   q, out [batch, q_heads, tokens] rows of dtype, Hq/Hkv in {1, 2, 4, 8}
+ *   partial_max, partial_sum  batch * q_heads * tokens * splits fp32 values, partial_out
+ *   head_dim times as many: scratch, unused (may be NULL) with splits == 1
+ *   strides [6]: q, out {batch, head, token}, multiples of 16 bytes
+ * Every sum in fp32. Results do not vary from call to call.
+ */
+int sfl_page_attention(const void* q, const void* k_codes, const void* v_codes, const float* k_scale,
+                       const float* v_scale, const int32_t* tables, const int32_t* lengths,
+                       const int32_t* counts, float* partial_max, float* partial_sum, float* partial_out,
+                       void* out, float* lse, const long* strides, int batch, int q_heads, int kv_heads,
+                       int tokens, int places, int pages, int page_size, int head_dim, int window_left,
+                       int splits, float scale, int dtype, void* stream);
+
+/*
+ * All at once, row b becomes what row parents[b] was: it leaves its pages and holds those
+ * that the parent's committed tokens are in. parents[b] == b: stays (as do entries outside
+ * [-1, batch)); -1: an empty row. tables, lengths and refs are updated.
+ */
+int sfl_page_fork(int32_t* tables, int32_t* lengths, int32_t* refs, const int32_t* parents, int batch,
+                  int places, int pages, int page_size, void* stream);
+
+/*
+ * Pages for the next counts[b] tokens of each sequence, one row after another, place by
+ * place: a place to be written that has no page, or one with refs > 1, gets the lowest free
+ * page; a shared page that holds committed tokens of the row is copied (all layers).
+ * granted [batch] int32: how many of the tokens then have a page of the row's own.
+ * scratch: 2 + 2 * batch int32, 8-byte aligned.
+ */
+int sfl_page_reserve(void* k_codes, void* v_codes, float* k_scale, float* v_scale, int32_t* tables,
+                     const int32_t* lengths, int32_t* refs, const int32_t* counts, int32_t* granted,
+                     int32_t* scratch, int batch, int places, int pages, int layers, int kv_heads,
+                     int page_size, int head_dim, void* stream);
+
+/*
+ * Moves the pages in use (refs > 0) into the first used[0] of the pool: those from there on,
+ * ascending, into the free ones below, ascending. tables and refs follow. used [1] int32.
+ * scratch: 4 + 2 * pages int32, 8-byte aligned.
+ */
+int sfl_page_compact(void* k_codes, void* v_codes, float* k_scale, float* v_scale, int32_t* tables,
+                     int32_t* refs, int32_t* used, int32_t* scratch, int batch, int places, int pages,
+                     int layers, int kv_heads, int page_size, int head_dim, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

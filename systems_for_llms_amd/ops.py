@@ -206,6 +206,67 @@ def launch_compact_slots(kept: torch.Tensor, k: torch.Tensor, v: torch.Tensor, w
           _strides_2(*k.stride()[:3], *v.stride()[:3]), batch, heads, capacity, kept.shape[2], dim, _lib.dtype_code(k.dtype))
 
 
+def launch_page_append(k: torch.Tensor, v: torch.Tensor, tables: torch.Tensor, lengths: torch.Tensor,
+                       counts: torch.Tensor | None, refs: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor,
+                       k_scale: torch.Tensor, v_scale: torch.Tensor, layer: int) -> None:
+    """New tokens quantised into one layer's pages (``sfl_page_append``)."""
+    batch, heads, tokens, dim = k.shape
+    pages, _, page_size = k_codes.shape[1:4]
+    codes, scales = layer * k_codes.stride(0), 4 * layer * k_scale.stride(0)
+    _call(k.device, "sfl_page_append", k.data_ptr(), v.data_ptr(), k_codes.data_ptr() + codes,
+          v_codes.data_ptr() + codes, k_scale.data_ptr() + scales, v_scale.data_ptr() + scales, tables.data_ptr(),
+          lengths.data_ptr(), _ptr(counts), refs.data_ptr(), _strides_2(*k.stride()[:3], *v.stride()[:3]), batch, heads,
+          tokens, tables.shape[1], pages, page_size, dim, _lib.dtype_code(k.dtype))
+
+
+def launch_page_attention(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor, k_scale: torch.Tensor,
+                          v_scale: torch.Tensor, tables: torch.Tensor, lengths: torch.Tensor,
+                          counts: torch.Tensor | None, partial_max: torch.Tensor, partial_sum: torch.Tensor,
+                          partial_output: torch.Tensor, out: torch.Tensor, lse: torch.Tensor, layer: int,
+                          window_left: int, splits: int, scale: float) -> None:
+    """Attention of new tokens over one layer's pages into ``out`` and ``lse`` (``sfl_page_attention``)."""
+    batch, heads, tokens, dim = q.shape
+    pages, kv_heads, page_size = k_codes.shape[1:4]
+    codes, scales = layer * k_codes.stride(0), 4 * layer * k_scale.stride(0)
+    _call(q.device, "sfl_page_attention", q.data_ptr(), k_codes.data_ptr() + codes, v_codes.data_ptr() + codes,
+          k_scale.data_ptr() + scales, v_scale.data_ptr() + scales, tables.data_ptr(), lengths.data_ptr(), _ptr(counts),
+          partial_max.data_ptr(), partial_sum.data_ptr(), partial_output.data_ptr(), out.data_ptr(), lse.data_ptr(),
+          _strides_2(*q.stride()[:3], *out.stride()[:3]), batch, heads, kv_heads, tokens, tables.shape[1], pages,
+          page_size, dim, window_left, splits, scale, _lib.dtype_code(q.dtype))
+
+
+def launch_page_fork(parents: torch.Tensor, tables: torch.Tensor, lengths: torch.Tensor, refs: torch.Tensor,
+                     page_size: int) -> None:
+    """Every row of the tables becomes its parent's (``sfl_page_fork``)."""
+    batch, places = tables.shape
+    _call(tables.device, "sfl_page_fork", tables.data_ptr(), lengths.data_ptr(), refs.data_ptr(), parents.data_ptr(),
+          batch, places, refs.shape[0], page_size)
+
+
+def _pools(k_codes, v_codes, k_scale, v_scale):
+    return k_codes.data_ptr(), v_codes.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr()
+
+
+def launch_page_reserve(lengths: torch.Tensor, counts: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor,
+                        k_scale: torch.Tensor, v_scale: torch.Tensor, tables: torch.Tensor, refs: torch.Tensor,
+                        granted: torch.Tensor, scratch: torch.Tensor) -> None:
+    """Pages for the next tokens, shared ones copied (``sfl_page_reserve``)."""
+    batch, places = tables.shape
+    layers, pages, heads, page_size, dim = k_codes.shape
+    _call(tables.device, "sfl_page_reserve", *_pools(k_codes, v_codes, k_scale, v_scale), tables.data_ptr(),
+          lengths.data_ptr(), refs.data_ptr(), counts.data_ptr(), granted.data_ptr(), scratch.data_ptr(), batch, places,
+          pages, layers, heads, page_size, dim)
+
+
+def launch_page_compact(k_codes: torch.Tensor, v_codes: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                        tables: torch.Tensor, refs: torch.Tensor, used: torch.Tensor, scratch: torch.Tensor) -> None:
+    """The pages in use moved to the front of the pool (``sfl_page_compact``)."""
+    batch, places = tables.shape
+    layers, pages, heads, page_size, dim = k_codes.shape
+    _call(tables.device, "sfl_page_compact", *_pools(k_codes, v_codes, k_scale, v_scale), tables.data_ptr(),
+          refs.data_ptr(), used.data_ptr(), scratch.data_ptr(), batch, places, pages, layers, heads, page_size, dim)
+
+
 def _nothing(*args):
     return None
 
@@ -217,6 +278,13 @@ _CACHE_OPS = {
     "accept_path": (launch_accept_path, ("k", "v", "weights", "positions", "new_lengths")),
     "select_slots": (launch_select_slots, ("kept", "new_lengths")),
     "compact_slots": (launch_compact_slots, ("k", "v", "weights", "positions")),
+    "page_append": (launch_page_append, ("k_codes", "v_codes", "k_scale", "v_scale")),
+    "page_attention": (launch_page_attention, ("partial_max", "partial_sum", "partial_output", "out", "lse")),
+    "page_fork": (launch_page_fork, ("tables", "lengths", "refs")),
+    "page_reserve": (launch_page_reserve, ("k_codes", "v_codes", "k_scale", "v_scale", "tables", "refs", "granted",
+                                           "scratch")),
+    "page_compact": (launch_page_compact, ("k_codes", "v_codes", "k_scale", "v_scale", "tables", "refs", "used",
+                                           "scratch")),
 }
 for _name, (_launch, _written) in _CACHE_OPS.items():
     torch.library.custom_op(f"sfl::{_name}", mutates_args=_written)(_launch).register_fake(_nothing)

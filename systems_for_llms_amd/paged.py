@@ -1,0 +1,290 @@
+"""A KV cache in pages that sequences share, held in 8 bits, and attention over it.
+
+Beside the contiguous 16-bit caches of ``decode``, ``rotary`` and ``tree``: here the cache of
+all layers is one pool of pages. A page holds ``page_size`` tokens of every KV head as float8
+(e4m3) codes, with a power-of-two scale for each head's keys and values in it; a sequence is a
+row of ``tables``, which names its pages, and of ``lengths``. A serving step is
+
+    fork(cache, parents)                     # rows that end, start anew or continue others
+    granted = reserve(cache, counts)         # pages for the next tokens, shared ones copied
+    append(cache, k, v, layer=i)             # each layer: quantised into the pages
+    out = prepared()                         # ``prepare(q, cache, layer=i)``
+    cache.lengths += accepted                # what the program keeps of them
+
+``compact`` moves the pages in use to the front of the pool. A page that several rows hold
+(``refs`` counts them) is never written: ``reserve`` gives a row its own copy of the one it
+goes on writing in. All calls but ``create`` only touch the device and can be captured;
+``cache.lengths`` and the tensors given may be changed in place between calls and replays.
+Inference only: ``requires_grad`` inputs are refused.
+"""
+
+from __future__ import annotations
+
+import math
+from dataclasses import dataclass
+
+import torch
+
+from . import _lib
+from . import cache as _cache
+from . import ops  # registers torch.ops.sfl
+
+CODES = torch.float8_e4m3fn
+PAGE_SIZES = (16, 32, 64, 128)
+MAX_PAGES = 1 << 24
+MAX_ROWS = 1024
+MAX_TOKENS = _cache.MAX_DRAFTS
+MAX_SPLITS = 128
+
+
+@dataclass(frozen=True)
+class PagedCache:
+    """The tensors of a paged cache, contiguous on one device; a program may allocate them itself.
+
+    ``k`` ``[L, P, Hkv, page, D]`` and ``v`` ``[L, P, Hkv, D, page]`` float8_e4m3fn codes of L layers
+    and P pages (of 16, 32, 64 or 128 tokens), ``k_scale`` and ``v_scale`` fp32 ``[L, P, Hkv]``:
+    a value is its code times its page's scale, a power of two. ``tables`` int32 ``[B, M]``: the
+    page of a row's tokens from ``place * page`` on, -1 for none. ``lengths`` int32 ``[B]``:
+    committed tokens. ``refs`` int32 ``[P]``: in how many rows a page is, 0 for a free one.
+    Up to 1024 rows.
+    """
+
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: torch.Tensor
+    v_scale: torch.Tensor
+    tables: torch.Tensor
+    lengths: torch.Tensor
+    refs: torch.Tensor
+
+    def __post_init__(self):
+        k, tables = self.k, self.tables
+        if k.ndim != 5 or 0 in k.shape or tables.ndim != 2 or 0 in tables.shape:
+            raise ValueError("k must be [L, P, Hkv, page, D] and tables [B, M], not empty")
+        layers, pages, heads, page, dim = k.shape
+        if page not in PAGE_SIZES:
+            raise ValueError("supported page sizes are 16/32/64/128")
+        if dim not in _cache.SUPPORTED_DIMS:
+            raise ValueError("supported head dimensions are 16/32/64/128")
+        if pages > MAX_PAGES:
+            raise ValueError(f"at most {MAX_PAGES} pages are supported")
+        if tables.shape[0] > MAX_ROWS:
+            raise ValueError(f"at most {MAX_ROWS} rows are supported")
+        if tables.shape[1] * page > _cache.MAX_ROWS:
+            raise ValueError(f"a row must have at most {_cache.MAX_ROWS} slots")
+        index = k.get_device()
+        for name, dtype, shape in (("k", CODES, k.shape), ("v", CODES, (layers, pages, heads, dim, page)),
+                                   ("k_scale", torch.float32, (layers, pages, heads)),
+                                   ("v_scale", torch.float32, (layers, pages, heads)),
+                                   ("tables", torch.int32, tables.shape), ("lengths", torch.int32, tables.shape[:1]),
+                                   ("refs", torch.int32, (pages,))):
+            _cache.check_vector("paged cache", name, getattr(self, name), dtype, shape, index)
+        if k.data_ptr() % 16 or self.v.data_ptr() % 16:
+            raise ValueError("k and v must be 16-byte aligned")
+
+    @property
+    def layers(self) -> int:
+        return self.k.shape[0]
+
+    @property
+    def page_size(self) -> int:
+        return self.k.shape[3]
+
+    @property
+    def capacity(self) -> int:
+        """Slots of a row."""
+        return self.tables.shape[1] * self.k.shape[3]
+
+
+def create(batch, capacity, kv_heads, head_dim, pages, *, layers=1, page_size=64, device="cuda") -> PagedCache:
+    """A cache of ``batch`` empty rows of up to ``capacity`` tokens over ``pages`` free pages."""
+    for name, value in (("batch", batch), ("capacity", capacity), ("kv_heads", kv_heads), ("pages", pages),
+                        ("layers", layers)):
+        if type(value) is not int or value < 1:
+            raise ValueError(f"{name} must be a positive integer")
+    if page_size not in PAGE_SIZES:
+        raise ValueError("supported page sizes are 16/32/64/128")
+
+    def zeros(*shape, dtype=torch.int32):
+        return torch.zeros(shape, dtype=dtype, device=device)
+
+    codes = (zeros(layers, pages, kv_heads, *rows, dtype=torch.uint8).view(CODES)
+             for rows in ((page_size, head_dim), (head_dim, page_size)))
+    scales = (zeros(layers, pages, kv_heads, dtype=torch.float32) for _ in range(2))
+    return PagedCache(*codes, *scales, zeros(batch, -(-capacity // page_size)) - 1, zeros(batch), zeros(pages))
+
+
+def _check_cache(operator, cache):
+    if not isinstance(cache, PagedCache):
+        raise TypeError(f"{operator}: cache must be a PagedCache")
+    return cache.k.get_device()
+
+
+def _check_layer(cache, layer):
+    if type(layer) is not int or not 0 <= layer < cache.k.shape[0]:
+        raise ValueError("layer must be an integer in [0, layers)")
+
+
+def fork(cache, parents) -> None:
+    """All at once, row b becomes what row ``parents[b]`` was (int32 ``[B]``), in place.
+
+    It leaves its own pages and shares those that the parent's committed tokens are in, with
+    the parent's length. ``parents[b] == b``: the row stays; -1: it is freed. (Entries that name
+    no row stay, too.) One call reorders, copies and frees any rows.
+    """
+    index = _check_cache("fork", cache)
+    _cache.check_vector("fork", "parents", parents, torch.int32, cache.lengths.shape, index)
+    _cache.check_device(index)
+    written = (cache.tables, cache.lengths, cache.refs)
+    ops.dispatch(torch.ops.sfl.page_fork, (parents, *written), written, cache.k.shape[3], checked=True)
+
+
+def reserve(cache, counts) -> torch.Tensor:
+    """Pages for the next ``counts[b]`` tokens of each row (int32 ``[B]``); returns how many are granted.
+
+    One row after another, place by place: a place that the tokens will be written to and
+    that has no page, or one that other rows hold too, gets the lowest free page; where the
+    shared one holds committed tokens of the row it is copied, in all layers. (Of several rows
+    that go on writing in one page the last keeps it.) ``granted`` int32 ``[B]``, a new tensor:
+    the tokens that have a place of their own; less than asked for where the pool or the row
+    is full.
+    """
+    index = _check_cache("reserve", cache)
+    _cache.check_vector("reserve", "counts", counts, torch.int32, cache.lengths.shape, index)
+    _cache.check_device(index)
+    _lib.lib()  # fail here, before allocating, if the library is not built
+    granted = torch.empty_like(cache.lengths)
+    scratch = torch.empty(2 + 2 * granted.shape[0], dtype=torch.int32, device=granted.device)
+    written = (cache.k, cache.v, cache.k_scale, cache.v_scale, cache.tables, cache.refs, granted, scratch)
+    ops.dispatch(torch.ops.sfl.page_reserve, (cache.lengths, counts, *written), written, checked=True)
+    return granted
+
+
+def compact(cache) -> torch.Tensor:
+    """Move the pages in use to the front of the pool, in place; returns how many they are (int32 ``[1]``).
+
+    Pages past that number, ascending, go into the free ones below it, ascending, in all
+    layers; ``tables`` and ``refs`` follow. Pages in front stay where they are.
+    """
+    index = _check_cache("compact", cache)
+    _cache.check_device(index)
+    _lib.lib()
+    used = torch.empty(1, dtype=torch.int32, device=cache.k.device)
+    scratch = torch.empty(4 + 2 * cache.refs.shape[0], dtype=torch.int32, device=cache.k.device)
+    written = (cache.k, cache.v, cache.k_scale, cache.v_scale, cache.tables, cache.refs, used, scratch)
+    ops.dispatch(torch.ops.sfl.page_compact, written, written, checked=True)
+    return used
+
+
+def append(cache, k, v, *, layer=0, counts=None) -> None:
+    """Quantise new tokens ``k``, ``v`` ``[B, Hkv, T, D]`` (fp16, bf16 or fp32 views) into a layer's pages, in place.
+
+    Token t of row b goes to slot ``lengths[b] + t``; those from ``counts[b]`` on (int32 ``[B]``)
+    are padding. ``lengths`` is not changed. Tokens whose place has no page, or one that other
+    rows hold, are left out: ``reserve`` comes first. For each page and head the scale becomes
+    the least power of two (from 2^-100 on) under which the new values fit codes of up to 448;
+    where the page holds committed tokens it does not become smaller, and where it grows their
+    codes are rounded again under the new one. Infinities, NaN and magnitudes from 2^127 on
+    become NaN.
+    """
+    index = _check_cache("append", cache)
+    if _cache.check_rows("append", ("k", "v"), (k, v)) != index:
+        _cache.check_device(-1)
+    _check_layer(cache, layer)
+    heads, _, dim = cache.k.shape[2:]
+    if v.shape != k.shape or k.shape[0] != cache.lengths.shape[0] or k.shape[1] != heads or k.shape[3] != dim:
+        raise ValueError("k, v and the cache must agree in rows, heads and head dimension")
+    if counts is not None:
+        _cache.check_vector("append", "counts", counts, torch.int32, cache.lengths.shape, index)
+    _cache.check_device(index)
+    written = (cache.k, cache.v, cache.k_scale, cache.v_scale)
+    ops.dispatch(torch.ops.sfl.page_append, (k, v, cache.tables, cache.lengths, counts, cache.refs, *written), written,
+                 layer, checked=True)
+
+
+def auto_splits(batch: int, kv_heads: int, capacity: int, rows: int) -> int:
+    """Workgroups that share a KV head's slots, for ``rows`` query rows over each (new tokens times
+    query heads of the KV head)."""
+    blocks = batch * kv_heads * math.ceil(rows / 32)
+    return max(1, min(32, round(512 / blocks), math.ceil(capacity / 256)))
+
+
+@dataclass
+class PreparedPaged:
+    q: torch.Tensor
+    cache: PagedCache
+    counts: torch.Tensor | None
+    partial_max: torch.Tensor
+    partial_sum: torch.Tensor
+    partial_output: torch.Tensor
+    output: torch.Tensor
+    lse: torch.Tensor
+    layer: int
+    window_left: int
+    splits: int
+    scale: float
+
+    def __call__(self) -> torch.Tensor:
+        """The output ``[B, Hq, T, D]``, overwritten by every call; ``lse`` goes with it."""
+        c = self.cache
+        written = (self.partial_max, self.partial_sum, self.partial_output, self.output, self.lse)
+        ops.dispatch(torch.ops.sfl.page_attention,
+                     (self.q, c.k, c.v, c.k_scale, c.v_scale, c.tables, c.lengths, self.counts, *written), written,
+                     self.layer, self.window_left, self.splits, self.scale, checked=True)
+        return self.output
+
+    @property
+    def scratch_bytes(self) -> int:
+        return sum(x.numel() * x.element_size() for x in (self.partial_max, self.partial_sum, self.partial_output))
+
+
+def prepare(q, cache, *, layer=0, counts=None, window_left=None, splits=None, scale=None) -> PreparedPaged:
+    """Validate and allocate, then return a reusable operation: attention of new tokens over a layer's pages.
+
+    ``q`` ``[B, Hq, T, D]`` (fp16, bf16 or fp32, T at most 128) may be a strided view with 16-byte
+    aligned rows. New token t of row b is in slot ``lengths[b] + t`` (``append``) and sees the slots
+    up to that one that have a page; with ``window_left`` only the last ``window_left`` before it,
+    and itself. ``counts`` int32 ``[B]``: tokens in use; the rows of the others are zeros with an
+    ``lse`` (fp32 ``[B, Hq, T]``) of -inf, as are those of tokens that see nothing or have no slot. What
+    a token does not see has no part in its row, NaN included. Scores and sums are fp32, and
+    no code is rounded again: probabilities are rounded to bf16 for bf16 ``q``, to two such
+    pieces for fp16, three for fp32. ``splits``: workgroups that share a KV head's slots, 1 to
+    128 (default by size). Like ``tree.PreparedTree`` the operation owns its scratch and output
+    and holds its inputs by reference; concurrent calls on one race.
+    """
+    if splits is not None and (type(splits) is not int or not 1 <= splits <= MAX_SPLITS):
+        raise ValueError("splits must be an integer in [1, 128]")
+    if window_left is not None and (type(window_left) is not int or window_left < 0):
+        raise ValueError("window_left must be a non-negative integer or None")
+    index = _check_cache("paged attention", cache)
+    if _cache.check_rows("paged attention", ("q",), (q,)) != index:
+        _cache.check_device(-1)
+    _check_layer(cache, layer)
+    batch, heads, tokens, dim = q.shape
+    kv_heads = cache.k.shape[2]
+    if batch != cache.lengths.shape[0] or dim != cache.k.shape[4]:
+        raise ValueError("q and the cache must agree in rows and head dimension")
+    _cache.check_heads(heads, kv_heads)
+    if tokens > MAX_TOKENS:
+        raise ValueError(f"at most {MAX_TOKENS} new tokens are supported")
+    if counts is not None:
+        _cache.check_vector("paged attention", "counts", counts, torch.int32, (batch,), index)
+    scale = dim ** -0.5 if scale is None else scale
+    if not math.isfinite(scale) or scale <= 0:
+        raise ValueError("scale must be finite and positive")
+    _cache.check_device(index)
+    _lib.lib()  # fail here, before allocation, if the library is not built
+    if splits is None:
+        splits = auto_splits(batch, kv_heads, cache.capacity, tokens * (heads // kv_heads))
+    window = -1 if window_left is None else min(window_left, cache.capacity)
+    maximum = torch.empty((batch, heads, tokens, splits if splits > 1 else 0), device=q.device, dtype=torch.float32)
+    numerator = torch.empty((*maximum.shape, dim), device=q.device, dtype=torch.float32)
+    lse = torch.empty((batch, heads, tokens), device=q.device, dtype=torch.float32)
+    return PreparedPaged(q, cache, counts, maximum, torch.empty_like(maximum), numerator, torch.empty_like(q), lse,
+                         layer, window, splits, float(scale))
+
+
+def attend(q, cache, *, layer=0, counts=None, window_left=None, splits=None, scale=None):
+    """``prepare`` and compute once on the current stream: ``(out, lse)``."""
+    op = prepare(q, cache, layer=layer, counts=counts, window_left=window_left, splits=splits, scale=scale)
+    return op(), op.lse

@@ -1,0 +1,720 @@
+"""GPU parity of the paged 8-bit cache's operators with their float64 and list forms (``oracle/paged.py``).
+
+Codes, scales and books are equal bit for bit. Error bounds of the attention count what
+the kernels do: a stored result is rounded once, by half a step (``finfo.eps / 2`` of the
+value); codes become bf16 exactly; probabilities go into the products with V as sums of one
+(bf16), two (fp16) or three (fp32) bf16 pieces, off by 2^-8, 2^-16 or 2^-24 of p |v|; scores
+are fp32 sums of as many times D products, off by at most (pieces D + 8) 2^-24 of sum |q k|
+and a few roundings of the scaled value, which enter exp as a relative error; sums over n
+keys are off by at most n 2^-24 of sum |terms|.
+"""
+
+import pytest
+import torch
+
+from oracle import paged as op_
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
+PIECES = {BF16: 1, FP16: 2, FP32: 3}
+TINY = {BF16: 1e-38, FP16: 2.0 ** -25, FP32: 1e-38}  # half a step of the smallest numbers
+NAMES = ("k", "v", "k_scale", "v_scale", "tables", "lengths", "refs")
+NAN_CODE = 0x7F
+
+
+def randn(g, *shape, dtype=FP32, scale=1.0):
+    return (torch.randn(shape, generator=g) * scale).to(dtype)
+
+
+def within(got, want, bound, what=""):
+    got, want = got.double().cpu(), want.double()
+    assert got.shape == want.shape, what
+    same = (got == want) | (got.isnan() & want.isnan())
+    off = torch.where(same, 0.0, (got - want).abs())
+    assert not bool((off.isnan() | (off > bound)).any()), f"{what}: {(off / bound).nan_to_num(9e9).max()} of the bound"
+
+
+def bits(codes):
+    """Codes as bytes, one byte for NaN."""
+    x = codes.cpu().view(torch.uint8)
+    return torch.where(x & 0x7F == NAN_CODE, NAN_CODE, x)
+
+
+def same_cache(cache, want, names=NAMES):
+    for n in names:
+        x, y = getattr(cache, n), want[n]
+        assert torch.equal(bits(x), bits(y)) if n in ("k", "v") else torch.equal(x.cpu(), y), n
+
+
+def on_gpu(state):
+    from systems_for_llms_amd import paged
+
+    return paged.PagedCache(*(state[n].cuda() for n in NAMES))
+
+
+def codes_like(g, *shape):
+    """Any codes but NaN."""
+    x = torch.randint(0, 254, shape, generator=g, dtype=torch.uint8)
+    return (x + (x >= NAN_CODE).to(torch.uint8)).view(op_.F8)
+
+
+def random_cache(g, lengths, heads, dim, page, *, layers=1, spare=5, room=0, codes=None, exponents=(-8, -5)):
+    """Rows of these lengths with room for more tokens, on pages in random order, all places with a page."""
+    places = max(-(-(n + room) // page) for n in lengths)
+    batch = len(lengths)
+    pages = batch * places + spare
+    state = {}
+    for name, rows in (("k", (page, dim)), ("v", (dim, page))):
+        e = torch.randint(*exponents, (layers, pages, heads), generator=g)
+        state[name + "_scale"] = torch.ldexp(torch.ones(e.shape), e)
+        if codes == "any":
+            state[name] = codes_like(g, layers, pages, heads, *rows)
+        else:
+            state[name] = (torch.randn(layers, pages, heads, *rows, generator=g) * 128).clamp(-448, 448).to(op_.F8)
+    state["tables"] = torch.randperm(pages, generator=g)[: batch * places].reshape(batch, places).to(torch.int32)
+    state["lengths"] = torch.tensor(lengths, dtype=torch.int32)
+    state["refs"] = torch.zeros(pages, dtype=torch.int32)
+    state["refs"][state["tables"].flatten().long()] = 1
+    return state
+
+
+# ---- append -------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("dim", [16, 32, 64, 128])
+@pytest.mark.parametrize("page", [16, 32, 64, 128])
+def test_append(dtype, dim, page):
+    """Prompts, drafts and single tokens after one another, values whose size changes between the calls."""
+    from systems_for_llms_amd import paged
+
+    g = torch.Generator().manual_seed(dim * 1000 + page)
+    state = random_cache(g, [0, 3, page - 1, 2 * page], 3, dim, page, room=3 * page + 40, codes="any")
+    cache = on_gpu(state)
+    for tokens, size in ((2 * page + 5, 1.0), (1, 3.0), (5, 40.0), (page, 0.01), (1, 0.0), (7, 1e4), (1, 1.0)):
+        qkv = randn(g, 4, tokens, 6, dim, dtype=dtype, scale=size).transpose(1, 2)
+        counts = torch.tensor([tokens, (tokens + 1) // 2, tokens, 0 if tokens == 5 else tokens], dtype=torch.int32)
+        k, v = qkv.cuda().split([3, 3], 1)
+        paged.append(cache, k, v, counts=counts.cuda())
+        state = op_.append(state, *qkv.split([3, 3], 1), counts)
+        same_cache(cache, state)
+        state["lengths"] = state["lengths"] + counts.clamp(max=tokens // 2 + 1)  # some drafts are not kept
+        cache.lengths.copy_(state["lengths"])
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+def test_append_rounds_to_nearest_even_and_marks_what_has_no_code(dtype):
+    from systems_for_llms_amd import paged
+
+    g = torch.Generator().manual_seed(5)
+    page, dim = 32, 64
+    state = random_cache(g, [0, 4], 2, dim, page, room=2 * page)
+    steps = torch.arange(0, 16 * 64, dtype=torch.float64) / 64  # every tie of the normal codes
+    k = torch.cat([steps, 448 - steps, steps * 2.0 ** -12, 2.0 ** -9 * steps]).reshape(1, 1, -1, dim)
+    k = k.expand(2, 2, -1, -1)[:, :, :40].to(dtype).contiguous()
+    k[1, 1, 3, 5], k[1, 1, 4, 6], k[1, 1, 5, 7] = float("inf"), float("-inf"), float("nan")
+    v = -k.flip(-1).contiguous()
+    v[0, 0, 1, 1] = float("nan")
+    v[1, 0, 0, :] = 448.0  # the largest code of scale 1
+    v[1, 1, 0, :] = 449.0 if dtype == FP32 else 450.0
+    if dtype != FP16:
+        k[0, 1, 0, 0], k[0, 1, 1, 0], k[0, 1, 2, 0] = 2.0 ** 127, 1.99 * 2.0 ** 126, 1e-36
+        k[0, 1, 3, :] = 2.0 ** -108
+    tokens = k.shape[2]
+    cache = on_gpu(state)
+    paged.append(cache, k.cuda(), v.cuda())
+    want = op_.append(state, k, v)
+    same_cache(cache, want)
+    assert bool((bits(want["k"]) == NAN_CODE).any()) and tokens == 40
+
+
+def test_append_of_zeros_and_of_the_smallest_values():
+    from systems_for_llms_amd import paged
+
+    g = torch.Generator().manual_seed(6)
+    state = random_cache(g, [0, 0, 0], 1, 32, 16, room=16)
+    k = torch.zeros(3, 1, 5, 32)
+    k[1] = 2.0 ** -140
+    k[2] = randn(g, 1, 5, 32, scale=2.0 ** -105)
+    cache = on_gpu(state)
+    paged.append(cache, k.cuda(), k.cuda())
+    want = op_.append(state, k, k)
+    assert float(want["k_scale"][0, state["tables"][0, 0], 0]) == 2.0 ** -100
+    same_cache(cache, want)
+
+
+def test_append_leaves_missing_shared_and_full_places_as_they_are():
+    from systems_for_llms_amd import paged
+
+    g = torch.Generator().manual_seed(7)
+    state = random_cache(g, [10, 10, 10, 10, 30], 2, 64, 16, room=20, codes="any")
+    state["tables"][0, 1] = -1
+    state["tables"][1, 1] = state["refs"].numel()
+    state["refs"][state["tables"][2, 0]] = 2
+    state["refs"][state["tables"][3, 1]] = 0
+    state["lengths"][4] = state["tables"].shape[1] * 16 - 3
+    k, v = randn(g, 5, 2, 25, 64, dtype=BF16), randn(g, 5, 2, 25, 64, dtype=BF16)
+    for lengths in (state["lengths"], torch.tensor([-5, 2 ** 31 - 1, 7, -2 ** 31, 64], dtype=torch.int32)):
+        state["lengths"] = lengths
+        clamped = {**state, "lengths": lengths.clamp(0, state["tables"].shape[1] * 16)}
+        cache = on_gpu(state)
+        paged.append(cache, k.cuda(), v.cuda(), counts=torch.tensor([25, 30, 25, -1, 25], dtype=torch.int32).cuda())
+        want = op_.append(clamped, k, v, torch.tensor([25, 25, 25, 0, 25]))
+        same_cache(cache, {**want, "lengths": lengths})
+
+
+def test_append_of_strided_views_into_one_layer():
+    from systems_for_llms_amd import paged
+
+    g = torch.Generator().manual_seed(8)
+    state = random_cache(g, [17, 40], 2, 64, 32, layers=3, room=33)
+    wide = randn(g, 2, 33, 3, 2, 96, dtype=FP16)
+    k, v = wide[:, :, 0, :, 16:80].transpose(1, 2), wide[:, :, 2, :, 32:].transpose(1, 2)
+    moved = wide.cuda()
+    cache = on_gpu(state)
+    paged.append(cache, moved[:, :, 0, :, 16:80].transpose(1, 2), moved[:, :, 2, :, 32:].transpose(1, 2), layer=1)
+    same_cache(cache, op_.append(state, k, v, layer=1))
+
+
+# ---- attention ----------------------------------------------------------------------
+
+
+def bounds(dtype, dim, keys, out, lse, spread, size):
+    high = size + lse.abs().nan_to_num(0, 0, 0)
+    ds = (PIECES[dtype] * dim + 8) * U * size + 6 * U * high + 4 * U
+    p = {BF16: 2.0 ** -8, FP16: 2.0 ** -16, FP32: 2.0 ** -24}[dtype]
+    out_bound = torch.finfo(dtype).eps / 2 * out.abs() + TINY[dtype] + spread * (
+        (p + 2 * ds + 2 * (PIECES[dtype] * keys + 8) * U)[..., None])
+    return out_bound * 1.01, ds + (keys + 8) * U + 4 * U * lse.abs().nan_to_num(0, 0, 0)
+
+
+def check(q, state, *, cache=None, got=None, counts=None, window=None, splits=None, scale=None, layer=0):
+    from systems_for_llms_amd import paged
+
+    if got is None:
+        cache = on_gpu(state) if cache is None else cache
+        used = None if counts is None else counts.cuda()
+        got = paged.attend(q.cuda(), cache, layer=layer, counts=used, window_left=window, splits=splits, scale=scale)
+    out, lse, spread, size = op_.attention(q, state, layer, counts, window, scale)
+    keys = int(state["lengths"].max()) + q.shape[2]
+    bound, lse_bound = bounds(q.dtype, q.shape[3], keys, out, lse, spread, size)
+    within(got[1], lse, lse_bound, "lse")
+    within(got[0], out, bound, "out")
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("dim", [16, 32, 64, 128])
+@pytest.mark.parametrize("group", [1, 2, 4, 8])
+def test_attention(dtype, dim, group):
+    g = torch.Generator().manual_seed(dim + group)
+    for tokens, keys, page in ((1, 0, 16), (1, 33, 32), (3, 70, 64), (16, 200, 128), (17, 31, 16), (9, 700, 64)):
+        state = random_cache(g, [keys, 0, keys // 2], 2, dim, page, room=tokens)
+        q = randn(g, 3, 2 * group, tokens, dim, dtype=dtype, scale=1.5)
+        counts = torch.tensor([tokens, (tokens + 1) // 2, 0 if tokens % 2 else tokens], dtype=torch.int32)
+        cache = on_gpu(state)
+        for splits in (1, 3, None):
+            check(q, state, cache=cache, counts=counts, splits=splits)
+    check(q, state, splits=2, scale=0.21)
+
+
+@pytest.mark.parametrize("page", [16, 32, 64, 128])
+@pytest.mark.parametrize("window", [0, 1, 15, 63, 64, 100, 511])
+def test_attention_windows(page, window):
+    g = torch.Generator().manual_seed(page + window)
+    state = random_cache(g, [0, 40, 333, 520], 2, 64, page, room=7)
+    for dtype, tokens, group in ((BF16, 1, 4), (FP16, 7, 2), (FP32, 5, 8)):
+        q = randn(g, 4, 2 * group, tokens, 64, dtype=dtype)
+        for splits in (1, 4):
+            check(q, state, window=window, splits=splits)
+
+
+@pytest.mark.parametrize("tokens, group", [(32, 2), (64, 1), (128, 1), (65, 8), (128, 8)])
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+def test_attention_of_many_rows(tokens, group, dtype):
+    g = torch.Generator().manual_seed(tokens)
+    state = random_cache(g, [90, 300], 1, 128, 64, room=tokens)
+    q = randn(g, 2, group, tokens, 128, dtype=dtype)
+    counts = torch.tensor([tokens - 1, tokens // 3], dtype=torch.int32)
+    for splits, window in ((1, None), (3, None), (2, 50)):
+        check(q, state, counts=counts, splits=splits, window=window)
+
+
+@pytest.mark.parametrize("dtype, dim, group, tokens", [(BF16, 128, 8, 1), (FP16, 64, 4, 3), (FP32, 32, 2, 3)])
+@pytest.mark.parametrize("splits", [9, 17, 128])
+def test_attention_of_many_splits(dtype, dim, group, tokens, splits):
+    g = torch.Generator().manual_seed(splits)
+    state = random_cache(g, [3000, 100], 1, dim, 16, room=tokens)
+    check(randn(g, 2, group, tokens, dim, dtype=dtype), state, splits=splits)
+
+
+def test_attention_pages_of_very_different_scales():
+    """Scales from 2^-100 to 2^90 in one row, values of zero among them."""
+    g = torch.Generator().manual_seed(11)
+    for dtype in (BF16, FP32):
+        state = random_cache(g, [500], 2, 64, 16, room=1, exponents=(-100, 91))
+        state["k_scale"] = random_cache(g, [500], 2, 64, 16, room=1)["k_scale"]
+        state["v"][:, 3] = torch.zeros(2, 64, 16).to(op_.F8)
+        check(randn(g, 1, 4, 1, 64, dtype=dtype), state, splits=3)
+        # One key in front of all others, in a page of small values.
+        state["v_scale"][:] = 2.0 ** -90
+        check(randn(g, 1, 4, 1, 64, dtype=dtype), state)
+
+
+def test_attention_keeps_the_tail_behind_a_heavy_key():
+    """Thousands of keys of weight 2^-20 beside one of 1: together a part that may not be lost."""
+    for dtype, tokens in ((BF16, 1), (FP16, 1), (FP16, 5), (FP32, 3)):
+        g = torch.Generator().manual_seed(12)
+        state = random_cache(g, [9000], 1, 64, 64, room=tokens)
+        state["k"][:] = torch.zeros(64, 64).to(op_.F8)
+        state["k_scale"][:] = 1.0
+        at, off = int(state["tables"][0, 4000 // 64]), 4000 % 64
+        state["k"][0, at, 0, off, 0] = torch.tensor(16.0).to(op_.F8)
+        state["v"][:] = torch.full((64, 64), 1.0).to(op_.F8)
+        state["v_scale"][:] = 1.0
+        state["v"][0, at, 0, :, off] = torch.zeros(64).to(op_.F8)
+        q = torch.zeros(1, 2, tokens, 64, dtype=dtype)
+        q[..., 0] = 20 * 0.6931471805599453 / 16  # a weight of about 2^-20 for the others
+        check(q, state, scale=1.0)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("dim", [16, 32, 64, 128])
+@pytest.mark.parametrize("tokens, page", [(1, 16), (6, 64), (20, 32)])
+def test_attention_ignores_what_it_does_not_see(dtype, dim, tokens, page):
+    """NaN codes behind the row, in pages of nobody, before the window, and in slots that only some tokens see."""
+    g = torch.Generator().manual_seed(dim + tokens)
+    state = random_cache(g, [130, 61, 250], 2, dim, page, room=page + tokens)
+    nan = torch.full((2, dim), NAN_CODE, dtype=torch.uint8).view(op_.F8)
+
+    def poison(b, slot):
+        at, off = int(state["tables"][b, slot // page]), slot % page
+        state["k"][0, at, :, off], state["v"][0, at, :, :, off] = nan, nan
+
+    for b, n in enumerate(state["lengths"].tolist()):
+        for slot in range(n + tokens, state["tables"].shape[1] * page):
+            poison(b, slot)
+        for slot in range(max(0, n - 100)):
+            poison(b, slot)
+    free = (state["refs"] == 0).nonzero()[:, 0]
+    state["k"][0, free] = torch.full((page, dim), NAN_CODE, dtype=torch.uint8).view(op_.F8)
+    q = randn(g, 3, 8, tokens, dim, dtype=dtype)
+    for splits in (1, 2):
+        check(q, state, window=100 - tokens, splits=splits)
+    if tokens > 1:
+        poison(0, 130 + tokens - 2)  # seen by the last two tokens of row 0
+        poison(2, 250 - (100 - tokens))  # seen by the first token of row 2
+        for splits in (1, 2):
+            check(q, state, window=100 - tokens, splits=splits)
+        out = op_.attention(q, state, 0, None, 100 - tokens)[0]
+        assert not out[0, :, : tokens - 2].isnan().any() and out[0, :, tokens - 2:].isnan().all()
+        assert out[2, :, 0].isnan().all() and not out[2, :, 1:].isnan().any()
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+def test_attention_of_nothing_but_nan(dtype):
+    """Rows whose every score is NaN are not empty; neither are those with one value of NaN."""
+    g = torch.Generator().manual_seed(13)
+    state = random_cache(g, [30, 30, 30], 1, 32, 16, room=1)
+    at = state["tables"].long()
+    state["k"][0, at[0]] = torch.full((16, 32), NAN_CODE, dtype=torch.uint8).view(op_.F8)
+    state["v"][0, at[1, 0], 0, 7, 3] = torch.tensor(float("nan")).to(op_.F8)
+    q = randn(g, 3, 2, 1, 32, dtype=dtype)
+    for splits in (1, 3):
+        check(q, state, splits=splits)
+    q[2, 0, 0, 4] = float("nan")
+    check(q, state)
+
+
+def test_attention_of_missing_pages():
+    g = torch.Generator().manual_seed(14)
+    state = random_cache(g, [100, 200, 50], 2, 64, 16, room=20)
+    state["tables"][0, 2:5] = -1
+    state["tables"][1, ::2] = state["refs"].numel() + 7
+    state["tables"][2] = -1
+    for dtype, tokens in ((BF16, 1), (FP16, 20)):
+        q = randn(g, 3, 4, tokens, 64, dtype=dtype)
+        for splits, window in ((1, None), (4, None), (2, 33)):
+            check(q, state, splits=splits, window=window)
+    # A row as long as its table: tokens without a slot see nothing.
+    state["lengths"][1] = state["tables"].shape[1] * 16 - 3
+    check(q, state)
+    # Lengths that no row has are taken as the nearest that one has.
+    state["lengths"] = torch.tensor([-7, 2 ** 31 - 1, -2 ** 31], dtype=torch.int32)
+    check(q, state)
+
+
+def test_attention_strided_queries_and_layers():
+    g = torch.Generator().manual_seed(15)
+    state = random_cache(g, [77, 130], 2, 64, 32, layers=3, room=4)
+    wide = randn(g, 2, 4, 3, 8, 96, dtype=FP16)
+    moved = wide.cuda()
+    from systems_for_llms_amd import paged
+
+    cache = on_gpu(state)
+    got = paged.attend(moved[:, :, 1, :, 32:].transpose(1, 2), cache, layer=2)
+    check(wide[:, :, 1, :, 32:].transpose(1, 2), state, got=got, layer=2)
+
+
+def test_pools_past_32_bits():
+    """Codes of more than 4 GiB, the pages of two rows at both ends."""
+    from systems_for_llms_amd import paged
+
+    page, heads, dim, pages = 128, 8, 128, 35000  # 128 KiB a page
+    cache = paged.create(2, 512, heads, dim, pages, page_size=page)
+    assert cache.k.numel() > 2 ** 32
+    g = torch.Generator().manual_seed(16)
+    at = torch.tensor([[pages - 1, 0, pages - 3, 17000], [16384, pages - 2, 32768, 1]], dtype=torch.int32)
+    cache.tables.copy_(at)
+    cache.refs[at.flatten().long().cuda()] = 1
+    k, v = randn(g, 2, heads, 500, dim, dtype=BF16), randn(g, 2, heads, 500, dim, dtype=BF16)
+    paged.append(cache, k.cuda(), v.cuda())
+    q = randn(g, 2, 16, 1, dim, dtype=BF16)
+    cache.lengths.fill_(499)
+    got = paged.attend(q.cuda(), cache)
+    small = {n: getattr(cache, n).view(torch.uint8)[:, at.flatten().long().cuda()].cpu().view(op_.F8) for n in ("k", "v")}
+    small |= {n: getattr(cache, n)[:, at.flatten().long().cuda()].cpu() for n in ("k_scale", "v_scale")}
+    small |= {"tables": torch.arange(8, dtype=torch.int32).reshape(2, 4), "lengths": torch.tensor([0, 0], dtype=torch.int32),
+              "refs": torch.ones(8, dtype=torch.int32)}
+    blank = {n: torch.zeros_like(small[n].view(torch.uint8)).view(op_.F8) if n in "kv" else small[n] for n in small}
+    want = op_.append(blank, k, v)
+    for n in ("k", "v"):
+        assert torch.equal(bits(small[n]), bits(want[n]))
+    want["lengths"] = torch.tensor([499, 499], dtype=torch.int32)
+    check(q, want, got=got)
+    # The pages at the end move to the front, past the free ones.
+    cache.refs.zero_()
+    cache.refs[at[0].long().cuda()] = 1
+    cache.tables[1] = -1
+    assert int(paged.compact(cache)) == 4
+    got = paged.attend(q.cuda(), cache)
+    check(q[:1], {**want, "tables": want["tables"][:1], "lengths": want["lengths"][:1]}, got=[x[:1] for x in got])
+
+
+# ---- books --------------------------------------------------------------------------
+
+
+def random_books(g, batch, places, pages, page, lengths=None):
+    """Rows that share pages of the same place, some with pages past their length."""
+    free = torch.randperm(pages, generator=g).tolist()
+    tables, refs, used = [], [0] * pages, []
+    for b in range(batch):
+        n = int(torch.randint(0, places * page // 2 + 1, (1,), generator=g)) if lengths is None else lengths[b]
+        filled = min(places, -(-n // page) + (b % 3 == 0))
+        row = []
+        if b and b % 2:
+            row = [x for x in tables[b - 1] if x >= 0][: int(torch.randint(0, filled + 1, (1,), generator=g))]
+        while len(row) < filled and free:
+            row.append(free.pop())
+        for x in row:
+            refs[x] += 1
+        tables.append(row + [-1] * (places - len(row)))
+        used.append(min(n, len(row) * page))
+    return tables, used, refs
+
+
+def books_state(g, batch, places, pages, page=16, heads=2, dim=32, layers=2, lengths=None):
+    tables, used, refs = random_books(g, batch, places, pages, page, lengths)
+    return {"k": codes_like(g, layers, pages, heads, page, dim), "v": codes_like(g, layers, pages, heads, dim, page),
+            "k_scale": torch.rand(layers, pages, heads, generator=g), "v_scale": torch.rand(layers, pages, heads, generator=g),
+            "tables": torch.tensor(tables, dtype=torch.int32), "lengths": torch.tensor(used, dtype=torch.int32),
+            "refs": torch.tensor(refs, dtype=torch.int32)}
+
+
+@pytest.mark.parametrize("batch, places, pages", [(1, 1, 1), (1, 5, 9), (7, 6, 40), (64, 9, 700), (33, 700, 9000), (1024, 20, 9000)])
+def test_fork(batch, places, pages):
+    from systems_for_llms_amd import paged
+
+    g = torch.Generator().manual_seed(batch + places)
+    state = books_state(g, batch, places, pages, heads=1, dim=16, layers=1)
+    cache = on_gpu(state)
+    for kind in ("swap", "copy", "free", "wild", "stay"):
+        parents = torch.arange(batch)
+        if kind == "swap":
+            parents = torch.randperm(batch, generator=g)
+        elif kind == "copy":
+            parents = torch.randint(0, batch, (batch,), generator=g)
+        elif kind == "free":
+            parents[torch.rand(batch, generator=g) < 0.3] = -1
+        elif kind == "wild":
+            parents[torch.rand(batch, generator=g) < 0.5] = batch
+            parents[torch.rand(batch, generator=g) < 0.2] = -2 ** 31
+        parents = parents.to(torch.int32)
+        paged.fork(cache, parents.cuda())
+        state = op_.fork(state, parents)
+        same_cache(cache, state)
+        held = state["tables"][state["tables"] >= 0].long()
+        assert torch.equal(torch.bincount(held, minlength=pages).to(torch.int32), state["refs"])
+
+
+@pytest.mark.parametrize("batch, places, pages", [(1, 1, 1), (1, 40, 30), (7, 6, 60), (40, 9, 200), (64, 40, 6000),
+                                                  (1024, 5, 3000), (3, 2000, 20000)])
+def test_reserve(batch, places, pages):
+    """Until the pool is empty; rows that share the page they go on in, rows rolled back, rows without wishes."""
+    from systems_for_llms_amd import paged
+
+    g = torch.Generator().manual_seed(batch + pages)
+    page = 16
+    state = books_state(g, batch, places, pages, page)
+    for step in range(5):
+        parents = torch.where(torch.rand(batch, generator=g) < 0.5, torch.randint(0, batch, (batch,), generator=g),
+                              torch.arange(batch)).to(torch.int32)
+        if step:
+            state = op_.fork(state, parents)
+        if step % 2:  # some rows lose tokens
+            state["lengths"] = (state["lengths"] - torch.randint(0, 40, (batch,), generator=g)).clamp(min=0).to(torch.int32)
+        cache = on_gpu(state)
+        most = places * page // 3 if step % 2 else 3
+        counts = torch.randint(-1, most + 2, (batch,), generator=g).to(torch.int32)
+        granted = paged.reserve(cache, counts.cuda())
+        want, state = op_.reserve(state, counts)
+        assert torch.equal(granted.cpu(), want), step
+        same_cache(cache, state)
+        state["lengths"] = state["lengths"] + want
+
+
+def test_reserve_when_the_pool_runs_out():
+    """Rows that share a page, and fewer pages than they need: nobody writes into what others hold."""
+    from systems_for_llms_amd import paged
+
+    g = torch.Generator().manual_seed(21)
+    for free in range(5):
+        state = books_state(g, 6, 4, 8, lengths=[0] * 6)
+        state["tables"][:] = -1
+        state["tables"][:4, 0] = 5
+        state["tables"][4:, 0] = 2
+        state["lengths"] = torch.tensor([10, 10, 10, 10, 16, 9], dtype=torch.int32)
+        state["refs"] = torch.tensor([1] * (6 - free) + [0] * (free + 2), dtype=torch.int32)
+        state["refs"][5], state["refs"][2] = 4, 2
+        for counts in ([1] * 6, [8] * 6, [0, 1, 0, 1, 1, 1], [1, 20, 1, 1, 60, 1]):
+            cache = on_gpu(state)
+            granted = paged.reserve(cache, torch.tensor(counts, dtype=torch.int32).cuda())
+            want, after = op_.reserve(state, torch.tensor(counts))
+            assert torch.equal(granted.cpu(), want), (free, counts)
+            same_cache(cache, after)
+
+
+@pytest.mark.parametrize("batch, places, pages", [(1, 1, 1), (1, 5, 9), (7, 6, 60), (40, 9, 200), (64, 40, 6000), (5, 2000, 20000)])
+def test_compact(batch, places, pages):
+    from systems_for_llms_amd import paged
+
+    g = torch.Generator().manual_seed(batch + pages)
+    state = books_state(g, batch, places, pages)
+    for drop in (0.0, 0.4, 0.4, 1.0):
+        parents = torch.where(torch.rand(batch, generator=g) < drop, -1, torch.arange(batch)).to(torch.int32)
+        state = op_.fork(state, parents)
+        cache = on_gpu(state)
+        used = paged.compact(cache)
+        want, after = op_.compact(state)
+        assert used.tolist() == [want]
+        live = slice(0, want)
+        for n in ("k", "v"):
+            assert torch.equal(bits(getattr(cache, n))[:, live], bits(after[n])[:, live])
+        same_cache(cache, after)
+        state = after
+
+
+def test_books_of_large_pages_and_many_layers():
+    from systems_for_llms_amd import paged
+
+    g = torch.Generator().manual_seed(22)
+    state = books_state(g, 5, 4, 20, page=128, heads=3, dim=128, layers=5)
+    cache = on_gpu(state)
+    parents = torch.tensor([0, 0, 0, 3, -1], dtype=torch.int32)
+    state["lengths"][0] = cache.lengths[0] = 200
+    paged.fork(cache, parents.cuda())
+    state = op_.fork(state, parents)
+    granted = paged.reserve(cache, torch.full((5,), 90, dtype=torch.int32).cuda())
+    want, state = op_.reserve(state, torch.full((5,), 90))
+    assert torch.equal(granted.cpu(), want)
+    same_cache(cache, state)
+    paged.fork(cache, torch.tensor([-1, 1, -1, 3, 4], dtype=torch.int32).cuda())
+    state = op_.fork(state, torch.tensor([-1, 1, -1, 3, 4]))
+    assert int(paged.compact(cache)) == op_.compact(state)[0]
+    same_cache(cache, op_.compact(state)[1])
+
+
+# ---- as they are used together --------------------------------------------------------
+
+
+def serve(g, cache, steps, layers, heads, dim, dtype, check_rows):
+    """A serving loop: rows end, start and continue one another, and every row gets tokens; yields each step's work."""
+    from systems_for_llms_amd import paged
+
+    batch, kv = cache.lengths.shape[0], cache.k.shape[2]
+    kept = [[([], []) for _ in range(layers)] for _ in range(batch)]  # what was appended, by row and layer
+    for step in range(steps):
+        parents = torch.arange(batch)
+        if step:
+            move = torch.rand(batch, generator=g)
+            parents = torch.where(move < 0.15, -1, torch.where(move < 0.4, torch.randint(0, batch, (batch,), generator=g), parents))
+        paged.fork(cache, parents.to(torch.int32).cuda())
+        kept = [[(list(ks), list(vs)) for ks, vs in kept[p]] if p >= 0 else [([], []) for _ in range(layers)]
+                for p in parents.tolist()]
+        tokens = 40 if step % 5 == 0 else 1 + step % 4
+        wish = torch.randint(1, tokens + 1, (batch,), generator=g).to(torch.int32)
+        granted = paged.reserve(cache, wish.cuda())
+        accepted = torch.minimum(granted.cpu(), torch.randint(1, tokens + 1, (batch,), generator=g).to(torch.int32))
+        for layer in range(layers):
+            k, v = (randn(g, batch, kv, tokens, dim, dtype=dtype) for _ in range(2))
+            q = randn(g, batch, heads, tokens, dim, dtype=dtype)
+            paged.append(cache, k.cuda(), v.cuda(), layer=layer, counts=granted)
+            out, lse = paged.attend(q.cuda(), cache, layer=layer, counts=granted)
+            check_rows(kept, q, k, v, granted.cpu(), layer, out, lse)
+            for b in range(batch):
+                kept[b][layer][0].extend(k[b, :, : accepted[b]].unbind(1))
+                kept[b][layer][1].extend(v[b, :, : accepted[b]].unbind(1))
+        cache.lengths.add_(accepted.cuda())
+        if step % 7 == 6:
+            used = int(paged.compact(cache))
+            refs = cache.refs.cpu()
+            assert bool((refs[:used] > 0).all()) and not bool(refs[used:].any())
+        held = cache.tables[cache.tables >= 0].long().cpu()
+        assert torch.equal(torch.bincount(held, minlength=cache.refs.numel()).to(torch.int32), cache.refs.cpu())
+
+
+@pytest.mark.parametrize("dtype, page", [(BF16, 16), (FP16, 32)])
+def test_serving_loop(dtype, page):
+    """Forks, reservations, appends, attention and compaction over and over. Against the tokens as they were given,
+    each key and value off by at most 2^-4 of itself (a code's half step) and 2^-10 of its page's largest
+    (half a step of the smallest codes, 2^-10 of a scale that is at most 2^-7 of the largest after one growth by
+    rounding; a few re-roundings)."""
+    from systems_for_llms_amd import paged
+
+    g = torch.Generator().manual_seed(page)
+    batch, kv, heads, dim, layers = 6, 2, 4, 32, 2
+    cache = paged.create(batch, 400, kv, dim, 200, layers=layers, page_size=page)
+    seen = [0]
+
+    def check_rows(kept, q, k, v, granted, layer, out, lse):
+        out, lse = out.double().cpu(), lse.double().cpu()
+        for b in range(batch):
+            c = int(granted[b])
+            assert not out[b, :, c:].any() and bool((lse[b, :, c:] == -float("inf")).all())
+            if not c:
+                continue
+            ks, vs = (torch.stack(list(x) + list(y[b, :, :c].unbind(1)), 1).double().repeat_interleave(2, 0)
+                      for x, y in zip(kept[b][layer], (k, v)))
+            n = ks.shape[1] - c
+            x = q[b, :, :c].double() @ ks.mT / dim ** 0.5
+            row = (torch.arange(n + c) <= n + torch.arange(c)[:, None])
+            x = x.masked_fill(~row, -float("inf"))
+            p = x.softmax(-1)
+            want = p @ vs
+            # Scores off by 2^-4 of sum |q k| at most, on average far less: a key's errors are independent.
+            off = 2.0 ** -4 * (q[b, :, :c].double().square() @ ks.square().mT).sqrt() / dim ** 0.5
+            lift = off.masked_fill(~row, 0.0).amax(-1, keepdim=True) * 4
+            bound = (2 * lift.exp() - 2) * (p @ vs.abs()) + 2.0 ** -3 * (p @ vs.abs()) + 2.0 ** -6
+            assert bool(((out[b, :, :c] - want).abs() <= bound).all())
+            assert bool(((lse[b, :, :c] - x.logsumexp(-1)).abs() <= lift[..., 0] + 1e-3).all())
+            seen[0] += 1
+
+    serve(g, cache, 24, layers, heads, dim, dtype, check_rows)
+    assert seen[0] > 100
+
+
+@pytest.mark.parametrize("pages", [24, 5])
+def test_serving_loop_when_the_pool_is_small(pages):
+    """Rows that get fewer tokens than they ask for; what is there stays right."""
+    from systems_for_llms_amd import paged
+
+    g = torch.Generator().manual_seed(31)
+    cache = paged.create(5, 300, 2, 32, pages, layers=1, page_size=16)
+    short = [0]
+
+    def check_rows(kept, q, k, v, granted, layer, out, lse):
+        state = {n: getattr(cache, n).cpu() for n in NAMES}
+        check(q, state, got=(out, lse), counts=granted)
+        short[0] += int((granted == 0).sum())
+
+    serve(g, cache, 16, 1, 4, 32, FP16, check_rows)
+    assert short[0] > 0 or pages > 5
+
+
+def test_captured_step_replays():
+    """A step's calls in one HIP graph, replayed with eager work of the same kind in between."""
+    from systems_for_llms_amd import paged
+
+    g = torch.Generator().manual_seed(41)
+    state = books_state(g, 4, 12, 60, dim=64, layers=1)
+
+    def inputs():
+        return {"parents": torch.tensor([0, 0, 2, -1], dtype=torch.int32)[torch.randperm(4, generator=g)],
+                "counts": torch.randint(0, 4, (4,), generator=g).to(torch.int32), "k": randn(g, 4, 2, 3, 64, dtype=FP16),
+                "v": randn(g, 4, 2, 3, 64, dtype=FP16), "q": randn(g, 4, 4, 3, 64, dtype=FP16)}
+
+    def step(cache, s, op):
+        paged.fork(cache, s["parents"])
+        granted = paged.reserve(cache, s["counts"])
+        paged.append(cache, s["k"], s["v"], counts=granted)
+        op.counts.copy_(granted)
+        op()
+        cache.lengths.add_(granted)
+        return granted, paged.compact(cache), op.output, op.lse
+
+    def prepared(cache, s):
+        return paged.prepare(s["q"], cache, counts=torch.zeros(4, dtype=torch.int32, device="cuda"), splits=2)
+
+    def restore(cache, s, books, given):
+        for n in NAMES:
+            getattr(cache, n).view(torch.uint8 if n in "kv" else getattr(cache, n).dtype).copy_(
+                books[n].view(torch.uint8 if n in "kv" else books[n].dtype))
+        for n in given:
+            s[n].copy_(given[n])
+
+    cache, static = on_gpu(state), {n: x.cuda() for n, x in inputs().items()}
+    op = prepared(cache, static)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step(cache, static, op)
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step(cache, static, op)
+    for _ in range(5):
+        given = inputs()
+        books = books_state(g, 4, 12, 60, dim=64, layers=1)
+        restore(cache, static, books, given)
+        graph.replay()
+        other, eager = on_gpu(books), {n: x.cuda() for n, x in given.items()}
+        want = step(other, eager, prepared(other, eager))
+        torch.cuda.synchronize()
+        for x, y in zip(captured, want):
+            assert torch.equal(x, y)
+        for n in NAMES:
+            assert torch.equal(bits(getattr(cache, n)), bits(getattr(other, n))) if n in "kv" else \
+                torch.equal(getattr(cache, n), getattr(other, n)), n
+
+
+def test_calls_on_two_streams_at_once():
+    from systems_for_llms_amd import paged
+
+    g = torch.Generator().manual_seed(51)
+    ops, cpu = [], []
+    for i in range(2):
+        state = random_cache(g, [2990, 1500 + i], 2, 64, 64, room=5)
+        q = randn(g, 2, 8, 5, 64, dtype=BF16)
+        cpu.append((q, state))
+        ops.append(paged.prepare(q.cuda(), on_gpu(state), splits=4))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(3):
+        for op, stream in zip(ops, streams):
+            with torch.cuda.stream(stream):
+                op()
+    torch.cuda.synchronize()
+    for op, (q, state) in zip(ops, cpu):
+        check(q, state, got=(op.output, op.lse))
+
+
+def test_results_repeat_bit_for_bit():
+    from systems_for_llms_amd import paged
+
+    g = torch.Generator().manual_seed(61)
+    state = random_cache(g, [3980], 2, 128, 64, room=20)
+    op = paged.prepare(randn(g, 1, 8, 20, 128, dtype=FP16).cuda(), on_gpu(state), splits=7)
+    first, lse = op().clone(), op.lse.clone()
+    for _ in range(2):
+        assert torch.equal(op(), first) and torch.equal(op.lse, lse)
