@@ -11,6 +11,8 @@
 // power of two), on their way into the matrix cores; what has more bits goes in as a sum of
 // bf16 pieces: q and the probabilities of fp16 as two, of fp32 as three, so the only
 // roundings are those of the probabilities to the sum of their pieces and of fp32 sums.
+#include <limits.h>
+
 #include <algorithm>
 #include <type_traits>
 
@@ -23,7 +25,6 @@ namespace {
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
-constexpr int kPagedWaves = 4;
 constexpr int kPagedTile = 64;  // keys of a wave's tile
 constexpr int kMaxTokens = 128;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -57,6 +58,38 @@ __device__ __forceinline__ PagedRow paged_row(const PagedArgs& a, int b) {
   r.count = a.counts ? min(max(Constant(a.counts)[b], 0), a.tokens) : a.tokens;
   r.count = min(r.count, r.cap - r.len);  // tokens that have a slot
   return r;
+}
+
+// A workgroup's work: some rows of a KV head of sequence b over a part of its tiles.
+struct Work {
+  int b, hk, part, group;  // group: the head among those of all sequences
+  int r0, rows;            // first row of the block; rows of a sequence
+  int t0, t1;              // tokens of the block
+  int start, end;          // slots that some row of the block sees
+  int begin, count;        // its tiles
+  PagedRow row;
+};
+__device__ __forceinline__ bool find_work(const PagedArgs& a, int block, Work& w) {
+  // Row blocks of one unit run on one XCD, whose L2 then holds its pages.
+  const int slice = int(blockIdx.x) / kXcds;
+  const int unit = slice / a.row_blocks * kXcds + int(blockIdx.x) % kXcds;
+  if (unit >= a.groups * a.splits) return false;
+  w.r0 = slice % a.row_blocks * block;
+  w.group = __builtin_amdgcn_readfirstlane(unit / a.splits);
+  w.part = unit - w.group * a.splits;
+  w.b = __builtin_amdgcn_readfirstlane(w.group / a.kv_heads);
+  w.hk = w.group - w.b * a.kv_heads;
+  w.row = paged_row(a, w.b);
+  w.rows = a.tokens << a.group_log2;
+  w.t0 = w.r0 >> a.group_log2, w.t1 = min((min(w.r0 + block, w.rows) - 1) >> a.group_log2, w.row.count - 1);
+  w.end = w.t1 >= w.t0 ? w.row.len + w.t1 + 1 : 0;
+  w.start = a.window >= 0 ? max(w.row.len + w.t0 - a.window, 0) : 0;
+  // The tiles from that of `start` on are shared out evenly, however long the row is.
+  const int first = w.start / kPagedTile, tiles = max((w.end + kPagedTile - 1) / kPagedTile - first, 0);
+  const int each = tiles / a.splits, more = tiles - each * a.splits;  // one more in the first ones
+  w.begin = first + w.part * each + min(w.part, more);
+  w.count = each + (w.part < more);
+  return true;
 }
 
 __device__ __forceinline__ f32x4 mfma16(const u32x4& a, const u32x4& b, f32x4 c) {
@@ -94,27 +127,28 @@ struct Tile {
   // Dims of step s in lane group g: heads of 64 and 128 take 16 bytes in a row for two steps.
   static __device__ __forceinline__ int dim(int s, int g) { return D >= 64 ? s / 2 * 64 + g * 16 + s % 2 * 8 : 8 * g; }
 
-  static __device__ __forceinline__ void load_k(const uint8_t* row, int g, uint32_t (&w)[kWords]) {
+  // Of the lane's part of a row of K.
+  static __device__ __forceinline__ int part(int g) { return D >= 64 ? 16 * g : D == 32 ? 8 * g : 8 * (g & 1); }
+  static __device__ __forceinline__ void load_k(const uint8_t* at, int g, uint32_t (&w)[kWords]) {
     if constexpr (D >= 64) {
 #pragma unroll
       for (int e = 0; e < D / 64; ++e) {
-        const u32x4 r = *reinterpret_cast<const u32x4*>(row + 64 * e + 16 * g);
+        const u32x4 r = *reinterpret_cast<const u32x4*>(at + 64 * e);
 #pragma unroll
         for (int x = 0; x < 4; ++x) w[4 * e + x] = r[x];
       }
     } else {
-      const u32x2 r = *reinterpret_cast<const u32x2*>(row + (D == 32 ? 8 * g : 8 * (g & 1)));
+      const u32x2 r = *reinterpret_cast<const u32x2*>(at);
       w[0] = D == 16 && g > 1 ? 0u : r[0], w[1] = D == 16 && g > 1 ? 0u : r[1];
     }
   }
 };
 
-// One query row's operand of step s, as pieces.
-template <typename T, int D>
-__device__ __forceinline__ void load_q(const T* row, int s, int g, u32x4 (&q)[pieces_of<T>()]) {
+// Eight values of q as pieces, cut rather than rounded so that the pieces' sum is the value
+// (zeros where not `on`).
+template <typename T>
+__device__ __forceinline__ void load_pieces(const T* at, bool on, u32x4 (&q)[pieces_of<T>()]) {
   constexpr int P = pieces_of<T>(), E = vec_elems<T>();
-  const bool on = D > 16 || g < 2;
-  const T* at = row + Tile<D>::dim(s, D > 16 ? g : g & 1);
   if constexpr (P == 1) {
     const uint4 r = load16(at);
     q[0] = on ? u32x4{r.x, r.y, r.z, r.w} : u32x4{0u, 0u, 0u, 0u};
@@ -127,21 +161,36 @@ __device__ __forceinline__ void load_q(const T* row, int s, int g, u32x4 (&q)[pi
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const uint32_t lo = __float_as_uint(x[2 * e]), hi = __float_as_uint(x[2 * e + 1]);
-        q[p][e] = on ? (lo >> 16) | (hi & 0xffff0000u) : 0u;  // cut, so that the pieces' sum is x
+        q[p][e] = on ? (lo >> 16) | (hi & 0xffff0000u) : 0u;
         x[2 * e] -= __uint_as_float(lo & 0xffff0000u);
         x[2 * e + 1] -= __uint_as_float(hi & 0xffff0000u);
       }
   }
 }
 
-// Where a lane's keys lie.
-struct Spot {
-  int page;  // 0 where there is none
-  bool on;
-};
-__device__ __forceinline__ Spot spot_of(const PagedArgs& a, int entry, int slot, int cap) {
-  const bool on = slot < cap && entry >= 0 && entry < a.pages;
-  return Spot{on ? entry : 0, on};
+// Eight probabilities as pieces, each what the ones before it leave, rounded.
+template <int P>
+__device__ __forceinline__ void split_pieces(float (&x)[8], u32x4 (&prob)[P]) {
+#pragma unroll
+  for (int p = 0; p < P; ++p)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t w = pack2<bf16_t>(x[2 * e], x[2 * e + 1]);
+      prob[p][e] = w;
+      x[2 * e] -= bf16_lo(w), x[2 * e + 1] -= bf16_hi(w);
+    }
+}
+
+// Ones in bf16 where eight codes are NaN, zeros elsewhere.
+__device__ __forceinline__ u32x4 nan_ones(uint32_t lo, uint32_t hi) {
+  const uint32_t m[2] = {nan_bytes(lo), nan_bytes(hi)};
+  u32x4 r;
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    r[2 * x] = (m[x] & 0xff ? 0x3f80u : 0u) | (m[x] & 0xff00 ? 0x3f800000u : 0u);
+    r[2 * x + 1] = (m[x] & 0xff0000 ? 0x3f80u : 0u) | (m[x] & 0xff000000u ? 0x3f800000u : 0u);
+  }
+  return r;
 }
 
 template <typename T>
@@ -153,33 +202,32 @@ __device__ __forceinline__ void store4(T* p, const float* v) {
   }
 }
 
+// Values are read once, past the caches, where a tile has whole lines of them. Pages of 128
+// tokens have two tiles to a line.
+template <int kPage>
+__device__ __forceinline__ u32x4 load_v(const uint8_t* at) {
+  const u32x4* p = reinterpret_cast<const u32x4*>(at);
+  return kPage == 128 ? *p : __builtin_nontemporal_load(p);
+}
+
 // A workgroup has up to 16 NC query rows (the G heads of a KV head times the tokens, row
 // r = t G + g) and a split of the keys; its waves take the split's tiles in turn and are
 // joined through LDS at the end.
-template <typename T, int D, int NC>
-__global__ __launch_bounds__(kPagedWaves * kWave) void paged_attention_kernel(const PagedArgs a) {
+template <typename T, int D, int NC, int kPage, int W>
+__global__ __launch_bounds__(W * kWave, D == 128 && NC == 2 ? 1 : 2) void paged_attention_kernel(const PagedArgs a) {
   using L = Tile<D>;
-  constexpr int P = pieces_of<T>(), W = kPagedWaves, BT = kPagedTile, kRows = 16 * NC, kLine = D + 4;
+  constexpr bool kWide = kPage >= kPagedTile;
+  constexpr int P = pieces_of<T>(), BT = kPagedTile, kRows = 16 * NC, kLine = D + 4;
   __shared__ float merged[W][kRows][kLine];
   __shared__ float tops[W][kRows], sums[W][kRows];
   const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave);
   const int lane = threadIdx.x % kWave, g = lane / 16, n = lane % 16;
-  // Row blocks of one unit run on one XCD, whose L2 then holds its pages.
-  const int slice = int(blockIdx.x) / kXcds;
-  const int unit = slice / a.row_blocks * kXcds + int(blockIdx.x) % kXcds;
-  if (unit >= a.groups * a.splits) return;
-  const int r0 = slice % a.row_blocks * kRows;
-  const int group = __builtin_amdgcn_readfirstlane(unit / a.splits), part = unit - group * a.splits;
-  const int b = __builtin_amdgcn_readfirstlane(group / a.kv_heads), hk = group - b * a.kv_heads;
-  const PagedRow row = paged_row(a, b);
-  const int rows = a.tokens << a.group_log2, G = 1 << a.group_log2;
-  const int t0 = r0 >> a.group_log2, t1 = min((min(r0 + kRows, rows) - 1) >> a.group_log2, row.count - 1);  // tokens
-
-  // Slots that some row of the block sees, in whole tiles of which this split has some.
-  const int end = t1 >= t0 ? row.len + t1 + 1 : 0;
-  const int start = a.window >= 0 ? max(row.len + t0 - a.window, 0) : 0;
-  const int tile0 = start / BT, tiles = max((end + BT - 1) / BT - tile0, 0);
-  const int begin = tile0 + int(long(tiles) * part / a.splits), stop = tile0 + int(long(tiles) * (part + 1) / a.splits);
+  Work work;
+  if (!find_work(a, kRows, work)) return;
+  const int b = work.b, hk = work.hk, r0 = work.r0, rows = work.rows, G = 1 << a.group_log2;
+  const PagedRow row = work.row;
+  const int t0 = work.t0, t1 = work.t1, start = work.start, end = work.end;
+  const int begin = work.begin, stop = work.begin + work.count;
 
   u32x4 q[NC][L::kSteps][P];
   int seen_from[NC], seen_to[NC];  // first and last slot of the lane's query row
@@ -188,7 +236,7 @@ __global__ __launch_bounds__(kPagedWaves * kWave) void paged_attention_kernel(co
     const int r = min(r0 + 16 * c + n, rows - 1), t = r >> a.group_log2, head = (hk << a.group_log2) + (r & (G - 1));
     const T* at = static_cast<const T*>(a.q) + b * a.qs[0] + head * a.qs[1] + t * a.qs[2];
 #pragma unroll
-    for (int s = 0; s < L::kSteps; ++s) load_q<T, D>(at, s, g, q[c][s]);
+    for (int s = 0; s < L::kSteps; ++s) load_pieces<T>(at + L::dim(s, D > 16 ? g : g & 1), D > 16 || g < 2, q[c][s]);
     seen_to[c] = t < row.count ? row.len + t : -1;
     seen_from[c] = a.window >= 0 ? row.len + t - a.window : 0;
   }
@@ -201,37 +249,61 @@ __global__ __launch_bounds__(kPagedWaves * kWave) void paged_attention_kernel(co
     for (int d = 0; d < L::kDims; ++d) o[c][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
+  // The pages of the wave's next tiles, one or (pages of less than a tile) four to a tile, and
+  // their scales, a lane each: nothing in the loop below waits for a page before it can ask
+  // for its rows.
+  constexpr int kSpots = kWide ? 1 : 4, kBatch = kWave / kSpots;
   const int32_t* table = a.tables + long(b) * a.places;
   const int page_mask = (1 << a.page_log2) - 1;
-  const int off_k = n / 4 * 16, off_v = g * 16;  // of the lane's keys in a tile
-  const auto entry = [&](int slot) { return table[min(slot >> a.page_log2, a.places - 1)]; };
-  uint32_t kw[4][L::kWords];
-  float ks = 0.f;
-  const auto fetch_k = [&](int tile, int e) {
-    const int slot = tile * BT + off_k;
-    const long block = long(spot_of(a, e, slot, row.cap).page) * a.kv_heads + hk;
-    ks = a.k_scale[block];
-    const uint8_t* at = a.k + ((block << a.page_log2) + (slot & page_mask) + n % 4) * D;
-#pragma unroll
-    for (int t = 0; t < 4; ++t) L::load_k(at + 4 * t * D, g, kw[t]);
+  const int count = stop - begin - wave > 0 ? (stop - begin - wave + W - 1) / W : 0;  // the wave's tiles
+  const auto tile_of = [&](int i) { return begin + wave + W * i; };
+  int spots = -1;  // -1: no page
+  float spots_ks = 0.f, spots_vs = 0.f;
+  const auto look_up = [&](int i) {
+    const int slot = tile_of(min(i + lane / kSpots, count - 1)) * BT + lane % kSpots * 16;
+    const int page = table[min(slot >> a.page_log2, a.places - 1)];
+    spots = slot < row.cap && page >= 0 && page < a.pages ? page : -1;
+    const long block = long(max(spots, 0)) * a.kv_heads + hk;
+    spots_ks = a.k_scale[block], spots_vs = a.v_scale[block];
+  };
+  const auto pick = [&](auto x, int i, int sub) {  // of tile i's keys from 16 sub on
+    const uint32_t bits = __builtin_bit_cast(uint32_t, x);
+    const uint32_t got = kWide ? __builtin_amdgcn_readlane(bits, i % kBatch) : uint32_t(__shfl(int(bits), i % kBatch * kSpots + sub));
+    return __builtin_bit_cast(decltype(x), got);
   };
 
-  int tile = begin + wave, ek = 0, ev = 0;
-  if (tile < stop) {
-    ek = entry(tile * BT + off_k), ev = entry(tile * BT + off_v);
-    fetch_k(tile, ek);
-  }
-  for (; tile < stop; tile += W) {
-    const int slot0 = tile * BT;
-    const Spot spot = spot_of(a, ev, slot0 + off_v, row.cap);
-    u32x4 vw[L::kDims];
-    const long block = long(spot.page) * a.kv_heads + hk;
-    const float vs = a.v_scale[block];
-    const uint8_t* at = a.v + (((block * D) + n) << a.page_log2) + ((slot0 + off_v) & page_mask);
+  const int off_k = n / 4 * 16, off_v = g * 16;  // of the lane's keys in a tile
+  const int sub_k = kWide ? 0 : off_k, sub_v = kWide ? 0 : off_v;
+  uint32_t kw[4][L::kWords];
+  float ks = 0.f;
+  const auto fetch_k = [&](int i) {
+    const long block = long(max(pick(spots, i, n / 4), 0)) * a.kv_heads + hk;
+    ks = pick(spots_ks, i, n / 4);
+    const uint8_t* base = a.k + ((block << a.page_log2) + ((tile_of(i) * BT + sub_k) & page_mask)) * D;
+    const unsigned lane_at = unsigned(((kWide ? off_k : 0) + n % 4) * D + L::part(g));
 #pragma unroll
-    for (int d = 0; d < L::kDims; ++d) vw[d] = *reinterpret_cast<const u32x4*>(at + (d * 16 << a.page_log2));
-    const int next = min(tile + W, stop - 1);
-    ek = entry(next * BT + off_k), ev = entry(next * BT + off_v);
+    for (int t = 0; t < 4; ++t) L::load_k(base + lane_at + 4 * t * D, g, kw[t]);
+  };
+  // Tiles that some row does not see whole.
+  const auto partly_seen = [&](int slot0, int spot) {
+    return slot0 + BT - 1 > row.len + t0 || (a.window >= 0 && slot0 < row.len + t1 - a.window) || __any(spot < 0);
+  };
+  const auto sees = [&](int c, int slot, int spot) { return spot >= 0 && slot <= seen_to[c] && slot >= seen_from[c]; };
+  bool found = false;  // NaN among the values of such a tile
+
+  if (count > 0) {
+    look_up(0);
+    fetch_k(0);
+  }
+  for (int i = 0; i < count; ++i) {
+    const int slot0 = tile_of(i) * BT, spot = pick(spots, i, g);
+    u32x4 vw[L::kDims];
+    const float vs = pick(spots_vs, i, g);
+    const uint8_t* base = a.v + (((long(max(spot, 0)) * a.kv_heads + hk) * D) << a.page_log2) + ((slot0 + sub_v) & page_mask);
+    const unsigned lane_at = unsigned((n << a.page_log2) + (kWide ? off_v : 0));
+#pragma unroll
+    for (int d = 0; d < L::kDims; ++d)
+      vw[d] = load_v<kPage>(base + (d * 16 << a.page_log2) + lane_at);
 
     f32x4 s[NC][4];
 #pragma unroll
@@ -247,23 +319,17 @@ __global__ __launch_bounds__(kPagedWaves * kWave) void paged_attention_kernel(co
           for (int p = P - 1; p >= 0; --p) s[c][t] = mfma16(key, q[c][st][p], s[c][t]);
       }
     }
-    fetch_k(next, ek);
+    if (i + 1 < count) {
+      if ((i + 1) % kBatch == 0) look_up(i + 1);
+      fetch_k(i + 1);
+    }
 
-    // Tiles that some row does not see whole.
-    uint32_t seen[NC];
-    const bool masked = slot0 + BT - 1 > row.len + t0 || (a.window >= 0 && slot0 < row.len + t1 - a.window) || __any(!spot.on);
+    const bool masked = partly_seen(slot0, spot);
     if (masked) {
 #pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        seen[c] = 0;
+      for (int c = 0; c < NC; ++c)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int slot = slot0 + off_v + e;
-          const bool on = spot.on && slot <= seen_to[c] && slot >= seen_from[c];
-          seen[c] |= uint32_t(on) << e;
-          s[c][e / 4][e % 4] = on ? s[c][e / 4][e % 4] : -INFINITY;
-        }
-      }
+        for (int e = 0; e < 16; ++e) s[c][e / 4][e % 4] = sees(c, slot0 + off_v + e, spot) ? s[c][e / 4][e % 4] : -INFINITY;
     }
     u32x4 prob[NC][2][P];
 #pragma unroll
@@ -284,60 +350,33 @@ __global__ __launch_bounds__(kPagedWaves * kWave) void paged_attention_kernel(co
         for (int d = 0; d < L::kDims; ++d) o[c][d] *= keep;
       }
       const float base = top[c] == -INFINITY ? 0.f : top[c];
-      float x[16];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) x[e] = __builtin_amdgcn_exp2f(fmaf(s[c][e / 4][e % 4], a.cs, -base));
-#pragma unroll
-      for (int e = 0; e < 16; ++e) sum[c] += x[e];
-#pragma unroll
-      for (int p = 0; p < P; ++p)
+      for (int y = 0; y < 2; ++y) {
+        float x[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const uint32_t w = pack2<bf16_t>(x[2 * e], x[2 * e + 1]);
-          prob[c][e / 4][p][e % 4] = w;
-          x[2 * e] -= bf16_lo(w), x[2 * e + 1] -= bf16_hi(w);
+          x[e] = __builtin_amdgcn_exp2f(fmaf(s[c][2 * y + e / 4][e % 4], a.cs, -base));
+          sum[c] += x[e];
         }
+        split_pieces(x, prob[c][y]);
+      }
     }
     if (masked) {
       // Values of slots that nobody sees become zeros: old codes there may be NaN. NaN in slots
-      // that some rows see makes the sums of those rows NaN, and only those.
-      const int from = start - (slot0 + off_v), to = spot.on ? end - (slot0 + off_v) : 0;
+      // that some rows see and some do not is zero here, too, and put into its rows below.
+      const int from = start - (slot0 + off_v), to = spot >= 0 ? end - (slot0 + off_v) : 0;
       uint32_t bad = 0;
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
         const uint32_t keep = first_bytes(to - 4 * x) & ~first_bytes(from - 4 * x);
 #pragma unroll
         for (int d = 0; d < L::kDims; ++d) {
-          vw[d][x] &= keep;
-          bad |= nan_bytes(vw[d][x]);
+          const uint32_t w = vw[d][x] & keep, is_nan = nan_bytes(w);
+          vw[d][x] = w & ~is_nan;
+          bad |= is_nan;
         }
       }
-      if (__any(bad != 0)) {
-        u32x4 sees[NC][2];
-#pragma unroll
-        for (int c = 0; c < NC; ++c)
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            sees[c][e / 4][e % 4] = (seen[c] >> (2 * e) & 1 ? 0x3f80u : 0u) | (seen[c] >> (2 * e + 1) & 1 ? 0x3f800000u : 0u);
-#pragma unroll
-        for (int d = 0; d < L::kDims; ++d) {
-          u32x4 is_nan[2];
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const uint32_t m = nan_bytes(vw[d][x]);
-            vw[d][x] &= ~m;
-            is_nan[x / 2][x % 2 * 2] = (m & 0xff ? 0x3f80u : 0u) | (m & 0xff00 ? 0x3f800000u : 0u);
-            is_nan[x / 2][x % 2 * 2 + 1] = (m & 0xff0000 ? 0x3f80u : 0u) | (m & 0xff000000u ? 0x3f800000u : 0u);
-          }
-#pragma unroll
-          for (int c = 0; c < NC; ++c) {
-            f32x4 hit = mfma16(is_nan[0], sees[c][0], f32x4{0.f, 0.f, 0.f, 0.f});
-            hit = mfma16(is_nan[1], sees[c][1], hit);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[c][d][e] = hit[e] > 0.f ? NAN : o[c][d][e];
-          }
-        }
-      }
+      found |= __any(bad != 0);
     }
 #pragma unroll
     for (int d = 0; d < L::kDims; ++d)
@@ -349,6 +388,34 @@ __global__ __launch_bounds__(kPagedWaves * kWave) void paged_attention_kernel(co
 #pragma unroll
           for (int p = P - 1; p >= 0; --p) o[c][d] = mfma16(value, prob[c][h][p], o[c][d]);
       }
+  }
+  if (found) {
+    // Which rows see a NaN, as products of what is NaN with what is seen.
+    for (int i = 0; i < count; ++i) {
+      if (i % kBatch == 0) look_up(i);
+      const int slot0 = tile_of(i) * BT, spot = pick(spots, i, g);
+      if (!partly_seen(slot0, spot)) continue;
+      u32x4 on[NC][2];
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          on[c][e / 4][e % 4] = (sees(c, slot0 + off_v + 2 * e, spot) ? 0x3f80u : 0u) |
+                                (sees(c, slot0 + off_v + 2 * e + 1, spot) ? 0x3f800000u : 0u);
+      const uint8_t* at = a.v + (((long(max(spot, 0)) * a.kv_heads + hk) * D + n) << a.page_log2) + ((slot0 + off_v) & page_mask);
+#pragma unroll
+      for (int d = 0; d < L::kDims; ++d) {
+        const u32x4 w = *reinterpret_cast<const u32x4*>(at + (d * 16 << a.page_log2));
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          f32x4 hits = mfma16(nan_ones(w[0], w[1]), on[c][0], f32x4{0.f, 0.f, 0.f, 0.f});
+          hits = mfma16(nan_ones(w[2], w[3]), on[c][1], hits);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[c][d][e] = hits[e] > 0.f ? NAN : o[c][d][e];
+        }
+        __builtin_amdgcn_sched_barrier(0);  // few registers rather than many loads at once
+      }
+    }
   }
 
 #pragma unroll
@@ -378,7 +445,7 @@ __global__ __launch_bounds__(kPagedWaves * kWave) void paged_attention_kernel(co
     }
     const int t = r >> a.group_log2, head = (hk << a.group_log2) + (r & (G - 1));
     if (a.splits > 1) {
-      const long to = (long(group) * a.splits + part) * rows + r;
+      const long to = (long(work.group) * a.splits + work.part) * rows + r;
       if (d == 0) a.pmax[to] = base, a.psum[to] = den;
       store4<float>(a.pout + to * D + d, num);
     } else {
@@ -391,28 +458,273 @@ __global__ __launch_bounds__(kPagedWaves * kWave) void paged_attention_kernel(co
   }
 }
 
-// The splits of a row joined: a wave to a row, kRound splits' loads at a time.
-template <typename T, int D>
+// The same for more rows: W waves with 32 query rows each, and tiles of 64 keys that they
+// share. The codes of a tile are read once, become bf16 on the way into LDS (K [key][dim],
+// V [dim][key], 16-byte slots swizzled by row), and are operands of 32 x 32 x 16 MFMAs from
+// there, the next tile's codes under way meanwhile. Row m of S^T takes the key
+// 16 (m / 16) + 8 (m / 4 % 2) + 4 (m / 8 % 2) + m % 4 of its 32, so that lane (h, n), lane =
+// 32 h + n, holds the scores of keys 16 x + 8 h .. + 7 of query row n: its k-slots in the
+// product with V.
+template <typename T, int D, int kPage, int W>
+__global__ __launch_bounds__(W * kWave, 2) void paged_rows_kernel(const PagedArgs a) {
+  constexpr bool kWide = kPage >= kPagedTile;
+  constexpr int P = pieces_of<T>(), BT = kPagedTile, kRows = 32 * W, kThreads = W * kWave;
+  constexpr int kSteps = D / 16, kTiles = D / 32;          // of the products with K, of dims of V
+  constexpr int kPieces = BT * D / 16 / kThreads;          // of 16 codes of a tile's keys a thread stages
+  constexpr int kSpots = kWide ? 1 : 4, kBatch = kWave / kSpots;
+  __shared__ u32x4 keys[BT * D / 8], values[D * BT / 8];
+  __shared__ int found;
+  const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave);
+  const int lane = threadIdx.x % kWave, h = lane / 32, n = lane % 32;
+  Work work;
+  if (!find_work(a, kRows, work)) return;
+  const int b = work.b, hk = work.hk, r0 = work.r0, rows = work.rows, G = 1 << a.group_log2;
+  const PagedRow row = work.row;
+  const int t0 = work.t0, t1 = work.t1, start = work.start, end = work.end, begin = work.begin, count = work.count;
+
+  const bool active = r0 + 32 * wave < rows;
+  const int r = min(r0 + 32 * wave + n, rows - 1), t = r >> a.group_log2, head = (hk << a.group_log2) + (r & (G - 1));
+  const int seen_to = t < row.count ? row.len + t : -1, seen_from = a.window >= 0 ? row.len + t - a.window : 0;
+  u32x4 q[kSteps][P];
+  {
+    const T* at = static_cast<const T*>(a.q) + b * a.qs[0] + head * a.qs[1] + t * a.qs[2] + 8 * h;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) load_pieces<T>(at + 16 * s, true, q[s]);
+  }
+  f32x16 o[kTiles];
+#pragma unroll
+  for (int d = 0; d < kTiles; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
+  float top = -INFINITY, sum = 0.f;
+
+  const int32_t* table = a.tables + long(b) * a.places;
+  const int page_mask = (1 << a.page_log2) - 1;
+  int spots = -1;
+  float spots_ks = 0.f, spots_vs = 0.f;
+  const auto look_up = [&](int i) {
+    const int slot = (begin + min(i + lane / kSpots, count - 1)) * BT + lane % kSpots * 16;
+    const int page = table[min(slot >> a.page_log2, a.places - 1)];
+    spots = slot < row.cap && page >= 0 && page < a.pages ? page : -1;
+    const long block = long(max(spots, 0)) * a.kv_heads + hk;
+    spots_ks = a.k_scale[block], spots_vs = a.v_scale[block];
+  };
+  const auto pick = [&](auto x, int i, int sub) {
+    const uint32_t bits = __builtin_bit_cast(uint32_t, x);
+    const uint32_t got = kWide ? __builtin_amdgcn_readlane(bits, i % kBatch) : uint32_t(__shfl(int(bits), i % kBatch * kSpots + sub));
+    return __builtin_bit_cast(decltype(x), got);
+  };
+  // A thread's pieces: 16 dims of a key, 16 keys of a dim.
+  u32x4 kw[kPieces], vw[kPieces];
+  float ks[kPieces], vs[kPieces];
+  bool kept[kPieces];
+  const auto fetch = [&](int i) {
+    const int slot0 = (begin + i) * BT;
+#pragma unroll
+    for (int e = 0; e < kPieces; ++e) {
+      const int x = int(threadIdx.x) + kThreads * e, key = x / (D / 16), dim = x / 4;
+      const int page_k = pick(spots, i, key / 16), page_v = pick(spots, i, x % 4);
+      ks[e] = pick(spots_ks, i, key / 16), vs[e] = pick(spots_vs, i, x % 4);
+      kept[e] = page_v >= 0;
+      const long block_k = long(max(page_k, 0)) * a.kv_heads + hk, block_v = long(max(page_v, 0)) * a.kv_heads + hk;
+      kw[e] = *reinterpret_cast<const u32x4*>(a.k + ((block_k << a.page_log2) + ((slot0 + key) & page_mask)) * D + x % (D / 16) * 16);
+      vw[e] = *reinterpret_cast<const u32x4*>(a.v + ((block_v * D + dim) << a.page_log2) + ((slot0 + x % 4 * 16) & page_mask));
+    }
+  };
+  const auto partly_seen = [&](int slot0, bool whole) {
+    return slot0 + BT - 1 > row.len + t0 || (a.window >= 0 && slot0 < row.len + t1 - a.window) || !whole;
+  };
+  // Whether all of tile i's keys have a page.
+  const auto whole_tile = [&](int i) { return kWide ? pick(spots, i, 0) >= 0 : !__any(pick(spots, i, lane % 4) < 0); };
+  const int key_row = 16 * (n / 16) + 8 * (n / 4 % 2) + 4 * (n / 8 % 2) + n % 4;
+
+  if (threadIdx.x == 0) found = 0;
+  if (count > 0) {
+    look_up(0);
+    fetch(0);
+  }
+  for (int i = 0; i < count; ++i) {
+    const int slot0 = (begin + i) * BT;
+    const bool masked = partly_seen(slot0, whole_tile(i));
+    const int missing = masked ? (kWide ? (pick(spots, i, 0) < 0 ? 15 : 0) : int(__ballot(pick(spots, i, lane % 4) < 0) & 15)) : 0;
+    if (masked) {
+      // Values that nobody sees become zeros, and so does NaN, which goes to its rows at the end.
+      uint32_t bad = 0;
+#pragma unroll
+      for (int e = 0; e < kPieces; ++e) {
+        const int at = slot0 + (int(threadIdx.x) + kThreads * e) % 4 * 16;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const uint32_t keep = kept[e] ? first_bytes(end - at - 4 * x) & ~first_bytes(start - at - 4 * x) : 0u;
+          const uint32_t w = vw[e][x] & keep, is_nan = nan_bytes(w);
+          vw[e][x] = w & ~is_nan;
+          bad |= is_nan;
+        }
+      }
+      if (bad) found = 1;
+    }
+    __syncthreads();  // the last tile's operands are read
+#pragma unroll
+    for (int e = 0; e < kPieces; ++e) {
+      const int x = int(threadIdx.x) + kThreads * e, key = x / (D / 16), dim = x / 4;
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        keys[key * (D / 8) + ((x % (D / 16) * 2 + y) ^ k_swizzle<D>(key))] = from_codes(kw[e][2 * y], kw[e][2 * y + 1], ks[e]);
+        values[dim * (BT / 8) + ((x % 4 * 2 + y) ^ k_swizzle<64>(dim))] = from_codes(vw[e][2 * y], vw[e][2 * y + 1], vs[e]);
+      }
+    }
+    __syncthreads();
+    if (i + 1 < count) {
+      if ((i + 1) % kBatch == 0) look_up(i + 1);
+      fetch(i + 1);
+    }
+    if (!active) continue;
+
+    f32x16 s[2];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[half][e] = 0.f;
+      const int key = 32 * half + key_row;
+#pragma unroll
+      for (int st = 0; st < kSteps; ++st) {
+        const u32x4 w = keys[key * (D / 8) + ((2 * st + h) ^ k_swizzle<D>(key))];
+#pragma unroll
+        for (int p = P - 1; p >= 0; --p) s[half] = mfma32<bf16_t>(w, q[st][p], s[half]);
+      }
+    }
+    if (masked) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int at = 32 * half + 16 * (e / 8) + 8 * h + e % 8;
+          const bool on = slot0 + at <= seen_to && slot0 + at >= seen_from && !(missing >> (2 * half + e / 8) & 1);
+          s[half][e] = on ? s[half][e] : -INFINITY;
+        }
+    }
+    float high = s[0][0];
+#pragma unroll
+    for (int e = 1; e < 32; ++e) high = fmaxf(high, s[e / 16][e % 16]);
+    high = fmaxf(high, lane_xor(high, 32)) * a.cs;
+    const bool raise = high > top + kLazyMax;
+    if (__any(raise)) {
+      const float now = raise ? high : top;
+      const float keep = raise ? __builtin_amdgcn_exp2f(top - now) : 1.f;
+      top = now;
+      sum *= keep;
+#pragma unroll
+      for (int d = 0; d < kTiles; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[d][e] *= keep;
+    }
+    const float base = top == -INFINITY ? 0.f : top;
+    u32x4 prob[4][P];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      float y[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        y[e] = __builtin_amdgcn_exp2f(fmaf(s[x / 2][x % 2 * 8 + e], a.cs, -base));
+        sum += y[e];
+      }
+      split_pieces(y, prob[x]);
+    }
+#pragma unroll
+    for (int d = 0; d < kTiles; ++d) {
+      const int dim = 32 * d + n;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const u32x4 w = values[dim * (BT / 8) + ((2 * x + h) ^ k_swizzle<64>(dim))];
+#pragma unroll
+        for (int p = P - 1; p >= 0; --p) o[d] = mfma32<bf16_t>(w, prob[x][p], o[d]);
+      }
+    }
+  }
+  __syncthreads();
+  if (!active) return;
+  if (found) {
+    for (int i = 0; i < count; ++i) {
+      if (i % kBatch == 0) look_up(i);
+      const int slot0 = (begin + i) * BT;
+      if (!partly_seen(slot0, whole_tile(i))) continue;
+#pragma unroll 1
+      for (int x = 0; x < 4; ++x) {
+        const int spot = pick(spots, i, x), slot = slot0 + 16 * x + 8 * h;
+        u32x4 on;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const auto sees = [&](int at) { return spot >= 0 && at <= seen_to && at >= seen_from; };
+          on[e] = (sees(slot + 2 * e) ? 0x3f80u : 0u) | (sees(slot + 2 * e + 1) ? 0x3f800000u : 0u);
+        }
+        const uint8_t* at = a.v + (((long(max(spot, 0)) * a.kv_heads + hk) * D + n) << a.page_log2) + (slot & page_mask);
+#pragma unroll
+        for (int d = 0; d < kTiles; ++d) {
+          const u32x2 w = *reinterpret_cast<const u32x2*>(at + (d * 32 << a.page_log2));
+          f32x16 hits;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) hits[e] = 0.f;
+          hits = mfma32<bf16_t>(nan_ones(w[0], w[1]), on, hits);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[d][e] = hits[e] > 0.f ? NAN : o[d][e];
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+    }
+  }
+  sum += lane_xor(sum, 32);
+  if (top == -INFINITY && sum != sum) top = 0.f;  // as above
+  if (r0 + 32 * wave + n >= rows) return;
+  const bool empty = top == -INFINITY || t >= row.count;
+  const long to = (long(work.group) * a.splits + work.part) * rows + r;
+  if (h == 0) {
+    if (a.splits > 1)
+      a.pmax[to] = top, a.psum[to] = sum;
+    else
+      a.lse[(long(b) * a.kv_heads * G + head) * a.tokens + t] = empty ? -INFINITY : (top + __builtin_log2f(sum)) * kLn2;
+  }
+  T* out = static_cast<T*>(a.out) + b * a.os[0] + head * a.os[1] + t * a.os[2];
+  const float share = a.splits > 1 ? 1.f : empty ? 0.f : 1.f / sum;
+#pragma unroll
+  for (int d = 0; d < kTiles; ++d)
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      float num[4];
+      const int dim = 32 * d + 8 * x + 4 * h;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) num[e] = empty && a.splits == 1 ? 0.f : o[d][4 * x + e] * share;
+      if (a.splits > 1)
+        store4<float>(a.pout + to * D + dim, num);
+      else
+        store4<T>(out + dim, num);
+    }
+}
+
+// The splits of a row joined. A wave has a row, or with `kShared` a workgroup has one and
+// its four waves every fourth round of splits; kRound splits' loads go out together.
+template <typename T, int D, bool kShared>
 __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedArgs a) {
-  constexpr int DPL = (D + kWave - 1) / kWave, kRound = 8;
-  const int lane = threadIdx.x % kWave;
+  constexpr int DPL = (D + kWave - 1) / kWave, kRound = 8, W = kShared ? 4 : 1;
+  __shared__ float nums[kShared ? 4 : 1][D], tops[4], dens[4];
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
   const int rows = a.tokens << a.group_log2, G = 1 << a.group_log2;
-  const long at = long(blockIdx.x) * 4 + threadIdx.x / kWave;
+  const long at = kShared ? long(blockIdx.x) : long(blockIdx.x) * 4 + wave;
   if (at >= long(a.groups) * rows) return;
-  const int group = int(at / rows), r = int(at - long(group) * rows);
+  const int group = __builtin_amdgcn_readfirstlane(int(at / rows)), r = int(at - long(group) * rows);
   const int b = group / a.kv_heads, hk = group - b * a.kv_heads;
   const PagedRow row = paged_row(a, b);
   const int t = r >> a.group_log2, head = (hk << a.group_log2) + (r & (G - 1));
   float top = -INFINITY, den = 0.f, num[DPL] = {};
-  for (int s0 = 0; s0 < a.splits; s0 += kRound) {
+  for (int s0 = kShared ? wave * kRound : 0; s0 < a.splits; s0 += kRound * W) {
     const auto part = [&](int s) { return (long(group) * a.splits + min(s0 + s, a.splits - 1)) * rows + r; };
     const bool on = lane < kRound && s0 + lane < a.splits;
-    const float mine = on ? a.pmax[part(lane % kRound)] : -INFINITY, sum = a.psum[part(lane % kRound)];
+    const float high = a.pmax[part(lane % kRound)], sum = a.psum[part(lane % kRound)];
     float x[kRound][DPL];
 #pragma unroll
     for (int s = 0; s < kRound; ++s)
 #pragma unroll
       for (int i = 0; i < DPL; ++i) x[s][i] = a.pout[part(s) * D + min(lane + i * kWave, D - 1)];
+    const float mine = on ? high : -INFINITY;
     const float now = fmaxf(top, wave_max(mine));
     const float base = now == -INFINITY ? 0.f : now;
     const float keep = __builtin_amdgcn_exp2f(top - base);
@@ -429,6 +741,26 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedArgs a) {
     }
     top = now;
   }
+  if constexpr (kShared) {
+#pragma unroll
+    for (int i = 0; i < DPL; ++i)
+      if (lane + i * kWave < D) nums[wave][lane + i * kWave] = num[i];
+    if (lane == 0) tops[wave] = top, dens[wave] = den;
+    __syncthreads();
+    if (wave) return;
+    top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+    den = 0.f;
+#pragma unroll
+    for (int i = 0; i < DPL; ++i) num[i] = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const bool on = tops[w] != -INFINITY;
+      const float weight = on ? __builtin_amdgcn_exp2f(tops[w] - top) : 0.f;
+      den = on ? fmaf(weight, dens[w], den) : den;
+#pragma unroll
+      for (int i = 0; i < DPL; ++i) num[i] = on ? fmaf(weight, nums[w][min(lane + i * kWave, D - 1)], num[i]) : num[i];
+    }
+  }
   const bool empty = top == -INFINITY || t >= row.count;
   T* o = static_cast<T*>(a.out) + b * a.os[0] + head * a.os[1] + t * a.os[2];
 #pragma unroll
@@ -444,17 +776,34 @@ template <typename T, int D>
 int launch_paged(PagedArgs& a, hipStream_t stream) {
   const char* what = "page_attention";
   const int rows = a.tokens << a.group_log2;
-  const int block = rows <= 16 ? 16 : 32;
+  constexpr bool kShares = pieces_of<T>() < 3 && D >= 64;
+  const int block = rows <= 16 ? 16 : rows <= 32 || !kShares ? 32 : rows <= 64 ? 64 : 128;
   a.row_blocks = (rows + block - 1) / block;
   const long units = (long(a.groups) * a.splits + kXcds - 1) / kXcds * kXcds;
   const long merged = long(a.groups) * rows;
-  if (units * a.row_blocks >= kMostGroups || merged / 4 >= kMostGroups - 1)
+  if (units * a.row_blocks >= kMostGroups || merged >= kMostGroups - 1)
     return set_error(SFL_ERR_UNSUPPORTED, "%s: too many workgroups", what);
-  const auto kernel = rows <= 16 ? paged_attention_kernel<T, D, 1> : paged_attention_kernel<T, D, 2>;
-  hipLaunchKernelGGL(kernel, dim3(unsigned(units * a.row_blocks)), dim3(kPagedWaves * kWave), 0, stream, a);
+  const auto launch = [&](auto kernel, int waves) {
+    hipLaunchKernelGGL(kernel, dim3(unsigned(units * a.row_blocks)), dim3(unsigned(waves * kWave)), 0, stream, a);
+  };
+  const auto run = [&](auto page) {
+    constexpr int kPage = decltype(page)::value;
+    if constexpr (kShares) {
+      if (rows > 64) return launch(paged_rows_kernel<T, D, kPage, 4>, 4);
+      if (rows > 32) return launch(paged_rows_kernel<T, D, kPage, 2>, 2);
+    }
+    if (rows > 16) return launch(paged_attention_kernel<T, D, 2, kPage, 4>, 4);
+    launch(paged_attention_kernel<T, D, 1, kPage, 8>, 8);
+  };
+  if (a.page_log2 == 7) run(std::integral_constant<int, 128>{});
+  else if (a.page_log2 == 6) run(std::integral_constant<int, 64>{});
+  else run(std::integral_constant<int, 16>{});  // pages of less than a tile
   if (int rc = check_launch(what)) return rc;
   if (a.splits == 1) return SFL_OK;
-  hipLaunchKernelGGL((paged_merge_kernel<T, D>), dim3(unsigned((merged + 3) / 4)), dim3(256), 0, stream, a);
+  if (a.splits > 8)
+    hipLaunchKernelGGL((paged_merge_kernel<T, D, true>), dim3(unsigned(merged)), dim3(256), 0, stream, a);
+  else
+    hipLaunchKernelGGL((paged_merge_kernel<T, D, false>), dim3(unsigned((merged + 3) / 4)), dim3(256), 0, stream, a);
   return check_launch(what);
 }
 
