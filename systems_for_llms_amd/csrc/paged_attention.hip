@@ -776,8 +776,15 @@ template <typename T, int D>
 int launch_paged(PagedArgs& a, hipStream_t stream) {
   const char* what = "page_attention";
   const int rows = a.tokens << a.group_log2;
-  constexpr bool kShares = pieces_of<T>() < 3 && D >= 64;
-  const int block = rows <= 16 ? 16 : rows <= 32 || !kShares ? 32 : rows <= 64 ? 64 : 128;
+  // By rows, us at the best number of splits with blocks of 16 / 32 rows / 128 that share
+  // tiles: bf16 D 128 2 x 8000 keys of 8 heads 32 rows 15.2 / 16.3 / 20.4, 8 x 4000 of 16
+  // heads 40 rows 52.9 / 36.9 / 46.4, 8 x 8000 of 8 heads 64 rows 53.8 / 41.4 / 45.7, 4 x
+  // 8000 128 rows - / 40.5 / 37.8, 16 x 4000 128 rows - / 69 / 62, 32000 keys 512 rows - /
+  // 121 / 89; fp16, whose pieces leave blocks of 32 rows too few registers, 8 x up to 8000 40
+  // rows 37.3 / 43.6 / 59, D 64 8 x 8000 128 rows - / 49.9 / 48; fp32 4 x 4000 128 rows 32.3 /
+  // 39.4, D 64 8 x 4000 128 rows 34.1 / 37.2; D 32 8 x 4000 128 rows 17.7 / 21.1.
+  constexpr bool kPairs = pieces_of<T>() == 1 && D >= 64, kShares = pieces_of<T>() < 3 && D >= 64;
+  const int block = rows > 64 && kShares ? 128 : rows > 32 && kPairs ? 32 : 16;
   a.row_blocks = (rows + block - 1) / block;
   const long units = (long(a.groups) * a.splits + kXcds - 1) / kXcds * kXcds;
   const long merged = long(a.groups) * rows;
@@ -788,11 +795,10 @@ int launch_paged(PagedArgs& a, hipStream_t stream) {
   };
   const auto run = [&](auto page) {
     constexpr int kPage = decltype(page)::value;
-    if constexpr (kShares) {
-      if (rows > 64) return launch(paged_rows_kernel<T, D, kPage, 4>, 4);
-      if (rows > 32) return launch(paged_rows_kernel<T, D, kPage, 2>, 2);
-    }
-    if (rows > 16) return launch(paged_attention_kernel<T, D, 2, kPage, 4>, 4);
+    if constexpr (kShares)
+      if (block == 128) return launch(paged_rows_kernel<T, D, kPage, 4>, 4);
+    if constexpr (kPairs)
+      if (block == 32) return launch(paged_attention_kernel<T, D, 2, kPage, 4>, 4);
     launch(paged_attention_kernel<T, D, 1, kPage, 8>, 8);
   };
   if (a.page_log2 == 7) run(std::integral_constant<int, 128>{});

@@ -202,11 +202,26 @@ def append(cache, k, v, *, layer=0, counts=None) -> None:
                  layer, checked=True)
 
 
-def auto_splits(batch: int, kv_heads: int, capacity: int, rows: int) -> int:
+def auto_splits(batch: int, kv_heads: int, capacity: int, rows: int, dim: int, dtype: torch.dtype,
+                window_left: int | None = None) -> int:
     """Workgroups that share a KV head's slots, for ``rows`` query rows over each (new tokens times
-    query heads of the KV head)."""
-    blocks = batch * kv_heads * math.ceil(rows / 32)
-    return max(1, min(32, round(512 / blocks), math.ceil(capacity / 256)))
+    query heads of the KV head).
+
+    A workgroup takes 16 rows, or in bf16 32 of up to 64, or 128 of more than 64 (16-bit heads of
+    64 and 128). About as many as run at once, 256; 512 of the last kind, and where sequences
+    may differ in length, so that long ones have more of them. At least 1024 slots each, at
+    most 64 splits. Measured, us at 1 / 2 / 4 / 8 splits, bf16, 8 KV heads of 128: 32 rows of 8000 slots
+    84 / 89 / 92 / -, of 1K to 8K 64 / 56 / 60 / 68; 16 of 4000 29 / 27 / 28 / 31, of 2K to 16K 99 / 64 /
+    52 / 56; 8 of 4000 28 / 21 / 17 / 19; 8 of 1000 11.6 / 13.9 / 14.2 / -; 16 heads of 64 with a window
+    of 4095 24 / 29 / 33 / 45; 1 of 131072 at 16 / 32 / 64 splits 76 / 52 / 55; 27 tokens of 4 heads
+    over 8 of 1K to 8K 185 / 102 / 59 / 44.
+    """
+    tiled = dtype != torch.float32 and dim >= 64
+    block = 128 if tiled and rows > 64 else 32 if tiled and dtype == torch.bfloat16 and rows > 32 else 16
+    blocks = batch * kv_heads * math.ceil(rows / block)
+    target = 512 if block == 128 or rows <= 16 and batch > 1 and window_left is None else 256
+    reach = capacity if window_left is None else min(capacity, window_left + 1)
+    return max(1, min(64, round(target / blocks), round(reach / 1024)))
 
 
 @dataclass
@@ -275,7 +290,7 @@ def prepare(q, cache, *, layer=0, counts=None, window_left=None, splits=None, sc
     _cache.check_device(index)
     _lib.lib()  # fail here, before allocation, if the library is not built
     if splits is None:
-        splits = auto_splits(batch, kv_heads, cache.capacity, tokens * (heads // kv_heads))
+        splits = auto_splits(batch, kv_heads, cache.capacity, tokens * (heads // kv_heads), dim, q.dtype, window_left)
     window = -1 if window_left is None else min(window_left, cache.capacity)
     maximum = torch.empty((batch, heads, tokens, splits if splits > 1 else 0), device=q.device, dtype=torch.float32)
     numerator = torch.empty((*maximum.shape, dim), device=q.device, dtype=torch.float32)
