@@ -260,19 +260,48 @@ __device__ __forceinline__ int32_t load_now(const int32_t* p) {
   return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
+// The lowest free pages from page `from` on, up to `most` of them into `found`; returns how
+// many there are. Every thread of the workgroup calls it.
+__device__ __forceinline__ int find_free(const BookArgs& a, int from, int most, int* found, int* sums) {
+  constexpr int kScan = 8;  // pages looked at by a thread at a time
+  int have = 0;
+  for (int base = from & ~(kBookThreads * kScan - 1); have < most && base < a.pages; base += kBookThreads * kScan) {
+    const int page = base + int(threadIdx.x) * kScan;
+    int refs[kScan];
+#pragma unroll
+    for (int e = 0; e < kScan; ++e) refs[e] = a.refs[min(page + e, a.pages - 1)];
+    unsigned free = 0;
+#pragma unroll
+    for (int e = 0; e < kScan; ++e) free |= unsigned(refs[e] == 0 && page + e >= from && page + e < a.pages) << e;
+    int frees;
+    int k = have + scan(__builtin_popcount(free), sums, frees);
+#pragma unroll
+    for (int e = 0; e < kScan; ++e)
+      if (free >> e & 1) {
+        if (k < most) found[k] = page + e;
+        ++k;
+      }
+    have = min(have + frees, most);
+  }
+  __syncthreads();
+  return have;
+}
+
 // One workgroup serves the rows one after another, place by place: a place that its row
 // will write and that has no page, or one that others hold too, gets the lowest free page.
 // 1024 places at a time are looked at together. What the rows before it in the same round
-// do to a place's page is found from the tables: of r holders, the first r - 1 that write
-// it leave it, and the last then has it alone.
+// do to a place's page is found from the pages they hold: of r holders, the first r - 1 that
+// write it leave it, and the last then has it alone. (Those of earlier rounds have left, or
+// there are no free pages any more.) Bound by its chain of loads and barriers: 64 rows, 16 of
+// them with 6 new places and 16 that share a page, of 1600 pages RESERVE us.
 __global__ __launch_bounds__(kBookThreads) void reserve_kernel(const BookArgs a, const int32_t* counts, int32_t* granted,
                                                                int2* copies, int* copied) {
-  constexpr int kScan = 8;  // pages looked at by a thread at a time
   __shared__ int sums[kBookThreads / kWave];
   __shared__ int lens[kMostRows], ends[kMostRows], starts[kMostRows + 1], failed[kMostRows];
   __shared__ int rank_of[kBookThreads], found[kBookThreads];
+  __shared__ __align__(16) int shared_page[kBookThreads];  // of places whose page others hold too, else -1
   __shared__ int made, position;
-  const int tid = threadIdx.x, page = 1 << a.page_log2, cap = a.places << a.page_log2;
+  const int tid = threadIdx.x, cap = a.places << a.page_log2;
   int wanted = 0;  // places of this thread's row
   if (tid < a.batch) {
     const int len = min(max(a.lengths[tid], 0), cap), end = len + min(max(counts[tid], 0), cap - len);
@@ -287,8 +316,7 @@ __global__ __launch_bounds__(kBookThreads) void reserve_kernel(const BookArgs a,
   __syncthreads();
   for (int base = 0; base < items; base += kBookThreads) {
     const int item = base + tid;
-    int b = 0, place = 0, held = -1, last = -1;
-    bool lacks = false, stays = false;
+    int b = 0, place = 0, held = -1, holders = 0;
     if (item < items) {
       int hi = a.batch - 1;  // the last row whose places start at or before the item
       while (b < hi) {
@@ -298,46 +326,28 @@ __global__ __launch_bounds__(kBookThreads) void reserve_kernel(const BookArgs a,
       place = (lens[b] >> a.page_log2) + item - starts[b];
       held = load_now(&a.tables[long(b) * a.places + place]);
       if (!is_page(a, held)) held = -1;
-      lacks = held < 0;
-      if (held >= 0) {
-        const int holders = load_now(&a.refs[held]);
-        if (holders > 1) {
-          int before = 0;
-          for (int r = 0; r < b; ++r)
-            if (starts[r] < starts[r + 1] && place >= lens[r] >> a.page_log2 && place <= (ends[r] - 1) >> a.page_log2 &&
-                load_now(&a.tables[long(r) * a.places + place]) == held)
-              ++before, last = r;
-          lacks = before < holders - 1;
-          stays = !lacks;
-        }
+      if (held >= 0) holders = load_now(&a.refs[held]);
+    }
+    shared_page[tid] = holders > 1 ? held : -1;
+    __syncthreads();
+    bool lacks = item < items && held < 0, stays = false;
+    int last = -1;  // the place before it with the same page
+    if (holders > 1) {
+      int before = 0;
+      for (int j = 0; j < tid; j += 4) {
+        const int4 x = *reinterpret_cast<const int4*>(shared_page + j);
+        const int pages[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (pages[e] == held && j + e < tid) ++before, last = j + e;
       }
+      lacks = before < holders - 1;
+      stays = !lacks;
     }
     int lacking;
     const int rank = scan(lacks, sums, lacking);
     rank_of[tid] = rank;
-    // The lowest free pages from `position` on, as many as are lacking.
-    int have = 0;
-    __syncthreads();
-    int from = position;
-    while (have < lacking && from < a.pages) {
-      const int page0 = (from & ~(kBookThreads * kScan - 1)) + tid * kScan;
-      unsigned free = 0;
-#pragma unroll
-      for (int e = 0; e < kScan; ++e)
-        if (page0 + e >= from && page0 + e < a.pages && a.refs[page0 + e] == 0) free |= 1u << e;
-      int frees;
-      int k = have + scan(__builtin_popcount(free), sums, frees);
-#pragma unroll
-      for (int e = 0; e < kScan; ++e)
-        if (free >> e & 1) {
-          if (k < lacking) found[k] = page0 + e;
-          ++k;
-        }
-      have = min(have + frees, lacking);
-      from = (from & ~(kBookThreads * kScan - 1)) + kBookThreads * kScan;
-    }
-    __syncthreads();
-    if (tid == 0 && have > 0) position = found[have - 1] + 1;
+    const int have = find_free(a, position, lacking, found, sums);
     const bool got = lacks && rank < have;
     if (got) {
       const int now = found[rank];
@@ -349,12 +359,9 @@ __global__ __launch_bounds__(kBookThreads) void reserve_kernel(const BookArgs a,
       }
     }
     // A row has a shared page alone only once the one before it has left.
-    bool bad = lacks && !got;
-    if (stays && last >= 0) {
-      const int other = starts[last] + place - (lens[last] >> a.page_log2) - base;
-      bad = other < 0 || rank_of[other] >= have;
-    }
-    if (bad) atomicMin(&failed[b], place);
+    if ((lacks && !got) || (stays && last >= 0 && rank_of[last] >= have)) atomicMin(&failed[b], place);
+    __syncthreads();
+    if (tid == 0 && have > 0) position = found[have - 1] + 1;
     settle();
   }
   if (tid < a.batch) {
