@@ -55,30 +55,38 @@ __global__ __launch_bounds__(1024) void append_kernel(const AppendArgs a) {
   u >>= 1;
   const unsigned row = u / unsigned(a.kv_heads), h = u - row * unsigned(a.kv_heads);
   const unsigned b = row / unsigned(a.reach), s = row - b * unsigned(a.reach);
+  // What is the same for the workgroup comes by scalar loads, whose chain (length, page,
+  // holders) then runs beside the tokens' own.
+  typedef const __attribute__((address_space(4))) int32_t* Constant;
+  typedef const __attribute__((address_space(4))) float* ConstantF;
   const int cap = a.places << a.page_log2;
-  const int len = min(max(a.lengths[b], 0), cap);
-  const int count = min(a.counts ? min(max(a.counts[b], 0), a.tokens) : a.tokens, cap - len);
+  const int len = min(max(Constant(a.lengths)[b], 0), cap);
+  const int count = min(a.counts ? min(max(Constant(a.counts)[b], 0), a.tokens) : a.tokens, cap - len);
   const int place = (len >> a.page_log2) + int(s);
   const int first = place << a.page_log2;  // the page's first slot
   const int lo = max(len - first, 0), hi = min(len + count - first, page);
   if (lo >= hi) return;
-  const int at = a.tables[long(b) * a.places + place];
-  if (at < 0 || at >= a.pages || a.refs[at] != 1) return;
-  const long block = long(at) * a.kv_heads + h;
-  uint8_t* codes = (values ? a.v_codes : a.k_codes) + (block << a.page_log2) * D;
-  float* scale = (values ? a.v_scale : a.k_scale) + block;
-  const int held = int(__float_as_uint(*scale) >> 23) - 127;  // read before anyone writes it, below
+  const int at = Constant(a.tables)[long(b) * a.places + place];
 
   const int i = int(threadIdx.x) / PIECES, j = int(threadIdx.x) % PIECES;  // tokens 4 i .. 4 i + 3, piece j
   const long step = values ? a.st[1][2] : a.st[0][2];
   const T* x = static_cast<const T*>(values ? a.v : a.k) + b * (values ? a.st[1][0] : a.st[0][0]) +
                h * (values ? a.st[1][1] : a.st[0][1]) + VEC * j;
-  float v[4][VEC] = {};
-  float amax = 0.f;
-  if (4 * i + 3 >= lo && 4 * i < hi) {
-    uint4 raw[4];
+  const bool some = 4 * i + 3 >= lo && 4 * i < hi;
+  uint4 raw[4] = {};
+  if (some) {
 #pragma unroll
     for (int c = 0; c < 4; ++c) raw[c] = load16(x + long(first + min(max(4 * i + c, lo), hi - 1) - len) * step);
+  }
+  if (at < 0 || at >= a.pages || Constant(a.refs)[at] != 1) return;
+  const long block = long(at) * a.kv_heads + h;
+  uint8_t* codes = (values ? a.v_codes : a.k_codes) + (block << a.page_log2) * D;
+  float* scale = (values ? a.v_scale : a.k_scale) + block;
+  const int held = int(__float_as_uint(ConstantF(scale)[0]) >> 23) - 127;
+
+  float v[4][VEC] = {};
+  float amax = 0.f;
+  if (some) {
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
       unpack16<T>(raw[c], v[c]);
