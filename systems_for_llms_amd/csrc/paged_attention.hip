@@ -104,6 +104,10 @@ __device__ __forceinline__ u32x4 from_codes(uint32_t lo, uint32_t hi, float scal
                __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true))};
 }
 
+// A scale as it is, or 1 for what a page that was never written may hold: the codes beside
+// tokens in sight are zeros then, and zeros have to stay.
+__device__ __forceinline__ float usable(float scale) { return fabsf(scale) < INFINITY ? scale : 1.f; }
+
 // 0xff in each byte of w that is the code of NaN.
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
   const uint32_t t = (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
@@ -264,7 +268,7 @@ __global__ __launch_bounds__(W * kWave, D == 128 && NC == 2 ? 1 : 2) void paged_
     const int page = table[min(slot >> a.page_log2, a.places - 1)];
     spots = slot < row.cap && page >= 0 && page < a.pages ? page : -1;
     const long block = long(max(spots, 0)) * a.kv_heads + hk;
-    spots_ks = a.k_scale[block], spots_vs = a.v_scale[block];
+    spots_ks = usable(a.k_scale[block]), spots_vs = usable(a.v_scale[block]);
   };
   const auto pick = [&](auto x, int i, int sub) {  // of tile i's keys from 16 sub on
     const uint32_t bits = __builtin_bit_cast(uint32_t, x);
@@ -507,7 +511,7 @@ __global__ __launch_bounds__(W * kWave, 2) void paged_rows_kernel(const PagedArg
     const int page = table[min(slot >> a.page_log2, a.places - 1)];
     spots = slot < row.cap && page >= 0 && page < a.pages ? page : -1;
     const long block = long(max(spots, 0)) * a.kv_heads + hk;
-    spots_ks = a.k_scale[block], spots_vs = a.v_scale[block];
+    spots_ks = usable(a.k_scale[block]), spots_vs = usable(a.v_scale[block]);
   };
   const auto pick = [&](auto x, int i, int sub) {
     const uint32_t bits = __builtin_bit_cast(uint32_t, x);

@@ -174,7 +174,7 @@ int launch_append(const AppendArgs& a, int batch, hipStream_t stream) {
   const long blocks = 2L * batch * a.reach * a.kv_heads;
   const int page = 1 << a.page_log2;
   const int threads = std::max(kWave, page / 4 * (D / vec_elems<T>()));  // at most 1024
-  if (blocks >= (1L << 22)) return set_error(SFL_ERR_UNSUPPORTED, "page_append: too many workgroups");
+  if (blocks * threads >= (1L << 32)) return set_error(SFL_ERR_UNSUPPORTED, "page_append: too many workgroups");
   hipLaunchKernelGGL((append_kernel<T, D>), dim3(unsigned(blocks)), dim3(unsigned(threads)), unsigned(D * (page + 4)), stream, a);
   return check_launch("page_append");
 }
@@ -301,7 +301,7 @@ __device__ __forceinline__ int find_free(const BookArgs& a, int from, int most, 
 // do to a place's page is found from the pages they hold: of r holders, the first r - 1 that
 // write it leave it, and the last then has it alone. (Those of earlier rounds have left, or
 // there are no free pages any more.) Bound by its chain of loads and barriers: 64 rows, 16 of
-// them with 6 new places and 16 that share a page, of 1600 pages RESERVE us.
+// them with 6 new places and 16 that share a page, of 1600 pages 9.7 us.
 __global__ __launch_bounds__(kBookThreads) void reserve_kernel(const BookArgs a, const int32_t* counts, int32_t* granted,
                                                                int2* copies, int* copied) {
   __shared__ int sums[kBookThreads / kWave];
@@ -312,7 +312,10 @@ __global__ __launch_bounds__(kBookThreads) void reserve_kernel(const BookArgs a,
   const int tid = threadIdx.x, cap = a.places << a.page_log2;
   int wanted = 0;  // places of this thread's row
   if (tid < a.batch) {
-    const int len = min(max(a.lengths[tid], 0), cap), end = len + min(max(counts[tid], 0), cap - len);
+    const int len = min(max(a.lengths[tid], 0), cap);
+    // No row gets more places than there are pages: one more shows what fails.
+    const long most = ((long(len) >> a.page_log2) + a.pages + 1) << a.page_log2;
+    const int end = int(min(long(len) + min(max(counts[tid], 0), cap - len), most));
     lens[tid] = len, ends[tid] = end, failed[tid] = a.places;
     wanted = end > len ? ((end - 1) >> a.page_log2) - (len >> a.page_log2) + 1 : 0;
   }
@@ -369,7 +372,7 @@ __global__ __launch_bounds__(kBookThreads) void reserve_kernel(const BookArgs a,
     // A row has a shared page alone only once the one before it has left.
     if ((lacks && !got) || (stays && last >= 0 && rank_of[last] >= have)) atomicMin(&failed[b], place);
     __syncthreads();
-    if (tid == 0 && have > 0) position = found[have - 1] + 1;
+    if (tid == 0) position = have < lacking ? a.pages : have > 0 ? found[have - 1] + 1 : position;
     settle();
   }
   if (tid < a.batch) {
@@ -562,6 +565,7 @@ extern "C" int sfl_page_reserve(void* k, void* v, float* k_scale, float* v_scale
   if (int rc = fill_copy(c, what, k, v, k_scale, v_scale, layers, pages, kv_heads, page_size, head_dim)) return rc;
   if (!lengths || !counts || !granted || !scratch) return set_error(SFL_ERR_INVALID, "%s: null pointer argument", what);
   const hipStream_t on = static_cast<hipStream_t>(stream);
+  if (long(batch) * std::min(places, pages + 1) >= (1L << 31)) return set_error(SFL_ERR_UNSUPPORTED, "%s: too many places", what);
   int2* copies = reinterpret_cast<int2*>(scratch + 2);
   hipLaunchKernelGGL(reserve_kernel, dim3(1), dim3(kBookThreads), 0, on, a, counts, granted, copies, scratch);
   if (int rc = check_launch(what)) return rc;

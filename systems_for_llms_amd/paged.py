@@ -37,7 +37,7 @@ MAX_TOKENS = _cache.MAX_DRAFTS
 MAX_SPLITS = 128
 
 
-@dataclass(frozen=True)
+@dataclass(frozen=True, eq=False)
 class PagedCache:
     """The tensors of a paged cache, contiguous on one device; a program may allocate them itself.
 
@@ -81,6 +81,9 @@ class PagedCache:
             _cache.check_vector("paged cache", name, getattr(self, name), dtype, shape, index)
         if k.data_ptr() % 16 or self.v.data_ptr() % 16:
             raise ValueError("k and v must be 16-byte aligned")
+        held = (k, self.v, self.k_scale, self.v_scale, tables, self.lengths, self.refs)
+        if len({t.data_ptr() for t in held}) < len(held) and index >= 0:
+            raise ValueError("the tensors of a cache must not share memory")
 
     @property
     def layers(self) -> int:
@@ -134,6 +137,8 @@ def fork(cache, parents) -> None:
     """
     index = _check_cache("fork", cache)
     _cache.check_vector("fork", "parents", parents, torch.int32, cache.lengths.shape, index)
+    if parents.data_ptr() == cache.lengths.data_ptr():
+        raise ValueError("parents must not be the cache's lengths")
     _cache.check_device(index)
     written = (cache.tables, cache.lengths, cache.refs)
     ops.dispatch(torch.ops.sfl.page_fork, (parents, *written), written, cache.k.shape[3], checked=True)

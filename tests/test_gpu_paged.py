@@ -281,7 +281,7 @@ def test_attention_keeps_the_tail_behind_a_heavy_key():
 
 @pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
 @pytest.mark.parametrize("dim", [16, 32, 64, 128])
-@pytest.mark.parametrize("tokens, page", [(1, 16), (6, 64), (20, 32)])
+@pytest.mark.parametrize("tokens, page", [(1, 16), (6, 64), (10, 128), (20, 32)])
 def test_attention_ignores_what_it_does_not_see(dtype, dim, tokens, page):
     """NaN codes behind the row, in pages of nobody, before the window, and in slots that only some tokens see."""
     g = torch.Generator().manual_seed(dim + tokens)
@@ -718,3 +718,65 @@ def test_results_repeat_bit_for_bit():
     first, lse = op().clone(), op.lse.clone()
     for _ in range(2):
         assert torch.equal(op(), first) and torch.equal(op.lse, lse)
+
+
+def test_attention_beside_pages_that_were_never_written():
+    """Scales and codes of missing, free and reserved pages may be anything, NaN and infinity too."""
+    g = torch.Generator().manual_seed(71)
+    for page in (16, 64):
+        state = random_cache(g, [2 * page + 3, 5 * page, 70], 2, 64, page, room=3 * page)
+        state["tables"][0, 1] = -1
+        state["tables"][1, 4] = -1
+        used = torch.zeros(state["refs"].numel(), dtype=torch.bool)
+        for b, n in enumerate(state["lengths"].tolist()):
+            held = state["tables"][b, : -(-(n + 2) // page)]
+            used[held[held >= 0].long()] = True
+        junk = torch.full((page, 64), NAN_CODE, dtype=torch.uint8).view(op_.F8)
+        for i in range(used.numel()):
+            if not used[i]:
+                state["k"][0, i], state["v"][0, i] = junk, junk.view(torch.uint8).T.contiguous().view(op_.F8)
+                state["k_scale"][0, i], state["v_scale"][0, i] = (float("nan"), float("inf"), -float("inf"))[i % 3], float("nan")
+        for dtype, tokens, group in ((BF16, 2, 1), (FP16, 2, 4), (FP32, 2, 2), (BF16, 2, 8)):
+            for splits in (1, 3):
+                check(randn(g, 3, 2 * group, tokens, 64, dtype=dtype), state, splits=splits)
+        counts = torch.tensor([2, 1, 2], dtype=torch.int32)
+        check(randn(g, 3, 16, 20, 64, dtype=BF16), state, counts=counts)  # rows of many tokens, two in use
+
+
+def test_reserve_asked_for_more_than_there_is():
+    """Tables of a million places, counts up to the largest: the pool is what ends it."""
+    from systems_for_llms_amd import paged
+
+    cache = paged.create(3, 16 << 20, 1, 16, 50, page_size=16)
+    state = {n: getattr(cache, n).cpu() for n in NAMES}
+    counts = torch.tensor([100, 2 ** 31 - 1, 5], dtype=torch.int32)
+    granted = paged.reserve(cache, counts.cuda())
+    assert granted.tolist() == [100, 43 * 16, 0]
+    assert cache.tables[:2, :50].cpu().tolist() == [list(range(7)) + [-1] * 43, list(range(7, 50)) + [-1] * 7]
+    assert int((cache.tables >= 0).sum()) == 50 and cache.refs.tolist() == [1] * 50
+    assert paged.reserve(cache, counts.cuda()).tolist() == [100, 43 * 16, 0]
+    assert torch.equal(state["lengths"], cache.lengths.cpu())
+
+
+def test_append_and_attention_of_many_pages_and_rows():
+    """Batches beyond a wave of sequences, prompts over hundreds of pages."""
+    from systems_for_llms_amd import paged
+
+    g = torch.Generator().manual_seed(72)
+    state = random_cache(g, [int(x) for x in torch.randint(0, 90, (100,), generator=g)], 1, 32, 16, room=2)
+    cache = on_gpu(state)
+    k, v, q = (randn(g, 100, h, 2, 32, dtype=FP16) for h in (1, 1, 4))
+    paged.append(cache, k.cuda(), v.cuda())
+    state = op_.append(state, k, v)
+    same_cache(cache, state)
+    for splits in (1, 3):
+        check(q, state, cache=cache, splits=splits)
+    state = random_cache(g, [5, 0], 1, 16, 16, room=9000)
+    cache = on_gpu(state)
+    k, v, q = (randn(g, 2, h, 9000, 16, dtype=BF16) for h in (1, 1, 1))
+    paged.append(cache, k.cuda(), v.cuda())
+    state = op_.append(state, k, v)
+    same_cache(cache, state)
+    state["lengths"] += 8990
+    cache.lengths.add_(8990)
+    check(q[:, :, :5], state, cache=cache)
