@@ -463,12 +463,12 @@ __global__ __launch_bounds__(W * kWave, D == 128 && NC == 2 ? 1 : 2) void paged_
 }
 
 // The same for more rows: W waves with 32 query rows each, and tiles of 64 keys that they
-// share. The codes of a tile are read once, become bf16 on the way into LDS (K [key][dim],
-// V [dim][key], 16-byte slots swizzled by row), and are operands of 32 x 32 x 16 MFMAs from
-// there, the next tile's codes under way meanwhile. Row m of S^T takes the key
-// 16 (m / 16) + 8 (m / 4 % 2) + 4 (m / 8 % 2) + m % 4 of its 32, so that lane (h, n), lane =
-// 32 h + n, holds the scores of keys 16 x + 8 h .. + 7 of query row n: its k-slots in the
-// product with V.
+// share. A tile's codes are read once into LDS as they are (K [key][dim], V [dim][key],
+// 16-byte slots swizzled by row) and become bf16 operands of 32 x 32 x 16 MFMAs on their way
+// out of it, the next tile's codes under way meanwhile. A lane's 16 codes are its k-slots in
+// two products: in those with K dims 32 x + 16 h .. + 15 of a key, in those with V keys
+// 32 x + 16 h .. + 15 of a dim (lane = 32 h + n). So that lane (h, n) holds the scores of the
+// latter, row m of S^T takes the key 16 (m / 4 % 2) + 8 (m / 16) + 4 (m / 8 % 2) + m % 4 of its 32.
 template <typename T, int D, int kPage, int W>
 __global__ __launch_bounds__(W * kWave, 2) void paged_rows_kernel(const PagedArgs a) {
   constexpr bool kWide = kPage >= kPagedTile;
@@ -476,7 +476,7 @@ __global__ __launch_bounds__(W * kWave, 2) void paged_rows_kernel(const PagedArg
   constexpr int kSteps = D / 16, kTiles = D / 32;          // of the products with K, of dims of V
   constexpr int kPieces = BT * D / 16 / kThreads;          // of 16 codes of a tile's keys a thread stages
   constexpr int kSpots = kWide ? 1 : 4, kBatch = kWave / kSpots;
-  __shared__ u32x4 keys[BT * D / 8], values[D * BT / 8];
+  __shared__ u32x4 keys[BT * D / 16], values[D * BT / 16];
   __shared__ int found;
   const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave);
   const int lane = threadIdx.x % kWave, h = lane / 32, n = lane % 32;
@@ -491,9 +491,9 @@ __global__ __launch_bounds__(W * kWave, 2) void paged_rows_kernel(const PagedArg
   const int seen_to = t < row.count ? row.len + t : -1, seen_from = a.window >= 0 ? row.len + t - a.window : 0;
   u32x4 q[kSteps][P];
   {
-    const T* at = static_cast<const T*>(a.q) + b * a.qs[0] + head * a.qs[1] + t * a.qs[2] + 8 * h;
+    const T* at = static_cast<const T*>(a.q) + b * a.qs[0] + head * a.qs[1] + t * a.qs[2] + 16 * h;
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) load_pieces<T>(at + 16 * s, true, q[s]);
+    for (int s = 0; s < kSteps; ++s) load_pieces<T>(at + s / 2 * 32 + s % 2 * 8, true, q[s]);
   }
   f32x16 o[kTiles];
 #pragma unroll
@@ -520,7 +520,6 @@ __global__ __launch_bounds__(W * kWave, 2) void paged_rows_kernel(const PagedArg
   };
   // A thread's pieces: 16 dims of a key, 16 keys of a dim.
   u32x4 kw[kPieces], vw[kPieces];
-  float ks[kPieces], vs[kPieces];
   bool kept[kPieces];
   const auto fetch = [&](int i) {
     const int slot0 = (begin + i) * BT;
@@ -528,7 +527,6 @@ __global__ __launch_bounds__(W * kWave, 2) void paged_rows_kernel(const PagedArg
     for (int e = 0; e < kPieces; ++e) {
       const int x = int(threadIdx.x) + kThreads * e, key = x / (D / 16), dim = x / 4;
       const int page_k = pick(spots, i, key / 16), page_v = pick(spots, i, x % 4);
-      ks[e] = pick(spots_ks, i, key / 16), vs[e] = pick(spots_vs, i, x % 4);
       kept[e] = page_v >= 0;
       const long block_k = long(max(page_k, 0)) * a.kv_heads + hk, block_v = long(max(page_v, 0)) * a.kv_heads + hk;
       kw[e] = *reinterpret_cast<const u32x4*>(a.k + ((block_k << a.page_log2) + ((slot0 + key) & page_mask)) * D + x % (D / 16) * 16);
@@ -540,7 +538,9 @@ __global__ __launch_bounds__(W * kWave, 2) void paged_rows_kernel(const PagedArg
   };
   // Whether all of tile i's keys have a page.
   const auto whole_tile = [&](int i) { return kWide ? pick(spots, i, 0) >= 0 : !__any(pick(spots, i, lane % 4) < 0); };
-  const int key_row = 16 * (n / 16) + 8 * (n / 4 % 2) + 4 * (n / 8 % 2) + n % 4;
+  const int key_row = 16 * (n / 4 % 2) + 8 * (n / 16) + 4 * (n / 8 % 2) + n % 4;
+  const auto key_slot = [](int key, int x) { return key * (D / 16) + (x ^ (D == 128 ? key / 2 % 8 : key / 4 % 4)); };
+  const auto value_slot = [](int dim, int x) { return dim * 4 + (x ^ dim / 4 % 4); };
 
   if (threadIdx.x == 0) found = 0;
   if (count > 0) {
@@ -570,13 +570,14 @@ __global__ __launch_bounds__(W * kWave, 2) void paged_rows_kernel(const PagedArg
     __syncthreads();  // the last tile's operands are read
 #pragma unroll
     for (int e = 0; e < kPieces; ++e) {
-      const int x = int(threadIdx.x) + kThreads * e, key = x / (D / 16), dim = x / 4;
-#pragma unroll
-      for (int y = 0; y < 2; ++y) {
-        keys[key * (D / 8) + ((x % (D / 16) * 2 + y) ^ k_swizzle<D>(key))] = from_codes(kw[e][2 * y], kw[e][2 * y + 1], ks[e]);
-        values[dim * (BT / 8) + ((x % 4 * 2 + y) ^ k_swizzle<64>(dim))] = from_codes(vw[e][2 * y], vw[e][2 * y + 1], vs[e]);
-      }
+      const int x = int(threadIdx.x) + kThreads * e;
+      keys[key_slot(x / (D / 16), x % (D / 16))] = kw[e];
+      values[value_slot(x / 4, x % 4)] = vw[e];
     }
+    float ks[2], vs[2];  // of the lane's keys in the two halves of the tile
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+      ks[half] = pick(spots_ks, i, 2 * half + key_row / 16), vs[half] = pick(spots_vs, i, 2 * half + h);
     __syncthreads();
     if (i + 1 < count) {
       if ((i + 1) % kBatch == 0) look_up(i + 1);
@@ -591,10 +592,14 @@ __global__ __launch_bounds__(W * kWave, 2) void paged_rows_kernel(const PagedArg
       for (int e = 0; e < 16; ++e) s[half][e] = 0.f;
       const int key = 32 * half + key_row;
 #pragma unroll
-      for (int st = 0; st < kSteps; ++st) {
-        const u32x4 w = keys[key * (D / 8) + ((2 * st + h) ^ k_swizzle<D>(key))];
+      for (int st = 0; st < kSteps; st += 2) {
+        const u32x4 w = keys[key_slot(key, st + h)];
 #pragma unroll
-        for (int p = P - 1; p >= 0; --p) s[half] = mfma32<bf16_t>(w, q[st][p], s[half]);
+        for (int y = 0; y < 2; ++y) {
+          const u32x4 x = from_codes(w[2 * y], w[2 * y + 1], ks[half]);
+#pragma unroll
+          for (int p = P - 1; p >= 0; --p) s[half] = mfma32<bf16_t>(x, q[st + y][p], s[half]);
+        }
       }
     }
     if (masked) {
@@ -602,8 +607,8 @@ __global__ __launch_bounds__(W * kWave, 2) void paged_rows_kernel(const PagedArg
       for (int half = 0; half < 2; ++half)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const int at = 32 * half + 16 * (e / 8) + 8 * h + e % 8;
-          const bool on = slot0 + at <= seen_to && slot0 + at >= seen_from && !(missing >> (2 * half + e / 8) & 1);
+          const int at = 32 * half + 16 * h + e;
+          const bool on = slot0 + at <= seen_to && slot0 + at >= seen_from && !(missing >> (2 * half + h) & 1);
           s[half][e] = on ? s[half][e] : -INFINITY;
         }
     }
@@ -635,15 +640,17 @@ __global__ __launch_bounds__(W * kWave, 2) void paged_rows_kernel(const PagedArg
       split_pieces(y, prob[x]);
     }
 #pragma unroll
-    for (int d = 0; d < kTiles; ++d) {
-      const int dim = 32 * d + n;
+    for (int d = 0; d < kTiles; ++d)
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const u32x4 w = values[dim * (BT / 8) + ((2 * x + h) ^ k_swizzle<64>(dim))];
+      for (int x = 0; x < 2; ++x) {
+        const u32x4 w = values[value_slot(32 * d + n, 2 * x + h)];
 #pragma unroll
-        for (int p = P - 1; p >= 0; --p) o[d] = mfma32<bf16_t>(w, prob[x][p], o[d]);
+        for (int y = 0; y < 2; ++y) {
+          const u32x4 v = from_codes(w[2 * y], w[2 * y + 1], vs[x]);
+#pragma unroll
+          for (int p = P - 1; p >= 0; --p) o[d] = mfma32<bf16_t>(v, prob[2 * x + y][p], o[d]);
+        }
       }
-    }
   }
   __syncthreads();
   if (!active) return;
@@ -654,7 +661,7 @@ __global__ __launch_bounds__(W * kWave, 2) void paged_rows_kernel(const PagedArg
       if (!partly_seen(slot0, whole_tile(i))) continue;
 #pragma unroll 1
       for (int x = 0; x < 4; ++x) {
-        const int spot = pick(spots, i, x), slot = slot0 + 16 * x + 8 * h;
+        const int spot = pick(spots, i, x / 2 * 2 + h), slot = slot0 + x / 2 * 32 + 16 * h + x % 2 * 8;
         u32x4 on;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
