@@ -21,7 +21,7 @@ Inference only: ``requires_grad`` inputs are refused.
 from __future__ import annotations
 
 import math
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 
 import torch
 
@@ -56,6 +56,10 @@ class PagedCache:
     tables: torch.Tensor
     lengths: torch.Tensor
     refs: torch.Tensor
+    # What the calls ask for each time: the device's index, rows, KV heads, head dimension; their workspace.
+    _index: int = field(init=False, repr=False)
+    _shape: tuple = field(init=False, repr=False)
+    _scratch: torch.Tensor = field(init=False, repr=False)
 
     def __post_init__(self):
         k, tables = self.k, self.tables
@@ -84,6 +88,10 @@ class PagedCache:
         held = (k, self.v, self.k_scale, self.v_scale, tables, self.lengths, self.refs)
         if len({t.data_ptr() for t in held}) < len(held) and index >= 0:
             raise ValueError("the tensors of a cache must not share memory")
+        object.__setattr__(self, "_index", index)
+        object.__setattr__(self, "_shape", (tables.shape[0], heads, dim))
+        scratch = torch.empty(4 + 2 * max(pages, tables.shape[0]), dtype=torch.int32, device=k.device)
+        object.__setattr__(self, "_scratch", scratch)
 
     @property
     def layers(self) -> int:
@@ -120,7 +128,7 @@ def create(batch, capacity, kv_heads, head_dim, pages, *, layers=1, page_size=64
 def _check_cache(operator, cache):
     if not isinstance(cache, PagedCache):
         raise TypeError(f"{operator}: cache must be a PagedCache")
-    return cache.k.get_device()
+    return cache._index
 
 
 def _check_layer(cache, layer):
@@ -159,8 +167,7 @@ def reserve(cache, counts) -> torch.Tensor:
     _cache.check_device(index)
     _lib.lib()  # fail here, before allocating, if the library is not built
     granted = torch.empty_like(cache.lengths)
-    scratch = torch.empty(2 + 2 * granted.shape[0], dtype=torch.int32, device=granted.device)
-    written = (cache.k, cache.v, cache.k_scale, cache.v_scale, cache.tables, cache.refs, granted, scratch)
+    written = (cache.k, cache.v, cache.k_scale, cache.v_scale, cache.tables, cache.refs, granted, cache._scratch)
     ops.dispatch(torch.ops.sfl.page_reserve, (cache.lengths, counts, *written), written, checked=True)
     return granted
 
@@ -175,8 +182,7 @@ def compact(cache) -> torch.Tensor:
     _cache.check_device(index)
     _lib.lib()
     used = torch.empty(1, dtype=torch.int32, device=cache.k.device)
-    scratch = torch.empty(4 + 2 * cache.refs.shape[0], dtype=torch.int32, device=cache.k.device)
-    written = (cache.k, cache.v, cache.k_scale, cache.v_scale, cache.tables, cache.refs, used, scratch)
+    written = (cache.k, cache.v, cache.k_scale, cache.v_scale, cache.tables, cache.refs, used, cache._scratch)
     ops.dispatch(torch.ops.sfl.page_compact, written, written, checked=True)
     return used
 
@@ -196,8 +202,8 @@ def append(cache, k, v, *, layer=0, counts=None) -> None:
     if _cache.check_rows("append", ("k", "v"), (k, v)) != index:
         _cache.check_device(-1)
     _check_layer(cache, layer)
-    heads, _, dim = cache.k.shape[2:]
-    if v.shape != k.shape or k.shape[0] != cache.lengths.shape[0] or k.shape[1] != heads or k.shape[3] != dim:
+    shape = k.shape
+    if v.shape != shape or (shape[0], shape[1], shape[3]) != cache._shape:
         raise ValueError("k, v and the cache must agree in rows, heads and head dimension")
     if counts is not None:
         _cache.check_vector("append", "counts", counts, torch.int32, cache.lengths.shape, index)
@@ -281,8 +287,8 @@ def prepare(q, cache, *, layer=0, counts=None, window_left=None, splits=None, sc
         _cache.check_device(-1)
     _check_layer(cache, layer)
     batch, heads, tokens, dim = q.shape
-    kv_heads = cache.k.shape[2]
-    if batch != cache.lengths.shape[0] or dim != cache.k.shape[4]:
+    rows, kv_heads, width = cache._shape
+    if batch != rows or dim != width:
         raise ValueError("q and the cache must agree in rows and head dimension")
     _cache.check_heads(heads, kv_heads)
     if tokens > MAX_TOKENS:
