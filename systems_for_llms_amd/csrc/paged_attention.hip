@@ -27,6 +27,7 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kPagedTile = 64;  // keys of a wave's tile
 constexpr int kMaxTokens = 128;
+constexpr int kRowWaves = 4;    // of the kernel for many rows
 constexpr float kLn2 = 0.6931471805599453f;
 
 struct PagedArgs {
@@ -216,7 +217,14 @@ __device__ __forceinline__ u32x4 load_v(const uint8_t* at) {
 
 // A workgroup has up to 16 NC query rows (the G heads of a KV head times the tokens, row
 // r = t G + g) and a split of the keys; its waves take the split's tiles in turn and are
-// joined through LDS at the end.
+// joined through LDS at the end. Codes go from memory to registers, a tile's values under
+// way during its scores, the next tile's keys during its softmax. Bound by HBM: 32 rows of
+// 8000 tokens of 8 heads of 128 84 us (537 MB, 6.4 TB/s), of 1K to 8K 51 (310 MB, 6.0), one of
+// 131072 48 (268 MB, 5.6); a CU alone reads 35 GB/s, so a head wants about 30 workgroups.
+// Both ways measured, us at those two: values past the caches 58, 57 and through them 63, 52
+// (pages of 64, pages of 128); both tiles' values ahead 58, 57; 4, 6, 8 and 12 waves 57, 56,
+// 56, 56 at their best splits, 8 for one short row (11 us for 1024 keys, where two splits and
+// their merge take 13.5); three waves a SIMD instead of two 60.
 template <typename T, int D, int NC, int kPage, int W>
 __global__ __launch_bounds__(W * kWave, D == 128 && NC == 2 ? 1 : 2) void paged_attention_kernel(const PagedArgs a) {
   using L = Tile<D>;
@@ -469,10 +477,17 @@ __global__ __launch_bounds__(W * kWave, D == 128 && NC == 2 ? 1 : 2) void paged_
 // two products: in those with K dims 32 x + 16 h .. + 15 of a key, in those with V keys
 // 32 x + 16 h .. + 15 of a dim (lane = 32 h + n). So that lane (h, n) holds the scores of the
 // latter, row m of S^T takes the key 16 (m / 4 % 2) + 8 (m / 16) + 4 (m / 8 % 2) + m % 4 of its 32.
-template <typename T, int D, int kPage, int W>
-__global__ __launch_bounds__(W * kWave, 2) void paged_rows_kernel(const PagedArgs a) {
+// Bound by a wave's chain and its vector instructions (128 conversions, 32 exponentials and
+// their like beside 32 products of 32 cycles to a tile of 32 rows of 128): 512 rows over 32000
+// keys of 8 heads 87 us with the merge (770 TFLOP/s), 27 tokens of 4 heads over 8 rows of 1K to
+// 8K 37. Measured: tiles staged as bf16 (a conversion for four waves, twice the LDS bytes) 89;
+// two buffers and one barrier a tile 90; the products of the tile before between this tile's
+// exponentials 89 to 95; two teams of four waves to a workgroup 86 at half the splits, but 51
+// where 37 + 7 stand for rows of different length.
+template <typename T, int D, int kPage>
+__global__ __launch_bounds__(kRowWaves * kWave, 2) void paged_rows_kernel(const PagedArgs a) {
   constexpr bool kWide = kPage >= kPagedTile;
-  constexpr int P = pieces_of<T>(), BT = kPagedTile, kRows = 32 * W, kThreads = W * kWave;
+  constexpr int P = pieces_of<T>(), BT = kPagedTile, kRows = 32 * kRowWaves, kThreads = kRowWaves * kWave;
   constexpr int kSteps = D / 16, kTiles = D / 32;          // of the products with K, of dims of V
   constexpr int kPieces = BT * D / 16 / kThreads;          // of 16 codes of a tile's keys a thread stages
   constexpr int kSpots = kWide ? 1 : 4, kBatch = kWave / kSpots;
@@ -543,6 +558,7 @@ __global__ __launch_bounds__(W * kWave, 2) void paged_rows_kernel(const PagedArg
   const auto value_slot = [](int dim, int x) { return dim * 4 + (x ^ dim / 4 % 4); };
 
   if (threadIdx.x == 0) found = 0;
+  __syncthreads();  // before a wave that is ahead finds something
   if (count > 0) {
     look_up(0);
     fetch(0);
@@ -712,7 +728,9 @@ __global__ __launch_bounds__(W * kWave, 2) void paged_rows_kernel(const PagedArg
 }
 
 // The splits of a row joined. A wave has a row, or with `kShared` a workgroup has one and
-// its four waves every fourth round of splits; kRound splits' loads go out together.
+// its four waves every fourth round of splits; kRound splits' loads go out together. A
+// chain of latencies for few rows (1024 of 2 splits 4.7 us; 32 of 32 splits 4.6, with a wave to
+// a row 6.0), memory for many (6912 of 8 splits, 29 MB, 7.8).
 template <typename T, int D, bool kShared>
 __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedArgs a) {
   constexpr int DPL = (D + kWave - 1) / kWave, kRound = 8, W = kShared ? 4 : 1;
@@ -807,7 +825,7 @@ int launch_paged(PagedArgs& a, hipStream_t stream) {
   const auto run = [&](auto page) {
     constexpr int kPage = decltype(page)::value;
     if constexpr (kShares)
-      if (block == 128) return launch(paged_rows_kernel<T, D, kPage, 4>, 4);
+      if (block == 128) return launch(paged_rows_kernel<T, D, kPage>, kRowWaves);
     if constexpr (kPairs)
       if (block == 32) return launch(paged_attention_kernel<T, D, 2, kPage, 4>, 4);
     launch(paged_attention_kernel<T, D, 1, kPage, 8>, 8);
