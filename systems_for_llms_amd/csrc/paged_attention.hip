@@ -11,8 +11,6 @@
 // power of two), on their way into the matrix cores; what has more bits goes in as a sum of
 // bf16 pieces: q and the probabilities of fp16 as two, of fp32 as three, so the only
 // roundings are those of the probabilities to the sum of their pieces and of fp32 sums.
-#include <limits.h>
-
 #include <algorithm>
 #include <type_traits>
 

@@ -126,6 +126,7 @@ __global__ __launch_bounds__(1024) void append_kernel(const AppendArgs a) {
     }
     e = max(e, before);
   }
+  asm volatile("" : "+v"(e));  // from the held scale, which is read before it is replaced
   settle();  // the words above are written before the new tokens' bytes beside them
   if (threadIdx.x == 0) *scale = power_of_two(e);
   const float up = power_of_two(-e);

@@ -14,7 +14,8 @@ row of ``tables``, which names its pages, and of ``lengths``. A serving step is
 ``compact`` moves the pages in use to the front of the pool. A page that several rows hold
 (``refs`` counts them) is never written: ``reserve`` gives a row its own copy of the one it
 goes on writing in. All calls but ``create`` only touch the device and can be captured;
-``cache.lengths`` and the tensors given may be changed in place between calls and replays.
+``cache.lengths`` and the tensors given may be changed in place between calls and replays. Calls
+on a cache, replays too, run one after the other; only ``prepared()`` ones may overlap.
 Inference only: ``requires_grad`` inputs are refused.
 """
 
@@ -37,7 +38,7 @@ MAX_TOKENS = _cache.MAX_DRAFTS
 MAX_SPLITS = 128
 
 
-@dataclass(frozen=True, eq=False)
+@dataclass(eq=False)
 class PagedCache:
     """The tensors of a paged cache, contiguous on one device; a program may allocate them itself.
 
@@ -46,7 +47,7 @@ class PagedCache:
     a value is its code times its page's scale, a power of two. ``tables`` int32 ``[B, M]``: the
     page of a row's tokens from ``place * page`` on, -1 for none. ``lengths`` int32 ``[B]``:
     committed tokens. ``refs`` int32 ``[P]``: in how many rows a page is, 0 for a free one.
-    Up to 1024 rows.
+    Up to 1024 rows. The tensors change in place; none is replaced.
     """
 
     k: torch.Tensor
@@ -60,6 +61,13 @@ class PagedCache:
     _index: int = field(init=False, repr=False)
     _shape: tuple = field(init=False, repr=False)
     _scratch: torch.Tensor = field(init=False, repr=False)
+    _spans: tuple = field(init=False, repr=False)  # of memory that calls write: first and last address of each tensor
+
+    def __setattr__(self, name, value):
+        # What was checked stays; ``cache.lengths += n`` sets the tensor that it has changed in place.
+        if self.__dict__.get(name, value) is not value:
+            raise AttributeError(f"{name} of a paged cache is changed in place, not replaced")
+        object.__setattr__(self, name, value)
 
     def __post_init__(self):
         k, tables = self.k, self.tables
@@ -86,12 +94,12 @@ class PagedCache:
         if k.data_ptr() % 16 or self.v.data_ptr() % 16:
             raise ValueError("k and v must be 16-byte aligned")
         held = (k, self.v, self.k_scale, self.v_scale, tables, self.lengths, self.refs)
-        if len({t.data_ptr() for t in held}) < len(held) and index >= 0:
+        self._spans = tuple(sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in held if t.data_ptr()))
+        if any(last > start for (_, last), (start, _) in zip(self._spans, self._spans[1:])):
             raise ValueError("the tensors of a cache must not share memory")
-        object.__setattr__(self, "_index", index)
-        object.__setattr__(self, "_shape", (tables.shape[0], heads, dim))
-        scratch = torch.empty(4 + 2 * max(pages, tables.shape[0]), dtype=torch.int32, device=k.device)
-        object.__setattr__(self, "_scratch", scratch)
+        self._index = index
+        self._shape = (tables.shape[0], heads, dim)
+        self._scratch = torch.empty(4 + 2 * max(pages, tables.shape[0]), dtype=torch.int32, device=k.device)
 
     @property
     def layers(self) -> int:
@@ -131,6 +139,15 @@ def _check_cache(operator, cache):
     return cache._index
 
 
+def _check_apart(cache, name, t):
+    """A vector that a call reads while it writes the cache."""
+    first = t.data_ptr()
+    last = first + 4 * t.numel()
+    for start, end in cache._spans:
+        if first < end and start < last:
+            raise ValueError(f"{name} must not share memory with the cache (its lengths, tables or pages)")
+
+
 def _check_layer(cache, layer):
     if type(layer) is not int or not 0 <= layer < cache.k.shape[0]:
         raise ValueError("layer must be an integer in [0, layers)")
@@ -145,8 +162,7 @@ def fork(cache, parents) -> None:
     """
     index = _check_cache("fork", cache)
     _cache.check_vector("fork", "parents", parents, torch.int32, cache.lengths.shape, index)
-    if parents.data_ptr() == cache.lengths.data_ptr():
-        raise ValueError("parents must not be the cache's lengths")
+    _check_apart(cache, "parents", parents)
     _cache.check_device(index)
     written = (cache.tables, cache.lengths, cache.refs)
     ops.dispatch(torch.ops.sfl.page_fork, (parents, *written), written, cache.k.shape[3], checked=True)
@@ -164,6 +180,7 @@ def reserve(cache, counts) -> torch.Tensor:
     """
     index = _check_cache("reserve", cache)
     _cache.check_vector("reserve", "counts", counts, torch.int32, cache.lengths.shape, index)
+    _check_apart(cache, "counts", counts)
     _cache.check_device(index)
     _lib.lib()  # fail here, before allocating, if the library is not built
     granted = torch.empty_like(cache.lengths)
@@ -273,8 +290,8 @@ def prepare(q, cache, *, layer=0, counts=None, window_left=None, splits=None, sc
     and itself. ``counts`` int32 ``[B]``: tokens in use; the rows of the others are zeros with an
     ``lse`` (fp32 ``[B, Hq, T]``) of -inf, as are those of tokens that see nothing or have no slot. What
     a token does not see has no part in its row, NaN included. Scores and sums are fp32, and
-    no code is rounded again: probabilities are rounded to bf16 for bf16 ``q``, to two such
-    pieces for fp16, three for fp32. ``splits``: workgroups that share a KV head's slots, 1 to
+    no code is rounded again: probabilities, of up to 2^8 before the division by their sum, are rounded
+    to bf16 for bf16 ``q``, to two such pieces for fp16, three for fp32. ``splits``: workgroups that share a KV head's slots, 1 to
     128 (default by size). Like ``tree.PreparedTree`` the operation owns its scratch and output
     and holds its inputs by reference; concurrent calls on one race.
     """

@@ -212,3 +212,29 @@ def test_float64_forms_agree_with_torch_and_the_older_oracle():
     freed = op_.fork(both, torch.tensor([-1, 1]))
     used, packed = op_.compact(op_.fork(freed, torch.tensor([0, 1])))
     assert used == 3 and packed["tables"].tolist() == [[-1] * 3, [0, 1, 2]]
+
+
+def test_lengths_move_in_place_and_nothing_is_replaced():
+    cache = small()
+    lengths = cache.lengths
+    cache.lengths += torch.tensor([3, 1], dtype=torch.int32)
+    assert cache.lengths is lengths and lengths.tolist() == [3, 1]
+    for name in ("k", "lengths", "_scratch"):
+        with pytest.raises(AttributeError, match="in place"):
+            setattr(cache, name, getattr(cache, name).clone())
+
+
+def test_shared_memory_is_refused():
+    cache = small()
+    books = torch.zeros(20, dtype=torch.int32)
+    small(tables=books[:6].view(2, 3), lengths=books[6:8], refs=books[8:15])
+    for lengths, refs in ((books[4:6], books[8:15]), (books[6:8], books[7:14]), (books[:2], books[8:15])):
+        with pytest.raises(ValueError, match="share memory"):
+            small(tables=books[:6].view(2, 3), lengths=lengths, refs=refs)
+    with pytest.raises(ValueError, match="share memory"):
+        small(v_scale=cache.k_scale, k_scale=cache.k_scale)
+    for vector in (cache.lengths, cache.refs[3:5], cache.tables.view(-1)[1:3], cache.k_scale.view(-1).view(torch.int32)[7:9]):
+        with pytest.raises(ValueError, match="parents must not share"):
+            paged.fork(cache, vector)
+        with pytest.raises(ValueError, match="counts must not share"):
+            paged.reserve(cache, vector)
