@@ -27,4 +27,7 @@ Pinning (what fixes each function independently of its own formula):
 * ``cache.*`` (the KV-cache operators, which the reference does not have): float64 and
   row by row from the definitions; one draft of ``tree_attention`` equals
   ``attention.decode_reference``, a row's ``tree_weights`` add up to one.
+* ``paged.*`` (the paged 8-bit cache, likewise): codes equal torch's own e4m3 rounding under
+  the page's scale, attention equals ``cache.tree_attention`` over the gathered values, and
+  the books are lists that forks, reservations and moves rewrite one by one.
 """
