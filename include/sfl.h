@@ -518,8 +518,10 @@ int sfl_rotate(const void* q, const void* k, const void* v, const int32_t* posit
  * in its row, whatever their rows hold.
  *   q, out [batch, q_heads, tokens] rows, Hq/Hkv in {1, 2, 4, 8}
  *   mask   uint8, strides {batch, t, j} (0 for a shared one); counts [batch] or NULL
- *   partial_max, partial_sum  batch * q_heads * tokens * splits fp32 values, partial_out
- *   head_dim times as many: scratch, unused (may be NULL) with splits == 1
+ *   splits: parts that each KV head's slots are read in, side by side. most_splits >= splits:
+ *   those of sequences that hold far more than their share of the batch's slots
+ *   partial_max, partial_sum  batch * q_heads * tokens * most_splits fp32 values, partial_out
+ *   head_dim times as many: scratch, unused (may be NULL) with most_splits == 1
  *   strides [15]: q, k, v, out, mask. q, k, v, out 16-byte aligned, their strides
  *   multiples of 16 bytes
  * Every sum in fp32. Results do not vary from call to call.
@@ -633,7 +635,7 @@ int sfl_page_attention(const void* q, const void* k_codes, const void* v_codes, 
                        const int32_t* counts, float* partial_max, float* partial_sum, float* partial_out,
                        void* out, float* lse, const long* strides, int batch, int q_heads, int kv_heads,
                        int tokens, int places, int pages, int page_size, int head_dim, int window_left,
-                       int splits, float scale, int dtype, void* stream);
+                       int splits, int most_splits, float scale, int dtype, void* stream);
 
 /*
  * All at once, row b becomes what row parents[b] was: it leaves its pages and holds those

@@ -71,7 +71,7 @@ SIGNATURES: dict[str, list] = {
     "sfl_select_slots": [P] * 5 + [c_int] * 5 + [P],
     "sfl_compact_slots": [P] * 5 + [P] + [c_int] * 6 + [P],
     "sfl_page_append": [P] * 10 + [P] + [c_int] * 8 + [P],
-    "sfl_page_attention": [P] * 13 + [P] + [c_int] * 10 + [c_float, c_int, P],
+    "sfl_page_attention": [P] * 13 + [P] + [c_int] * 11 + [c_float, c_int, P],
     "sfl_page_fork": [P] * 4 + [c_int] * 4 + [P],
     "sfl_page_reserve": [P] * 10 + [c_int] * 7 + [P],
     "sfl_page_compact": [P] * 8 + [c_int] * 7 + [P],

@@ -26,6 +26,7 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 constexpr int kPagedTile = 64;  // keys of a wave's tile
 constexpr int kMaxTokens = 128;
 constexpr int kRowWaves = 4;    // of the kernel for many rows
+constexpr int kAtOnce = 256;    // workgroups that a call in need of more parts aims at
 constexpr float kLn2 = 0.6931471805599453f;
 
 struct PagedArgs {
@@ -37,9 +38,13 @@ struct PagedArgs {
   void* out;
   float* lse;
   long qs[3], os[3];  // strides in elements: batch, head, token
-  int kv_heads, places, pages, page_log2, tokens, group_log2, row_blocks, splits, groups;
-  int window;  // slots before its own that a token sees; < 0: all
-  float cs;    // scale * log2(e): scores are kept in base 2
+  int kv_heads, places, pages, page_log2, tokens, group_log2, row_blocks, groups;
+  int splits, most;  // parts of a head's tiles: of sequences of the usual length, of long ones
+  int more;          // workgroups (to a row block) for the latter's, where they may have more
+  int batch;
+  int window;   // slots before its own that a token sees; < 0: all
+  float share;  // of the tiles of all sequences that a part is meant to have
+  float cs;     // scale * log2(e): scores are kept in base 2
 };
 
 template <typename T> constexpr int pieces_of() { return std::is_same<T, bf16_t>::value ? 1 : std::is_same<T, f16_t>::value ? 2 : 3; }
@@ -48,20 +53,76 @@ template <typename T> constexpr int pieces_of() { return std::is_same<T, bf16_t>
 struct PagedRow {
   int len, count, cap;
 };
-__device__ __forceinline__ PagedRow paged_row(const PagedArgs& a, int b) {
-  typedef const __attribute__((address_space(4))) int32_t* Constant;  // read by scalar loads
-  b = __builtin_amdgcn_readfirstlane(b);
+template <typename P>
+__device__ __forceinline__ PagedRow paged_row(const PagedArgs& a, P lengths, P counts, int b) {
   PagedRow r;
   r.cap = a.places << a.page_log2;
-  r.len = min(max(Constant(a.lengths)[b], 0), r.cap);
-  r.count = a.counts ? min(max(Constant(a.counts)[b], 0), a.tokens) : a.tokens;
+  r.len = min(max(lengths[b], 0), r.cap);
+  r.count = counts ? min(max(counts[b], 0), a.tokens) : a.tokens;
   r.count = min(r.count, r.cap - r.len);  // tokens that have a slot
   return r;
+}
+__device__ __forceinline__ PagedRow paged_row(const PagedArgs& a, int b) {
+  typedef const __attribute__((address_space(4))) int32_t* Constant;  // read by scalar loads
+  return paged_row(a, Constant(a.lengths), Constant(a.counts), __builtin_amdgcn_readfirstlane(b));
+}
+
+// Tiles that the tokens of a sequence see.
+__device__ __forceinline__ int tiles_seen(const PagedArgs& a, const PagedRow& r) {
+  if (r.count <= 0) return 0;
+  return (r.len + r.count + kPagedTile - 1) / kPagedTile - (a.window >= 0 ? max(r.len - a.window, 0) / kPagedTile : 0);
+}
+
+// Into how many parts a head's tiles of a sequence go: `splits`, or, where the call has room
+// for more, as many as it takes that none is more than the batch's tiles over kAtOnce. With
+// `splits` by the number of heads only sequences far longer than the others get more: us
+// without and with, 8 heads, 32 rows of 500 tokens but one of 131000 371 / 58 (78 where it is
+// the last), 64 of 2000 743 / 94, 8 of 500 but one of 32000 with 108 query rows 92 / 55; for
+// rows of one length the sum costs 1 to 4 of 170 to 320. More parts for every row by its
+// share: rows of 1K to 8K 51.5 / 52.5, 108 query rows 44 / 52. Whole waves call it; it is one
+// sum in one order, so all of them come to the same.
+__device__ __forceinline__ int fair_part(const PagedArgs& a) {
+  float total = 0.f;
+  for (int b = threadIdx.x % kWave; b < a.batch; b += kWave) total += float(tiles_seen(a, paged_row(a, a.lengths, a.counts, b)));
+  return int(fminf(wave_sum(total) * a.share, 0x1p24f)) + 1;
+}
+__device__ __forceinline__ int parts_of(const PagedArgs& a, const PagedRow& row, int fair) {
+  const int tiles = tiles_seen(a, row);
+  return (tiles + a.splits - 1) / a.splits > fair ? min((tiles + fair - 1) / fair, a.most) : a.splits;
+}
+__device__ __forceinline__ int parts_of(const PagedArgs& a, const PagedRow& row) {
+  return __builtin_expect(a.most == a.splits, 1) ? a.splits : __builtin_amdgcn_readfirstlane(parts_of(a, row, fair_part(a)));
+}
+
+// The sequence that the x-th of the parts beyond `splits` belongs to, a head's parts behind each
+// other, and the part's number there. No parts: there are not so many.
+struct More {
+  int b, parts, x;
+};
+__device__ __forceinline__ More find_more(const PagedArgs& a, int x) {
+  const int fair = fair_part(a), lane = threadIdx.x % kWave;
+  int of = 0, parts = 0, at_x = 0;
+  for (int b0 = 0; b0 < a.batch && parts == 0; b0 += kWave) {
+    const int mine = b0 + lane < a.batch ? parts_of(a, paged_row(a, a.lengths, a.counts, b0 + lane), fair) : a.splits;
+    const int own = (mine - a.splits) * a.kv_heads;
+    int sum = own;  // becomes that of the lanes up to this one
+#pragma unroll
+    for (int m = 1; m < kWave; m <<= 1) {
+      const int other = __shfl_up(sum, m);
+      sum += lane >= m ? other : 0;
+    }
+    const uint64_t past = __ballot(sum > x);
+    const int at = past ? __builtin_ctzll(past) : kWave - 1;
+    of = b0 + at, parts = past ? __builtin_amdgcn_readlane(mine, at) : 0, at_x = x - __builtin_amdgcn_readlane(sum - own, at);
+    x -= __builtin_amdgcn_readlane(sum, kWave - 1);
+  }
+  return {of, parts, at_x};
 }
 
 // A workgroup's work: some rows of a KV head of sequence b over a part of its tiles.
 struct Work {
-  int b, hk, part, group;  // group: the head among those of all sequences
+  int b, hk, group;        // group: the head among those of all sequences
+  int part, parts;
   int r0, rows;            // first row of the block; rows of a sequence
   int t0, t1;              // tokens of the block
   int start, end;          // slots that some row of the block sees
@@ -72,22 +133,40 @@ __device__ __forceinline__ bool find_work(const PagedArgs& a, int block, Work& w
   // Row blocks of one unit run on one XCD, whose L2 then holds its pages.
   const int slice = int(blockIdx.x) / kXcds;
   const int unit = slice / a.row_blocks * kXcds + int(blockIdx.x) % kXcds;
-  if (unit >= a.groups * a.splits) return false;
   w.r0 = slice % a.row_blocks * block;
-  w.group = __builtin_amdgcn_readfirstlane(unit / a.splits);
-  w.part = unit - w.group * a.splits;
+  const int usual = unit - a.more;  // the parts that only long sequences have come first
+  if (usual >= a.groups * a.splits) return false;
+  int group = usual / a.splits, more_parts = 0;
+  w.part = usual - group * a.splits;
+  if (__builtin_expect(usual < 0, 0)) {
+    const More more = find_more(a, unit);
+    if (more.parts == 0) return false;
+    const int extra = more.parts - a.splits;
+    group = more.b * a.kv_heads + more.x / extra, w.part = a.splits + more.x % extra, more_parts = more.parts;
+  }
+  w.group = __builtin_amdgcn_readfirstlane(group), w.part = __builtin_amdgcn_readfirstlane(w.part);
   w.b = __builtin_amdgcn_readfirstlane(w.group / a.kv_heads);
   w.hk = w.group - w.b * a.kv_heads;
   w.row = paged_row(a, w.b);
+  w.parts = __builtin_amdgcn_readfirstlane(more_parts ? more_parts : parts_of(a, w.row));
   w.rows = a.tokens << a.group_log2;
   w.t0 = w.r0 >> a.group_log2, w.t1 = min((min(w.r0 + block, w.rows) - 1) >> a.group_log2, w.row.count - 1);
   w.end = w.t1 >= w.t0 ? w.row.len + w.t1 + 1 : 0;
   w.start = a.window >= 0 ? max(w.row.len + w.t0 - a.window, 0) : 0;
-  // The tiles from that of `start` on are shared out evenly, however long the row is.
+  // The tiles from that of `start` on are shared out evenly.
   const int first = w.start / kPagedTile, tiles = max((w.end + kPagedTile - 1) / kPagedTile - first, 0);
-  const int each = tiles / a.splits, more = tiles - each * a.splits;  // one more in the first ones
+  const int each = tiles / w.parts, more = tiles - each * w.parts;  // one more in the first ones
   w.begin = first + w.part * each + min(w.part, more);
   w.count = each + (w.part < more);
+  return true;
+}
+
+// A part without tiles of a row that others share: the merge looks no further than its maximum.
+template <int kRows, int kThreads>
+__device__ __forceinline__ bool nothing_to_do(const PagedArgs& a, const Work& w) {
+  if (w.parts == 1 || w.count > 0) return false;
+  for (int i = threadIdx.x; i < min(kRows, w.rows - w.r0); i += kThreads)
+    a.pmax[(long(w.group) * a.most + w.part) * w.rows + w.r0 + i] = -INFINITY;
   return true;
 }
 
@@ -233,7 +312,7 @@ __global__ __launch_bounds__(W * kWave, D == 128 && NC == 2 ? 1 : 2) void paged_
   const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave);
   const int lane = threadIdx.x % kWave, g = lane / 16, n = lane % 16;
   Work work;
-  if (!find_work(a, kRows, work)) return;
+  if (!find_work(a, kRows, work) || nothing_to_do<kRows, W * kWave>(a, work)) return;
   const int b = work.b, hk = work.hk, r0 = work.r0, rows = work.rows, G = 1 << a.group_log2;
   const PagedRow row = work.row;
   const int t0 = work.t0, t1 = work.t1, start = work.start, end = work.end;
@@ -454,8 +533,8 @@ __global__ __launch_bounds__(W * kWave, D == 128 && NC == 2 ? 1 : 2) void paged_
       for (int e = 0; e < 4; ++e) num[e] = tops[w][i] == -INFINITY ? num[e] : fmaf(weight, part_o[e], num[e]);
     }
     const int t = r >> a.group_log2, head = (hk << a.group_log2) + (r & (G - 1));
-    if (a.splits > 1) {
-      const long to = (long(work.group) * a.splits + work.part) * rows + r;
+    if (work.parts > 1) {
+      const long to = (long(work.group) * a.most + work.part) * rows + r;
       if (d == 0) a.pmax[to] = base, a.psum[to] = den;
       store4<float>(a.pout + to * D + d, num);
     } else {
@@ -494,7 +573,7 @@ __global__ __launch_bounds__(kRowWaves * kWave, 2) void paged_rows_kernel(const 
   const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave);
   const int lane = threadIdx.x % kWave, h = lane / 32, n = lane % 32;
   Work work;
-  if (!find_work(a, kRows, work)) return;
+  if (!find_work(a, kRows, work) || nothing_to_do<kRows, kThreads>(a, work)) return;
   const int b = work.b, hk = work.hk, r0 = work.r0, rows = work.rows, G = 1 << a.group_log2;
   const PagedRow row = work.row;
   const int t0 = work.t0, t1 = work.t1, start = work.start, end = work.end, begin = work.begin, count = work.count;
@@ -701,15 +780,15 @@ __global__ __launch_bounds__(kRowWaves * kWave, 2) void paged_rows_kernel(const 
   if (top == -INFINITY && sum != sum) top = 0.f;  // as above
   if (r0 + 32 * wave + n >= rows) return;
   const bool empty = top == -INFINITY || t >= row.count;
-  const long to = (long(work.group) * a.splits + work.part) * rows + r;
+  const long to = (long(work.group) * a.most + work.part) * rows + r;
   if (h == 0) {
-    if (a.splits > 1)
+    if (work.parts > 1)
       a.pmax[to] = top, a.psum[to] = sum;
     else
       a.lse[(long(b) * a.kv_heads * G + head) * a.tokens + t] = empty ? -INFINITY : (top + __builtin_log2f(sum)) * kLn2;
   }
   T* out = static_cast<T*>(a.out) + b * a.os[0] + head * a.os[1] + t * a.os[2];
-  const float share = a.splits > 1 ? 1.f : empty ? 0.f : 1.f / sum;
+  const float share = work.parts > 1 ? 1.f : empty ? 0.f : 1.f / sum;
 #pragma unroll
   for (int d = 0; d < kTiles; ++d)
 #pragma unroll
@@ -717,8 +796,8 @@ __global__ __launch_bounds__(kRowWaves * kWave, 2) void paged_rows_kernel(const 
       float num[4];
       const int dim = 32 * d + 8 * x + 4 * h;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) num[e] = empty && a.splits == 1 ? 0.f : o[d][4 * x + e] * share;
-      if (a.splits > 1)
+      for (int e = 0; e < 4; ++e) num[e] = empty && work.parts == 1 ? 0.f : o[d][4 * x + e] * share;
+      if (work.parts > 1)
         store4<float>(a.pout + to * D + dim, num);
       else
         store4<T>(out + dim, num);
@@ -740,11 +819,13 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedArgs a) {
   const int group = __builtin_amdgcn_readfirstlane(int(at / rows)), r = int(at - long(group) * rows);
   const int b = group / a.kv_heads, hk = group - b * a.kv_heads;
   const PagedRow row = paged_row(a, b);
+  const int parts = parts_of(a, row);
+  if (parts == 1) return;  // written already
   const int t = r >> a.group_log2, head = (hk << a.group_log2) + (r & (G - 1));
   float top = -INFINITY, den = 0.f, num[DPL] = {};
-  for (int s0 = kShared ? wave * kRound : 0; s0 < a.splits; s0 += kRound * W) {
-    const auto part = [&](int s) { return (long(group) * a.splits + min(s0 + s, a.splits - 1)) * rows + r; };
-    const bool on = lane < kRound && s0 + lane < a.splits;
+  for (int s0 = kShared ? wave * kRound : 0; s0 < parts; s0 += kRound * W) {
+    const auto part = [&](int s) { return (long(group) * a.most + min(s0 + s, parts - 1)) * rows + r; };
+    const bool on = lane < kRound && s0 + lane < parts;
     const float high = a.pmax[part(lane % kRound)], sum = a.psum[part(lane % kRound)];
     float x[kRound][DPL];
 #pragma unroll
@@ -813,7 +894,10 @@ int launch_paged(PagedArgs& a, hipStream_t stream) {
   constexpr bool kPairs = pieces_of<T>() == 1 && D >= 64, kShares = pieces_of<T>() < 3 && D >= 64;
   const int block = rows > 64 && kShares ? 128 : rows > 32 && kPairs ? 32 : 16;
   a.row_blocks = (rows + block - 1) / block;
-  const long units = (long(a.groups) * a.splits + kXcds - 1) / kXcds * kXcds;
+  a.share = float(a.kv_heads) * a.row_blocks / kAtOnce;
+  // Sequences of more than `splits` parts have together fewer parts than kAtOnce / row_blocks.
+  a.more = a.most > a.splits ? kAtOnce / a.row_blocks + 1 : 0;
+  const long units = (long(a.groups) * a.splits + a.more + kXcds - 1) / kXcds * kXcds;
   const long merged = long(a.groups) * rows;
   if (units * a.row_blocks >= kMostGroups || merged >= kMostGroups - 1)
     return set_error(SFL_ERR_UNSUPPORTED, "%s: too many workgroups", what);
@@ -832,8 +916,8 @@ int launch_paged(PagedArgs& a, hipStream_t stream) {
   else if (a.page_log2 == 6) run(std::integral_constant<int, 64>{});
   else run(std::integral_constant<int, 16>{});  // pages of less than a tile
   if (int rc = check_launch(what)) return rc;
-  if (a.splits == 1) return SFL_OK;
-  if (a.splits > 8)
+  if (a.most == 1) return SFL_OK;
+  if (a.splits > 8 || (a.most > 8 && merged <= 2048))
     hipLaunchKernelGGL((paged_merge_kernel<T, D, true>), dim3(unsigned(merged)), dim3(256), 0, stream, a);
   else
     hipLaunchKernelGGL((paged_merge_kernel<T, D, false>), dim3(unsigned((merged + 3) / 4)), dim3(256), 0, stream, a);
@@ -850,7 +934,7 @@ extern "C" int sfl_page_attention(const void* q, const void* k_codes, const void
                                   const int32_t* counts, float* partial_max, float* partial_sum, float* partial_out,
                                   void* out, float* lse, const long* strides, int batch, int q_heads, int kv_heads,
                                   int tokens, int places, int pages, int page_size, int head_dim, int window_left,
-                                  int splits, float scale, int dtype, void* stream) {
+                                  int splits, int most_splits, float scale, int dtype, void* stream) {
   using namespace sfl;
   const char* what = "page_attention";
   if (!q || !k_codes || !v_codes || !k_scale || !v_scale || !tables || !lengths || !out || !lse || !strides)
@@ -867,8 +951,9 @@ extern "C" int sfl_page_attention(const void* q, const void* k_codes, const void
   if (dtype != SFL_DTYPE_F32 && dtype != SFL_DTYPE_BF16 && dtype != SFL_DTYPE_F16)
     return set_error(SFL_ERR_UNSUPPORTED, "%s: dtype must be F32, BF16 or F16", what);
   if (!(scale > 0.f) || !__builtin_isfinite(scale)) return set_error(SFL_ERR_INVALID, "%s: scale must be finite and positive", what);
-  if (splits < 1 || splits > 1024) return set_error(SFL_ERR_INVALID, "%s: splits must be in [1, 1024]", what);
-  if (splits > 1 && (!partial_max || !partial_sum || !partial_out))
+  if (splits < 1 || most_splits < splits || most_splits > 1024)
+    return set_error(SFL_ERR_INVALID, "%s: splits must be in [1, 1024], most_splits in [splits, 1024]", what);
+  if (most_splits > 1 && (!partial_max || !partial_sum || !partial_out))
     return set_error(SFL_ERR_INVALID, "%s: null pointer argument", what);
   if (long(batch) * kv_heads > (1L << 24)) return set_error(SFL_ERR_UNSUPPORTED, "%s: too many KV heads", what);
   if (!aligned16(q) || !aligned16(out) || !aligned16(k_codes) || !aligned16(v_codes))
@@ -880,7 +965,8 @@ extern "C" int sfl_page_attention(const void* q, const void* k_codes, const void
               counts, partial_max, partial_sum, partial_out, out, lse};
   for (int i = 0; i < 3; ++i) a.qs[i] = strides[i], a.os[i] = strides[3 + i];
   a.kv_heads = kv_heads, a.places = places, a.pages = pages, a.page_log2 = log2_of(page_size), a.tokens = tokens;
-  a.group_log2 = ratio == 8 ? 3 : ratio / 2, a.splits = splits, a.groups = batch * kv_heads;
+  a.group_log2 = ratio == 8 ? 3 : ratio / 2, a.groups = batch * kv_heads;
+  a.splits = splits, a.most = most_splits, a.batch = batch;
   a.window = std::max(window_left, -1);
   a.cs = scale * kLog2e;
   return paged_types(dtype, head_dim, [&](auto t, auto d) {

@@ -232,7 +232,7 @@ def launch_page_attention(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch
           k_scale.data_ptr() + scales, v_scale.data_ptr() + scales, tables.data_ptr(), lengths.data_ptr(), _ptr(counts),
           partial_max.data_ptr(), partial_sum.data_ptr(), partial_output.data_ptr(), out.data_ptr(), lse.data_ptr(),
           _strides_2(*q.stride()[:3], *out.stride()[:3]), batch, heads, kv_heads, tokens, tables.shape[1], pages,
-          page_size, dim, window_left, splits, scale, _lib.dtype_code(q.dtype))
+          page_size, dim, window_left, splits, max(splits, partial_max.shape[3]), scale, _lib.dtype_code(q.dtype))
 
 
 def launch_page_fork(parents: torch.Tensor, tables: torch.Tensor, lengths: torch.Tensor, refs: torch.Tensor,

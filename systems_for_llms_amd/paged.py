@@ -244,12 +244,29 @@ def auto_splits(batch: int, kv_heads: int, capacity: int, rows: int, dim: int, d
     of 4095 24 / 29 / 33 / 45; 1 of 131072 at 16 / 32 / 64 splits 76 / 52 / 55; 27 tokens of 4 heads
     over 8 of 1K to 8K 185 / 102 / 59 / 44.
     """
+    block, blocks, reach = _blocks(batch, kv_heads, capacity, rows, dim, dtype, window_left)
+    target = 512 if block == 128 or rows <= 16 and batch > 1 and window_left is None else 256
+    return max(1, min(64, round(target / blocks), round(reach / 1024)))
+
+
+def _blocks(batch, kv_heads, capacity, rows, dim, dtype, window_left):
+    """Query rows of a workgroup, such blocks of all sequences, slots that a token may see."""
     tiled = dtype != torch.float32 and dim >= 64
     block = 128 if tiled and rows > 64 else 32 if tiled and dtype == torch.bfloat16 and rows > 32 else 16
-    blocks = batch * kv_heads * math.ceil(rows / block)
-    target = 512 if block == 128 or rows <= 16 and batch > 1 and window_left is None else 256
-    reach = capacity if window_left is None else min(capacity, window_left + 1)
-    return max(1, min(64, round(target / blocks), round(reach / 1024)))
+    return (block, batch * kv_heads * math.ceil(rows / block),
+            capacity if window_left is None else min(capacity, window_left + 1))
+
+
+def auto_most_splits(splits: int, batch: int, kv_heads: int, capacity: int, rows: int, dim: int, dtype: torch.dtype,
+                     window_left: int | None = None) -> int:
+    """Those that sequences may have that hold far more than their share of the batch's slots, where
+    ``splits`` could leave their workgroups more than 8192 slots each (4096 and 2048 for blocks of 32
+    and 128 rows): with 256 more workgroups for the call, of heads and blocks of such sequences.
+    """
+    block, blocks, reach = _blocks(batch, kv_heads, capacity, rows, dim, dtype, window_left)
+    if batch == 1 or reach <= splits * {16: 8192, 32: 4096, 128: 2048}[block]:
+        return splits
+    return max(splits, min(64, splits + 256 * batch // blocks))
 
 
 @dataclass
@@ -292,7 +309,7 @@ def prepare(q, cache, *, layer=0, counts=None, window_left=None, splits=None, sc
     a token does not see has no part in its row, NaN included. Scores and sums are fp32, and
     no code is rounded again: probabilities, of up to 2^8 before the division by their sum, are rounded
     to bf16 for bf16 ``q``, to two such pieces for fp16, three for fp32. ``splits``: workgroups that share a KV head's slots, 1 to
-    128 (default by size). Like ``tree.PreparedTree`` the operation owns its scratch and output
+    128; by default as many as the sizes ask for, and more for sequences far longer than the others. Like ``tree.PreparedTree`` the operation owns its scratch and output
     and holds its inputs by reference; concurrent calls on one race.
     """
     if splits is not None and (type(splits) is not int or not 1 <= splits <= MAX_SPLITS):
@@ -317,10 +334,13 @@ def prepare(q, cache, *, layer=0, counts=None, window_left=None, splits=None, sc
         raise ValueError("scale must be finite and positive")
     _cache.check_device(index)
     _lib.lib()  # fail here, before allocation, if the library is not built
+    most = splits
     if splits is None:
-        splits = auto_splits(batch, kv_heads, cache.capacity, tokens * (heads // kv_heads), dim, q.dtype, window_left)
+        size = batch, kv_heads, cache.capacity, tokens * (heads // kv_heads), dim, q.dtype, window_left
+        splits = auto_splits(*size)
+        most = auto_most_splits(splits, *size)
     window = -1 if window_left is None else min(window_left, cache.capacity)
-    maximum = torch.empty((batch, heads, tokens, splits if splits > 1 else 0), device=q.device, dtype=torch.float32)
+    maximum = torch.empty((batch, heads, tokens, most if most > 1 else 0), device=q.device, dtype=torch.float32)
     numerator = torch.empty((*maximum.shape, dim), device=q.device, dtype=torch.float32)
     lse = torch.empty((batch, heads, tokens), device=q.device, dtype=torch.float32)
     return PreparedPaged(q, cache, counts, maximum, torch.empty_like(maximum), numerator, torch.empty_like(q), lse,

@@ -164,13 +164,13 @@ def test_entry_points_refuse_before_any_launch():
         (10, strides((2, 60)), INVALID)))
     assert _status("sfl_page_append", *append[:11], 1 << 20, 1 << 12, *append[13:]) == UNSUPPORTED  # workgroups
 
-    attention = [p] * 13 + [strides(), 1, 4, 2, 3, 4, 9, 16, 64, -1, 1, 0.125, f, None]
+    attention = [p] * 13 + [strides(), 1, 4, 2, 3, 4, 9, 16, 64, -1, 1, 1, 0.125, f, None]
     refused("sfl_page_attention", attention, (
         *((i, None, INVALID) for i in (0, 1, 2, 3, 4, 5, 6, 11, 12, 13)), (0, 72, INVALID), (2, 72, INVALID), (11, 72, INVALID),
         (14, 0, INVALID), (15, 3, INVALID), (15, 6, UNSUPPORTED), (17, 129, UNSUPPORTED), (17, 0, INVALID), (18, 0, INVALID),
-        (20, 8, UNSUPPORTED), (21, 80, UNSUPPORTED), (23, 0, INVALID), (23, 1025, INVALID), (24, -1.0, INVALID),
-        (24, math.inf, INVALID), (25, 7, UNSUPPORTED), (13, strides((4, 63)), INVALID)))
-    assert _status("sfl_page_attention", *[p] * 8, None, p, p, *attention[11:23], 2, 0.125, f, None) == INVALID  # no scratch
+        (20, 8, UNSUPPORTED), (21, 80, UNSUPPORTED), (23, 0, INVALID), (23, 2, INVALID), (24, 1025, INVALID), (25, -1.0, INVALID),
+        (25, math.inf, INVALID), (26, 7, UNSUPPORTED), (13, strides((4, 63)), INVALID)))
+    assert _status("sfl_page_attention", *[p] * 8, None, p, p, *attention[11:23], 1, 2, 0.125, f, None) == INVALID  # no scratch
 
     fork = [p] * 4 + [2, 4, 9, 16, None]
     refused("sfl_page_fork", fork, (*((i, None, INVALID) for i in range(4)), (4, 1025, UNSUPPORTED), (5, 0, INVALID),
@@ -238,3 +238,22 @@ def test_shared_memory_is_refused():
             paged.fork(cache, vector)
         with pytest.raises(ValueError, match="counts must not share"):
             paged.reserve(cache, vector)
+
+
+def test_most_splits_bounds():
+    bf16, fp16, fp32 = torch.bfloat16, torch.float16, torch.float32
+    for size, most in (((32, 8, 8192, 4, 128, bf16), 2),         # rows of up to 8192 slots: nothing to win
+                       ((32, 8, 131072, 4, 128, bf16), 34),      # 256 more workgroups of 8 heads
+                       ((1, 8, 131072, 4, 128, bf16), 32),       # a sequence alone has all of them
+                       ((8, 8, 8192, 108, 128, fp16), 8), ((8, 8, 32768, 108, 128, fp16), 40),
+                       ((32, 8, 131072, 4, 128, bf16, 4095), 1), ((600, 1, 9024, 1, 128, fp16), 64)):
+        splits = paged.auto_splits(*size)
+        assert paged.auto_most_splits(splits, *size) == most
+    for batch in (2, 64, 1024):
+        for rows in (1, 40, 100, 1024):
+            for dtype in (bf16, fp32):
+                size = (batch, 8, 1 << 20, rows, 128, dtype)
+                splits = paged.auto_splits(*size)
+                most = paged.auto_most_splits(splits, *size)
+                # No sequence can need more: the further workgroups are 256, a block of a head's rows each.
+                assert splits <= most <= 64
