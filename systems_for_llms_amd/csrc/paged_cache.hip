@@ -305,7 +305,7 @@ __device__ __forceinline__ int find_free(const BookArgs& a, int from, int most, 
 // do to a place's page is found from the pages they hold: of r holders, the first r - 1 that
 // write it leave it, and the last then has it alone. (Those of earlier rounds have left, or
 // there are no free pages any more.) Bound by its chain of loads and barriers: 64 rows, 16 of
-// them with 6 new places and 16 that share a page, of 1600 pages 9.7 us.
+// them with 6 new places and 16 that share a page, of 1600 pages 10 to 11 us.
 __global__ __launch_bounds__(kBookThreads) void reserve_kernel(const BookArgs a, const int32_t* counts, int32_t* granted,
                                                                int2* copies, int* copied) {
   __shared__ int sums[kBookThreads / kWave];
@@ -439,7 +439,7 @@ constexpr int kCopyPieces = 4, kCopyPart = 256 * 16 * kCopyPieces;
 
 // Pages copied, all layers: workgroups walk (move, layer, keys or values, 16 KB of it), as a
 // plan made on the device is not known to the launch. Bound by memory: 491 pages of 8 layers,
-// 1.03 GB read and written, 196 us (5.3 TB/s); 94 MB 20 (4.6).
+// 1.03 GB read and written, 198 to 212 us (4.9 to 5.2 TB/s); 94 MB 20 (4.6).
 __device__ __forceinline__ void copy_pages(const CopyArgs& c) {
   const long items = long(*c.moved) * c.layers * 2 * c.parts;
   for (long y = blockIdx.x; y < items; y += gridDim.x) {

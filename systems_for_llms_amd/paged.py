@@ -101,6 +101,9 @@ class PagedCache:
         self._shape = (tables.shape[0], heads, dim)
         self._scratch = torch.empty(4 + 2 * max(pages, tables.shape[0]), dtype=torch.int32, device=k.device)
 
+    def __reduce__(self):  # copies and loaded caches are looked at anew: their tensors are others
+        return PagedCache, (self.k, self.v, self.k_scale, self.v_scale, self.tables, self.lengths, self.refs)
+
     @property
     def layers(self) -> int:
         return self.k.shape[0]

@@ -1,6 +1,8 @@
 """Host side of the paged 8-bit cache (no GPU): refusals, schemas, C argument checks, the plain forms against each other."""
 
+import copy
 import ctypes
+import io
 import math
 
 import pytest
@@ -222,6 +224,22 @@ def test_lengths_move_in_place_and_nothing_is_replaced():
     for name in ("k", "lengths", "_scratch"):
         with pytest.raises(AttributeError, match="in place"):
             setattr(cache, name, getattr(cache, name).clone())
+
+
+def test_copies_are_caches_of_their_own():
+    cache = small()
+    cache.lengths += 5
+    file = io.BytesIO()
+    torch.save(cache, file)
+    file.seek(0)
+    for other in (copy.deepcopy(cache), torch.load(file, weights_only=False)):
+        assert other.lengths.tolist() == [5, 5] and other.k.shape == cache.k.shape and other._spans != cache._spans
+        other.lengths += 1
+        assert cache.lengths.tolist() == [5, 5]
+        with pytest.raises(ValueError, match="must not share"):
+            paged.fork(other, other.lengths)
+        with pytest.raises(ValueError, match="same CUDA"):
+            paged.fork(other, cache.lengths)
 
 
 def test_shared_memory_is_refused():
