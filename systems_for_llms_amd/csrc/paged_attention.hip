@@ -119,10 +119,19 @@ __device__ __forceinline__ More find_more(const PagedArgs& a, int x) {
   return {of, parts, at_x};
 }
 
+// How many such parts the sequences before b have.
+__device__ __forceinline__ int more_before(const PagedArgs& a, int b) {
+  const int fair = fair_part(a);
+  float sum = 0.f;
+  for (int x = threadIdx.x % kWave; x < b; x += kWave)
+    sum += float(parts_of(a, paged_row(a, a.lengths, a.counts, x), fair) - a.splits);
+  return __builtin_amdgcn_readfirstlane(int(wave_sum(sum)) * a.kv_heads);
+}
+
 // A workgroup's work: some rows of a KV head of sequence b over a part of its tiles.
 struct Work {
   int b, hk, group;        // group: the head among those of all sequences
-  int part, parts;
+  int part, parts, slot;   // slot: of the partial results of its head's rows
   int r0, rows;            // first row of the block; rows of a sequence
   int t0, t1;              // tokens of the block
   int start, end;          // slots that some row of the block sees
@@ -149,6 +158,7 @@ __device__ __forceinline__ bool find_work(const PagedArgs& a, int block, Work& w
   w.hk = w.group - w.b * a.kv_heads;
   w.row = paged_row(a, w.b);
   w.parts = __builtin_amdgcn_readfirstlane(more_parts ? more_parts : parts_of(a, w.row));
+  w.slot = usual < 0 ? a.groups * a.splits + unit : usual;
   w.rows = a.tokens << a.group_log2;
   w.t0 = w.r0 >> a.group_log2, w.t1 = min((min(w.r0 + block, w.rows) - 1) >> a.group_log2, w.row.count - 1);
   w.end = w.t1 >= w.t0 ? w.row.len + w.t1 + 1 : 0;
@@ -166,7 +176,7 @@ template <int kRows, int kThreads>
 __device__ __forceinline__ bool nothing_to_do(const PagedArgs& a, const Work& w) {
   if (w.parts == 1 || w.count > 0) return false;
   for (int i = threadIdx.x; i < min(kRows, w.rows - w.r0); i += kThreads)
-    a.pmax[(long(w.group) * a.most + w.part) * w.rows + w.r0 + i] = -INFINITY;
+    a.pmax[long(w.slot) * w.rows + w.r0 + i] = -INFINITY;
   return true;
 }
 
@@ -534,7 +544,7 @@ __global__ __launch_bounds__(W * kWave, D == 128 && NC == 2 ? 1 : 2) void paged_
     }
     const int t = r >> a.group_log2, head = (hk << a.group_log2) + (r & (G - 1));
     if (work.parts > 1) {
-      const long to = (long(work.group) * a.most + work.part) * rows + r;
+      const long to = long(work.slot) * rows + r;
       if (d == 0) a.pmax[to] = base, a.psum[to] = den;
       store4<float>(a.pout + to * D + d, num);
     } else {
@@ -780,7 +790,7 @@ __global__ __launch_bounds__(kRowWaves * kWave, 2) void paged_rows_kernel(const 
   if (top == -INFINITY && sum != sum) top = 0.f;  // as above
   if (r0 + 32 * wave + n >= rows) return;
   const bool empty = top == -INFINITY || t >= row.count;
-  const long to = (long(work.group) * a.most + work.part) * rows + r;
+  const long to = long(work.slot) * rows + r;
   if (h == 0) {
     if (work.parts > 1)
       a.pmax[to] = top, a.psum[to] = sum;
@@ -821,10 +831,16 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedArgs a) {
   const PagedRow row = paged_row(a, b);
   const int parts = parts_of(a, row);
   if (parts == 1) return;  // written already
+  int more = 0;  // slot of the row's first part beyond `splits`, less that part's number
+  if (parts > a.splits)
+    more = a.groups * a.splits + min(more_before(a, b) + hk * (parts - a.splits), a.more - (parts - a.splits)) - a.splits;
   const int t = r >> a.group_log2, head = (hk << a.group_log2) + (r & (G - 1));
   float top = -INFINITY, den = 0.f, num[DPL] = {};
   for (int s0 = kShared ? wave * kRound : 0; s0 < parts; s0 += kRound * W) {
-    const auto part = [&](int s) { return (long(group) * a.most + min(s0 + s, parts - 1)) * rows + r; };
+    const auto part = [&](int s) {
+      const int x = min(s0 + s, parts - 1);
+      return long(x < a.splits ? group * a.splits + x : more + x) * rows + r;
+    };
     const bool on = lane < kRound && s0 + lane < parts;
     const float high = a.pmax[part(lane % kRound)], sum = a.psum[part(lane % kRound)];
     float x[kRound][DPL];

@@ -223,7 +223,7 @@ def launch_page_attention(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch
                           v_scale: torch.Tensor, tables: torch.Tensor, lengths: torch.Tensor,
                           counts: torch.Tensor | None, partial_max: torch.Tensor, partial_sum: torch.Tensor,
                           partial_output: torch.Tensor, out: torch.Tensor, lse: torch.Tensor, layer: int,
-                          window_left: int, splits: int, scale: float) -> None:
+                          window_left: int, splits: int, most_splits: int, scale: float) -> None:
     """Attention of new tokens over one layer's pages into ``out`` and ``lse`` (``sfl_page_attention``)."""
     batch, heads, tokens, dim = q.shape
     pages, kv_heads, page_size = k_codes.shape[1:4]
@@ -232,7 +232,7 @@ def launch_page_attention(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch
           k_scale.data_ptr() + scales, v_scale.data_ptr() + scales, tables.data_ptr(), lengths.data_ptr(), _ptr(counts),
           partial_max.data_ptr(), partial_sum.data_ptr(), partial_output.data_ptr(), out.data_ptr(), lse.data_ptr(),
           _strides_2(*q.stride()[:3], *out.stride()[:3]), batch, heads, kv_heads, tokens, tables.shape[1], pages,
-          page_size, dim, window_left, splits, max(splits, partial_max.shape[3]), scale, _lib.dtype_code(q.dtype))
+          page_size, dim, window_left, splits, most_splits, scale, _lib.dtype_code(q.dtype))
 
 
 def launch_page_fork(parents: torch.Tensor, tables: torch.Tensor, lengths: torch.Tensor, refs: torch.Tensor,

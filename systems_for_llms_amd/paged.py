@@ -285,6 +285,7 @@ class PreparedPaged:
     layer: int
     window_left: int
     splits: int
+    most_splits: int
     scale: float
 
     def __call__(self) -> torch.Tensor:
@@ -293,7 +294,7 @@ class PreparedPaged:
         written = (self.partial_max, self.partial_sum, self.partial_output, self.output, self.lse)
         ops.dispatch(torch.ops.sfl.page_attention,
                      (self.q, c.k, c.v, c.k_scale, c.v_scale, c.tables, c.lengths, self.counts, *written), written,
-                     self.layer, self.window_left, self.splits, self.scale, checked=True)
+                     self.layer, self.window_left, self.splits, self.most_splits, self.scale, checked=True)
         return self.output
 
     @property
@@ -337,17 +338,20 @@ def prepare(q, cache, *, layer=0, counts=None, window_left=None, splits=None, sc
         raise ValueError("scale must be finite and positive")
     _cache.check_device(index)
     _lib.lib()  # fail here, before allocation, if the library is not built
-    most = splits
+    most, group_rows = splits, tokens * (heads // kv_heads)
     if splits is None:
-        size = batch, kv_heads, cache.capacity, tokens * (heads // kv_heads), dim, q.dtype, window_left
+        size = batch, kv_heads, cache.capacity, group_rows, dim, q.dtype, window_left
         splits = auto_splits(*size)
         most = auto_most_splits(splits, *size)
     window = -1 if window_left is None else min(window_left, cache.capacity)
-    maximum = torch.empty((batch, heads, tokens, most if most > 1 else 0), device=q.device, dtype=torch.float32)
-    numerator = torch.empty((*maximum.shape, dim), device=q.device, dtype=torch.float32)
+    parts = batch * heads * tokens * splits if most > 1 else 0
+    if most > splits:
+        parts += 256 * (128 if group_rows > 64 else 32) + group_rows
+    maximum = torch.empty(parts, device=q.device, dtype=torch.float32)
+    numerator = torch.empty((parts, dim), device=q.device, dtype=torch.float32)
     lse = torch.empty((batch, heads, tokens), device=q.device, dtype=torch.float32)
     return PreparedPaged(q, cache, counts, maximum, torch.empty_like(maximum), numerator, torch.empty_like(q), lse,
-                         layer, window, splits, float(scale))
+                         layer, window, splits, most, float(scale))
 
 
 def attend(q, cache, *, layer=0, counts=None, window_left=None, splits=None, scale=None):

@@ -813,7 +813,7 @@ def test_attention_of_few_long_rows_among_short_ones(dtype, dim, group, heads, t
         counts[list(at)] = tokens
         q = randn(g, batch, heads * group, tokens, dim, dtype=dtype)
         op = paged.prepare(q.cuda(), cache, counts=counts.cuda())
-        assert op.partial_max.shape[3] > op.splits
+        assert op.most_splits > op.splits
         check(q, state, got=(op(), op.lse), counts=counts)
         again = op().clone()
         # The same operation after the long row has ended and another has grown.
@@ -836,8 +836,13 @@ def test_attention_with_room_for_more_parts(dtype, dim, group, tokens, page, spl
     q = randn(g, 6, 2 * group, tokens, dim, dtype=dtype)
     for window in (None, 333):
         op = paged.prepare(q.cuda(), on_gpu(state), counts=counts.cuda(), window_left=window, splits=splits)
-        op.partial_max = torch.full((*q.shape[:3], most), float("nan"), device="cuda")
+        op.most_splits = most
+        rows = tokens * group
+        parts = 12 * rows * splits + 256 * (128 if rows > 64 else 32) + rows
+        # Nothing is read that no part has written, nothing written behind the last of them.
+        op.partial_max = torch.full((parts + 64,), float("nan"), device="cuda")
         op.partial_sum = torch.full_like(op.partial_max, float("nan"))
-        op.partial_output = torch.full((*op.partial_max.shape, dim), float("nan"), device="cuda")
+        op.partial_output = torch.full((parts + 64, dim), float("nan"), device="cuda")
         op.output.fill_(float("nan"))
         check(q, state, got=(op(), op.lse), counts=counts, window=window)
+        assert all(bool(x[parts:].isnan().all()) for x in (op.partial_max, op.partial_sum, op.partial_output))

@@ -133,7 +133,7 @@ def test_schemas_and_meta_dispatch():
     torch.ops.sfl.page_append(new, new, m.tables, m.lengths, None, m.refs, m.k, m.v, m.k_scale, m.v_scale, 0)
     torch.ops.sfl.page_attention(q, m.k, m.v, m.k_scale, m.v_scale, m.tables, m.lengths, n, f, f.clone(),
                                  torch.empty(2, 4, 3, 2, 64, device="meta"), torch.empty_like(q),
-                                 torch.empty(2, 4, 3, device="meta"), 0, -1, 2, 0.125)
+                                 torch.empty(2, 4, 3, device="meta"), 0, -1, 2, 2, 0.125)
     torch.ops.sfl.page_fork(n, m.tables, m.lengths, m.refs, 16)
 
 
