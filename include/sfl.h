@@ -518,11 +518,8 @@ int sfl_rotate(const void* q, const void* k, const void* v, const int32_t* posit
  * in its row, whatever their rows hold.
  *   q, out [batch, q_heads, tokens] rows, Hq/Hkv in {1, 2, 4, 8}
  *   mask   uint8, strides {batch, t, j} (0 for a shared one); counts [batch] or NULL
- *   splits: parts that each KV head's slots are read in, side by side. most_splits >= splits:
- *   those of sequences that hold far more than their share of the batch's slots
- *   partial_max, partial_sum  batch * q_heads * tokens * splits fp32 values, and with most_splits >
- *   splits 256 * (32, or 128 of more than 64 rows) + rows more, rows = tokens * q_heads / kv_heads;
- *   partial_out head_dim times as many: scratch, unused (may be NULL) with most_splits == 1
+ *   partial_max, partial_sum  batch * q_heads * tokens * splits fp32 values, partial_out
+ *   head_dim times as many: scratch, unused (may be NULL) with splits == 1
  *   strides [15]: q, k, v, out, mask. q, k, v, out 16-byte aligned, their strides
  *   multiples of 16 bytes
  * Every sum in fp32. Results do not vary from call to call.
@@ -626,8 +623,11 @@ int sfl_page_append(const void* k, const void* v, void* k_codes, void* v_codes, 
  * lies past counts[b] or has no slot has a zero row and lse -inf. What a token does not see
  * has no part in its row, NaN codes included.
  *   q, out [batch, q_heads, tokens] rows of dtype, Hq/Hkv in {1, 2, 4, 8}
- *   partial_max, partial_sum  batch * q_heads * tokens * splits fp32 values, partial_out
- *   head_dim times as many: scratch, unused (may be NULL) with splits == 1
+ *   splits: parts that each KV head's slots are read in, side by side. most_splits >= splits:
+ *   those of sequences that hold far more than their share of the batch's slots
+ *   partial_max, partial_sum  batch * q_heads * tokens * splits fp32 values, and with most_splits >
+ *   splits 256 * (32, or 128 of more than 64 rows) + rows more, rows = tokens * q_heads / kv_heads;
+ *   partial_out head_dim times as many: scratch, unused (may be NULL) with most_splits == 1
  *   strides [6]: q, out {batch, head, token}, multiples of 16 bytes
  * Every sum in fp32. Results do not vary from call to call.
  */
