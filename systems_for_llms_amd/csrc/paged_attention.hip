@@ -9,8 +9,11 @@
 //
 // in one pass over the pages, m and l running. Codes become bf16, exactly (four bits and a
 // power of two), on their way into the matrix cores; what has more bits goes in as a sum of
-// bf16 pieces: q and the probabilities of fp16 as two, of fp32 as three, so the only
-// roundings are those of the probabilities to the sum of their pieces and of fp32 sums.
+// bf16 pieces: q of fp16 as two, of fp32 as three, and the probabilities of 16-bit rows as two,
+// of fp32 as three, so the only roundings are those of the probabilities to the sum of their
+// pieces (2^-16 or 2^-24 of them) and of fp32 sums. bf16 rows beyond 32 to a KV head have
+// one piece (2^-8): there the matrix cores are what a second one waits for, see
+// paged_attention_kernel.
 #include <algorithm>
 #include <type_traits>
 
@@ -311,12 +314,17 @@ __device__ __forceinline__ u32x4 load_v(const uint8_t* at) {
 // Both ways measured, us at those two: values past the caches 58, 57 and through them 63, 52
 // (pages of 64, pages of 128); both tiles' values ahead 58, 57; 4, 6, 8 and 12 waves 57, 56,
 // 56, 56 at their best splits, 8 for one short row (11 us for 1024 keys, where two splits and
-// their merge take 13.5); three waves a SIMD instead of two 60.
+// their merge take 13.5); three waves a SIMD instead of two 60. Probabilities of bf16 rows as
+// one piece and as two: 16 rows (NC 1) 54.9 / 55.6, 52.4 / 52.6 (16 of up to 16000 tokens),
+// 12.0 / 12.0 (1024 keys), so two; 32 rows (NC 2) 64 rows over 8 x 8000 39.3 / 45.2, 40 of 64
+// dims 25.5 / 28.3, and paged_rows_kernel 108 over 8 of 1K to 8K 44.4 / 52.6, 512 over 32000
+// 93.8 / 116.5, so one there, as in the framework's other bf16 attention.
 template <typename T, int D, int NC, int kPage, int W>
 __global__ __launch_bounds__(W * kWave, D == 128 && NC == 2 ? 1 : 2) void paged_attention_kernel(const PagedArgs a) {
   using L = Tile<D>;
   constexpr bool kWide = kPage >= kPagedTile;
   constexpr int P = pieces_of<T>(), BT = kPagedTile, kRows = 16 * NC, kLine = D + 4;
+  constexpr int kProb = NC == 1 ? std::max(P, 2) : P;  // pieces of the probabilities
   __shared__ float merged[W][kRows][kLine];
   __shared__ float tops[W][kRows], sums[W][kRows];
   const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave);
@@ -430,7 +438,7 @@ __global__ __launch_bounds__(W * kWave, D == 128 && NC == 2 ? 1 : 2) void paged_
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[c][e / 4][e % 4] = sees(c, slot0 + off_v + e, spot) ? s[c][e / 4][e % 4] : -INFINITY;
     }
-    u32x4 prob[NC][2][P];
+    u32x4 prob[NC][2][kProb];
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       float high = s[c][0][0];
@@ -485,7 +493,7 @@ __global__ __launch_bounds__(W * kWave, D == 128 && NC == 2 ? 1 : 2) void paged_
 #pragma unroll
         for (int c = 0; c < NC; ++c)
 #pragma unroll
-          for (int p = P - 1; p >= 0; --p) o[c][d] = mfma16(value, prob[c][h][p], o[c][d]);
+          for (int p = kProb - 1; p >= 0; --p) o[c][d] = mfma16(value, prob[c][h][p], o[c][d]);
       }
   }
   if (found) {

@@ -312,9 +312,11 @@ def prepare(q, cache, *, layer=0, counts=None, window_left=None, splits=None, sc
     ``lse`` (fp32 ``[B, Hq, T]``) of -inf, as are those of tokens that see nothing or have no slot. What
     a token does not see has no part in its row, NaN included. Scores and sums are fp32, and
     no code is rounded again: probabilities, of up to 2^8 before the division by their sum, are rounded
-    to bf16 for bf16 ``q``, to two such pieces for fp16, three for fp32. ``splits``: workgroups that share a KV head's slots, 1 to
-    128; by default as many as the sizes ask for, and more for sequences far longer than the others. Like ``tree.PreparedTree`` the operation owns its scratch and output
-    and holds its inputs by reference; concurrent calls on one race.
+    to two bf16 pieces (off by 2^-16) for 16-bit ``q``, three for fp32, and to one (2^-8) for bf16 ``q``
+    of 64 or 128 dims with more than 32 rows to a KV head (T times Hq / Hkv). ``splits``: workgroups
+    that share a KV head's slots, 1 to 128; by default as many as the sizes ask for, and more for
+    sequences far longer than the others. Like ``tree.PreparedTree`` the operation owns its scratch
+    and output and holds its inputs by reference; concurrent calls on one race.
     """
     if splits is not None and (type(splits) is not int or not 1 <= splits <= MAX_SPLITS):
         raise ValueError("splits must be an integer in [1, 128]")

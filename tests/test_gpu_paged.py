@@ -3,7 +3,7 @@
 Codes, scales and books are equal bit for bit. Error bounds of the attention count what
 the kernels do: a stored result is rounded once, by half a step (``finfo.eps / 2`` of the
 value); codes become bf16 exactly; probabilities go into the products with V as sums of one
-(bf16), two (fp16) or three (fp32) bf16 pieces, off by 2^-8, 2^-16 or 2^-24 of p |v|; scores
+(bf16: two up to 32 rows), two (fp16) or three (fp32) bf16 pieces, off by 2^-8, 2^-16 or 2^-24 of p |v|; scores
 are fp32 sums of as many times D products, off by at most (pieces D + 8) 2^-24 of sum |q k|
 and a few roundings of the scaled value, which enter exp as a relative error; sums over n
 keys are off by at most n 2^-24 of sum |terms|.
@@ -846,3 +846,22 @@ def test_attention_with_room_for_more_parts(dtype, dim, group, tokens, page, spl
         op.output.fill_(float("nan"))
         check(q, state, got=(op(), op.lse), counts=counts, window=window)
         assert all(bool(x[parts:].isnan().all()) for x in (op.partial_max, op.partial_sum, op.partial_output))
+
+
+@pytest.mark.parametrize("dim", [16, 32, 64, 128])
+@pytest.mark.parametrize("tokens, group", [(1, 1), (1, 8), (4, 8)])
+def test_bf16_attention_loses_no_more_than_its_result_s_rounding(dim, tokens, group):
+    """Probabilities of up to 32 bf16 rows as two pieces: off by 2^-16 of p |v|, where one piece is off by 2^-8. Few
+    keys, and elements of results near zero among them, so that one piece shows beside the result's own half step."""
+    from systems_for_llms_amd import paged
+
+    g = torch.Generator().manual_seed(dim + tokens + group)
+    state = random_cache(g, [1, 3, 7, 30, 90], 2, dim, 64, room=tokens)
+    q = randn(g, 5, 2 * group, tokens, dim, dtype=BF16)
+    out, lse, spread, size = op_.attention(q, state)
+    keys = 90 + tokens
+    ds = (dim + 8) * U * size + 6 * U * (size + lse.abs()) + 4 * U
+    bound = 2.0 ** -8 * out.abs() + 1e-38 + spread * (2.0 ** -16 + 2 * ds + 2 * (2 * keys + 8) * U)[..., None]
+    cache = on_gpu(state)
+    for splits in (1, 3):
+        within(paged.attend(q.cuda(), cache, splits=splits)[0], out, bound * 1.01, "out")
