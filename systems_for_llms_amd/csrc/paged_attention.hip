@@ -28,7 +28,7 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kPagedTile = 64;  // keys of a wave's tile
 constexpr int kMaxTokens = 128;
-constexpr int kRowWaves = 4;    // of the kernel for many rows
+constexpr int kRowWaves = 4;    // of the kernels for blocks of 32 and more rows
 constexpr int kAtOnce = 256;    // workgroups that a call in need of more parts aims at
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -902,7 +902,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedArgs a) {
     a.lse[(long(b) * a.kv_heads * G + head) * a.tokens + t] = empty ? -INFINITY : (top + __builtin_log2f(den)) * kLn2;
 }
 
-constexpr long kMostGroups = 1L << 24;  // a launch holds fewer than 2^32 threads
+constexpr long kMostThreads = 1L << 32;  // a launch holds fewer
 
 template <typename T, int D>
 int launch_paged(PagedArgs& a, hipStream_t stream) {
@@ -917,24 +917,25 @@ int launch_paged(PagedArgs& a, hipStream_t stream) {
   // 39.4, D 64 8 x 4000 128 rows 34.1 / 37.2; D 32 8 x 4000 128 rows 17.7 / 21.1.
   constexpr bool kPairs = pieces_of<T>() == 1 && D >= 64, kShares = pieces_of<T>() < 3 && D >= 64;
   const int block = rows > 64 && kShares ? 128 : rows > 32 && kPairs ? 32 : 16;
+  const int threads = (block == 16 ? 8 : kRowWaves) * kWave;  // kernels below
   a.row_blocks = (rows + block - 1) / block;
   a.share = float(a.kv_heads) * a.row_blocks / kAtOnce;
   // Sequences of more than `splits` parts have together fewer parts than kAtOnce / row_blocks.
   a.more = a.most > a.splits ? kAtOnce / a.row_blocks + 1 : 0;
   const long units = (long(a.groups) * a.splits + a.more + kXcds - 1) / kXcds * kXcds;
   const long merged = long(a.groups) * rows;
-  if (units * a.row_blocks >= kMostGroups || merged >= kMostGroups - 1)
+  if (units * a.row_blocks * threads >= kMostThreads || (merged + 3) * 256 >= kMostThreads)
     return set_error(SFL_ERR_UNSUPPORTED, "%s: too many workgroups", what);
-  const auto launch = [&](auto kernel, int waves) {
-    hipLaunchKernelGGL(kernel, dim3(unsigned(units * a.row_blocks)), dim3(unsigned(waves * kWave)), 0, stream, a);
+  const auto launch = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(unsigned(units * a.row_blocks)), dim3(unsigned(threads)), 0, stream, a);
   };
   const auto run = [&](auto page) {
     constexpr int kPage = decltype(page)::value;
     if constexpr (kShares)
-      if (block == 128) return launch(paged_rows_kernel<T, D, kPage>, kRowWaves);
+      if (block == 128) return launch(paged_rows_kernel<T, D, kPage>);
     if constexpr (kPairs)
-      if (block == 32) return launch(paged_attention_kernel<T, D, 2, kPage, 4>, 4);
-    launch(paged_attention_kernel<T, D, 1, kPage, 8>, 8);
+      if (block == 32) return launch(paged_attention_kernel<T, D, 2, kPage, kRowWaves>);
+    launch(paged_attention_kernel<T, D, 1, kPage, 8>);
   };
   if (a.page_log2 == 7) run(std::integral_constant<int, 128>{});
   else if (a.page_log2 == 6) run(std::integral_constant<int, 64>{});

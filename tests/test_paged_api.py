@@ -275,3 +275,21 @@ def test_most_splits_bounds():
                 most = paged.auto_most_splits(splits, *size)
                 # No sequence can need more: the further workgroups are 256, a block of a head's rows each.
                 assert splits <= most <= 64
+
+
+def test_attention_of_more_threads_than_a_launch_holds_is_refused():
+    """2^23 workgroups of 512 threads, and as many of the kernels of 256 threads as reach 2^32."""
+    if not _lib.LIB_PATH.exists():
+        pytest.skip("libsfl.so not built")
+
+    def status(batch, heads, kv_heads, tokens, dim, splits, dtype):
+        strides = (ctypes.c_long * 6)(*[64] * 6)
+        return _status("sfl_page_attention", *[64] * 13, strides, batch, heads, kv_heads, tokens, 4, 9, 16, dim, -1, splits,
+                       splits, 0.125, dtype, None)
+
+    fp32, bf16, fp16 = 0, 1, 2
+    assert status(1024, 64, 64, 1, 64, 128, bf16) == UNSUPPORTED      # 2^23 of 8 waves
+    assert status(1024, 64, 64, 1, 64, 128, fp32) == UNSUPPORTED
+    assert status(512, 128, 16, 128, 64, 16, fp32) == UNSUPPORTED     # 64 blocks of rows
+    assert status(1024, 128, 64, 20, 128, 128, bf16) == UNSUPPORTED   # 2^24 of 4 waves, blocks of 32 rows
+    assert status(1024, 64, 64, 128, 128, 256, fp16) == UNSUPPORTED   # 2^24 of 4 waves, blocks of 128 rows
