@@ -172,12 +172,43 @@ __global__ __launch_bounds__(1024) void append_kernel(const AppendArgs a) {
   }
 }
 
+// Bytes from the first to past the last one of a tensor.
+struct Extent {
+  uintptr_t from, to;
+};
+Extent extent_of(const void* p, long bytes, long before = 0) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+  return {at - uintptr_t(before), at + uintptr_t(bytes)};
+}
+
+// Whether what is read while pages are written lies apart from them.
+bool apart(const AppendArgs& a, int batch, int dim, int element) {
+  const int sizes[3] = {batch, a.kv_heads, a.tokens};
+  Extent read[3] = {{}, {}, extent_of(a.counts, a.counts ? 4L * batch : 0)};
+  for (int x = 0; x < 2; ++x) {
+    long high = dim, low = 0;
+    for (int i = 0; i < 3; ++i) {
+      const long step = (sizes[i] - 1) * a.st[x][i];
+      high += std::max(step, 0L), low -= std::min(step, 0L);
+    }
+    read[x] = extent_of(x ? a.v : a.k, high * element, low * element);
+  }
+  const long heads = long(a.pages) * a.kv_heads, pool = (heads << a.page_log2) * dim;
+  for (const Extent& y : {extent_of(a.k_codes, pool), extent_of(a.v_codes, pool), extent_of(a.k_scale, 4 * heads),
+                          extent_of(a.v_scale, 4 * heads)})
+    for (const Extent& x : read)
+      if (x.from < y.to && y.from < x.to) return false;
+  return true;
+}
+
 template <typename T, int D>
 int launch_append(const AppendArgs& a, int batch, hipStream_t stream) {
   const long blocks = 2L * batch * a.reach * a.kv_heads;
   const int page = 1 << a.page_log2;
   const int threads = std::max(kWave, page / 4 * (D / vec_elems<T>()));  // at most 1024
   if (blocks * threads >= (1L << 32)) return set_error(SFL_ERR_UNSUPPORTED, "page_append: too many workgroups");
+  if (!apart(a, batch, D, sizeof(T)))
+    return set_error(SFL_ERR_INVALID, "page_append: k, v and counts must not share memory with the layer's pages");
   hipLaunchKernelGGL((append_kernel<T, D>), dim3(unsigned(blocks)), dim3(unsigned(threads)), unsigned(D * (page + 4)), stream, a);
   return check_launch("page_append");
 }

@@ -216,7 +216,7 @@ def append(cache, k, v, *, layer=0, counts=None) -> None:
     the least power of two (from 2^-100 on) under which the new values fit codes of up to 448;
     where the page holds committed tokens it does not become smaller, and where it grows their
     codes are rounded again under the new one. Infinities, NaN and magnitudes from 2^127 on
-    become NaN.
+    become NaN. Tokens and counts must not share memory with the pages and scales of the layer.
     """
     index = _check_cache("append", cache)
     if _cache.check_rows("append", ("k", "v"), (k, v)) != index:

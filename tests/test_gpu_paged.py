@@ -865,3 +865,18 @@ def test_bf16_attention_loses_no_more_than_its_result_s_rounding(dim, tokens, gr
     cache = on_gpu(state)
     for splits in (1, 3):
         within(paged.attend(q.cuda(), cache, splits=splits)[0], out, bound * 1.01, "out")
+
+
+def test_append_of_views_of_the_pool_is_refused():
+    from systems_for_llms_amd import paged
+
+    cache = paged.create(2, 64, 2, 64, 9, layers=2, page_size=16)
+    new = torch.zeros(2, 2, 4, 64, dtype=BF16, device="cuda")
+    inside = cache.v[0].view(torch.uint8).flatten().view(BF16)[1024:2048].view(2, 2, 4, 64)
+    for k, v in ((inside, new), (new, inside)):
+        with pytest.raises(RuntimeError, match="share memory"):
+            paged.append(cache, k, v)
+        paged.append(cache, k, v, layer=1)  # the other layer's pages are not read
+    with pytest.raises(RuntimeError, match="share memory"):
+        paged.append(cache, new, new, counts=cache.k_scale.view(torch.int32).flatten()[3:5])
+    paged.append(cache, new, new, counts=cache.lengths)

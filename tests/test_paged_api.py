@@ -293,3 +293,33 @@ def test_attention_of_more_threads_than_a_launch_holds_is_refused():
     assert status(512, 128, 16, 128, 64, 16, fp32) == UNSUPPORTED     # 64 blocks of rows
     assert status(1024, 128, 64, 20, 128, 128, bf16) == UNSUPPORTED   # 2^24 of 4 waves, blocks of 32 rows
     assert status(1024, 64, 64, 128, 128, 256, fp16) == UNSUPPORTED   # 2^24 of 4 waves, blocks of 128 rows
+
+
+def test_append_from_the_memory_that_it_writes_is_refused():
+    """Tokens or counts that overlap the layer's pages or scales; those beside them are not."""
+    if not _lib.LIB_PATH.exists():
+        pytest.skip("libsfl.so not built")
+    if torch.cuda.is_available():
+        pytest.skip("calls that are not refused here must not reach a GPU: their addresses are none")
+    page, heads, dim, pages, batch, tokens = 16, 2, 64, 9, 3, 5
+    pool, scales, row, lane = pages * heads * page * dim, 4 * pages * heads, 2 * dim, 2 * dim * heads
+    base = 1 << 20
+    at = dict(k_codes=base, v_codes=2 * base, k_scale=3 * base, v_scale=4 * base, k=5 * base, v=6 * base, counts=7 * base)
+    size = 2 * ((batch * tokens * heads - 1) * dim + dim)  # tokens as a projection leaves them: [B, T, H, D]
+
+    def refused(**moved):
+        x = {**at, **moved}
+        strides = (ctypes.c_long * 6)(*[lane // 2 * tokens, dim, lane // 2] * 2)
+        status = _status("sfl_page_append", x["k"], x["v"], x["k_codes"], x["v_codes"], x["k_scale"], x["v_scale"], 64, 64,
+                         x["counts"], 64, strides, batch, heads, tokens, 4, pages, page, dim, 1, None)
+        return status == INVALID and b"share memory" in _lib.lib().sfl_last_error()
+
+    for name, extent in (("k_codes", pool), ("v_codes", pool), ("k_scale", scales), ("v_scale", scales)):
+        for new in ("k", "v"):
+            assert refused(**{new: at[name]}) and refused(**{new: at[name] + (extent - 1) // 16 * 16})
+            assert refused(**{new: at[name] - size + 16})
+        assert refused(counts=at[name]) and refused(counts=at[name] + extent - 4) and refused(counts=at[name] - 4 * batch + 4)
+    for name, extent in (("k_codes", pool), ("v_scale", scales)):  # these end with the launch that fails without a GPU
+        assert not refused(k=at[name] + -(-extent // 16) * 16) and not refused(v=at[name] - size)
+        assert not refused(counts=at[name] + extent) and not refused(counts=at[name] - 4 * batch)
+    assert not refused() and not refused(counts=None)
