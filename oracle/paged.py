@@ -52,7 +52,7 @@ def append(cache, k, v, counts=None, layer=0):
                         codes = codes.T
                     scale = done[name + "_scale"][layer, at, h]
                     if lo:
-                        before = int(torch.frexp(scale)[1]) - 1
+                        before = max(int(torch.frexp(scale)[1]) - 1, LEAST) if scale else LEAST
                         if e > before:
                             codes[:lo] = nearest_code(codes[:lo] * 2.0 ** (before - e))
                         e = max(e, before)

@@ -880,3 +880,24 @@ def test_append_of_views_of_the_pool_is_refused():
     with pytest.raises(RuntimeError, match="share memory"):
         paged.append(cache, new, new, counts=cache.k_scale.view(torch.int32).flatten()[3:5])
     paged.append(cache, new, new, counts=cache.lengths)
+
+
+@pytest.mark.parametrize("page", [16, 64])
+def test_append_behind_tokens_of_a_page_that_was_never_written(page):
+    """Lengths set by hand over reserved pages: their scales are 0, their codes zeros, and stay so."""
+    from systems_for_llms_amd import paged
+
+    g = torch.Generator().manual_seed(page)
+    cache = paged.create(3, 4 * page, 2, 32, 12, page_size=page)
+    state = {n: getattr(cache, n).cpu() for n in NAMES}
+    counts = torch.tensor([9, page + 3, 2 * page], dtype=torch.int32)
+    granted, state = op_.reserve(state, counts)
+    assert torch.equal(paged.reserve(cache, counts.cuda()).cpu(), granted)
+    state["lengths"] = torch.tensor([5, page + 1, page - 1], dtype=torch.int32)
+    cache.lengths.copy_(state["lengths"])
+    for size in (2.0 ** -20, 2.0 ** -24, 1.0):
+        k, v = (randn(g, 3, 2, 4, 32, dtype=FP32, scale=size) for _ in range(2))
+        paged.append(cache, k.cuda(), v.cuda())
+        state = op_.append(state, k, v)
+        same_cache(cache, state)
+        check(randn(g, 3, 4, 4, 32, dtype=FP32), state, cache=cache)

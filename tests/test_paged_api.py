@@ -323,3 +323,15 @@ def test_append_from_the_memory_that_it_writes_is_refused():
         assert not refused(k=at[name] + -(-extent // 16) * 16) and not refused(v=at[name] - size)
         assert not refused(counts=at[name] + extent) and not refused(counts=at[name] - 4 * batch)
     assert not refused() and not refused(counts=None)
+
+
+def test_a_page_that_was_never_written_holds_no_scale():
+    """Behind committed tokens of a page whose scale is still 0 the new tokens alone choose it."""
+    cache = paged.create(1, 48, 1, 16, 3, page_size=16, device="cpu")
+    state = {n: getattr(cache, n) for n in ("k", "v", "k_scale", "v_scale", "tables", "lengths", "refs")}
+    _, state = op_.reserve(state, torch.tensor([20]))
+    state["lengths"] = torch.tensor([5], dtype=torch.int32)
+    new = torch.full((1, 1, 3, 16), 2.0 ** -20)
+    done = op_.append(state, new, 4 * new)
+    assert done["k_scale"][0, 0, 0] == 2.0 ** -28 and done["v_scale"][0, 0, 0] == 2.0 ** -26
+    assert torch.equal(done["k"][0, 0, 0, 5:8].float(), torch.full((3, 16), 256.0)) and not done["k"][0, 0, 0, :5].float().any()
