@@ -901,3 +901,76 @@ def test_append_behind_tokens_of_a_page_that_was_never_written(page):
         state = op_.append(state, k, v)
         same_cache(cache, state)
         check(randn(g, 3, 4, 4, 32, dtype=FP32), state, cache=cache)
+
+
+def given_and_held(state, b, layer, given):
+    """Whether a row's committed keys and values are those that were appended, as far as codes can hold them: off by
+    2^-4 of a value (half a step of a normal code) and by less than 2^-9 of its page's scale: half a step of the
+    smallest codes, 2^-10, under the present scale and under each one before it, which was at most half the next."""
+    page, n = state["k"].shape[3], len(given[0])
+    at = [int(state["tables"][b, s // page]) for s in range(n)]
+    for got, new, name in zip(op_.rows_of(state, b, range(n), layer), given, ("k_scale", "v_scale")):
+        want = torch.stack(new, 1).double()
+        unit = state[name][layer][at].T.double()[..., None]
+        if bool(((got - want).abs() > 2.0 ** -4 * want.abs() + 2.0 ** -9 * unit).any()):
+            return False
+    return True
+
+
+@pytest.mark.parametrize("dtype, page, pages, size", [(BF16, 16, 200, 1.0), (FP16, 32, 90, 1.0), (BF16, 64, 40, 8.0), (FP32, 16, 30, 8.0)])
+def test_serving_loop_beside_the_lists(dtype, page, pages, size):
+    """The loop of all calls on the device and, step by step, on the list forms: books, codes and scales the same,
+    attention within the counted bounds, and what the rows hold is what they were given."""
+    from systems_for_llms_amd import paged
+
+    g = torch.Generator().manual_seed(page + pages)
+    batch, kv, heads, dim, layers = 6, 2, 4, 32, 2
+    cache = paged.create(batch, 300, kv, dim, pages, layers=layers, page_size=page)
+    state = {n: getattr(cache, n).cpu() for n in NAMES}
+    given = [[([], []) for _ in range(layers)] for _ in range(batch)]
+    rows = longest = 0
+    for step in range(20):
+        parents = torch.arange(batch)
+        if step:
+            move = torch.rand(batch, generator=g)
+            parents = torch.where(move < 0.1, -1, torch.where(move < 0.35, torch.randint(0, batch, (batch,), generator=g), parents))
+        parents = parents.to(torch.int32)
+        paged.fork(cache, parents.cuda())
+        state = op_.fork(state, parents)
+        given = [[tuple(list(x) for x in layer) for layer in given[p]] if p >= 0 else [([], []) for _ in range(layers)]
+                 for p in parents.tolist()]
+        tokens = 40 if step % 5 == 0 else 1 + step % 4
+        wish = torch.randint(1, tokens + 1, (batch,), generator=g).to(torch.int32)
+        granted, (want, state) = paged.reserve(cache, wish.cuda()), op_.reserve(state, wish)
+        assert torch.equal(granted.cpu(), want)
+        accepted = torch.minimum(want, torch.randint(1, tokens + 1, (batch,), generator=g).to(torch.int32))
+        for layer in range(layers):
+            k, v = (randn(g, batch, kv, tokens, dim, dtype=dtype, scale=size ** float(torch.randn((), generator=g))) for _ in range(2))
+            q = randn(g, batch, heads, tokens, dim, dtype=dtype)
+            paged.append(cache, k.cuda(), v.cuda(), layer=layer, counts=granted)
+            state = op_.append(state, k, v, want, layer)
+            check(q, state, cache=cache, counts=want, layer=layer)
+            for b in range(batch):
+                for held, new in zip(given[b][layer], (k, v)):
+                    held.extend(new[b, :, : accepted[b]].unbind(1))
+        cache.lengths += accepted.cuda()
+        state["lengths"] = state["lengths"] + accepted
+        if step % 7 == 6:
+            used, (live, state) = paged.compact(cache), op_.compact(state)
+            assert used.tolist() == [live]
+        same_cache(cache, state)
+        for b in range(batch):
+            n = int(state["lengths"][b])
+            assert all(len(given[b][layer][0]) == n for layer in range(layers))
+            if n:
+                assert all(given_and_held(state, b, layer, given[b][layer]) for layer in range(layers))
+                rows, longest = rows + 1, max(longest, n)
+    assert rows > 90 and longest > page, (rows, longest)
+    # What the comparison is for: a page of another place, one of zeros, and codes under another scale are seen.
+    b = max(range(batch), key=lambda r: int(state["lengths"][r]))
+    first, second = state["tables"][b, :2].tolist()
+    for change in (lambda x: x["k"][0].__setitem__(first, x["k"][0, second].clone()),
+                   lambda x: x["v"].view(torch.uint8)[0, first].zero_(), lambda x: x["v_scale"][0, second].mul_(2)):
+        wrong = {n: x.clone() for n, x in state.items()}
+        change(wrong)
+        assert not given_and_held(wrong, b, 0, given[b][0])
