@@ -215,7 +215,7 @@ def append(cache, k, v, *, layer=0, counts=None) -> None:
     rows hold, are left out: ``reserve`` comes first. For each page and head the scale becomes
     the least power of two (from 2^-100 on) under which the new values fit codes of up to 448;
     where the page holds committed tokens it does not become smaller, and where it grows their
-    codes are rounded again under the new one. Infinities, NaN and magnitudes from 2^127 on
+    codes are rounded again under the new one, which stays if the new tokens are rejected. Infinities, NaN and magnitudes from 2^127 on
     become NaN. Tokens and counts must not share memory with the pages and scales of the layer.
     """
     index = _check_cache("append", cache)

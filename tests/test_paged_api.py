@@ -335,3 +335,30 @@ def test_a_page_that_was_never_written_holds_no_scale():
     done = op_.append(state, new, 4 * new)
     assert done["k_scale"][0, 0, 0] == 2.0 ** -28 and done["v_scale"][0, 0, 0] == 2.0 ** -26
     assert torch.equal(done["k"][0, 0, 0, 5:8].float(), torch.full((3, 16), 256.0)) and not done["k"][0, 0, 0, :5].float().any()
+
+
+def test_what_codes_hold_of_the_values_that_were_appended():
+    """Off by 2^-4 of the value or 2^-10 of the scale under the scale they were appended with; where it grew afterwards,
+    by 2^-4 of the value and less than 2^-9 of the scale: each rounding of a small code adds 2^-10 of a scale at most half the next."""
+    g = torch.Generator().manual_seed(3)
+    worst = 0.0
+    for trial in range(60):
+        cache = paged.create(1, 32, 1, 32, 1, page_size=32, device="cpu")
+        state = {n: getattr(cache, n) for n in ("k", "v", "k_scale", "v_scale", "tables", "lengths", "refs")}
+        _, state = op_.reserve(state, torch.tensor([32]))
+        given = []
+        size = 1.0
+        for _ in range(8):
+            x = torch.randn(1, 1, 4, 32, generator=g) * torch.exp2(-torch.randint(0, 18, (1, 1, 4, 32), generator=g).float()) * size
+            state = op_.append(state, x, x)
+            given.append(x)
+            state["lengths"] = state["lengths"] + 4
+            want, unit = torch.cat(given, 2)[0].double(), float(state["k_scale"][0, 0, 0])
+            held = op_.rows_of(state, 0, range(want.shape[1]))
+            assert torch.equal(held[0], held[1])
+            off = (held[0] - want).abs()
+            assert bool((off[:, -4:] <= torch.maximum(2.0 ** -4 * want.abs(), torch.tensor(2.0 ** -10 * unit))[:, -4:]).all())
+            assert bool((off <= 2.0 ** -4 * want.abs() + 2.0 ** -9 * unit).all())
+            worst = max(worst, float((off / torch.maximum(2.0 ** -4 * want.abs(), torch.tensor(2.0 ** -10 * unit))).max()))
+            size *= float(torch.randint(1, 4, (), generator=g))
+    assert worst > 1.3  # once rounded again, values are further off than one rounding says
