@@ -240,8 +240,8 @@ def auto_splits(batch: int, kv_heads: int, capacity: int, rows: int, dim: int, d
 
     A workgroup takes 16 rows, or in bf16 32 of up to 64, or 128 of more than 64 (16-bit heads of
     64 and 128). About as many as run at once, 256; 512 of the last kind, and where sequences
-    may differ in length, so that long ones have more of them. At least 1024 slots each, at
-    most 64 splits. Measured, us at 1 / 2 / 4 / 8 splits, bf16, 8 KV heads of 128: 32 rows of 8000 slots
+    may differ in length, so that long ones have more of them. About 1024 slots each (to the
+    nearest number of splits: 768 at least), at most 64 splits. Measured, us at 1 / 2 / 4 / 8 splits, bf16, 8 KV heads of 128: 32 rows of 8000 slots
     84 / 89 / 92 / -, of 1K to 8K 64 / 56 / 60 / 68; 16 of 4000 29 / 27 / 28 / 31, of 2K to 16K 99 / 64 /
     52 / 56; 8 of 4000 28 / 21 / 17 / 19; 8 of 1000 11.6 / 13.9 / 14.2 / -; 16 heads of 64 with a window
     of 4095 24 / 29 / 33 / 45; 1 of 131072 at 16 / 32 / 64 splits 76 / 52 / 55; 27 tokens of 4 heads

@@ -362,3 +362,13 @@ def test_what_codes_hold_of_the_values_that_were_appended():
             worst = max(worst, float((off / torch.maximum(2.0 ** -4 * want.abs(), torch.tensor(2.0 ** -10 * unit))).max()))
             size *= float(torch.randint(1, 4, (), generator=g))
     assert worst > 1.3  # once rounded again, values are further off than one rounding says
+
+
+def test_auto_splits_leave_768_slots_each():
+    """Capacities between the multiples of 1024: the number of splits is the nearest one."""
+    for reach, splits in ((1, 1), (1535, 1), (1537, 2), (2559, 2), (2561, 3), (3583, 3), (3585, 4), (66000, 64)):
+        assert paged.auto_splits(1, 1, reach, 1, 128, torch.bfloat16) == splits
+        assert paged.auto_splits(1, 1, 1 << 20, 1, 128, torch.bfloat16, reach - 1) == splits
+    for reach in range(1, 9000):
+        splits = paged.auto_splits(1, 1, reach, 1, 128, torch.bfloat16)
+        assert splits == 1 or reach // splits >= 768
