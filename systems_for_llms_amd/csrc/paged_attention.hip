@@ -11,9 +11,7 @@
 // power of two), on their way into the matrix cores; what has more bits goes in as a sum of
 // bf16 pieces: q of fp16 as two, of fp32 as three, and the probabilities of 16-bit rows as two,
 // of fp32 as three, so the only roundings are those of the probabilities to the sum of their
-// pieces (2^-16 or 2^-24 of them) and of fp32 sums. bf16 rows beyond 32 to a KV head have
-// one piece (2^-8): there the matrix cores are what a second one waits for, see
-// paged_attention_kernel.
+// pieces (2^-16 or 2^-24 of them) and of fp32 sums.
 #include <algorithm>
 #include <type_traits>
 
@@ -51,6 +49,11 @@ struct PagedArgs {
 };
 
 template <typename T> constexpr int pieces_of() { return std::is_same<T, bf16_t>::value ? 1 : std::is_same<T, f16_t>::value ? 2 : 3; }
+// Of probabilities. With one piece for bf16 rows, off by 2^-8, results are 2.2e-3 from 64 bits, with
+// two 1.7e-3, which is their own rounding. us with one and with two: 32 rows of up to 8191 tokens
+// 54.9 / 55.6, one of 1024 12.0 / 12.0; where the matrix cores are busy, 64 query rows over 8 x
+// 8000 keys 39.4 / 45.9, 108 over 8 of 1K to 8K 44.5 / 53.0, 512 over 32000 86.8 / 109.9.
+template <typename T> constexpr int prob_pieces_of() { return std::is_same<T, float>::value ? 3 : 2; }
 
 // What a sequence has: committed tokens, new ones in use, slots.
 struct PagedRow {
@@ -314,17 +317,13 @@ __device__ __forceinline__ u32x4 load_v(const uint8_t* at) {
 // Both ways measured, us at those two: values past the caches 58, 57 and through them 63, 52
 // (pages of 64, pages of 128); both tiles' values ahead 58, 57; 4, 6, 8 and 12 waves 57, 56,
 // 56, 56 at their best splits, 8 for one short row (11 us for 1024 keys, where two splits and
-// their merge take 13.5); three waves a SIMD instead of two 60. Probabilities of bf16 rows as
-// one piece and as two: 16 rows (NC 1) 54.9 / 55.6, 52.4 / 52.6 (16 of up to 16000 tokens),
-// 12.0 / 12.0 (1024 keys), so two; 32 rows (NC 2) 64 rows over 8 x 8000 39.3 / 45.2, 40 of 64
-// dims 25.5 / 28.3, and paged_rows_kernel 108 over 8 of 1K to 8K 44.4 / 52.6, 512 over 32000
-// 93.8 / 116.5, so one there, as in the framework's other bf16 attention.
+// their merge take 13.5); three waves a SIMD instead of two 60.
 template <typename T, int D, int NC, int kPage, int W>
 __global__ __launch_bounds__(W * kWave, D == 128 && NC == 2 ? 1 : 2) void paged_attention_kernel(const PagedArgs a) {
   using L = Tile<D>;
   constexpr bool kWide = kPage >= kPagedTile;
   constexpr int P = pieces_of<T>(), BT = kPagedTile, kRows = 16 * NC, kLine = D + 4;
-  constexpr int kProb = NC == 1 ? std::max(P, 2) : P;  // pieces of the probabilities
+  constexpr int kProb = prob_pieces_of<T>();
   __shared__ float merged[W][kRows][kLine];
   __shared__ float tops[W][kRows], sums[W][kRows];
   const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave);
@@ -583,6 +582,7 @@ template <typename T, int D, int kPage>
 __global__ __launch_bounds__(kRowWaves * kWave, 2) void paged_rows_kernel(const PagedArgs a) {
   constexpr bool kWide = kPage >= kPagedTile;
   constexpr int P = pieces_of<T>(), BT = kPagedTile, kRows = 32 * kRowWaves, kThreads = kRowWaves * kWave;
+  constexpr int kProb = prob_pieces_of<T>();
   constexpr int kSteps = D / 16, kTiles = D / 32;          // of the products with K, of dims of V
   constexpr int kPieces = BT * D / 16 / kThreads;          // of 16 codes of a tile's keys a thread stages
   constexpr int kSpots = kWide ? 1 : 4, kBatch = kWave / kSpots;
@@ -739,7 +739,7 @@ __global__ __launch_bounds__(kRowWaves * kWave, 2) void paged_rows_kernel(const 
         for (int e = 0; e < 16; ++e) o[d][e] *= keep;
     }
     const float base = top == -INFINITY ? 0.f : top;
-    u32x4 prob[4][P];
+    u32x4 prob[4][kProb];
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
       float y[8];
@@ -759,7 +759,7 @@ __global__ __launch_bounds__(kRowWaves * kWave, 2) void paged_rows_kernel(const 
         for (int y = 0; y < 2; ++y) {
           const u32x4 v = from_codes(w[2 * y], w[2 * y + 1], vs[x]);
 #pragma unroll
-          for (int p = P - 1; p >= 0; --p) o[d] = mfma32<bf16_t>(v, prob[2 * x + y][p], o[d]);
+          for (int p = kProb - 1; p >= 0; --p) o[d] = mfma32<bf16_t>(v, prob[2 * x + y][p], o[d]);
         }
       }
   }

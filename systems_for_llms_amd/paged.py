@@ -245,7 +245,7 @@ def auto_splits(batch: int, kv_heads: int, capacity: int, rows: int, dim: int, d
     84 / 89 / 92 / -, of 1K to 8K 64 / 56 / 60 / 68; 16 of 4000 29 / 27 / 28 / 31, of 2K to 16K 99 / 64 /
     52 / 56; 8 of 4000 28 / 21 / 17 / 19; 8 of 1000 11.6 / 13.9 / 14.2 / -; 16 heads of 64 with a window
     of 4095 24 / 29 / 33 / 45; 1 of 131072 at 16 / 32 / 64 splits 76 / 52 / 55; 27 tokens of 4 heads
-    over 8 of 1K to 8K 185 / 102 / 59 / 44.
+    over 8 of 1K to 8K 206 / 113 / 65 / 50.
     """
     block, blocks, reach = _blocks(batch, kv_heads, capacity, rows, dim, dtype, window_left)
     target = 512 if block == 128 or rows <= 16 and batch > 1 and window_left is None else 256
@@ -312,11 +312,10 @@ def prepare(q, cache, *, layer=0, counts=None, window_left=None, splits=None, sc
     ``lse`` (fp32 ``[B, Hq, T]``) of -inf, as are those of tokens that see nothing or have no slot. What
     a token does not see has no part in its row, NaN included. Scores and sums are fp32, and
     no code is rounded again: probabilities, of up to 2^8 before the division by their sum, are rounded
-    to two bf16 pieces (off by 2^-16) for 16-bit ``q``, three for fp32, and to one (2^-8) for bf16 ``q``
-    of 64 or 128 dims with more than 32 rows to a KV head (T times Hq / Hkv). ``splits``: workgroups
-    that share a KV head's slots, 1 to 128; by default as many as the sizes ask for, and more for
-    sequences far longer than the others. Like ``tree.PreparedTree`` the operation owns its scratch
-    and output and holds its inputs by reference; concurrent calls on one race.
+    to two bf16 pieces (off by 2^-16) for 16-bit ``q``, to three for fp32. ``splits``: workgroups that
+    share a KV head's slots, 1 to 128; by default as many as the sizes ask for, and more for sequences
+    far longer than the others. Like ``tree.PreparedTree`` the operation owns its scratch and output
+    and holds its inputs by reference; concurrent calls on one race.
     """
     if splits is not None and (type(splits) is not int or not 1 <= splits <= MAX_SPLITS):
         raise ValueError("splits must be an integer in [1, 128]")
