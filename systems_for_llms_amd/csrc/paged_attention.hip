@@ -310,11 +310,14 @@ __device__ __forceinline__ u32x4 load_v(const uint8_t* at) {
 
 // A workgroup has up to 16 NC query rows (the G heads of a KV head times the tokens, row
 // r = t G + g) and a split of the keys; its waves take the split's tiles in turn and are
-// joined through LDS at the end. Codes go from memory to registers, a tile's values under
-// way during its scores, the next tile's keys during its softmax. Bound by HBM: 32 rows of
-// 8000 tokens of 8 heads of 128 84 us (537 MB, 6.4 TB/s), of 1K to 8K 51 (310 MB, 6.0), one of
-// 131072 48 (268 MB, 5.6); a CU alone reads 35 GB/s, so a head wants about 30 workgroups.
-// Both ways measured, us at those two: values past the caches 58, 57 and through them 63, 52
+// joined through LDS at the end. Codes go from memory to registers: a tile's values are asked
+// for before or among its products with K, the next tile's keys before its softmax. Nothing
+// stays under way from one tile to the next: keys are asked for on one of two paths (not on
+// the last tile's), so the waits before the products with V, which have to hold on both, let
+// the keys arrive, too; the other seven waves are what fills the time. Bound by HBM: 32 rows of
+// 8000 tokens of 8 heads of 128 84 us (537 MB, 6.4 TB/s), of 1K to 8K 52 (314 MB, 6.0, the matrix
+// cores busy for 13% of it, vector instructions for 28%), one of 131072 48 (274 MB, 5.6); a CU alone
+// reads 35 GB/s, so a head wants about 30 workgroups. Both ways measured, us at those two: values past the caches 58, 57 and through them 63, 52
 // (pages of 64, pages of 128); both tiles' values ahead 58, 57; 4, 6, 8 and 12 waves 57, 56,
 // 56, 56 at their best splits, 8 for one short row (11 us for 1024 keys, where two splits and
 // their merge take 13.5); three waves a SIMD instead of two 60.
@@ -571,13 +574,15 @@ __global__ __launch_bounds__(W * kWave, D == 128 && NC == 2 ? 1 : 2) void paged_
 // two products: in those with K dims 32 x + 16 h .. + 15 of a key, in those with V keys
 // 32 x + 16 h .. + 15 of a dim (lane = 32 h + n). So that lane (h, n) holds the scores of the
 // latter, row m of S^T takes the key 16 (m / 4 % 2) + 8 (m / 16) + 4 (m / 8 % 2) + m % 4 of its 32.
-// Bound by a wave's chain and its vector instructions (128 conversions, 32 exponentials and
-// their like beside 32 products of 32 cycles to a tile of 32 rows of 128): 512 rows over 32000
-// keys of 8 heads 87 us with the merge (770 TFLOP/s), 27 tokens of 4 heads over 8 rows of 1K to
-// 8K 37. Measured: tiles staged as bf16 (a conversion for four waves, twice the LDS bytes) 89;
-// two buffers and one barrier a tile 90; the products of the tile before between this tile's
-// exponentials 89 to 95; two teams of four waves to a workgroup 86 at half the splits, but 51
-// where 37 + 7 stand for rows of different length.
+// Bound by a wave's chain, its products and its vector instructions (48 products of 32 cycles
+// beside 128 conversions, 32 exponentials and their pieces, some 400 in all, to a tile of 32 rows
+// of 128 in bf16): 512 rows over 32000 keys of 8 heads 110 us with the merge (610 TFLOP/s), 27
+// tokens of 4 heads over 8 rows of 1K to 8K 46 (350), the matrix cores busy for 42% of it, vector
+// instructions for 57%. Measured with the probabilities as one piece, where those two took 87
+// and 37: tiles staged as bf16 (a conversion for four waves, twice the LDS bytes) 89; two buffers
+// and one barrier a tile 90; the products of the tile before between this tile's exponentials
+// 89 to 95; two teams of four waves to a workgroup 86 at half the splits, but 51 where 37 + 7
+// stand for rows of different length.
 template <typename T, int D, int kPage>
 __global__ __launch_bounds__(kRowWaves * kWave, 2) void paged_rows_kernel(const PagedArgs a) {
   constexpr bool kWide = kPage >= kPagedTile;
@@ -824,8 +829,8 @@ __global__ __launch_bounds__(kRowWaves * kWave, 2) void paged_rows_kernel(const 
 
 // The splits of a row joined. A wave has a row, or with `kShared` a workgroup has one and
 // its four waves every fourth round of splits; kRound splits' loads go out together. A
-// chain of latencies for few rows (1024 of 2 splits 4.7 us; 32 of 32 splits 4.6, with a wave to
-// a row 6.0), memory for many (6912 of 8 splits, 29 MB, 7.8).
+// chain of latencies for few rows (1024 of 2 splits 4.8 us; 32 of 32 splits 4.8, with a wave to
+// a row 6.0), memory for many (6912 of 8 splits, 32 MB read, 8.3).
 template <typename T, int D, bool kShared>
 __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedArgs a) {
   constexpr int DPL = (D + kWave - 1) / kWave, kRound = 8, W = kShared ? 4 : 1;
@@ -909,10 +914,10 @@ int launch_paged(PagedArgs& a, hipStream_t stream) {
   const char* what = "page_attention";
   const int rows = a.tokens << a.group_log2;
   // By rows, us at the best number of splits with blocks of 16 / 32 rows / 128 that share
-  // tiles: bf16 D 128 2 x 8000 keys of 8 heads 32 rows 15.2 / 16.3 / 20.4, 8 x 4000 of 16
-  // heads 40 rows 52.9 / 36.9 / 46.4, 8 x 8000 of 8 heads 64 rows 53.8 / 41.4 / 45.7, 4 x
-  // 8000 128 rows - / 40.5 / 37.8, 16 x 4000 128 rows - / 69 / 62, 32000 keys 512 rows - /
-  // 121 / 89; fp16, whose pieces leave blocks of 32 rows too few registers, 8 x up to 8000 40
+  // tiles: bf16 D 128 2 x 8000 keys of 8 heads 32 rows 15.6 / 16.7 / 21.5, 8 x 4000 of 16
+  // heads 40 rows 52.9 / 39.9 / 51.2, 8 x 8000 of 8 heads 64 rows 51.8 / 43.0 / 53.3, 8 of 1K
+  // to 8K 108 rows 67.5 / 56.7 / 49.6, 4 x 8000 128 rows 57.9 / 41.4 / 40.6, 16 x 4000 128 rows
+  // 104.8 / 72.6 / 67.7, 32000 keys 512 rows 190 / 128 / 107; fp16, whose pieces leave blocks of 32 rows too few registers, 8 x up to 8000 40
   // rows 37.3 / 43.6 / 59, D 64 8 x 8000 128 rows - / 49.9 / 48; fp32 4 x 4000 128 rows 32.3 /
   // 39.4, D 64 8 x 4000 128 rows 34.1 / 37.2; D 32 8 x 4000 128 rows 17.7 / 21.1.
   constexpr bool kPairs = pieces_of<T>() == 1 && D >= 64, kShares = pieces_of<T>() < 3 && D >= 64;

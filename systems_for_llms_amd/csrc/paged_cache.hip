@@ -234,7 +234,7 @@ __device__ __forceinline__ int parent_of(const int32_t* parents, int b, int batc
 
 // Every row takes the filled pages of its parent, all at once: a workgroup has some columns
 // of the tables, of all rows, and holds them in LDS before it writes the first. `alone`: the
-// grid is this workgroup, which then writes the lengths too (64 rows of 17 places 3.2 us;
+// grid is this workgroup, which then writes the lengths too (64 rows of 17 places 3.6 us;
 // other grids have another launch for them).
 __global__ __launch_bounds__(kBookThreads) void fork_kernel(const BookArgs a, const int32_t* parents, int columns, int alone) {
   extern __shared__ int32_t held[];  // [batch][columns], then [batch] filled pages
@@ -336,7 +336,7 @@ __device__ __forceinline__ int find_free(const BookArgs& a, int from, int most, 
 // do to a place's page is found from the pages they hold: of r holders, the first r - 1 that
 // write it leave it, and the last then has it alone. (Those of earlier rounds have left, or
 // there are no free pages any more.) Bound by its chain of loads and barriers: 64 rows, 16 of
-// them with 6 new places and 16 that share a page, of 1600 pages 10 to 11 us.
+// them with 6 new places and 16 that share a page, of 1600 pages 11 to 12 us.
 __global__ __launch_bounds__(kBookThreads) void reserve_kernel(const BookArgs a, const int32_t* counts, int32_t* granted,
                                                                int2* copies, int* copied) {
   __shared__ int sums[kBookThreads / kWave];
@@ -418,7 +418,7 @@ __global__ __launch_bounds__(kBookThreads) void reserve_kernel(const BookArgs a,
 }
 
 // Which pages move where: the k-th page in use past the first `used` to the k-th free one
-// among them. 2048 pages 6.3 us, a chain of loads and barriers.
+// among them. 2048 pages 6.5 us, a chain of loads and barriers.
 __global__ __launch_bounds__(kBookThreads) void compact_plan_kernel(const BookArgs a, int2* moves, int32_t* target, int* moved,
                                                                     int32_t* used) {
   constexpr int kScan = 8;
@@ -470,7 +470,7 @@ constexpr int kCopyPieces = 4, kCopyPart = 256 * 16 * kCopyPieces;
 
 // Pages copied, all layers: workgroups walk (move, layer, keys or values, 16 KB of it), as a
 // plan made on the device is not known to the launch. Bound by memory: 491 pages of 8 layers,
-// 1.03 GB read and written, 198 to 212 us (4.9 to 5.2 TB/s); 94 MB 20 (4.6).
+// 1.03 GB read and written, 209 us (4.9 TB/s); 94 MB 20 (4.7).
 __device__ __forceinline__ void copy_pages(const CopyArgs& c) {
   const long items = long(*c.moved) * c.layers * 2 * c.parts;
   for (long y = blockIdx.x; y < items; y += gridDim.x) {
