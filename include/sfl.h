@@ -609,7 +609,8 @@ int sfl_compact_slots(void* k, void* v, float* weights, int32_t* positions, cons
  * the code of NaN. Tokens are left out whose page is missing or has refs != 1.
  *   k, v [batch, kv_heads, tokens] rows of head_dim of dtype F32, BF16 or F16
  *   strides [6]: k, v {batch, head, token}, multiples of 16 bytes
- * k, v and counts must not share memory with the layer's codes and scales, which are written.
+ * k, v and counts must not share memory with the layer's codes and scales, which are written:
+ * no part of these may lie between the first and the last byte of those.
  */
 int sfl_page_append(const void* k, const void* v, void* k_codes, void* v_codes, float* k_scale, float* v_scale,
                     const int32_t* tables, const int32_t* lengths, const int32_t* counts, const int32_t* refs,
